@@ -10,5 +10,6 @@ namespace pdt {
 void multi_flatten_tensors(std::vector<at::Tensor>& srcs, std::vector<at::Tensor>& dsts, double scale);
 
 void bind_ops(pybind11::module& m);
+void bind_transformer_ops(pybind11::module& m);  // ops_transformer.cpp
 
 }  // namespace pdt

@@ -13,6 +13,7 @@ PYBIND11_MODULE(_C, m) {
     m.doc() = "MI355X (gfx950) native kernels, RCCL communicator and gradient reducer";
     m.attr("arch") = "gfx950";
     pdt::bind_ops(m);
+    pdt::bind_transformer_ops(m);
 
     py::class_<pdt::RcclComm, std::shared_ptr<pdt::RcclComm>>(m, "RcclComm")
         // unique_id arrives as std::string (converted from bytes while the GIL is still held); the

@@ -1,0 +1,347 @@
+// Torch bindings of attention_ext.hip and gated_norm.hip: every shape, type, stride, device and size that the kernels assume
+// is checked here (a faulting kernel can take the whole node down), outputs and workspaces come from the caching allocator,
+// launches go to the current stream of the operands' device.
+#include <ATen/ATen.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/extension.h>
+
+#include <cmath>
+
+#include "../kernels/attention_ext.h"
+#include "../kernels/gated_norm.h"
+#include "../kernels/kernels.h"
+#include "binding.h"
+
+namespace pdt {
+namespace {
+
+using at::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+void check_same_device(const Tensor& t, const Tensor& like, const char* name) {
+    TORCH_CHECK(t.device() == like.device(), name, ": expected on ", like.device(), ", got ", t.device());
+}
+// [B, rows, width] bf16 with contiguous, 16-B aligned, non-overlapping rows
+void check_rows(const Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 3, name, ": expected a bf16 GPU tensor [B, rows, width]");
+    TORCH_CHECK(t.numel() == 0 || (t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0), name,
+                ": expected contiguous rows, 16-B aligned");
+    TORCH_CHECK(t.size(1) < 2 || (t.stride(1) % 8 == 0 && t.stride(1) >= t.size(2) && t.stride(1) < (1L << 23)), name,
+                ": row stride ", t.stride(1));
+    TORCH_CHECK(t.size(0) < 2 || (t.stride(0) % 8 == 0 && t.stride(0) >= 0), name, ": batch stride ", t.stride(0));
+}
+void check_dense(const Tensor& t, at::IntArrayRef shape, at::ScalarType type, const Tensor& like, const char* name) {
+    TORCH_CHECK(t.scalar_type() == type && t.is_contiguous() && t.sizes() == shape, name, ": expected contiguous ", type, " ", shape,
+                ", got ", t.scalar_type(), " ", t.sizes());
+    TORCH_CHECK(t.numel() == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, ": data pointer must be 16-B aligned");
+    check_same_device(t, like, name);
+}
+ExtView view_of(const Tensor& t, int G) {
+    return {t.size(0) < 2 ? 0 : (long)t.stride(0), t.size(1) < 2 ? (long)t.size(2) : (long)t.stride(1), make_fastdiv((uint32_t)G)};
+}
+const __bf16* bf16_ptr(const Tensor& t) { return static_cast<const __bf16*>(t.data_ptr()); }
+
+// operands that forward and backward share; q [B,Sq,H*hd], k and v [B,Sk,Hkv*hd] with equal strides
+ExtArgs ext_args(const Tensor& q, const Tensor& k, const Tensor& v, int64_t heads, int64_t kv_heads, const OptTensor& lens, int64_t hd,
+                 bool self) {
+    TORCH_CHECK(hd == 32 || hd == 64 || hd == 128, "attention: head_dim ", hd, " not supported (32, 64 or 128)");
+    const long B = q.size(0), G = heads / kv_heads, M = q.size(1) * G;
+    TORCH_CHECK(M < (1L << 30) && k.size(1) < (1L << 30) && B < (1L << 30), "attention: lengths below 2^30");
+    ExtArgs a{};
+    a.q = bf16_ptr(q); a.k = bf16_ptr(k); a.v = bf16_ptr(v);
+    a.qv = view_of(q, (int)G); a.kv = view_of(k, 1);
+    a.o = {(long)(q.size(1) * heads * hd), (long)(heads * hd), make_fastdiv((uint32_t)G)};
+    TORCH_CHECK(a.o.rs < (1L << 23), "attention: width ", a.o.rs);
+    if (given(lens)) {
+        check_dense(*lens, {B}, at::kInt, q, "lengths");
+        a.lens = lens->data_ptr<int>();
+    }
+    a.self = self;
+    a.B = (int)B; a.Hkv = (int)kv_heads; a.G = (int)G; a.Sq = (int)q.size(1); a.Sk = (int)k.size(1);
+    a.M = (int)M; a.Mp = (int)((M + 63) / 64 * 64);
+    a.stat_n = B * kv_heads * a.Mp;
+    a.scale = (float)(1.0 / std::sqrt((double)hd));
+    a.c = (float)(1.4426950408889634 / std::sqrt((double)hd));
+    return a;
+}
+void check_grid(const ExtArgs& a, const ExtPlan& p) {
+    TORCH_CHECK((long)a.B * a.Hkv < (1L << 30) / std::max(1, p.tiles * p.splits), "attention: more than 2^30 workgroups");
+}
+void set_tables(ExtArgs& a, const Tensor& tab, const Tensor& codes, int64_t R) {
+    const long Sp = (a.Sk + 63) / 64 * 64, Rp = (R + 3) / 4 * 4;
+    TORCH_CHECK(R >= 1 && R <= kExtMaxEntries, "rel_bias_attention: ", R, " entries (1 to ", kExtMaxEntries, ")");
+    TORCH_CHECK(tab.sizes() == at::IntArrayRef({(long)a.Hkv, Rp}) && codes.sizes() == at::IntArrayRef({2, Sp}), "bias tables: shape");
+    a.tab = tab.data_ptr<float>();
+    a.q_codes4 = codes.data_ptr<int>();
+    a.k_codes4 = codes.data_ptr<int>() + Sp;
+    a.R = (int)R; a.Rp = (int)Rp;
+}
+
+// -> out, stat (with `grad`), out_lo (with `lo`)
+std::tuple<Tensor, Tensor, Tensor> ext_fwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, bool grad, bool lo) {
+    Tensor out = at::empty({a.B, a.Sq, heads * hd}, q.options().memory_format(at::MemoryFormat::Contiguous)), stat, out_lo;
+    const auto f32 = q.options().dtype(at::kFloat);
+    if (grad) stat = at::empty({2, (long)a.B * a.Hkv, a.Mp}, f32);
+    if (lo) out_lo = at::empty_like(out);
+    if (out.numel() == 0) return {out, stat, out_lo};
+    const long BH = (long)a.B * a.Hkv;
+    const ExtPlan p = ext_plan_fwd(BH, a.M, a.Sk, a.tab != nullptr);
+    check_grid(a, p);
+    Tensor part, ml;
+    if (p.splits > 1) {
+        part = at::empty({BH * p.splits * a.M * hd}, f32);
+        ml = at::empty({BH * p.splits * a.M * 2}, f32);
+    }
+    launch_ext_fwd(a, p, (int)hd, out.data_ptr(), lo ? out_lo.data_ptr() : nullptr, grad ? stat.data_ptr<float>() : nullptr,
+                   part.defined() ? part.data_ptr<float>() : nullptr, ml.defined() ? ml.data_ptr<float>() : nullptr, stream_of(q));
+    return {out, stat, out_lo};
+}
+
+// dq / dk / dv: views to fill; -> dtable [NB, H] when bucket_of is given
+Tensor ext_bwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, const Tensor& dout, const Tensor& out, const OptTensor& out_lo,
+               const Tensor& stat, Tensor dq, Tensor dk, Tensor dv, const OptTensor& bucket_of, int64_t NB) {
+    const long width = heads * hd, BH = (long)a.B * a.Hkv;
+    check_dense(dout, {a.B, a.Sq, width}, at::kBFloat16, q, "dout");
+    check_dense(out, {a.B, a.Sq, width}, at::kBFloat16, q, "out");
+    check_dense(stat, {2, BH, a.Mp}, at::kFloat, q, "stat");
+    const auto f32 = q.options().dtype(at::kFloat);
+    Tensor dtable;
+    if (given(bucket_of)) {
+        check_dense(*bucket_of, {a.R}, at::kInt, q, "bucket_of");
+        dtable = at::empty({NB, heads}, f32);
+    }
+    if (BH == 0 || a.M == 0 || a.Sk == 0) {
+        dq.zero_(); dk.zero_(); dv.zero_();
+        if (dtable.defined()) dtable.zero_();
+        return dtable;
+    }
+    ExtBwd w{};
+    w.out = out.data_ptr(); w.dout = dout.data_ptr();
+    if (given(out_lo)) {
+        check_dense(*out_lo, {a.B, a.Sq, width}, at::kBFloat16, q, "out_lo");
+        w.out_lo = out_lo->data_ptr();
+    }
+    w.stat = stat.data_ptr<float>();
+    w.dq = dq.data_ptr(); w.dk = dk.data_ptr(); w.dv = dv.data_ptr();
+    a.dqv = view_of(dq, a.G); a.dkv = view_of(dk, 1);
+    w.q = ext_plan_bwd(BH, a.M, a.Sk);
+    w.kv = ext_plan_bwd(BH, a.Sk, a.M);
+    check_grid(a, w.q); check_grid(a, w.kv);
+    Tensor dsum = at::empty({BH, a.Mp}, f32), pq, pk, pv, slab, mid;
+    w.dsum = dsum.data_ptr<float>();
+    if (w.q.splits > 1) {
+        pq = at::empty({BH * w.q.splits * a.M * hd}, f32);
+        w.part_q = pq.data_ptr<float>();
+    }
+    if (w.kv.splits > 1) {
+        pk = at::empty({BH * w.kv.splits * a.Sk * hd}, f32);
+        pv = at::empty_like(pk);
+        w.part_k = pk.data_ptr<float>();
+        w.part_v = pv.data_ptr<float>();
+    }
+    const int per_head = w.q.tiles * w.q.splits;
+    if (dtable.defined()) {
+        slab = at::empty({BH * per_head, a.Rp}, f32);
+        w.slab = slab.data_ptr<float>();
+    }
+    launch_ext_bwd(a, w, (int)hd, stream_of(q));
+    if (dtable.defined() && NB > 0) {
+        const int chunks = bias_grad_chunks(a.B * per_head);
+        mid = at::empty({chunks, (long)heads, a.Rp}, f32);
+        launch_bias_grad(w.slab, mid.data_ptr<float>(), bucket_of->data_ptr<int>(), dtable.data_ptr<float>(), a.R, a.Rp, (int)NB,
+                         (int)heads, a.B, per_head, chunks, stream_of(q));
+    }
+    return dtable;
+}
+
+// ------------------------------------------------------------------------------------ relative-position bias
+long packed_head_dim(const Tensor& qkv, int64_t heads) {
+    check_rows(qkv, "qkv");
+    TORCH_CHECK(heads > 0 && qkv.size(2) % (3 * heads) == 0, "rel_bias_attention: width ", qkv.size(2), " is not 3 * heads * head_dim");
+    return qkv.size(2) / (3 * heads);
+}
+
+// -> out, stat, out_lo, tab [H, Rp], codes [2, Sp]; stat with `grad`, out_lo with `lo`
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> rel_bias_attention_fwd(const Tensor& qkv, const Tensor& table, const Tensor& q_codes,
+                                                                          const Tensor& k_codes, const Tensor& bucket_of, int64_t heads,
+                                                                          const OptTensor& lens, bool grad, bool lo) {
+    const long hd = packed_head_dim(qkv, heads), D = heads * hd, S = qkv.size(1), R = bucket_of.size(0), NB = table.size(0);
+    TORCH_CHECK(R >= 1 && R <= kExtMaxEntries, "rel_bias_attention: ", R, " entries (1 to ", kExtMaxEntries, ")");
+    TORCH_CHECK(NB < (1L << 30) && S < (1L << 30), "rel_bias_attention: sizes below 2^30");
+    check_dense(table, {NB, heads}, at::kFloat, qkv, "table");
+    check_dense(q_codes, {S}, at::kInt, qkv, "q_codes");
+    check_dense(k_codes, {S}, at::kInt, qkv, "k_codes");
+    check_dense(bucket_of, {R}, at::kInt, qkv, "bucket_of");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(qkv.device());
+    const long Rp = (R + 3) / 4 * 4, Sp = (S + 63) / 64 * 64;
+    Tensor tab = at::empty({heads, Rp}, table.options()), codes = at::empty({2, Sp}, q_codes.options());
+    launch_bias_tables(table.data_ptr<float>(), bucket_of.data_ptr<int>(), q_codes.data_ptr<int>(), k_codes.data_ptr<int>(),
+                       tab.data_ptr<float>(), codes.data_ptr<int>(), codes.data_ptr<int>() + Sp, (int)R, (int)Rp, (int)NB, (int)heads,
+                       (int)S, (int)Sp, (float)std::sqrt((double)hd), stream_of(qkv));
+    const Tensor q = qkv.narrow(2, 0, D), k = qkv.narrow(2, D, D), v = qkv.narrow(2, 2 * D, D);
+    ExtArgs a = ext_args(q, k, v, heads, heads, lens, hd, true);
+    set_tables(a, tab, codes, R);
+    auto [out, stat, out_lo] = ext_fwd(a, q, heads, hd, grad, lo);
+    return {out, stat, out_lo, tab, codes};
+}
+
+// -> dqkv [B, S, 3 H hd], dtable [NB, H] fp32 (undefined without `want_table`)
+std::tuple<Tensor, Tensor> rel_bias_attention_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out, const OptTensor& out_lo,
+                                                  const Tensor& stat, const Tensor& tab, const Tensor& codes, const Tensor& bucket_of,
+                                                  int64_t NB, int64_t heads, const OptTensor& lens, bool want_table) {
+    const long hd = packed_head_dim(qkv, heads), D = heads * hd;
+    TORCH_CHECK(NB >= 0 && NB < (1L << 30), "rel_bias_attention: ", NB, " buckets");
+    check_same_device(tab, qkv, "tab"); check_same_device(codes, qkv, "codes");
+    TORCH_CHECK(tab.scalar_type() == at::kFloat && tab.is_contiguous() && codes.scalar_type() == at::kInt && codes.is_contiguous(),
+                "bias tables: as the forward made them");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(qkv.device());
+    const Tensor q = qkv.narrow(2, 0, D), k = qkv.narrow(2, D, D), v = qkv.narrow(2, 2 * D, D);
+    ExtArgs a = ext_args(q, k, v, heads, heads, lens, hd, true);
+    set_tables(a, tab, codes, bucket_of.size(0));
+    Tensor dqkv = at::empty({qkv.size(0), qkv.size(1), 3 * D}, qkv.options().memory_format(at::MemoryFormat::Contiguous));
+    Tensor dtable = ext_bwd(a, q, heads, hd, dout, out, out_lo, stat, dqkv.narrow(2, 0, D), dqkv.narrow(2, D, D), dqkv.narrow(2, 2 * D, D),
+                            want_table ? OptTensor(bucket_of) : OptTensor(), NB);
+    return {dqkv, dtable};
+}
+
+// ------------------------------------------------------------------------------------------- cross attention
+long cross_head_dim(const Tensor& q, const Tensor& kv, int64_t heads, int64_t kv_heads) {
+    check_rows(q, "q"); check_rows(kv, "kv");
+    check_same_device(kv, q, "kv");
+    TORCH_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "cross_attention: ", heads, " heads over ", kv_heads, " key heads");
+    TORCH_CHECK(q.size(2) % heads == 0 && kv.size(2) == 2 * kv_heads * (q.size(2) / heads), "cross_attention: widths ", q.size(2), " and ",
+                kv.size(2), " for ", heads, " heads and ", kv_heads, " key heads");
+    TORCH_CHECK(q.size(0) == kv.size(0), "cross_attention: batches ", q.size(0), " and ", kv.size(0));
+    return q.size(2) / heads;
+}
+// q [B, Sq, H hd], kv [B, Sk, 2 Hkv hd] (keys | values) -> out [B, Sq, H hd], stat (with `grad`)
+std::tuple<Tensor, Tensor> cross_attention_fwd(const Tensor& q, const Tensor& kv, int64_t heads, int64_t kv_heads, const OptTensor& lens,
+                                               bool grad) {
+    const long hd = cross_head_dim(q, kv, heads, kv_heads), W = kv_heads * hd;
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    ExtArgs a = ext_args(q, kv.narrow(2, 0, W), kv.narrow(2, W, W), heads, kv_heads, lens, hd, false);
+    auto [out, stat, lo] = ext_fwd(a, q, heads, hd, grad, false);
+    return {out, stat};
+}
+std::tuple<Tensor, Tensor> cross_attention_bwd(const Tensor& dout, const Tensor& q, const Tensor& kv, const Tensor& out, const Tensor& stat,
+                                               int64_t heads, int64_t kv_heads, const OptTensor& lens) {
+    const long hd = cross_head_dim(q, kv, heads, kv_heads), W = kv_heads * hd;
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    ExtArgs a = ext_args(q, kv.narrow(2, 0, W), kv.narrow(2, W, W), heads, kv_heads, lens, hd, false);
+    Tensor dq = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+    Tensor dkv = at::empty(kv.sizes(), kv.options().memory_format(at::MemoryFormat::Contiguous));
+    ext_bwd(a, q, heads, hd, dout, out, OptTensor(), stat, dq, dkv.narrow(2, 0, W), dkv.narrow(2, W, W), OptTensor(), 0);
+    return {dq, dkv};
+}
+
+// ---------------------------------------------------------------------------------------- gated residual norm
+// x, y [..., D] contiguous; gate [D], or [B, D] for x [B, ..., D]
+GatedNorm gated_norm_args(const Tensor& x, const Tensor& y, const Tensor& gate, const Tensor& w, const Tensor& b, const OptTensor& pw,
+                          const OptTensor& pb, double eps, double scale) {
+    TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kBFloat16 && x.dim() >= 2, "gated_residual_norm: expected a bf16 GPU tensor [..., D]");
+    check_dense(x, x.sizes(), at::kBFloat16, x, "x");
+    check_dense(y, x.sizes(), at::kBFloat16, x, "branch");
+    const long D = x.size(-1);
+    TORCH_CHECK(gated_norm_dim_ok(D), "gated_residual_norm: unsupported width ", D);
+    GatedNorm p{};
+    p.D = (int)D;
+    p.M = x.numel() / D;
+    p.per_sample = gate.dim() == 2;
+    if (p.per_sample) {
+        check_dense(gate, {x.size(0), D}, at::kFloat, x, "gate");
+        p.T = x.size(0) ? p.M / x.size(0) : 0;
+    } else {
+        check_dense(gate, {D}, at::kFloat, x, "gate");
+        p.T = p.M;
+    }
+    TORCH_CHECK(p.M < (1L << 32), "gated_residual_norm: ", p.M, " rows");
+    check_dense(w, {D}, at::kFloat, x, "weight"); check_dense(b, {D}, at::kFloat, x, "bias");
+    TORCH_CHECK(given(pw) == given(pb), "gated_residual_norm: post_weight and post_bias come together");
+    if (given(pw)) {
+        check_dense(*pw, {D}, at::kFloat, x, "post_weight"); check_dense(*pb, {D}, at::kFloat, x, "post_bias");
+        p.pw = pw->data_ptr<float>(); p.pb = pb->data_ptr<float>();
+    }
+    p.x = bf16_ptr(x); p.y = bf16_ptr(y);
+    p.gate = gate.data_ptr<float>(); p.w = w.data_ptr<float>(); p.b = b.data_ptr<float>();
+    p.a = (float)scale; p.eps = (float)eps;
+    return p;
+}
+// -> u, n, stats [2 or 4, M] (with `grad`)
+std::tuple<Tensor, Tensor, Tensor> gated_norm_fwd(const Tensor& x, const Tensor& y, const Tensor& gate, const Tensor& w, const Tensor& b,
+                                                  const OptTensor& pw, const OptTensor& pb, double eps, double scale, bool grad) {
+    const GatedNorm p = gated_norm_args(x, y, gate, w, b, pw, pb, eps, scale);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    Tensor u = at::empty_like(x), n = at::empty_like(x), stats;
+    if (grad) stats = at::empty({p.pw ? 4 : 2, p.M}, w.options());
+    if (p.M > 0) launch_gated_norm_fwd(p, u.data_ptr(), n.data_ptr(), grad ? stats.data_ptr<float>() : nullptr, stream_of(x));
+    return {u, n, stats};
+}
+// -> dx, dy, dgate, dw, db[, dpw, dpb]
+std::vector<Tensor> gated_norm_bwd(const OptTensor& du, const OptTensor& dn, const Tensor& x, const Tensor& y, const Tensor& gate,
+                                   const Tensor& w, const Tensor& b, const OptTensor& pw, const OptTensor& pb, const Tensor& stats,
+                                   double eps, double scale) {
+    const GatedNorm p = gated_norm_args(x, y, gate, w, b, pw, pb, eps, scale);
+    if (given(du)) check_dense(*du, x.sizes(), at::kBFloat16, x, "gradient of the stream");
+    if (given(dn)) check_dense(*dn, x.sizes(), at::kBFloat16, x, "gradient of the normalised");
+    const bool post = p.pw != nullptr;
+    check_dense(stats, {post ? 4 : 2, p.M}, at::kFloat, x, "stats");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    const long D = p.D;
+    Tensor dx = at::empty_like(x), dy = at::empty_like(x), dgate = at::empty(gate.sizes(), gate.options());
+    const int cols = post ? 4 : 2;
+    if (p.M == 0) {
+        Tensor z = at::zeros({cols, D}, w.options());
+        dgate.zero_();
+        std::vector<Tensor> r = {dx, dy, dgate, z[1], z[0]};
+        if (post) { r.push_back(z[3]); r.push_back(z[2]); }
+        return r;
+    }
+    const GatedNormPlan q = gated_norm_plan(x.size(0), p.T, p.M, p.per_sample);
+    // without a gate per sample a workgroup has one unit: its gate sums are one more column block of the slab
+    const int srow = (int)((cols + (p.per_sample ? 0 : 1)) * D);
+    Tensor slab = at::empty({q.blocks, srow}, w.options()), gate_part;
+    float* gp = slab.data_ptr<float>() + cols * D;
+    long gstride = srow;
+    if (p.per_sample) {
+        TORCH_CHECK(x.size(0) < (1L << 31) / ((D + 63) / 64), "gated_residual_norm: ", x.size(0), " samples");
+        gate_part = q.chunks > 1 ? at::empty({q.units, D}, w.options()) : dgate;
+        gp = gate_part.data_ptr<float>();
+        gstride = D;
+    }
+    launch_gated_norm_bwd(p, q, given(du) ? du->data_ptr() : nullptr, given(dn) ? dn->data_ptr() : nullptr, stats.data_ptr<float>(),
+                          dx.data_ptr(), dy.data_ptr(), gp, gstride, slab.data_ptr<float>(), srow, stream_of(x));
+    if (p.per_sample && q.chunks > 1)
+        launch_gate_sum(gp, dgate.data_ptr<float>(), x.size(0), p.D, q.chunks, stream_of(x));
+    Tensor sums;
+    if (q.blocks == 1) {
+        sums = slab.view({srow});
+    } else {
+        sums = at::empty({srow}, w.options());
+        Tensor tmp = at::empty({kReduceChunks, srow}, w.options());
+        launch_reduce_slab(slab.data_ptr<float>(), q.blocks, srow, srow, sums.data_ptr<float>(), tmp.data_ptr<float>(), stream_of(x));
+    } 
+    std::vector<Tensor> r = {dx, dy, p.per_sample ? dgate : sums.narrow(0, cols * D, D), sums.narrow(0, D, D), sums.narrow(0, 0, D)};
+    if (post) {
+        r.push_back(sums.narrow(0, 3 * D, D));
+        r.push_back(sums.narrow(0, 2 * D, D));
+    }
+    return r;
+}
+
+}  // namespace
+
+void bind_transformer_ops(pybind11::module& m) {
+    m.def("rel_bias_attention_fwd", &rel_bias_attention_fwd);
+    m.def("rel_bias_attention_bwd", &rel_bias_attention_bwd);
+    m.def("cross_attention_fwd", &cross_attention_fwd);
+    m.def("cross_attention_bwd", &cross_attention_bwd);
+    m.def("gated_norm_fwd", &gated_norm_fwd);
+    m.def("gated_norm_bwd", &gated_norm_bwd);
+    m.attr("rel_bias_max_entries") = kExtMaxEntries;
+}
+
+}  // namespace pdt

@@ -23,7 +23,8 @@ BUILD = os.path.join(HERE, "_build")
 ARCH = "gfx950"
 
 HIP_SOURCES = [
-    "kernels/elementwise.hip", "kernels/softmax_ce.hip", "kernels/bn.hip", "kernels/layernorm.hip", "kernels/attention.hip", "kernels/pool.hip",
+    "kernels/elementwise.hip", "kernels/softmax_ce.hip", "kernels/bn.hip", "kernels/layernorm.hip", "kernels/attention.hip", "kernels/attention_ext.hip",
+    "kernels/gated_norm.hip", "kernels/pool.hip",
     "kernels/gemm.hip", "kernels/gemm_tn.hip", "kernels/conv_win64.hip",
     "kernels/conv_stem_win.hip", "kernels/wgrad_win64.hip", "kernels/vit.hip", "kernels/conv_igemm.hip", "kernels/conv_wgrad.hip", "kernels/conv_wgrad_win.hip", "kernels/conv_stem.hip",
     "comm/ipc_allreduce.hip",
@@ -33,8 +34,11 @@ HIP_SOURCES = [
 # that decide whether a NaN stays visible.  They keep the rest of fast-math (contraction,
 # reassociation, approximate reciprocals); the GEMM-shaped kernels keep plain -ffast-math.
 NAN_AWARE = {"kernels/bn.hip", "kernels/softmax_ce.hip", "kernels/elementwise.hip", "kernels/pool.hip",
-             "kernels/layernorm.hip", "kernels/vit.hip", "comm/ipc_allreduce.hip"}
-CPP_SOURCES = ["binding/ops.cpp", "binding/module.cpp", "comm/rccl_comm.cpp", "comm/ipc_allreduce.cpp", "reducer/reducer.cpp"]
+             "kernels/layernorm.hip", "kernels/vit.hip", "kernels/attention_ext.hip", "kernels/gated_norm.hip", "comm/ipc_allreduce.hip"}
+# No packed fp32 instructions in device code: some forms that the compiler makes of ordinary float code have given wrong
+# results now and then on this hardware, without an error.
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+CPP_SOURCES = ["binding/ops.cpp", "binding/ops_transformer.cpp", "binding/module.cpp", "comm/rccl_comm.cpp", "comm/ipc_allreduce.cpp", "reducer/reducer.cpp"]
 
 
 def _torch_paths():
@@ -99,7 +103,8 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = True) ->
         obj = os.path.join(BUILD, rel.replace("/", "_") + ".o")
         objs.append(obj)
         is_hip = rel.endswith(".hip")
-        flags = hip_flags if is_hip else cpp_flags
+        flags = [*hip_flags, *NO_PACKED_FP32] if rel in ("kernels/attention_ext.hip", "kernels/gated_norm.hip") else (
+            hip_flags if is_hip else cpp_flags)
         if rel in NAN_AWARE:
             flags = [*flags, "-fno-finite-math-only"]
         stamp = digest + "|" + " ".join(flags)

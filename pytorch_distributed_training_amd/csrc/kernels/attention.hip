@@ -26,6 +26,7 @@
 #include <cmath>
 #include <cstdlib>
 
+#include "attn_tile.h"
 #include "common.h"
 #include "kernels.h"
 
@@ -34,10 +35,7 @@ namespace {
 
 constexpr int HD = 64;        // head dim
 constexpr int ROWB = HD * 2;  // LDS row bytes
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -1e30f;  // finite stand-in for -inf (the kernels are built with -ffast-math)
-
-typedef bf16x4 __attribute__((address_space(3))) * lds_bf16x4_ptr;
 
 __device__ __forceinline__ int swz(int row, int chunk) {
     const int x = (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
@@ -59,14 +57,6 @@ __device__ __forceinline__ bf16x8 frag_cols(const char* img, int r0, int colbase
     const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_ptr)(img + swz(rb, col >> 3) + (col & 7) * 2));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
-// accumulator tile regs [8*blk, 8*blk+8) -> bf16 A operand
-__device__ __forceinline__ bf16x8 acc_to_a(const f32x16& t, int blk) {
-    bf16x8 a;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = (bf16)t[8 * blk + j];
-    return a;
-}
-__device__ __forceinline__ int acc_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
 
 // stage rows [0, SP) of one of q/k/v (which = 0/1/2) or of a [B,S,H,64] tensor (which < 0) into an LDS image
 template <int NT, int NW>
@@ -764,57 +754,6 @@ __global__ __launch_bounds__(64 * NW) void k_attn_bwd_p(const bf16* __restrict__
 //    1.5x the matrix work of a one-sweep online softmax, on a path whose job is generality.
 //  * backward as two kernels (key-owner: dK, dV; query-owner: dQ) with D[q] = sum_d dO * O from a small pre-pass.
 //  * the softmax scale is applied to the fp32 scores (1/sqrt(32) is not a bf16 number).
-template <int HDT>
-struct AttnGeo {
-    static constexpr int ROWBYTES = HDT * 2, NCH = HDT / 8, STEPS = HDT / 16, DT = HDT / 32;
-    static __device__ __forceinline__ int swz(int row, int chunk) {
-        const int x = ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) & (NCH - 1);
-        return row * ROWBYTES + ((chunk ^ x) << 4);
-    }
-    static __device__ __forceinline__ bf16x8 rows(const char* img, int row, int step, int half) {
-        return *reinterpret_cast<const bf16x8*>(img + swz(row, 2 * step + half));
-    }
-    static __device__ __forceinline__ bf16x8 cols(const char* img, int r0, int colbase, int lane) {
-        const int q4 = (lane & 15) >> 2, p = lane & 3, h16 = (lane >> 4) & 1, half = lane >> 5;
-        const int col = colbase + h16 * 16 + p * 4;
-        const int ra = r0 + 4 * half + q4, rb = ra + 8;
-        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_ptr)(img + swz(ra, col >> 3) + (col & 7) * 2));
-        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4_ptr)(img + swz(rb, col >> 3) + (col & 7) * 2));
-        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-    // rows [r0, r0 + 64) of a [*, row_stride] tensor -> LDS image rows 0..63 (zeros past S); 256 threads
-    static __device__ __forceinline__ void stage64(char* img, const bf16* src, long row_stride, int r0, int S, int tid) {
-        // every load of the block is issued before the first LDS store (a load -> wait -> store loop pays the memory
-        // latency once per chunk); rows past S read row S - 1 and are zeroed by a select, so no load sits behind a branch
-        constexpr int IT = 64 * NCH / 256;
-        static_assert(IT >= 1 && 64 * NCH % 256 == 0, "a block is a whole number of chunks per thread");
-        bf16x8 v[IT];
-#pragma unroll
-        for (int t = 0; t < IT; ++t) {
-            const int i = tid + 256 * t, row = i / NCH, ch = i % NCH;
-            const int rr = r0 + row < S ? r0 + row : S - 1;
-            v[t] = *reinterpret_cast<const bf16x8*>(src + (long)rr * row_stride + ch * 8);
-        }
-#pragma unroll
-        for (int t = 0; t < IT; ++t) {
-            const int i = tid + 256 * t, row = i / NCH, ch = i % NCH;
-            if (r0 + row >= S) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[t][k] = (bf16)0.f;
-            }
-            *reinterpret_cast<bf16x8*>(img + swz(row, ch)) = v[t];
-        }
-    }
-    // a wave's own 32 rows as MFMA fragments straight from global memory (lane = row, 8 elements per step and half)
-    static __device__ __forceinline__ void own_rows(bf16x8* f, const bf16* src, long row_stride, int row, int S, int half) {
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) f[s][k] = (bf16)0.f;
-            if (row < S) f[s] = *reinterpret_cast<const bf16x8*>(src + (long)row * row_stride + s * 16 + half * 8);
-        }
-    }
-};
 
 template <int HDT>
 __global__ __launch_bounds__(256) void k_attn_fwd_kb(const bf16* __restrict__ qkv, bf16* __restrict__ out,

@@ -1,0 +1,52 @@
+// Host side of attention_ext.hip: operands, launch plans and launchers (the binding checks shapes and allocates).
+#pragma once
+#include <hip/hip_runtime_api.h>
+
+#include "fastdiv.h"
+
+namespace pdt {
+
+constexpr int kExtMaxEntries = 4096;  // entries of a relative-position table a head keeps in LDS, five times in the backward
+
+// rows of a [B, rows, heads, hd] tensor: element strides, and the division of a row by the heads that share a key head
+struct ExtView {
+    long bs, rs;
+    FastDiv g;
+};
+struct ExtArgs {
+    const __bf16 *q, *k, *v;
+    ExtView qv, kv, o, dqv, dkv;  // k and v share strides; `o` holds for out, out_lo and dout
+    const int* lens;              // [B] valid keys, or null
+    const float* tab;             // [H][Rp] bias per code difference, times sqrt(hd), or null
+    const int *q_codes4, *k_codes4;
+    int R, Rp;
+    int self;                     // rows past lens[b] are dead too
+    int B, Hkv, G, Sq, Sk, M, Mp; // M = Sq * G rows per key head, Mp = M rounded up to 64
+    long stat_n;                  // B * Hkv * Mp: the statistics are [2][stat_n], m and log2 l
+    float c, scale;               // log2(e) / sqrt(hd), 1 / sqrt(hd)
+};
+struct ExtPlan {
+    bool few;  // one tile of rows per key head: the waves split the keys
+    int tiles, splits;
+};
+struct ExtBwd {
+    const void *out, *out_lo, *dout;
+    const float* stat;
+    float* dsum;
+    void *dq, *dk, *dv;
+    float *part_q, *part_k, *part_v, *slab;
+    ExtPlan q, kv;
+};
+
+ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool bias);
+ExtPlan ext_plan_bwd(long BH, int own, int other);  // workgroups own tiles of `own`, `other` streams
+void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, void* out_lo, float* stat, float* part, float* part_ml,
+                    hipStream_t s);
+void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s);
+void launch_bias_tables(const float* table, const int* bucket_of, const int* q_codes, const int* k_codes, float* tab, int* q4,
+                        int* k4, int R, int Rp, int NB, int H, int S, int Sp, float inv_scale, hipStream_t s);
+int bias_grad_chunks(int rows);
+void launch_bias_grad(const float* slab, float* mid, const int* bucket_of, float* dtable, int R, int Rp, int NB, int H, int B,
+                      int per_head, int chunks, hipStream_t s);
+
+}  // namespace pdt

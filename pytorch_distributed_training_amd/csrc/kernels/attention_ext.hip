@@ -1,0 +1,1018 @@
+// Attention of queries over keys that are laid out apart from them (forward + backward) on the gfx950 matrix cores:
+// any two lengths, query heads that share a key head, valid key counts per sequence, and an additive bias that is learned
+// per bucket of relative positions.  One family serves self attention with such a bias (packed projection, strided views)
+// and cross attention to an encoder's states.
+//
+//   row r of a key head = (query position q = r / G, head g = r % G of its G query heads), M = Sq * G rows
+//   S[r, j]  = c (q_r . k_j) + bias(q, j) log2(e),  c = log2(e) / sqrt(hd)      (scores in base 2)
+//   P        = 2^(S - m) / l,  O = P V,  m = max_j S,  l = sum_j 2^(S - m)        j < len[b]; a row without keys is zero
+//   dS       = P (dO V^T - D),  D = sum_j P_rj (dO V^T)_rj = dO_r . O_r
+//   dQ       = dS K / sqrt(hd),  dK = dS^T Q / sqrt(hd),  dV = P^T dO  (the sum over r runs over the G heads too)
+//
+// The bias of (q, j) is tab[clamp(q_code[q] - k_code[j], 0, R-1)], a table of R floats per head in LDS: a position is one
+// integer, so neither an [S, S] index nor an [H, S, S] bias is ever read.
+//
+//  * Scores are produced TRANSPOSED in the passes that own rows (lane = row, registers = keys) and straight in the pass that
+//    owns keys (lane = key, registers = rows); the second product is transposed as well (V^T P^T, K^T dS^T, ...), so that
+//    running maximum, sums, rescaling and the stores (four neighbouring channels a lane) are all per lane.
+//  * The statistics that the backward gets are m (in units of q . k) and log2 l apart.  Where a bias of -1e9 holds for a whole
+//    row, their sum would not leave a bit of l, and 2^(c s - sum), a difference of two numbers rounded at 1e9, is anything.
+//    The backward's scores start at bias - m, so that no large number is left to round.
+//  * The axis that streams comes by LDS-DMA in blocks of 64 rows, two buffers, one barrier a block; rows past the valid
+//    length are sent out of range and arrive as zeros, so whatever they hold (NaN, infinities) is never multiplied.
+//  * Few rows: the streamed axis is cut into `splits`, each with its own workgroup and an fp32 partial that a small kernel
+//    joins in a fixed order.
+//  * No atomics in memory: the bias gradient is added up in a histogram per WAVE in LDS (program order), the waves and the
+//    workgroups are summed in a fixed order.
+#include <cmath>
+
+#include "attn_tile.h"
+#include "attention_ext.h"
+
+namespace pdt {
+namespace {
+
+constexpr float kInf = __builtin_inff();
+constexpr float kBiasFloor = 1e30f;  // finite biases are clamped here: times sqrt(hd) they stay finite (-inf stays -inf: never attended)
+
+// one 4-byte-aligned 16-B piece per lane into LDS (lane-linear), descriptor from wave-uniform words
+__device__ __forceinline__ i32x4 uniform_rsrc(const void* base, uint32_t bytes) {
+    i32x4 r = make_rsrc_words(base, bytes);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) r[k] = __builtin_amdgcn_readfirstlane(r[k]);
+    return r;
+}
+// every outstanding DMA and LDS access of this wave is done, and every wave is here; no memory access moves across
+__device__ __forceinline__ void dma_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+__device__ __forceinline__ int xcd_order(int id, int n) {
+    // workgroup id runs on XCD id % 8: neighbours in the result (which read the same keys) get the same XCD and its L2
+    const int q = n >> 3, r = n & 7, x = id & 7;
+    return x * q + (x < r ? x : r) + (id >> 3);
+}
+
+// rows [r0, r0 + 64) of a matrix -> LDS image; rows >= valid arrive as zeros.  `off(row)` = element offset of row r0 + row
+template <int HD, int NW, typename F>
+__device__ __forceinline__ void dma_block(uint32_t img, const bf16* base, uint32_t bytes, int valid, int wave, int lane, F off) {
+    using G = AttnGeo<HD>;
+    constexpr int RPP = 1024 / G::ROWBYTES, NP = 64 / RPP;
+    const i32x4 rsrc = uniform_rsrc(base, bytes);
+#pragma unroll
+    for (int i = 0; i < (NP + NW - 1) / NW; ++i) {
+        const int p = wave + i * NW;
+        if (NP % NW == 0 || p < NP) {
+            const int row = p * RPP + lane / G::NCH;
+            const int x = ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) & (G::NCH - 1);
+            const uint32_t o = row < valid ? (uint32_t)off(row) * 2u + (uint32_t)(((lane % G::NCH) ^ x) << 4) : kOOB;
+            lds_dma16(rsrc, o, (uint32_t)__builtin_amdgcn_readfirstlane((int)(img + (uint32_t)p * 1024u)));
+        }
+    }
+}
+// 64 consecutive 4-byte values -> LDS (the image takes 1 KiB: lanes 16.. write zeros)
+__device__ __forceinline__ void dma_words(uint32_t img, const void* base, int lane) {
+    lds_dma16(uniform_rsrc(base, 256u), lane < 16 ? (uint32_t)lane * 16u : kOOB, (uint32_t)__builtin_amdgcn_readfirstlane((int)img));
+}
+
+__device__ __forceinline__ int bias_at(int qc4, int kc4, int top4) {
+    const int d = qc4 - kc4;
+    return d < 0 ? 0 : d > top4 ? top4 : d;
+}
+
+__device__ __forceinline__ long row_offset(const ExtView& v, int r, int hkv, int G, int HD) {
+    const int q = (int)fdiv((uint32_t)r, v.g);
+    return (long)q * v.rs + (long)(hkv * G + (r - q * G)) * HD;
+}
+
+// what a workgroup works on
+struct Job {
+    int b, hkv, bh, tile, split, len, rows;  // len: valid keys; rows: live rows (self attention: those before len)
+};
+__device__ __forceinline__ Job job_of(const ExtArgs& a, int tiles, int splits) {
+    Job j;
+    int l = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    j.split = l % splits;
+    l /= splits;
+    j.tile = l % tiles;
+    j.bh = l / tiles;
+    j.b = j.bh / a.Hkv;
+    j.hkv = j.bh - j.b * a.Hkv;
+    int len = a.Sk;
+    if (a.lens) {
+        len = a.lens[j.b];
+        len = len < 0 ? 0 : len > a.Sk ? a.Sk : len;
+    }
+    j.len = __builtin_amdgcn_readfirstlane(len);
+    j.rows = a.self && j.len < a.M ? j.len : a.M;
+    return j;
+}
+
+// the row's statistics; where nothing was attended to, log2 l = +inf makes every P of the backward zero.  Where l was summed
+// from 2^(c s + base) with base = -c m rounded, `rounding` = c m + base goes into log2 l
+__device__ __forceinline__ void put_stat(const ExtArgs& a, float* stat, long at, bool some, float m, float l, float rounding) {
+    stat[at] = some ? m : 0.f;
+    stat[a.stat_n + at] = some ? __builtin_amdgcn_logf(l) - rounding : kInf;
+}
+
+template <int HD>
+__device__ __forceinline__ void own_frags(bf16x8* f, const bf16* p, bool live, int half) {
+    using G = AttnGeo<HD>;
+#pragma unroll
+    for (int s = 0; s < G::STEPS; ++s) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[s][k] = (bf16)0.f;
+        if (live) f[s] = *reinterpret_cast<const bf16x8*>(p + s * 16 + half * 8);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------- forward
+// One sweep with a running maximum.  4 waves own 32 rows each; keys in blocks of 64.
+// HL: P and O as two bf16 each (value and remainder), so that the backward's D = dO . O, and with it the fp32 gradient of
+// the bias table, does not carry the rounding of P and O to 8 bits of mantissa.
+template <int HD, bool BIAS, bool HL>
+__global__ __launch_bounds__(256) void k_ext_fwd(ExtArgs a, bf16* __restrict__ out, bf16* __restrict__ out_lo,
+                                                 float* __restrict__ stat, float* __restrict__ part, float* __restrict__ part_ml,
+                                                 int tiles, int splits) {
+    using G = AttnGeo<HD>;
+    constexpr int IMG = 64 * G::ROWBYTES;
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][K image, V image], [2][codes 1 KiB], table
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Job j = job_of(a, tiles, splits);
+    const uint32_t lds0 = lds_address(smem);
+    char* codes = smem + 4 * IMG;
+    const float* tab = reinterpret_cast<const float*>(smem + 4 * IMG + 2048);
+    const int r = j.tile * 128 + wave * 32 + l31;
+    const bool live = r < j.rows;
+    const long orow = r < a.M ? (long)j.b * a.o.bs + row_offset(a.o, r, j.hkv, a.G, HD) : 0;
+
+    const int nb = (j.len + 63) >> 6, per = (nb + splits - 1) / splits;
+    const int kb0 = j.split * per, kb1 = kb0 + per < nb ? kb0 + per : nb;
+    const bool any = j.tile * 128 < j.rows && kb0 < kb1;  // (uniform over the workgroup)
+
+    f32x16 o[G::DT];
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+    float m = -kInf, l = 0.f, base = 0.f;
+
+    if (any) {
+        const bf16* kbase = a.k + (long)j.b * a.kv.bs + (long)j.hkv * HD;
+        const bf16* vbase = a.v + (long)j.b * a.kv.bs + (long)j.hkv * HD;
+        const int krs = (int)a.kv.rs;
+        auto issue = [&](int kb, int buf) {
+            const int valid = j.len - kb * 64 < 64 ? j.len - kb * 64 : 64;
+            const uint32_t bytes = (uint32_t)(valid - 1) * (uint32_t)krs * 2u + G::ROWBYTES;
+            const long at = (long)kb * 64 * krs;
+            auto off = [&](int row) { return row * krs; };
+            dma_block<HD, 4>(lds0 + buf * 2 * IMG, kbase + at, bytes, valid, wave, lane, off);
+            dma_block<HD, 4>(lds0 + buf * 2 * IMG + IMG, vbase + at, bytes, valid, wave, lane, off);
+            if (BIAS && wave == 0) dma_words(lds0 + 4 * IMG + buf * 1024, a.k_codes4 + kb * 64, lane);
+        };
+        issue(kb0, 0);
+        if (BIAS) {  // the head's bias table
+            const i32x4 rsrc = uniform_rsrc(a.tab + (long)j.hkv * a.Rp, (uint32_t)a.Rp * 4u);
+            for (int p = wave; p * 256 < a.Rp; p += 4)
+                lds_dma16(rsrc, (uint32_t)(p * 1024 + lane * 16), (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + 4 * IMG + 2048 + p * 1024)));
+        }
+        bf16x8 bq[G::STEPS];
+        own_frags<HD>(bq, a.q + (long)j.b * a.qv.bs + row_offset(a.qv, live ? r : 0, j.hkv, a.G, HD), live, half);
+        const int qc = BIAS && live ? a.q_codes4[r] : 0, top4 = (a.R - 1) * 4;
+
+        for (int kb = kb0; kb < kb1; ++kb) {
+            const int buf = (kb - kb0) & 1;
+            dma_barrier();
+            if (kb + 1 < kb1) issue(kb + 1, buf ^ 1);
+            const char* Ks = smem + buf * 2 * IMG;
+            const char* Vs = Ks + IMG;
+            f32x16 st[2];
+            float mb = m;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                if (BIAS) {
+#pragma unroll
+                    for (int jj = 0; jj < 4; ++jj) {
+                        const i32x4 kc = *reinterpret_cast<const i32x4*>(codes + buf * 1024 + (kt * 32 + 8 * jj + 4 * half) * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            st[kt][4 * jj + e] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(tab) + bias_at(qc, kc[e], top4));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
+                }
+#pragma unroll
+                for (int s = 0; s < G::STEPS; ++s)
+                    st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::rows(Ks, kt * 32 + l31, s, half), bq[s], st[kt], 0, 0, 0);
+                if ((kb + 1) * 64 > j.len) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (kb * 64 + kt * 32 + acc_row(i, half) >= j.len) st[kt][i] = -kInf;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mb = fmaxf(mb, st[kt][i]);
+            }
+            mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
+            // (with a bias, s - m is taken before the product: a mask of -1e9 over a whole row leaves P in [0, 1]; without one
+            // scores are small enough for one multiply-add.  Every key so far forbidden: m counts as 0, all P are 0)
+            const float top = mb == -kInf ? 0.f : mb;
+            base = BIAS ? -top : -top * a.c;
+            if (__any(mb > m)) {
+                const float alpha = __builtin_amdgcn_exp2f(BIAS ? (m + base) * a.c : fmaf(m, a.c, base));
+                l *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+                m = mb;
+            }
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                float part_l = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    st[kt][i] = __builtin_amdgcn_exp2f(BIAS ? (st[kt][i] + base) * a.c : fmaf(st[kt][i], a.c, base));
+                    part_l += st[kt][i];
+                }
+                l += part_l;
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk) {
+                    const bf16x8 p = acc_to_a(st[kt], blk);
+                    bf16x8 plo;
+                    if (HL) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) plo[i] = (bf16)(st[kt][8 * blk + i] - (float)p[i]);
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < G::DT; ++dt) {
+                        const bf16x8 vt = G::cols(Vs, kt * 32 + blk * 16, dt * 32, lane);
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, p, o[dt], 0, 0, 0);
+                        if (HL) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, plo, o[dt], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (splits > 1) {
+        if (r < a.M) {
+            const long at = ((long)j.bh * splits + j.split) * a.M + r;
+#pragma unroll
+            for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    f32x4 t;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) t[e] = o[dt][4 * jj + e];
+                    *reinterpret_cast<f32x4*>(part + at * HD + dt * 32 + 8 * jj + 4 * half) = t;
+                }
+            if (half == 0) {
+                part_ml[2 * at] = m;
+                part_ml[2 * at + 1] = l;
+            }
+        }
+        return;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    if (stat && half == 0 && r < a.Mp) put_stat(a, stat, (long)j.bh * a.Mp + r, live && (l > 0.f || l != l), m, l, BIAS ? 0.f : fmaf(m, a.c, base));
+    if (r < a.M) {
+#pragma unroll
+        for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+                bf16x4 t, tl;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float v = live ? o[dt][4 * jj + e] * inv : 0.f;
+                    t[e] = (bf16)v;
+                    tl[e] = (bf16)(v - (float)t[e]);
+                }
+                *reinterpret_cast<bf16x4*>(out + orow + dt * 32 + 8 * jj + 4 * half) = t;
+                if (HL) *reinterpret_cast<bf16x4*>(out_lo + orow + dt * 32 + 8 * jj + 4 * half) = tl;
+            }
+    }
+}
+
+// Few rows (at most one tile of 32 for a key head: single tokens).  The four waves of a workgroup share the rows and take
+// every fourth tile of 32 keys each, through an LDS ring of their own (no barrier until the join): the kernel is a stream over
+// K and V, 16 to 64 KiB of it in flight per workgroup.
+template <int HD>
+__global__ __launch_bounds__(256) void k_ext_fwd_few(ExtArgs a, bf16* __restrict__ out, float* __restrict__ stat,
+                                                     float* __restrict__ part, float* __restrict__ part_ml, int splits) {
+    using G = AttnGeo<HD>;
+    constexpr int TIMG = 32 * G::ROWBYTES, STAGE = 2 * TIMG, RPP = 1024 / G::ROWBYTES, NP = 32 / RPP;
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // [4 waves][2 stages][K tile, V tile], then [4][32][2] floats
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Job j = job_of(a, 1, splits);
+    char* ring = smem + wave * 2 * STAGE;
+    const uint32_t ring_lds = lds_address(ring);
+    const bool live = l31 < a.M;
+    const int nt = (j.len + 31) >> 5, per = (nt + splits - 1) / splits;
+    const int t0 = j.split * per, t1 = t0 + per < nt ? t0 + per : nt;
+    const bf16* kbase = a.k + (long)j.b * a.kv.bs + (long)j.hkv * HD;
+    const bf16* vbase = a.v + (long)j.b * a.kv.bs + (long)j.hkv * HD;
+    const int krs = (int)a.kv.rs;
+
+    bf16x8 bq[G::STEPS];
+    own_frags<HD>(bq, a.q + (long)j.b * a.qv.bs + row_offset(a.qv, live ? l31 : 0, j.hkv, a.G, HD), live, half);
+#pragma unroll
+    for (int s = 0; s < G::STEPS; ++s) asm volatile("" : "+v"(bq[s])::"memory");  // the rows are here: only DMA is counted below
+
+    auto issue = [&](int t, int buf) {
+        const int valid = j.len - t * 32 < 32 ? j.len - t * 32 : 32;
+        const uint32_t bytes = (uint32_t)(valid - 1) * (uint32_t)krs * 2u + G::ROWBYTES;
+        const long at = (long)t * 32 * krs;
+        const i32x4 rk = uniform_rsrc(kbase + at, bytes), rv = uniform_rsrc(vbase + at, bytes);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const int row = p * RPP + lane / G::NCH;
+            const int x = ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) & (G::NCH - 1);
+            const uint32_t o = row < valid ? (uint32_t)(row * krs) * 2u + (uint32_t)(((lane % G::NCH) ^ x) << 4) : kOOB;
+            lds_dma16(rk, o, (uint32_t)__builtin_amdgcn_readfirstlane((int)(ring_lds + buf * STAGE + p * 1024)));
+            lds_dma16(rv, o, (uint32_t)__builtin_amdgcn_readfirstlane((int)(ring_lds + buf * STAGE + TIMG + p * 1024)));
+        }
+    };
+    f32x16 o[G::DT];
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+    float m = -kInf, l = 0.f;
+    int buf = 0;
+    if (t0 + wave < t1) issue(t0 + wave, 0);
+    for (int t = t0 + wave; t < t1; t += 4, buf ^= 1) {
+        // the reads of the other stage (last tile) are done before it is written again
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (t + 4 < t1) {
+            issue(t + 4, buf ^ 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NP) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const char* Ks = ring + buf * STAGE;
+        const char* Vs = Ks + TIMG;
+        f32x16 st;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < G::STEPS; ++s)
+            st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::rows(Ks, l31, s, half), bq[s], st, 0, 0, 0);
+        if ((t + 1) * 32 > j.len) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (t * 32 + acc_row(i, half) >= j.len) st[i] = -kInf;
+        }
+        float mb = m;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mb = fmaxf(mb, st[i]);
+        mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
+        const float base = -mb * a.c;
+        if (__any(mb > m)) {
+            const float alpha = __builtin_amdgcn_exp2f(fmaf(m, a.c, base));
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+            m = mb;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            st[i] = __builtin_amdgcn_exp2f(fmaf(st[i], a.c, base));
+            l += st[i];
+        }
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+            const bf16x8 p = acc_to_a(st, blk);
+#pragma unroll
+            for (int dt = 0; dt < G::DT; ++dt)
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Vs, blk * 16, dt * 32, lane), p, o[dt], 0, 0, 0);
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    // the waves' (m, l, O) through LDS, over their rings
+    float* ml = reinterpret_cast<float*>(smem + 8 * STAGE);
+    if (half == 0) {
+        ml[(wave * 32 + l31) * 2] = m;
+        ml[(wave * 32 + l31) * 2 + 1] = l;
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    float* acc = reinterpret_cast<float*>(ring);  // [32 rows][HD]: a wave's two stages are at least that large
+    static_assert(2 * STAGE >= 32 * HD * 4, "the join uses the ring");
+    if (live) {
+#pragma unroll
+        for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+                f32x4 t;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[e] = o[dt][4 * jj + e];
+                *reinterpret_cast<f32x4*>(acc + l31 * HD + dt * 32 + 8 * jj + 4 * half) = t;
+            }
+    }
+    __syncthreads();
+    for (int i = tid; i < a.M * (HD / 4); i += 256) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+        float mx = -kInf, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[(w * 32 + r) * 2]);
+        f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float mw = ml[(w * 32 + r) * 2], f = mw == -kInf ? 0.f : __builtin_amdgcn_exp2f((mw - mx) * a.c);
+            sum += ml[(w * 32 + r) * 2 + 1] * f;
+            const f32x4 u = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem + w * 2 * STAGE) + r * HD + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] += u[e] * f;
+        }
+        if (splits > 1) {
+            const long at = ((long)j.bh * splits + j.split) * a.M + r;
+            *reinterpret_cast<f32x4*>(part + at * HD + d) = t;
+            if (d == 0) {
+                part_ml[2 * at] = mx;
+                part_ml[2 * at + 1] = sum;
+            }
+        } else {
+            const float inv = j.len > 0 ? 1.f / sum : 0.f;
+            bf16x4 w4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w4[e] = (bf16)(t[e] * inv);
+            *reinterpret_cast<bf16x4*>(out + (long)j.b * a.o.bs + row_offset(a.o, r, j.hkv, a.G, HD) + d) = w4;
+            if (stat && d == 0) put_stat(a, stat, (long)j.bh * a.Mp + r, j.len > 0, mx, sum, 0.f);
+        }
+    }
+    if (stat && splits == 1)
+        for (int r = a.M + tid; r < a.Mp; r += 256) put_stat(a, stat, (long)j.bh * a.Mp + r, false, 0.f, 0.f, 0.f);
+}
+
+// (m, l, O) of the splits -> out (and stat); one thread per row and 4 channels, splits in order
+template <int HD>
+__global__ __launch_bounds__(256) void k_ext_join(ExtArgs a, const float* __restrict__ part, const float* __restrict__ part_ml,
+                                                  bf16* __restrict__ out, bf16* __restrict__ out_lo, float* __restrict__ stat,
+                                                  long total, int splits) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int d = (int)(i % (HD / 4)) * 4;
+    const long row = i / (HD / 4);
+    const int bh = (int)(row / a.Mp), r = (int)(row - (long)bh * a.Mp);
+    if (r >= a.M) {  // padding rows of the statistics
+        if (stat && d == 0) put_stat(a, stat, row, false, 0.f, 0.f, 0.f);
+        return;
+    }
+    const int b = bh / a.Hkv, hkv = bh - b * a.Hkv;
+    float mx = -kInf, sum = 0.f;
+    const long at0 = (long)bh * splits * a.M + r;
+    for (int s = 0; s < splits; ++s) mx = fmaxf(mx, part_ml[2 * (at0 + (long)s * a.M)]);
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+        const long at = at0 + (long)s * a.M;
+        const float ms = part_ml[2 * at], f = ms == -kInf ? 0.f : __builtin_amdgcn_exp2f((ms - mx) * a.c);
+        sum += part_ml[2 * at + 1] * f;
+        const f32x4 u = *reinterpret_cast<const f32x4*>(part + at * HD + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] += u[e] * f;
+    }
+    int rows = a.M;
+    if (a.self && a.lens) {
+        const int len = a.lens[b] < 0 ? 0 : a.lens[b];
+        rows = len < rows ? len : rows;
+    }
+    const bool some = (sum > 0.f || sum != sum) && r < rows;
+    const float inv = some ? 1.f / sum : 0.f;
+    const long o = (long)b * a.o.bs + row_offset(a.o, r, hkv, a.G, HD) + d;
+    bf16x4 w4, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float v = some ? t[e] * inv : 0.f;
+        w4[e] = (bf16)v;
+        lo[e] = (bf16)(v - (float)w4[e]);
+    }
+    *reinterpret_cast<bf16x4*>(out + o) = w4;
+    if (out_lo) *reinterpret_cast<bf16x4*>(out_lo + o) = lo;
+    if (stat && d == 0) put_stat(a, stat, row, some, mx, sum, 0.f);
+}
+
+// ------------------------------------------------------------------------------------------------------- backward
+// dst rows <- scale * (sum of the splits' fp32 partials, in order), or, for dead rows, what the partials hold: zeros
+template <int HD>
+__global__ __launch_bounds__(256) void k_ext_sum(const float* __restrict__ part, bf16* __restrict__ dst, ExtView v, int G,
+                                                 int Hkv, int rows, int splits, float scale, long total) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const int d = (int)(i % (HD / 4)) * 4;
+    const long row = i / (HD / 4);
+    const int bh = (int)(row / rows), r = (int)(row - (long)bh * rows);
+    const int b = bh / Hkv, hkv = bh - b * Hkv;
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+        const f32x4 u = *reinterpret_cast<const f32x4*>(part + (((long)bh * splits + s) * rows + r) * HD + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] += u[e];
+    }
+    bf16x4 w4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w4[e] = (bf16)(t[e] * scale);
+    *reinterpret_cast<bf16x4*>(dst + (long)b * v.bs + row_offset(v, r, hkv, G, HD) + d) = w4;
+}
+
+// a lane's accumulator columns: dst[d] for d = dt*32 + 8*jj + 4*half + e
+template <int HD>
+__device__ __forceinline__ void store_acc(const f32x16* t, bf16* dst, float scale, int half) {
+    using G = AttnGeo<HD>;
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+            bf16x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = (bf16)(t[dt][4 * jj + e] * scale);
+            *reinterpret_cast<bf16x4*>(dst + dt * 32 + 8 * jj + 4 * half) = w;
+        }
+}
+template <int HD>
+__device__ __forceinline__ void store_acc32(const f32x16* t, float* dst, int half) {
+    using G = AttnGeo<HD>;
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+            f32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = t[dt][4 * jj + e];
+            *reinterpret_cast<f32x4*>(dst + dt * 32 + 8 * jj + 4 * half) = w;
+        }
+}
+
+// Row owner: dQ, D for the key owner (written by split 0) and the histogram of dS over the table's entries.  A softmax over
+// one key is constant, so with len = 1 dS is zero, and is set so (as a difference of two rounded numbers it would not be).
+template <int HD, bool BIAS>
+__global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ out_lo,
+                                                   const bf16* __restrict__ dout, const float* __restrict__ stat,
+                                                   float* __restrict__ dsum, bf16* __restrict__ dq, float* __restrict__ part,
+                                                   float* __restrict__ slab, int tiles, int splits) {
+    using G = AttnGeo<HD>;
+    constexpr int IMG = 64 * G::ROWBYTES;
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][K, V], [2][codes 1 KiB], table [Rt], histograms [4][Rt]
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Job j = job_of(a, tiles, splits);
+    const uint32_t lds0 = lds_address(smem);
+    char* codes = smem + 4 * IMG;
+    char* tab = smem + 4 * IMG + 2048;
+    const int Rt = (a.Rp + 255) & ~255;
+    char* hist = tab + (long)Rt * 4 * (1 + wave);
+    const int r = j.tile * 128 + wave * 32 + l31;
+    const bool live = r < j.rows;
+    const int nb = (j.len + 63) >> 6, per = (nb + splits - 1) / splits;
+    const int kb0 = j.split * per, kb1 = kb0 + per < nb ? kb0 + per : nb;
+    const bool any = j.tile * 128 < j.rows && kb0 < kb1;
+
+    f32x16 acc[G::DT];
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+    const bf16* kbase = a.k + (long)j.b * a.kv.bs + (long)j.hkv * HD;
+    const bf16* vbase = a.v + (long)j.b * a.kv.bs + (long)j.hkv * HD;
+    const int krs = (int)a.kv.rs;
+    auto issue = [&](int kb, int buf) {
+        const int valid = j.len - kb * 64 < 64 ? j.len - kb * 64 : 64;
+        const uint32_t bytes = (uint32_t)(valid - 1) * (uint32_t)krs * 2u + G::ROWBYTES;
+        const long at = (long)kb * 64 * krs;
+        auto off = [&](int row) { return row * krs; };
+        dma_block<HD, 4>(lds0 + buf * 2 * IMG, kbase + at, bytes, valid, wave, lane, off);
+        dma_block<HD, 4>(lds0 + buf * 2 * IMG + IMG, vbase + at, bytes, valid, wave, lane, off);
+        if (BIAS && wave == 0) dma_words(lds0 + 4 * IMG + buf * 1024, a.k_codes4 + kb * 64, lane);
+    };
+    if (any) issue(kb0, 0);
+    if (BIAS) {
+        if (any) {
+            const i32x4 rsrc = uniform_rsrc(a.tab + (long)j.hkv * a.Rp, (uint32_t)a.Rp * 4u);
+            for (int p = wave; p * 256 < a.Rp; p += 4)
+                lds_dma16(rsrc, (uint32_t)(p * 1024 + lane * 16), (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + 4 * IMG + 2048 + p * 1024)));
+        }
+        for (int i = lane; i < Rt; i += 64) reinterpret_cast<float*>(hist)[i] = 0.f;
+    }
+    // own rows, and D from them
+    bf16x8 qf[G::STEPS], gf[G::STEPS];
+    float d = 0.f;
+    {
+        const long ro = row_offset(a.o, live ? r : 0, j.hkv, a.G, HD) + (long)j.b * a.o.bs;
+        own_frags<HD>(qf, a.q + (long)j.b * a.qv.bs + row_offset(a.qv, live ? r : 0, j.hkv, a.G, HD), live, half);
+        own_frags<HD>(gf, dout + ro, live, half);
+        bf16x8 of[G::STEPS], ol[G::STEPS];
+        own_frags<HD>(of, out + ro, live, half);
+        if (BIAS && out_lo) own_frags<HD>(ol, out_lo + ro, live, half);
+#pragma unroll
+        for (int s = 0; s < G::STEPS; ++s)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                float v = (float)of[s][k];
+                if (BIAS && out_lo) v += (float)ol[s][k];
+                d += v * (float)gf[s][k];
+            }
+        d += __shfl_xor(d, 32, 64);
+    }
+    if (j.split == 0 && half == 0 && r < a.Mp) dsum[(long)j.bh * a.Mp + r] = live ? d : 0.f;
+    const float mq = live ? stat[(long)j.bh * a.Mp + r] : 0.f, lq = live ? stat[a.stat_n + (long)j.bh * a.Mp + r] : kInf;
+    const int qc = BIAS && live ? a.q_codes4[r] : 0, top4 = (a.R - 1) * 4;
+    const float keep = j.len > 1 ? 1.f : 0.f;
+
+    if (any) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+            const int buf = (kb - kb0) & 1;
+            dma_barrier();
+            if (kb + 1 < kb1) issue(kb + 1, buf ^ 1);
+            const char* Ks = smem + buf * 2 * IMG;
+            const char* Vs = Ks + IMG;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                f32x16 sc, dp;
+                int at[16];
+                if (BIAS) {
+#pragma unroll
+                    for (int jj = 0; jj < 4; ++jj) {
+                        const i32x4 kc = *reinterpret_cast<const i32x4*>(codes + buf * 1024 + (kt * 32 + 8 * jj + 4 * half) * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            at[4 * jj + e] = bias_at(qc, kc[e], top4);
+                            sc[4 * jj + e] = *reinterpret_cast<const float*>(tab + at[4 * jj + e]) - mq;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (!BIAS) sc[i] = -mq;
+                    dp[i] = -d;
+                }
+#pragma unroll
+                for (int s = 0; s < G::STEPS; ++s) {
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::rows(Ks, kt * 32 + l31, s, half), qf[s], sc, 0, 0, 0);
+                    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::rows(Vs, kt * 32 + l31, s, half), gf[s], dp, 0, 0, 0);
+                }
+                if ((kb + 1) * 64 > j.len) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (kb * 64 + kt * 32 + acc_row(i, half) >= j.len) sc[i] = -kInf;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, -lq)) * keep;
+                if (BIAS && slab) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        __hip_atomic_fetch_add(reinterpret_cast<float*>(hist + at[i]), dp[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                }
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk) {
+                    const bf16x8 ds = acc_to_a(dp, blk);
+#pragma unroll
+                    for (int dt = 0; dt < G::DT; ++dt)
+                        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Ks, kt * 32 + blk * 16, dt * 32, lane), ds, acc[dt], 0, 0, 0);
+                }
+            }
+        }
+    }
+    if (BIAS && slab) {
+        __syncthreads();
+        float* dst = slab + (((long)j.bh * tiles + j.tile) * splits + j.split) * a.Rp;
+        for (int i = tid; i < a.Rp; i += 256) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) s += reinterpret_cast<const float*>(tab)[(long)Rt * (1 + w) + i];
+            dst[i] = s;
+        }
+    }
+    if (r >= a.M) return;
+    if (splits > 1) store_acc32<HD>(acc, part + (((long)j.bh * splits + j.split) * a.M + r) * HD, half);
+    else store_acc<HD>(acc, dq + (long)j.b * a.dqv.bs + row_offset(a.dqv, r, j.hkv, a.G, HD), a.scale, half);
+}
+
+// Key owner: dK and dV of 128 keys a workgroup; the rows of all G heads stream through.
+template <int HD, bool BIAS>
+__global__ __launch_bounds__(256) void k_ext_bwd_kv(ExtArgs a, const bf16* __restrict__ dout, const float* __restrict__ stat,
+                                                    const float* __restrict__ dsum, bf16* __restrict__ dk, bf16* __restrict__ dv,
+                                                    float* __restrict__ part_k, float* __restrict__ part_v, int tiles, int splits) {
+    using G = AttnGeo<HD>;
+    constexpr int IMG = 64 * G::ROWBYTES;
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][Q, dO], [2][log2 l, D, codes, m: 1 KiB each], table
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Job j = job_of(a, tiles, splits);
+    const uint32_t lds0 = lds_address(smem);
+    char* stat_s = smem + 4 * IMG;
+    char* tab = stat_s + 2 * 4096;
+    const int key = j.tile * 128 + wave * 32 + l31;
+    const bool live = key < j.len;
+    const int nb = (j.rows + 63) >> 6, per = (nb + splits - 1) / splits;
+    const int rb0 = j.split * per, rb1 = rb0 + per < nb ? rb0 + per : nb;
+    const bool any = j.tile * 128 < j.len && rb0 < rb1;
+
+    f32x16 ak[G::DT], av[G::DT];
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            ak[dt][i] = 0.f;
+            av[dt][i] = 0.f;
+        }
+    if (any) {
+        const bf16* qb = a.q + (long)j.b * a.qv.bs + (long)j.hkv * a.G * HD;
+        const bf16* gb = dout + (long)j.b * a.o.bs + (long)j.hkv * a.G * HD;
+        const int qrs = (int)a.qv.rs, grs = (int)a.o.rs;
+        const float* mrow = stat + (long)j.bh * a.Mp;
+        const float* lrow = mrow + a.stat_n;
+        const float* drow = dsum + (long)j.bh * a.Mp;
+        auto issue = [&](int rb, int buf) {
+            const int valid = j.rows - rb * 64 < 64 ? j.rows - rb * 64 : 64;
+            const int q0 = (int)fdiv((uint32_t)(rb * 64), a.qv.g), last = (int)fdiv((uint32_t)(rb * 64 + valid - 1), a.qv.g);
+            const uint32_t span = (uint32_t)(last - q0), width = (uint32_t)(a.G * HD * 2);
+            auto qoff = [&](int row) {
+                const int q = (int)fdiv((uint32_t)(rb * 64 + row), a.qv.g);
+                return (q - q0) * qrs + (rb * 64 + row - q * a.G) * HD;
+            };
+            auto goff = [&](int row) {
+                const int q = (int)fdiv((uint32_t)(rb * 64 + row), a.qv.g);
+                return (q - q0) * grs + (rb * 64 + row - q * a.G) * HD;
+            };
+            dma_block<HD, 4>(lds0 + buf * 2 * IMG, qb + (long)q0 * qrs, span * (uint32_t)qrs * 2u + width, valid, wave, lane, qoff);
+            dma_block<HD, 4>(lds0 + buf * 2 * IMG + IMG, gb + (long)q0 * grs, span * (uint32_t)grs * 2u + width, valid, wave, lane, goff);
+            const uint32_t st = lds0 + 4 * IMG + buf * 4096;
+            if (wave == 0) dma_words(st, lrow + rb * 64, lane);
+            if (wave == 1) dma_words(st + 1024, drow + rb * 64, lane);
+            if (BIAS && wave == 2) dma_words(st + 2048, a.q_codes4 + rb * 64, lane);
+            if (wave == 3) dma_words(st + 3072, mrow + rb * 64, lane);
+        };
+        issue(rb0, 0);
+        if (BIAS) {
+            const i32x4 rsrc = uniform_rsrc(a.tab + (long)j.hkv * a.Rp, (uint32_t)a.Rp * 4u);
+            for (int p = wave; p * 256 < a.Rp; p += 4)
+                lds_dma16(rsrc, (uint32_t)(p * 1024 + lane * 16), (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + 4 * IMG + 8192 + p * 1024)));
+        }
+        bf16x8 kf[G::STEPS], vf[G::STEPS];
+        const long ko = (long)j.b * a.kv.bs + (long)(live ? key : 0) * a.kv.rs + (long)j.hkv * HD;
+        own_frags<HD>(kf, a.k + ko, live, half);
+        own_frags<HD>(vf, a.v + ko, live, half);
+        const int kc = BIAS && live ? a.k_codes4[key] : 0, top4 = (a.R - 1) * 4;
+        const float keep = j.len > 1 ? 1.f : 0.f;
+
+        for (int rb = rb0; rb < rb1; ++rb) {
+            const int buf = (rb - rb0) & 1;
+            dma_barrier();
+            if (rb + 1 < rb1) issue(rb + 1, buf ^ 1);
+            const char* Qs = smem + buf * 2 * IMG;
+            const char* Gs = Qs + IMG;
+            const char* st = stat_s + buf * 4096;
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) {
+                f32x16 sc, dp;
+                f32x4 lr[4];
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj) {
+                    const int w = (rt * 32 + 8 * jj + 4 * half) * 4;
+                    lr[jj] = *reinterpret_cast<const f32x4*>(st + w);
+                    const f32x4 dr = *reinterpret_cast<const f32x4*>(st + 1024 + w), mr = *reinterpret_cast<const f32x4*>(st + 3072 + w);
+                    i32x4 qc = {0, 0, 0, 0};
+                    if (BIAS) qc = *reinterpret_cast<const i32x4*>(st + 2048 + w);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        sc[4 * jj + e] = BIAS ? *reinterpret_cast<const float*>(tab + bias_at(qc[e], kc, top4)) - mr[e] : -mr[e];
+                        dp[4 * jj + e] = -dr[e];
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < G::STEPS; ++s) {
+                    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::rows(Qs, rt * 32 + l31, s, half), kf[s], sc, 0, 0, 0);
+                    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::rows(Gs, rt * 32 + l31, s, half), vf[s], dp, 0, 0, 0);
+                }
+                // (no mask: a dead key is a lane of its own whose results are not stored; rows past the end have log2 l = +inf)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, -lr[i >> 2][i & 3]));
+                    sc[i] = p;
+                    dp[i] *= p * keep;
+                }
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk) {
+                    const bf16x8 p = acc_to_a(sc, blk), ds = acc_to_a(dp, blk);
+#pragma unroll
+                    for (int dt = 0; dt < G::DT; ++dt) {
+                        av[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Gs, rt * 32 + blk * 16, dt * 32, lane), p, av[dt], 0, 0, 0);
+                        ak[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Qs, rt * 32 + blk * 16, dt * 32, lane), ds, ak[dt], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    if (key >= a.Sk) return;
+    if (!live) {
+#pragma unroll
+        for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                ak[dt][i] = 0.f;
+                av[dt][i] = 0.f;
+            }
+    }
+    if (splits > 1) {
+        const long at = (((long)j.bh * splits + j.split) * a.Sk + key) * HD;
+        store_acc32<HD>(ak, part_k + at, half);
+        store_acc32<HD>(av, part_v + at, half);
+    } else {
+        const long at = (long)j.b * a.dkv.bs + (long)key * a.dkv.rs + (long)j.hkv * HD;
+        store_acc<HD>(ak, dk + at, a.scale, half);
+        store_acc<HD>(av, dv + at, 1.f, half);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------- bias tables
+// tab[h][r] = table[bucket_of[r]][h] * sqrt(hd) (the scores are scaled after the bias is added), zero where the entry names no
+// bucket; byte offsets of the position codes, padded with zeros to a multiple of 64
+__global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ table, const int* __restrict__ bucket_of,
+                                                     const int* __restrict__ q_codes, const int* __restrict__ k_codes,
+                                                     float* __restrict__ tab, int* __restrict__ q4, int* __restrict__ k4, int R,
+                                                     int Rp, int NB, int H, int S, int Sp, float inv_scale, long total) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    if (i < (long)H * Rp) {
+        const int h = (int)(i / Rp), r = (int)(i % Rp);
+        const int n = r < R ? bucket_of[r] : -1;
+        float v = n >= 0 && n < NB ? table[(long)n * H + h] : 0.f;
+        if (v < -kBiasFloor && v > -kInf) v = -kBiasFloor;
+        if (v > kBiasFloor && v < kInf) v = kBiasFloor;
+        tab[i] = v * inv_scale;
+        return;
+    }
+    const long w = i - (long)H * Rp;
+    const int at = (int)(w % Sp);
+    const int* src = w < Sp ? q_codes : k_codes;
+    int c = at < S ? src[at] : 0;
+    c = c < -(1 << 28) ? -(1 << 28) : c > (1 << 28) - 1 ? (1 << 28) - 1 : c;  // differences of the byte offsets fit 32 bits
+    (w < Sp ? q4 : k4)[at] = c * 4;
+}
+
+// mid[chunk][h][r] = sum of the slab rows of head h in this chunk, in order
+__global__ __launch_bounds__(256) void k_bias_slab(const float* __restrict__ slab, float* __restrict__ mid, int Rp, int H, int B,
+                                                   int per_head /* tiles * splits */, int chunks) {
+    const int r = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, ch = blockIdx.z;
+    if (r >= Rp) return;
+    const int rows = B * per_head, per = (rows + chunks - 1) / chunks;
+    const int i0 = ch * per, i1 = i0 + per < rows ? i0 + per : rows;
+    float s = 0.f;
+    for (int i = i0; i < i1; ++i) {
+        const int b = i / per_head, t = i - b * per_head;
+        s += slab[((long)(b * H + h) * per_head + t) * Rp + r];
+    }
+    mid[((long)ch * H + h) * Rp + r] = s;
+}
+
+// dtable[n][h] = sum over the entries r of bucket n: the head's entries and their buckets in LDS, one thread per bucket
+__global__ __launch_bounds__(256) void k_bias_buckets(const float* __restrict__ mid, const int* __restrict__ bucket_of,
+                                                      float* __restrict__ dtable, int R, int Rp, int NB, int H, int chunks) {
+    __shared__ __attribute__((aligned(16))) float sums[kExtMaxEntries];
+    __shared__ __attribute__((aligned(16))) int of[kExtMaxEntries];
+    const int h = blockIdx.y;
+    for (int r = threadIdx.x; r < Rp; r += 256) {
+        float s = 0.f;
+        for (int c = 0; c < chunks; ++c) s += mid[((long)c * H + h) * Rp + r];
+        sums[r] = s;
+        of[r] = r < R ? bucket_of[r] : -1;
+    }
+    __syncthreads();
+    const int n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= NB) return;
+    float s = 0.f;
+    for (int r = 0; r < Rp; r += 4) {
+        const i32x4 o = *reinterpret_cast<const i32x4*>(of + r);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(sums + r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (o[e] == n) s += v[e];
+    }
+    dtable[(long)n * H + h] = s;
+}
+
+template <typename K>
+void allow_lds(K kern, size_t bytes) {
+    if (bytes > 65536)
+        PDT_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+size_t table_bytes(const ExtArgs& a) { return a.tab ? (size_t)((a.Rp + 255) & ~255) * 4 : 0; }
+
+template <int HD>
+void fwd(const ExtArgs& a, const ExtPlan& p, void* out, void* out_lo, float* stat, float* part, float* part_ml, hipStream_t s) {
+    const unsigned grid = (unsigned)((long)a.B * a.Hkv * p.tiles * p.splits);
+    if (p.few) {
+        const size_t lds = (size_t)16 * 32 * HD * 2 + 4 * 32 * 2 * sizeof(float);
+        allow_lds(&k_ext_fwd_few<HD>, lds);
+        hipLaunchKernelGGL((k_ext_fwd_few<HD>), dim3(grid), dim3(256), lds, s, a, (bf16*)out, stat, part, part_ml, p.splits);
+    } else {
+        const size_t lds = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + table_bytes(a);
+#define PDT_EXT_FWD(BIAS, HL)                                                                                             \
+    allow_lds(&k_ext_fwd<HD, BIAS, HL>, lds);                                                                             \
+    hipLaunchKernelGGL((k_ext_fwd<HD, BIAS, HL>), dim3(grid), dim3(256), lds, s, a, (bf16*)out, (bf16*)out_lo, stat, part, \
+                       part_ml, p.tiles, p.splits);
+        if (a.tab && out_lo) {
+            PDT_EXT_FWD(true, true)
+        } else if (a.tab) {
+            PDT_EXT_FWD(true, false)
+        } else {
+            PDT_EXT_FWD(false, false)
+        }
+#undef PDT_EXT_FWD
+    }
+    if (p.splits > 1) {
+        const long total = (long)a.B * a.Hkv * a.Mp * (HD / 4);
+        hipLaunchKernelGGL((k_ext_join<HD>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a, (const float*)part,
+                           (const float*)part_ml, (bf16*)out, (bf16*)out_lo, stat, total, p.splits);
+    }
+}
+
+template <int HD>
+void bwd(const ExtArgs& a, const ExtBwd& w, hipStream_t s) {
+    const ExtPlan &pq = w.q, &pk = w.kv;
+    const dim3 gq((unsigned)((long)a.B * a.Hkv * pq.tiles * pq.splits)), gk((unsigned)((long)a.B * a.Hkv * pk.tiles * pk.splits));
+    const size_t lq = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + 5 * table_bytes(a);
+    const size_t lk = (size_t)4 * 64 * HD * 2 + 8192 + table_bytes(a);
+#define PDT_EXT_BWD(BIAS)                                                                                                  \
+    allow_lds(&k_ext_bwd_q<HD, BIAS>, lq);                                                                                 \
+    hipLaunchKernelGGL((k_ext_bwd_q<HD, BIAS>), gq, dim3(256), lq, s, a, (const bf16*)w.out, (const bf16*)w.out_lo,        \
+                       (const bf16*)w.dout, w.stat, w.dsum, (bf16*)w.dq, w.part_q, w.slab, pq.tiles, pq.splits);           \
+    allow_lds(&k_ext_bwd_kv<HD, BIAS>, lk);                                                                                \
+    hipLaunchKernelGGL((k_ext_bwd_kv<HD, BIAS>), gk, dim3(256), lk, s, a, (const bf16*)w.dout, w.stat, (const float*)w.dsum, \
+                       (bf16*)w.dk, (bf16*)w.dv, w.part_k, w.part_v, pk.tiles, pk.splits);
+    if (a.tab) {
+        PDT_EXT_BWD(true)
+    } else {
+        PDT_EXT_BWD(false)
+    }
+#undef PDT_EXT_BWD
+    const long BH = (long)a.B * a.Hkv;
+    if (pq.splits > 1) {
+        const long total = BH * a.M * (HD / 4);
+        hipLaunchKernelGGL((k_ext_sum<HD>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, (const float*)w.part_q,
+                           (bf16*)w.dq, a.dqv, a.G, a.Hkv, a.M, pq.splits, a.scale, total);
+    }
+    if (pk.splits > 1) {
+        const long total = BH * a.Sk * (HD / 4);
+        const dim3 g((unsigned)((total + 255) / 256));
+        hipLaunchKernelGGL((k_ext_sum<HD>), g, dim3(256), 0, s, (const float*)w.part_k, (bf16*)w.dk, a.dkv, 1, a.Hkv, a.Sk,
+                           pk.splits, a.scale, total);
+        hipLaunchKernelGGL((k_ext_sum<HD>), g, dim3(256), 0, s, (const float*)w.part_v, (bf16*)w.dv, a.dkv, 1, a.Hkv, a.Sk,
+                           pk.splits, 1.f, total);
+    }
+}
+
+// parts to cut `blocks` blocks of the streamed axis into, so that `groups` workgroups become about two per CU (512); a part
+// keeps at least `least` blocks
+int splits_for(long groups, long blocks, long least) {
+    if (groups >= 256 || blocks < 2 * least) return 1;
+    long s = (512 + groups - 1) / groups;
+    s = s < blocks / least ? s : blocks / least;
+    return (int)(s < 1 ? 1 : s > 128 ? 128 : s);
+}
+
+}  // namespace
+
+ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool bias) {
+    ExtPlan p;
+    p.few = !bias && M <= 32;
+    p.tiles = p.few ? 1 : (M + 127) / 128;
+    p.splits = p.few ? splits_for(BH, (Sk + 31) / 32, 8) : splits_for(BH * p.tiles, (Sk + 63) / 64, 4);
+    return p;
+}
+ExtPlan ext_plan_bwd(long BH, int own, int other) {
+    ExtPlan p;
+    p.few = false;
+    p.tiles = (own + 127) / 128;
+    p.splits = splits_for(BH * p.tiles, (other + 63) / 64, 4);
+    return p;
+}
+
+void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, void* out_lo, float* stat, float* part, float* part_ml,
+                    hipStream_t s) {
+    if (hd == 32) fwd<32>(a, p, out, out_lo, stat, part, part_ml, s);
+    else if (hd == 64) fwd<64>(a, p, out, out_lo, stat, part, part_ml, s);
+    else fwd<128>(a, p, out, out_lo, stat, part, part_ml, s);
+}
+void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s) {
+    if (hd == 32) bwd<32>(a, w, s);
+    else if (hd == 64) bwd<64>(a, w, s);
+    else bwd<128>(a, w, s);
+}
+void launch_bias_tables(const float* table, const int* bucket_of, const int* q_codes, const int* k_codes, float* tab, int* q4,
+                        int* k4, int R, int Rp, int NB, int H, int S, int Sp, float inv_scale, hipStream_t s) {
+    const long total = (long)H * Rp + 2L * Sp;
+    hipLaunchKernelGGL(k_bias_tables, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, table, bucket_of, q_codes, k_codes,
+                       tab, q4, k4, R, Rp, NB, H, S, Sp, inv_scale, total);
+}
+int bias_grad_chunks(int rows) { return rows < 32 ? 1 : rows < 32 * 32 ? (rows + 31) / 32 : 32; }
+void launch_bias_grad(const float* slab, float* mid, const int* bucket_of, float* dtable, int R, int Rp, int NB, int H, int B,
+                      int per_head, int chunks, hipStream_t s) {
+    hipLaunchKernelGGL(k_bias_slab, dim3((Rp + 255) / 256, H, chunks), dim3(256), 0, s, slab, mid, Rp, H, B, per_head, chunks);
+    hipLaunchKernelGGL(k_bias_buckets, dim3((NB + 255) / 256, H), dim3(256), 0, s, (const float*)mid, bucket_of, dtable, R, Rp, NB, H,
+                       chunks);
+}
+
+}  // namespace pdt

@@ -1,0 +1,343 @@
+// End of a residual block and start of the next in one pass over token-major activations [B, T, D], bf16 in and out, fp32
+// statistics and parameters:
+//
+//   z = LN(y; pw, pb)  (or z = y)      the norm after the branch
+//   u = a x + gate z                   gate [D], or [B, D] with a row for each sample
+//   n = LN(u; w, b)                    the norm before the next branch, of u before it is rounded for the stream
+//
+// Backward, with yh / uh the normalised y / u and g = du + LN'(dn):
+//   dx = a g,  dgate = sum g z,  dz = gate g,  dy = LN'(dz) (or dz),  dw = sum dn uh,  db = sum dn,  dpw = sum dz yh,  dpb = sum dz
+//
+// Bound by memory: forward 2 reads + 2 writes, backward 4 reads + 2 writes of 2 bytes per element.  x and y are what the
+// backward reads again (not u): u is recomputed in fp32, so the parameter gradients see the numbers that the forward normalised,
+// at no more traffic than a saved u would cost.  One wave holds a row in registers (4 channels a lane and piece, NP pieces of
+// 256 channels); the column sums stay in registers over all rows a wave visits, are added over the waves in LDS and over the
+// workgroups in a fixed order (no atomics).
+#include "common.h"
+#include "gated_norm.h"
+
+namespace pdt {
+namespace {
+
+constexpr int kMaxPieces = 8;  // D <= 2048
+
+__device__ __forceinline__ void load4(float* v, const bf16* p, bool in) {
+    bf16x4 t = {(bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f};
+    if (in) t = *reinterpret_cast<const bf16x4*>(p);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (float)t[k];
+}
+__device__ __forceinline__ f32x4 par4(const float* p, bool in) {
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    if (in) t = *reinterpret_cast<const f32x4*>(p);
+    return t;
+}
+
+template <int NP, bool POST>
+__global__ __launch_bounds__(256) void k_gn_fwd(GatedNorm p, bf16* __restrict__ u_out, bf16* __restrict__ n_out,
+                                                float* __restrict__ stats /* [4][M], or null */) {
+    const int lane = threadIdx.x & 63;
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= p.M) return;
+    const int D = p.D, np4 = D >> 2;
+    const float inv_d = 1.f / (float)D;
+    const float* gate = p.gate + (p.per_sample ? row / p.T * D : 0);
+    float x[NP][4], y[NP][4];
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int c = lane + 64 * j;
+        load4(x[j], p.x + row * D + 4 * c, c < np4);
+        load4(y[j], p.y + row * D + 4 * c, c < np4);
+    }
+    if (POST) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s += y[j][k];
+        const float mean = wave_sum(s) * inv_d;
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float d = lane + 64 * j < np4 ? y[j][k] - mean : 0.f;
+                q += d * d;
+            }
+        const float rstd = rsqrtf(wave_sum(q) * inv_d + p.eps);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const bool in = lane + 64 * j < np4;
+            const f32x4 w = par4(p.pw + 4 * (lane + 64 * j), in), b = par4(p.pb + 4 * (lane + 64 * j), in);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[j][k] = (y[j][k] - mean) * rstd * w[k] + b[k];
+        }
+        if (stats && lane == 0) {
+            stats[2 * p.M + row] = mean;
+            stats[3 * p.M + row] = rstd;
+        }
+    }
+    s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const bool in = lane + 64 * j < np4;
+        const f32x4 g = par4(gate + 4 * (lane + 64 * j), in);
+        bf16x4 o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            x[j][k] = p.a * x[j][k] + g[k] * y[j][k];
+            s += x[j][k];
+            o[k] = (bf16)x[j][k];
+        }
+        if (in) *reinterpret_cast<bf16x4*>(u_out + row * D + 4 * (lane + 64 * j)) = o;
+    }
+    const float mean = wave_sum(s) * inv_d;
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < NP; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float d = lane + 64 * j < np4 ? x[j][k] - mean : 0.f;
+            q += d * d;
+        }
+    const float rstd = rsqrtf(wave_sum(q) * inv_d + p.eps);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int c = lane + 64 * j;
+        const f32x4 w = par4(p.w + 4 * c, c < np4), b = par4(p.b + 4 * c, c < np4);
+        bf16x4 o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = (bf16)((x[j][k] - mean) * rstd * w[k] + b[k]);
+        if (c < np4) *reinterpret_cast<bf16x4*>(n_out + row * D + 4 * c) = o;
+    }
+    if (stats && lane == 0) {
+        stats[row] = mean;
+        stats[p.M + row] = rstd;
+    }
+}
+
+// the four waves' column sums -> dst[D] (wave order); `red` [3][NP * 256]
+template <int NP>
+__device__ __forceinline__ void column_sum(float (&v)[NP][4], float* red, float* dst, int lane, int wave, int np4) {
+    constexpr int DP = NP * 256;
+    __syncthreads();
+    if (wave > 0) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const f32x4 t = {v[j][0], v[j][1], v[j][2], v[j][3]};
+            *reinterpret_cast<f32x4*>(red + (wave - 1) * DP + 4 * (lane + 64 * j)) = t;
+        }
+    }
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            f32x4 t = {v[j][0], v[j][1], v[j][2], v[j][3]};
+#pragma unroll
+            for (int w = 0; w < 3; ++w) {
+                const f32x4 o = *reinterpret_cast<const f32x4*>(red + w * DP + 4 * (lane + 64 * j));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) t[k] += o[k];
+            }
+            if (lane + 64 * j < np4) *reinterpret_cast<f32x4*>(dst + 4 * (lane + 64 * j)) = t;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NP; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[j][k] = 0.f;
+}
+
+// A unit is one of `chunks` parts of a sample's rows; a workgroup takes the units blockIdx.x, + gridDim.x, ...  The gate's sums
+// leave after every unit (to gate_part + unit * gate_stride), the others at the end (slab [gridDim.x][srow]: db, dw, dpb, dpw).
+template <int NP, bool POST>
+__global__ __launch_bounds__(256) void k_gn_bwd(GatedNorm p, const bf16* __restrict__ du, const bf16* __restrict__ dn,
+                                                const float* __restrict__ stats, bf16* __restrict__ dx, bf16* __restrict__ dy,
+                                                float* __restrict__ gate_part, long gate_stride, float* __restrict__ slab, int srow,
+                                                int chunks, long units) {
+    extern __shared__ __attribute__((aligned(16))) float red[];  // [3][NP * 256]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int D = p.D, np4 = D >> 2;
+    const float inv_d = 1.f / (float)D;
+    float sg[NP][4], sw[NP][4], sb[NP][4], spw[POST ? NP : 1][4], spb[POST ? NP : 1][4];
+#pragma unroll
+    for (int j = 0; j < NP; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            sg[j][k] = sw[j][k] = sb[j][k] = 0.f;
+            if (POST) spw[j][k] = spb[j][k] = 0.f;
+        }
+    const long rows = p.per_sample ? p.T : p.M, per = (rows + chunks - 1) / chunks;
+    for (long unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const long b = unit / chunks, ch = unit - b * chunks;
+        const long r0 = b * rows + ch * per, r1 = r0 + per < (b + 1) * rows ? r0 + per : (b + 1) * rows;
+        const float* gate = p.gate + (p.per_sample ? b * D : 0);
+        for (long row = r0 + wave; row < r1; row += 4) {
+            float x[NP][4], y[NP][4], g[NP][4], d[NP][4];
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                const int c = lane + 64 * j;
+                const bool in = c < np4;
+                load4(x[j], p.x + row * D + 4 * c, in);
+                load4(y[j], p.y + row * D + 4 * c, in);
+                load4(d[j], dn + row * D + 4 * c, in && dn);
+                load4(g[j], du + row * D + 4 * c, in && du);
+            }
+            const float mu = stats[row], ru = stats[p.M + row];
+            float my = 0.f, ry = 1.f;
+            if (POST) {
+                my = stats[2 * p.M + row];
+                ry = stats[3 * p.M + row];
+            }
+            // x <- uh, y <- yh (or y), s1 / s2: sums of dn w and dn w uh
+            float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                const int c = lane + 64 * j;
+                const bool in = c < np4;
+                const f32x4 ga = par4(gate + 4 * c, in), w = par4(p.w + 4 * c, in);
+                f32x4 pw = {1.f, 1.f, 1.f, 1.f}, pb = {0.f, 0.f, 0.f, 0.f};
+                if (POST) {
+                    pw = par4(p.pw + 4 * c, in);
+                    pb = par4(p.pb + 4 * c, in);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float z = y[j][k];
+                    if (POST) {
+                        y[j][k] = (y[j][k] - my) * ry;
+                        z = y[j][k] * pw[k] + pb[k];
+                    }
+                    x[j][k] = in ? (p.a * x[j][k] + ga[k] * z - mu) * ru : 0.f;
+                    sw[j][k] += d[j][k] * x[j][k];
+                    sb[j][k] += d[j][k];
+                    const float t = d[j][k] * w[k];
+                    s1 += t;
+                    s2 += t * x[j][k];
+                }
+            }
+            s1 = wave_sum(s1) * inv_d;
+            s2 = wave_sum(s2) * inv_d;
+            float s3 = 0.f, s4 = 0.f;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                const int c = lane + 64 * j;
+                const bool in = c < np4;
+                const f32x4 ga = par4(gate + 4 * c, in), w = par4(p.w + 4 * c, in);
+                f32x4 pw = {1.f, 1.f, 1.f, 1.f}, pb = {0.f, 0.f, 0.f, 0.f};
+                if (POST) {
+                    pw = par4(p.pw + 4 * c, in);
+                    pb = par4(p.pb + 4 * c, in);
+                }
+                bf16x4 o;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float gk = in ? g[j][k] + ru * (d[j][k] * w[k] - s1 - x[j][k] * s2) : 0.f;
+                    o[k] = (bf16)(p.a * gk);
+                    const float z = POST ? y[j][k] * pw[k] + pb[k] : y[j][k];
+                    sg[j][k] += gk * z;
+                    const float dz = gk * ga[k];
+                    g[j][k] = dz;
+                    if (POST) {
+                        spw[j][k] += dz * y[j][k];
+                        spb[j][k] += dz;
+                        const float t = dz * pw[k];
+                        s3 += t;
+                        s4 += t * y[j][k];
+                    }
+                }
+                if (in) *reinterpret_cast<bf16x4*>(dx + row * D + 4 * c) = o;
+            }
+            if (POST) {
+                s3 = wave_sum(s3) * inv_d;
+                s4 = wave_sum(s4) * inv_d;
+            }
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                const int c = lane + 64 * j;
+                const bool in = c < np4;
+                f32x4 pw = {1.f, 1.f, 1.f, 1.f};
+                if (POST) pw = par4(p.pw + 4 * c, in);
+                bf16x4 o;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] = (bf16)(POST ? ry * (g[j][k] * pw[k] - s3 - y[j][k] * s4) : g[j][k]);
+                if (in) *reinterpret_cast<bf16x4*>(dy + row * D + 4 * c) = o;
+            }
+        }
+        column_sum<NP>(sg, red, gate_part + unit * gate_stride, lane, wave, np4);
+    }
+    float* out = slab + (long)blockIdx.x * srow;
+    column_sum<NP>(sb, red, out, lane, wave, np4);
+    column_sum<NP>(sw, red, out + D, lane, wave, np4);
+    if constexpr (POST) {
+        column_sum<NP>(spb, red, out + 2 * D, lane, wave, np4);
+        column_sum<NP>(spw, red, out + 3 * D, lane, wave, np4);
+    }
+}
+
+// dgate[b][c] = sum of the sample's units: a wave of 64 columns takes every fourth, the four waves are added in order
+__global__ __launch_bounds__(256) void k_gate_sum(const float* __restrict__ part, float* __restrict__ dgate, int D, int chunks) {
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blocks = (D + 63) / 64;
+    const long b = blockIdx.x / blocks;
+    const int c = (int)(blockIdx.x - b * blocks) * 64 + lane;
+    float s = 0.f;
+    if (c < D) {
+#pragma unroll 8
+        for (int k = wave; k < chunks; k += 4) s += part[(b * chunks + k) * D + c];
+    }
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < D) dgate[b * D + c] = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
+}
+
+}  // namespace
+
+bool gated_norm_dim_ok(long D) { return D >= 4 && D % 4 == 0 && D <= kMaxPieces * 256; }
+
+#define PDT_GN_CASE(N, ...) case N: { constexpr int NP = N; __VA_ARGS__; } break;
+#define PDT_GN_DISPATCH(D, ...)                                                                                       \
+    switch (((D) + 255) / 256) {                                                                                      \
+        PDT_GN_CASE(1, __VA_ARGS__) PDT_GN_CASE(2, __VA_ARGS__) PDT_GN_CASE(3, __VA_ARGS__) PDT_GN_CASE(4, __VA_ARGS__) \
+        PDT_GN_CASE(5, __VA_ARGS__) PDT_GN_CASE(6, __VA_ARGS__) PDT_GN_CASE(7, __VA_ARGS__) PDT_GN_CASE(8, __VA_ARGS__) \
+        default: break; /* (the binding refuses other widths) */                                                      \
+    }
+
+void launch_gated_norm_fwd(const GatedNorm& p, void* u, void* n, float* stats, hipStream_t s) {
+    const unsigned grid = (unsigned)((p.M + 3) / 4);
+    PDT_GN_DISPATCH(p.D, {
+        if (p.pw) hipLaunchKernelGGL((k_gn_fwd<NP, true>), dim3(grid), dim3(256), 0, s, p, (bf16*)u, (bf16*)n, stats);
+        else hipLaunchKernelGGL((k_gn_fwd<NP, false>), dim3(grid), dim3(256), 0, s, p, (bf16*)u, (bf16*)n, stats);
+    });
+}
+
+GatedNormPlan gated_norm_plan(long B, long T, long M, bool per_sample) {
+    // about 1024 workgroups (4 per CU) of at least 8 rows
+    GatedNormPlan q;
+    const long samples = per_sample ? B : 1, rows = per_sample ? T : M;
+    long c = (1024 + samples - 1) / samples;
+    if (c > (rows + 7) / 8) c = (rows + 7) / 8;
+    if (per_sample && c > 256) c = 256;  // (k_gate_sum walks over a sample's chunks)
+    q.chunks = (int)(c < 1 ? 1 : c);
+    q.units = samples * q.chunks;
+    q.blocks = (int)(q.units < 1024 ? q.units : 1024);
+    return q;
+}
+
+void launch_gated_norm_bwd(const GatedNorm& p, const GatedNormPlan& q, const void* du, const void* dn, const float* stats, void* dx,
+                           void* dy, float* gate_part, long gate_stride, float* slab, int srow, hipStream_t s) {
+    PDT_GN_DISPATCH(p.D, {
+        const size_t lds = (size_t)3 * NP * 256 * sizeof(float);
+        if (p.pw)
+            hipLaunchKernelGGL((k_gn_bwd<NP, true>), dim3(q.blocks), dim3(256), lds, s, p, (const bf16*)du, (const bf16*)dn, stats,
+                               (bf16*)dx, (bf16*)dy, gate_part, gate_stride, slab, srow, q.chunks, q.units);
+        else
+            hipLaunchKernelGGL((k_gn_bwd<NP, false>), dim3(q.blocks), dim3(256), lds, s, p, (const bf16*)du, (const bf16*)dn, stats,
+                               (bf16*)dx, (bf16*)dy, gate_part, gate_stride, slab, srow, q.chunks, q.units);
+    });
+}
+void launch_gate_sum(const float* part, float* dgate, long B, int D, int chunks, hipStream_t s) {
+    hipLaunchKernelGGL(k_gate_sum, dim3((unsigned)(B * ((D + 63) / 64))), dim3(256), 0, s, part, dgate, D, chunks);
+}
+
+}  // namespace pdt

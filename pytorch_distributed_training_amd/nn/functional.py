@@ -543,6 +543,195 @@ def layer_norm(x, weight, bias, eps: float = 1e-5, with_skip: bool = False):
     return (y, skip) if with_skip else y
 
 
+# ------------------------------------------------- attention with relative positions, cross attention, gated norms
+def _rows3(t):
+    """``t`` [B, rows, width] with contiguous, 16-B aligned, non-overlapping rows (a copy only where it has none)"""
+    ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and (t.shape[1] < 2 or (t.stride(1) % 8 == 0 and t.stride(1) >= t.shape[2]
+          and t.stride(1) < (1 << 23))) and (t.shape[0] < 2 or t.stride(0) % 8 == 0))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def _check_lengths(lengths, like, op: str) -> None:
+    if lengths is None:
+        return
+    if lengths.dim() != 1 or lengths.shape[0] != like.shape[0] or lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{op}: lengths must be [{like.shape[0]}] int32 or int64, got {tuple(lengths.shape)} {lengths.dtype}")
+    if lengths.device != like.device:
+        raise ValueError(f"{op}: lengths are on {lengths.device}, the input on {like.device}")
+
+
+class _RelBiasAttentionFn(torch.autograd.Function):
+    """The bias table's gradient is fp32 and summed without atomics; for it the forward also keeps the part of its output that
+    bf16 drops (``out_lo``), which the backward adds to D = dO . O."""
+
+    @staticmethod
+    def forward(ctx, qkv, table, q_codes, k_codes, bucket_of, heads, lengths, be):
+        want_table = ctx.needs_input_grad[1]
+        out, lse, lo, tab, codes = be.rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, True,
+                                                             want_table)
+        ctx.save_for_backward(qkv, out, lo, lse, tab, codes, bucket_of, lengths)
+        ctx.cfg = (be, heads, table.shape[0], table.dtype)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        qkv, out, lo, lse, tab, codes, bucket_of, lengths = ctx.saved_tensors
+        be, heads, buckets, tdt = ctx.cfg
+        dqkv, dtable = be.rel_bias_attention_bwd(dout, qkv, out, lo, lse, tab, codes, bucket_of, buckets, heads, lengths,
+                                                 ctx.needs_input_grad[1])
+        return dqkv, (None if dtable is None else dtable.to(tdt)), None, None, None, None, None, None
+
+
+def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None):
+    """Self-attention with a learned relative position bias on the packed in-projection output ``[B, S, 3*D]`` (q | k | v,
+    heads inside each) -> ``[B, S, D]``: ``softmax(q k^T / sqrt(head_dim) + bias) v``.
+
+    The bias of query ``i`` and key ``j`` in head ``h`` is ``table[bucket, h]`` (``table`` ``[buckets, heads]``, learned) with
+    ``bucket = bucket_of[clamp(q_codes[i] - k_codes[j], 0, len(bucket_of) - 1)]``; ``nn.grid_position_buckets`` and
+    ``nn.log_position_buckets`` make the three integer tensors (codes below 2^28 in magnitude).  An entry of ``bucket_of``
+    outside the table means no bias; a table entry of ``-inf`` forbids the pair.
+
+    ``lengths`` (``[B]`` integers, on the device of ``qkv``): sequence ``b`` is its first ``lengths[b]`` tokens; the rows behind
+    it are neither attended to nor read, their outputs and gradients are zero, and so is a row whose every key is forbidden.
+    On bf16 GPU tensors with head_dim 32 / 64 / 128 and at most 4096 entries the HIP kernels of csrc/kernels/attention_ext.hip run;
+    the PyTorch oracle elsewhere."""
+    heads = int(heads)
+    if qkv.dim() != 3 or heads < 1 or qkv.shape[2] % (3 * heads):
+        raise ValueError(f"rel_bias_attention: qkv {tuple(qkv.shape)} is not [B, S, 3 * {heads} * head_dim]")
+    if table.dim() != 2 or table.shape[1] != heads:
+        raise ValueError(f"rel_bias_attention: table {tuple(table.shape)} is not [buckets, {heads}]")
+    if bucket_of.dim() != 1 or bucket_of.shape[0] < 1:
+        raise ValueError(f"rel_bias_attention: bucket_of {tuple(bucket_of.shape)} is not [entries]")
+    for name, t in (("q_codes", q_codes), ("k_codes", k_codes)):
+        if tuple(t.shape) != (qkv.shape[1],):
+            raise ValueError(f"rel_bias_attention: {name} {tuple(t.shape)} for {qkv.shape[1]} tokens")
+    for name, t in (("table", table), ("q_codes", q_codes), ("k_codes", k_codes), ("bucket_of", bucket_of)):
+        if t.device != qkv.device:
+            raise ValueError(f"rel_bias_attention: {name} is on {t.device}, qkv on {qkv.device}")
+        if name != "table" and t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"rel_bias_attention: {name} must be integers, got {t.dtype}")
+    _check_lengths(lengths, qkv, "rel_bias_attention")
+    be = backend_for(qkv)
+    if be is not reference:
+        why = be.rel_bias_attention_unsupported_reason(qkv, heads, bucket_of)
+        if why is not None:
+            _note_fallback("rel_bias_attention", why)
+            be = reference
+    qkv = _rows3(qkv)
+    if not _wants_grad(qkv, table):
+        return be.rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, False, False)[0]
+    return _RelBiasAttentionFn.apply(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, be)
+
+
+class _CrossAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, kv, heads, kv_heads, lengths, be):
+        out, lse = be.cross_attention_fwd(q, kv, heads, kv_heads, lengths, True)
+        ctx.save_for_backward(q, kv, out, lse, lengths)
+        ctx.cfg = (be, heads, kv_heads)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, kv, out, lse, lengths = ctx.saved_tensors
+        be, heads, kv_heads = ctx.cfg
+        dq, dkv = be.cross_attention_bwd(dout, q, kv, out, lse, heads, kv_heads, lengths)
+        return dq, dkv, None, None, None, None
+
+
+def cross_attention(q, kv, heads: int, kv_heads: int | None = None, lengths=None):
+    """Attention of ``q`` ``[B, Sq, heads*head_dim]`` over an encoder's states ``kv`` ``[B, Sk, 2*kv_heads*head_dim]`` (keys |
+    values, heads inside each) -> ``[B, Sq, heads*head_dim]``; scale 1/sqrt(head_dim), no dropout.  ``kv_heads`` (default
+    ``heads``) divides ``heads``: query heads ``h*heads/kv_heads ...`` share key head ``h``.
+
+    ``lengths`` (``[B]`` integers, on the device of ``q``): only the first ``lengths[b]`` keys of sequence ``b`` are attended to;
+    the others are not read and get zero gradients; a sequence without keys gives zeros.  Single queries (``Sq = 1``) over
+    long states are split over the keys.  HIP kernels (csrc/kernels/attention_ext.hip) on bf16 GPU tensors with head_dim
+    32 / 64 / 128, the PyTorch oracle elsewhere."""
+    heads = int(heads)
+    kv_heads = heads if kv_heads is None else int(kv_heads)
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"cross_attention: {heads} heads over {kv_heads} key heads")
+    if q.dim() != 3 or kv.dim() != 3 or q.shape[0] != kv.shape[0] or q.shape[2] % heads or (
+            kv.shape[2] != 2 * kv_heads * (q.shape[2] // heads)):
+        raise ValueError(f"cross_attention: q {tuple(q.shape)} and kv {tuple(kv.shape)} for {heads} heads over {kv_heads}")
+    if q.device != kv.device or q.dtype != kv.dtype:
+        raise ValueError(f"cross_attention: q is {q.dtype} on {q.device}, kv {kv.dtype} on {kv.device}")
+    _check_lengths(lengths, q, "cross_attention")
+    be = backend_for(q)
+    if be is not reference:
+        why = be.cross_attention_unsupported_reason(q, heads)
+        if why is not None:
+            _note_fallback("cross_attention", why)
+            be = reference
+    q, kv = _rows3(q), _rows3(kv)
+    if not _wants_grad(q, kv):
+        return be.cross_attention_fwd(q, kv, heads, kv_heads, lengths, False)[0]
+    return _CrossAttentionFn.apply(q, kv, heads, kv_heads, lengths, be)
+
+
+class _GatedResidualNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, gate, weight, bias, post_weight, post_bias, eps, scale, be):
+        ps = [None if t is None else t.float().contiguous() for t in (gate, weight, bias, post_weight, post_bias)]
+        new, normed, stats = be.gated_norm_fwd(x, branch, *ps, eps, scale, True)
+        ctx.save_for_backward(x, branch, *ps, stats)
+        ctx.cfg = (be, eps, scale, [None if t is None else t.dtype for t in (gate, weight, bias, post_weight, post_bias)])
+        ctx.set_materialize_grads(False)
+        return new, normed
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dnew, dnormed):
+        if dnew is None and dnormed is None:
+            return (None,) * 10
+        x, branch, *ps, stats = ctx.saved_tensors
+        be, eps, scale, dts = ctx.cfg
+        dx, dy, *dps = be.gated_norm_bwd(dnew, dnormed, x, branch, *ps, stats, eps, scale)
+        dps += [None] * (5 - len(dps))
+        return (dx, dy, *(None if t is None else t.to(dt) for t, dt in zip(dps, dts)), None, None, None)
+
+
+def gated_residual_norm(x, branch, gate, weight, bias, eps: float = 1e-6, post_weight=None, post_bias=None,
+                        residual_scale: float = 1.0):
+    """The end of a residual block and the norm of the next one, in one pass -> ``(x_new, normed)``:
+    ``x_new = residual_scale * x + gate * post(branch)`` and ``normed = LayerNorm(x_new; weight, bias)``, with ``post`` the
+    LayerNorm of ``post_weight`` / ``post_bias`` (identity without them).  ``x`` and ``branch`` are ``[..., D]``; ``gate`` is
+    ``[D]`` (layer scale) or ``[B, D]``, one for each entry of the first dimension.  ``normed`` is taken of ``x_new`` before
+    that is rounded to the stream's type.  HIP kernel (csrc/kernels/gated_norm.hip) on bf16 GPU tensors, widths that are
+    multiples of 4 up to 2048; fp32 PyTorch oracle elsewhere."""
+    d = x.shape[-1] if x.dim() else 0
+    if x.dim() < 2 or x.shape != branch.shape or x.dtype != branch.dtype:
+        raise ValueError(f"gated_residual_norm: x {tuple(x.shape)} {x.dtype}, branch {tuple(branch.shape)} {branch.dtype}")
+    if tuple(gate.shape) not in ((d,), (x.shape[0], d)):
+        raise ValueError(f"gated_residual_norm: gate {tuple(gate.shape)} for x {tuple(x.shape)}")
+    if (post_weight is None) != (post_bias is None):
+        raise ValueError("gated_residual_norm: post_weight and post_bias come together")
+    for name, t in (("branch", branch), ("gate", gate), ("weight", weight), ("bias", bias), ("post_weight", post_weight),
+                    ("post_bias", post_bias)):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"gated_residual_norm: {name} is on {t.device}, x on {x.device}")
+        if t is not None and name not in ("branch", "gate") and tuple(t.shape) != (d,):
+            raise ValueError(f"gated_residual_norm: {name} {tuple(t.shape)} for width {d}")
+    be = backend_for(x)
+    if be is not reference:
+        why = be.layernorm_unsupported_reason(x)
+        if why is not None:
+            _note_fallback("gated_residual_norm", why)
+            be = reference
+    x, branch = x.contiguous(), branch.contiguous()
+    if not _wants_grad(x, branch, gate, weight, bias, post_weight, post_bias):
+        ps = [None if t is None else t.float().contiguous() for t in (gate, weight, bias, post_weight, post_bias)]
+        return be.gated_norm_fwd(x, branch, *ps, float(eps), float(residual_scale), False)[:2]
+    return _GatedResidualNormFn.apply(x, branch, gate, weight, bias, post_weight, post_bias, float(eps), float(residual_scale), be)
+
+
 # ------------------------------------------------------------------- linear
 def _lowp_weight(w, dtype):
     lp = getattr(w, "_lp", None)

@@ -11,6 +11,7 @@
 """
 from __future__ import annotations
 
+import math
 import os
 
 import torch
@@ -142,3 +143,41 @@ class CrossEntropyLoss(tnn.Module):
 
     def forward(self, logits, labels):
         return F.softmax_cross_entropy(logits, labels)
+
+
+def grid_position_buckets(height: int, width: int, prefix: int = 1):
+    """``(q_codes, k_codes, bucket_of)`` for ``functional.rel_bias_attention``: tokens are ``prefix`` leading tokens (class
+    token) and the cells of a ``height`` x ``width`` grid, row by row.  Each (dy, dx) has a bucket of its own,
+    ``(2*height-1) * (2*width-1)`` of them between three for the prefix: the first for a cell that reads a prefix token, the last
+    two for a prefix token that reads one and that reads a cell.  A cell's code is its row-major place in a grid of
+    width ``2*width-1``, so that a difference of codes names (dy, dx); the prefix codes lie so far out that their differences
+    fall past the ends."""
+    if height < 1 or width < 1 or prefix < 0:
+        raise ValueError(f"grid_position_buckets: {height} x {width} cells, {prefix} prefix tokens")
+    w = 2 * width - 1
+    top = (height - 1) * w + width - 1
+    if 4 * top + 3 >= 1 << 28:
+        raise ValueError(f"grid_position_buckets: {height} x {width} cells are too many")
+    cell = (torch.arange(height)[:, None] * w + torch.arange(width)[None, :]).reshape(-1)
+    q = torch.cat([torch.full((prefix,), 4 * top + 3), cell + top + 1])
+    k = torch.cat([torch.full((prefix,), 2 * top + 1), cell])
+    return q.int(), k.int(), torch.arange(2 * top + 4).int()
+
+
+def log_position_buckets(length: int, buckets: int = 32, far: int = 128, bidirectional: bool = True):
+    """``(q_codes, k_codes, bucket_of)`` for ``functional.rel_bias_attention`` on ``length`` positions in a row: with
+    ``bidirectional`` half of the ``buckets`` for keys behind the query's position and half for those after it, else all for
+    those behind (a key after it is in bucket 0).  Of those for one side, the first half are one distance each and the others
+    grow logarithmically up to ``far``, past which the last one holds."""
+    sides = buckets // 2 if bidirectional else buckets
+    exact = sides // 2
+    if length < 0 or exact < 1 or far <= exact:
+        raise ValueError(f"log_position_buckets: {buckets} buckets up to {far}")
+    pos = torch.arange(length)
+    ahead = far - torch.arange(2 * far + 1)  # key position - query position
+    d = ahead.abs() if bidirectional else (-ahead).clamp(min=0)
+    log = exact + (torch.log(d.clamp(min=1).double() / exact) / math.log(far / exact) * (sides - exact)).long()
+    of = torch.where(d < exact, d, log.clamp(max=sides - 1))
+    if bidirectional:
+        of = of + sides * (ahead > 0)
+    return (pos + far).int(), pos.int(), of.int()

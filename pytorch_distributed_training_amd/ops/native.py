@@ -258,6 +258,78 @@ def layernorm_bwd(dy, x, mean, rstd, gamma, addend=None):
                             None if addend is None else addend.contiguous())
 
 
+# -------------------------------- attention with relative positions, cross attention (csrc/kernels/attention_ext.hip)
+def _al(t):
+    """dense and 16-B aligned (a copy only where it is not: a slice that starts at an odd element)"""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _i32(t):
+    return None if t is None else _al(t if t.dtype == torch.int32 else t.to(torch.int32))
+
+
+def _f32(t):
+    return _al(t if t.dtype == torch.float32 else t.float())
+
+
+def cross_attention_unsupported_reason(q, heads: int):
+    if q.dtype != _BF16:
+        return f"dtype {q.dtype} (native attention is bf16)"
+    if q.shape[2] // heads not in (32, 64, 128):
+        return f"head_dim {q.shape[2] // heads} (native attention: head_dim 32, 64 or 128)"
+    return None
+
+
+def rel_bias_attention_unsupported_reason(qkv, heads: int, bucket_of):
+    if qkv.dtype != _BF16:
+        return f"dtype {qkv.dtype} (native attention is bf16)"
+    if qkv.shape[2] // (3 * heads) not in (32, 64, 128):
+        return f"head_dim {qkv.shape[2] // (3 * heads)} (native attention: head_dim 32, 64 or 128)"
+    if bucket_of.shape[0] > _C.rel_bias_max_entries:
+        return f"{bucket_of.shape[0]} relative positions (native: up to {_C.rel_bias_max_entries})"
+    return None
+
+
+def rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None, grad: bool = True,
+                           want_table: bool = True):
+    """-> (out [B, S, D], stat, out_lo, tab, codes): what ``rel_bias_attention_bwd`` wants back, the statistics with ``grad``,
+    ``out_lo`` with ``want_table``"""
+    return _C.rel_bias_attention_fwd(qkv, _f32(table), _i32(q_codes), _i32(k_codes), _i32(bucket_of), heads, _i32(lengths),
+                                     grad, want_table)
+
+
+def rel_bias_attention_bwd(dout, qkv, out, out_lo, lse, tab, codes, bucket_of, buckets: int, heads: int, lengths=None,
+                           want_table: bool = True):
+    """-> (dqkv, dtable [buckets, heads] fp32, or None)"""
+    return _C.rel_bias_attention_bwd(_al(dout), qkv, out, out_lo, lse, tab, codes, _i32(bucket_of), buckets, heads,
+                                     _i32(lengths), want_table)
+
+
+def cross_attention_fwd(q, kv, heads: int, kv_heads: int, lengths=None, grad: bool = True):
+    """-> (out [B, Sq, H*hd], statistics for the backward, or None)"""
+    return _C.cross_attention_fwd(q, kv, heads, kv_heads, _i32(lengths), grad)
+
+
+def cross_attention_bwd(dout, q, kv, out, lse, heads: int, kv_heads: int, lengths=None):
+    """-> (dq, dkv)"""
+    return _C.cross_attention_bwd(_al(dout), q, kv, out, lse, heads, kv_heads, _i32(lengths))
+
+
+# ------------------------------------------------------------------------- gated norm (csrc/kernels/gated_norm.hip)
+def gated_norm_fwd(x, branch, gate, weight, bias, post_weight, post_bias, eps: float, scale: float, grad: bool = True):
+    """-> (x_new, normed, statistics for the backward, or None); parameters fp32"""
+    return _C.gated_norm_fwd(_al(x), _al(branch), _al(gate), _al(weight), _al(bias), _al(post_weight), _al(post_bias), eps, scale, grad)
+
+
+def gated_norm_bwd(dnew, dnormed, x, branch, gate, weight, bias, post_weight, post_bias, stats, eps: float, scale: float):
+    """-> [dx, dbranch, dgate, dweight, dbias (, dpost_weight, dpost_bias)]; a gradient that is None counts as zeros"""
+    return _C.gated_norm_bwd(_al(dnew), _al(dnormed), _al(x), _al(branch), _al(gate), _al(weight), _al(bias), _al(post_weight),
+                             _al(post_bias), stats, eps, scale)
+
+
 # ------------------------------------------------------------------- linear
 def linear_unsupported_reason(x, w, padded_ok: bool = False):
     """``x [..., K]`` against ``w [N, K]``: why the MFMA GEMM (csrc/kernels/gemm.hip) cannot take it, or None.

@@ -200,6 +200,167 @@ def layernorm_bwd(dy, x, mean, rstd, gamma, addend=None):
     return dx.to(x.dtype).view_as(x), (dyf * xhat).sum(0), dyf.sum(0)
 
 
+# ----------------------- attention with relative positions, cross attention
+def _ext_probs(q, k, bias, lengths):
+    """fp32 softmax probabilities ``[B, H, Sq, Sk]`` over the first ``lengths[b]`` keys; rows without a key are zero"""
+    s = torch.matmul(q, k.transpose(2, 3)) * q.shape[-1] ** -0.5
+    if bias is not None:
+        s = s + bias
+    if lengths is not None:
+        dead = torch.arange(k.shape[2], device=k.device) >= lengths[:, None]
+        s = s.masked_fill(dead[:, None, None, :], float("-inf"))
+    if s.shape[-1] == 0:
+        return s
+    top = s.amax(-1, keepdim=True)
+    p = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top))
+    total = p.sum(-1, keepdim=True)
+    return p / torch.where(total == 0, torch.ones_like(total), total)
+
+
+def _no_dead_rows(t, lengths):
+    """``t`` ``[B, H, S, hd]`` with zeros in the rows past ``lengths`` (their values are not to be read)"""
+    if lengths is None:
+        return t
+    dead = torch.arange(t.shape[2], device=t.device) >= lengths[:, None]
+    return t.masked_fill(dead[:, None, :, None], 0.0)
+
+
+def _ext_grads(do, q, k, v, p):
+    dp = torch.matmul(do, v.transpose(2, 3))
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    scale = q.shape[-1] ** -0.5
+    return torch.matmul(ds, k) * scale, torch.matmul(ds.transpose(2, 3), q) * scale, torch.matmul(p.transpose(2, 3), do), ds
+
+
+def _work_type(t):
+    return torch.float64 if t.dtype == torch.float64 else torch.float32
+
+
+def _rel_parts(qkv, heads, lengths):
+    b, s, w = qkv.shape
+    x = qkv.to(_work_type(qkv)).view(b, s, 3, heads, w // (3 * heads)).permute(2, 0, 3, 1, 4)
+    return [_no_dead_rows(t, lengths) for t in x.unbind(0)]
+
+
+def _rel_buckets(q_codes, k_codes, bucket_of):
+    return bucket_of.long()[(q_codes.long()[:, None] - k_codes.long()[None, :]).clamp(0, bucket_of.shape[0] - 1)]
+
+
+def _rel_probs(q, k, table, bucket, lengths):
+    real = (bucket >= 0) & (bucket < table.shape[0])
+    bias = torch.zeros((table.shape[1], *bucket.shape), dtype=q.dtype, device=q.device)
+    if table.shape[0]:
+        rows = table.to(q.dtype)[bucket.clamp(0, table.shape[0] - 1)].permute(2, 0, 1)
+        bias = torch.where(real, rows, bias)
+    p = _ext_probs(q, k, bias, lengths)
+    if lengths is not None:
+        p = p * (torch.arange(q.shape[2], device=q.device) < lengths[:, None])[:, None, :, None]
+    return p, real
+
+
+def rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None, grad: bool = True,
+                           want_table: bool = True):
+    """Oracle of csrc/kernels/attention_ext.hip -> (out, None, None, table, codes)"""
+    b, s, w = qkv.shape
+    q, k, v = _rel_parts(qkv, heads, lengths)
+    p, _ = _rel_probs(q, k, table, _rel_buckets(q_codes, k_codes, bucket_of), lengths)
+    out = torch.matmul(p, v).transpose(1, 2).reshape(b, s, w // 3).to(qkv.dtype)
+    return out, None, None, table, torch.stack([q_codes, k_codes])
+
+
+def rel_bias_attention_bwd(dout, qkv, out, out_lo, lse, tab, codes, bucket_of, buckets: int, heads: int, lengths=None,
+                           want_table: bool = True):
+    b, s, w = qkv.shape
+    q, k, v = _rel_parts(qkv, heads, lengths)
+    bucket = _rel_buckets(codes[0], codes[1], bucket_of)
+    p, real = _rel_probs(q, k, tab, bucket, lengths)
+    do = _no_dead_rows(dout.to(q.dtype).view(b, s, heads, -1).transpose(1, 2), lengths)
+    dq, dk, dv, ds = _ext_grads(do, q, k, v, p)
+    dqkv = torch.stack([dq, dk, dv]).permute(1, 3, 0, 2, 4).reshape(b, s, w).to(qkv.dtype)
+    if not want_table:
+        return dqkv, None
+    dtable = torch.zeros((buckets, heads), dtype=q.dtype, device=q.device)
+    if buckets:
+        by_pair = (ds.sum(0) * real).view(heads, -1).t()
+        dtable.index_add_(0, bucket.clamp(0, buckets - 1).reshape(-1), by_pair.contiguous())
+    return dqkv, dtable
+
+
+def _cross_parts(q, kv, heads, kv_heads, lengths):
+    b, sq, w = q.shape
+    hd = w // heads
+    f = _work_type(q)
+    qf = q.to(f).view(b, sq, kv_heads, heads // kv_heads, hd).permute(0, 2, 3, 1, 4).reshape(b, kv_heads, -1, hd)
+    k, v = kv.to(f).view(b, kv.shape[1], 2, kv_heads, hd).permute(2, 0, 3, 1, 4).unbind(0)
+    return qf, _no_dead_rows(k, lengths), _no_dead_rows(v, lengths)
+
+
+def _cross_rows(t, q, heads, kv_heads):
+    """``[B, kv_heads, G*Sq, hd]`` -> the layout and type of ``q``"""
+    b, sq, w = q.shape
+    return t.view(b, kv_heads, heads // kv_heads, sq, w // heads).permute(0, 3, 1, 2, 4).reshape(b, sq, w).to(q.dtype)
+
+
+def cross_attention_fwd(q, kv, heads: int, kv_heads: int, lengths=None, grad: bool = True):
+    """Oracle of csrc/kernels/attention_ext.hip -> (out, None)"""
+    qf, k, v = _cross_parts(q, kv, heads, kv_heads, lengths)
+    return _cross_rows(torch.matmul(_ext_probs(qf, k, None, lengths), v), q, heads, kv_heads), None
+
+
+def cross_attention_bwd(dout, q, kv, out, lse, heads: int, kv_heads: int, lengths=None):
+    b, sk = kv.shape[:2]
+    qf, k, v = _cross_parts(q, kv, heads, kv_heads, lengths)
+    do = _cross_parts(dout, kv, heads, kv_heads, None)[0]
+    dq, dk, dv, _ = _ext_grads(do, qf, k, v, _ext_probs(qf, k, None, lengths))
+    dkv = torch.stack([dk, dv]).permute(1, 3, 0, 2, 4).reshape(b, sk, -1).to(kv.dtype)
+    return _cross_rows(dq, q, heads, kv_heads), dkv
+
+
+# --------------------------------------------------------- gated norm ----
+def _normalise(t, eps):
+    mean = t.mean(-1, keepdim=True)
+    rstd = torch.rsqrt((t - mean).square().mean(-1, keepdim=True) + eps)
+    return (t - mean) * rstd, rstd
+
+
+def _gated_parts(x, branch, gate, post_weight, post_bias, eps, scale):
+    f = _work_type(x)
+    xf, yf = x.to(f), branch.to(f)
+    g = gate.to(f)
+    if gate.dim() == 2:
+        g = g.view(gate.shape[0], *[1] * (x.dim() - 2), gate.shape[1])
+    yh, yr = _normalise(yf, eps) if post_weight is not None else (yf, None)
+    z = yh * post_weight.to(f) + post_bias.to(f) if post_weight is not None else yh
+    return g, yh, yr, z, scale * xf + g * z
+
+
+def gated_norm_fwd(x, branch, gate, weight, bias, post_weight, post_bias, eps: float, scale: float, grad: bool = True):
+    """Oracle of csrc/kernels/gated_norm.hip -> (x_new, normed, None)"""
+    new = _gated_parts(x, branch, gate, post_weight, post_bias, eps, scale)[4]
+    normed = _normalise(new, eps)[0] * weight.to(new.dtype) + bias.to(new.dtype)
+    return new.to(x.dtype), normed.to(x.dtype), None
+
+
+def gated_norm_bwd(dnew, dnormed, x, branch, gate, weight, bias, post_weight, post_bias, stats, eps: float, scale: float):
+    g, yh, yr, z, new = _gated_parts(x, branch, gate, post_weight, post_bias, eps, scale)
+    f = new.dtype
+    nh, nr = _normalise(new, eps)
+
+    def norm_grad(t, hat, r):
+        return r * (t - t.mean(-1, keepdim=True) - hat * (t * hat).mean(-1, keepdim=True))
+
+    dn = torch.zeros_like(new) if dnormed is None else dnormed.to(f)
+    du = norm_grad(dn * weight.to(f), nh, nr)
+    if dnew is not None:
+        du = du + dnew.to(f)
+    rows = tuple(range(x.dim() - 1))
+    dz = du * g
+    dy = dz if post_weight is None else norm_grad(dz * post_weight.to(f), yh, yr)
+    grads = [(scale * du).to(x.dtype), dy.to(x.dtype), (du * z).sum(rows if gate.dim() == 1 else rows[1:]), (dn * nh).sum(rows),
+             dn.sum(rows)]
+    return grads if post_weight is None else grads + [(dz * yh).sum(rows), dz.sum(rows)]
+
+
 # ---------------------------------------------------------------- pools ----
 def maxpool3x3s2_fwd(x):
     """-> (y, aux); the oracle needs no aux"""

@@ -1,0 +1,582 @@
+"""Attention with a learned relative position bias, cross attention and gated residual norms against plain forms in 64 bits.
+
+The tolerances count roundings: a bf16 rounding is off by at most 2^-8 of its value.  The attention kernels round P (for P V and
+P^T dO), dS (for dS K and dS^T Q) and each output once, and D = dO . O carries the error of the rounded O; every bound below is
+that sum of absolute values, element by element, plus 2^-13 of the same absolute sums for what is done in 32 bits (products of
+up to 128 terms, scores up to 2^6 whose error an exponential passes on as a relative one: 2^6 * 2^7 * 2^-24 * a margin of 16)."""
+import math
+
+import pytest
+import torch
+
+import pytorch_distributed_training_amd as pdt
+from pytorch_distributed_training_amd.nn import functional as F
+
+U = torch.finfo(torch.bfloat16).eps / 2
+SLACK = 2.0 ** -13
+TINY = 1e-30
+gpu = pytest.mark.gpu
+
+
+def _dev(device):
+    if device == "cuda":
+        pdt.require_native()
+    return torch.device(device)
+
+
+def _rand(g, *shape, std=1.0, dtype=torch.bfloat16, device="cpu"):
+    return (torch.randn(*shape, generator=g) * std).to(dtype).to(device)
+
+
+def _within(got, want, bound, what):
+    got, want, bound = got.double().cpu(), want.cpu(), bound.cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert torch.isfinite(got).all(), what
+    over = (got - want).abs() - bound
+    assert (over <= TINY).all(), f"{what}: {int((over > TINY).sum())} of {got.numel()} off, worst by {over.max():.3e}"
+
+
+# ----------------------------------------------------------------------------------------- the plain form in 64 bits
+def _attention64(q, k, v, bias, key_live, row_live, do):
+    """q [B,H,Sq,hd] ... in 64 bits; masks [B,Sk] / [B,Sq] -> out, dq, dk, dv, dS and the bounds of the first four"""
+    scale = q.shape[-1] ** -0.5
+    s = q @ k.transpose(-1, -2) * scale
+    if bias is not None:
+        s = s + bias
+    s = s.masked_fill(~key_live[:, None, None, :], -math.inf)
+    top = s.amax(-1, keepdim=True) if s.shape[-1] else s.new_zeros(*s.shape[:-1], 1)
+    p = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
+    p = p / p.sum(-1, keepdim=True).clamp(min=1e-300) * row_live[:, None, :, None]
+    out = p @ v
+    spread = p @ v.abs()
+    e_out = U * (out.abs() + spread) + SLACK * spread
+    dp = do @ v.transpose(-1, -2)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    e_d = (do.abs() * e_out).sum(-1, keepdim=True)
+    e_ds = U * ds.abs() + p * (e_d + SLACK * (do.abs() @ v.abs().transpose(-1, -2)))
+    dq, dk, dv = ds @ k * scale, ds.transpose(-1, -2) @ q * scale, p.transpose(-1, -2) @ do
+    e_dq = U * dq.abs() + scale * (e_ds @ k.abs())
+    e_dk = U * dk.abs() + scale * (e_ds.transpose(-1, -2) @ q.abs())
+    e_dv = U * dv.abs() + (U + SLACK) * (p.transpose(-1, -2) @ do.abs())
+    return (out, dq, dk, dv, ds, p), (e_out, e_dq, e_dk, e_dv)
+
+
+def _live(lengths, b, n, device):
+    if lengths is None:
+        return torch.ones(b, n, dtype=torch.bool, device=device)
+    return torch.arange(n, device=device) < torch.tensor(lengths, device=device)[:, None]
+
+
+def _rel_case(device, b, codes, heads, hd, lengths=None, seed=0, table=None, poison=False):
+    g = torch.Generator().manual_seed(seed)
+    qc, kc, of = (t.to(device) for t in codes)
+    n = qc.numel()
+    qkv = _rand(g, b, n, 3 * heads * hd, device=device)
+    if table is None:
+        table = _rand(g, int(of.max()) + 1, heads, dtype=torch.float32)
+    table = table.to(device)
+    do = _rand(g, b, n, heads * hd, std=0.1, device=device)
+    live = _live(lengths, b, n, device)
+    clean = qkv.double() * live[..., None], do.double() * live[..., None]
+    if poison:  # what stands behind the last token is not to be read
+        qkv = qkv.masked_fill(~live[..., None], math.nan)
+        do = do.masked_fill(~live[..., None], math.inf)
+    return qkv, table, qc, kc, of, do, live, clean
+
+
+def _check_rel(device, b, codes, heads, hd, lengths=None, seed=0, table=None, poison=False):
+    qkv, table, qc, kc, of, do, live, (qkv64, do64) = _rel_case(device, b, codes, heads, hd, lengths, seed, table, poison)
+    n = qc.numel()
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=device)
+    leaf, tleaf = qkv.clone().requires_grad_(), table.clone().requires_grad_()
+    out = F.rel_bias_attention(leaf, tleaf, qc, kc, of, heads, lens)
+    dqkv, dtable = torch.autograd.grad(out, [leaf, tleaf], do)
+    with torch.no_grad():
+        only = F.rel_bias_attention(qkv, table, qc, kc, of, heads, lens)
+    q, k, v = qkv64.view(b, n, 3, heads, hd).permute(2, 0, 3, 1, 4)
+    bucket = of.long()[(qc.long()[:, None] - kc.long()[None]).clamp(0, of.numel() - 1)]
+    real = (bucket >= 0) & (bucket < table.shape[0])
+    bias = torch.where(real, table.double()[bucket.clamp(0, table.shape[0] - 1)].permute(2, 0, 1), 0.0)
+    do4 = do64.view(b, n, heads, hd).transpose(1, 2)
+    (o, dq, dk, dv, ds, p), es = _attention64(q, k, v, bias, live, live.double(), do4)
+
+    def flat(t):
+        return t.transpose(1, 2).reshape(b, n, heads * hd)
+
+    _within(out, flat(o), flat(es[0]), "out")
+    _within(only, flat(o), flat(es[0]), "out without gradients")
+    for i, (name, w, e) in enumerate((("dq", dq, es[1]), ("dk", dk, es[2]), ("dv", dv, es[3]))):
+        _within(dqkv[..., i * heads * hd:(i + 1) * heads * hd], flat(w), flat(e), name)
+    # the table's gradient is kept in 32 bits: P and O come in two halves (2^-16 each), the sums have up to n * b terms
+    err = p * (2.0 ** -15 * (do4.abs() * (o.abs() + p @ v.abs())).sum(-1, keepdim=True) + SLACK / 8 * (do4.abs() @ v.abs().transpose(-1, -2)))
+
+    def by_bucket(t):
+        z = torch.zeros(table.shape[0], heads, dtype=torch.float64, device=t.device)
+        return z.index_add_(0, bucket.clamp(0, table.shape[0] - 1).reshape(-1), (t.sum(0) * real).reshape(heads, -1).t().contiguous())
+
+    _within(dtable, by_bucket(ds), by_bucket(err) + 2.0 ** -20 * by_bucket(ds.abs()), "dtable")
+    return out, dqkv, dtable
+
+
+def _check_cross(device, b, nq, nk, heads, kv_heads, hd, lengths=None, seed=0, poison=False, grads=True):
+    g = torch.Generator().manual_seed(seed)
+    q = _rand(g, b, nq, heads * hd, device=device)
+    kv = _rand(g, b, nk, 2 * kv_heads * hd, device=device)
+    do = _rand(g, b, nq, heads * hd, std=0.1, device=device)
+    live = _live(lengths, b, nk, device)
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=device)
+    kv64 = kv.double() * live[..., None]
+    if poison:
+        kv = kv.masked_fill(~live[..., None], math.nan)
+    q4 = q.double().view(b, nq, heads, hd).transpose(1, 2)
+    k1, v1 = kv64.view(b, nk, 2, kv_heads, hd).permute(2, 0, 3, 1, 4)
+    k4, v4 = (t.repeat_interleave(heads // kv_heads, 1) for t in (k1, v1))
+    rows = torch.ones(b, nq, dtype=torch.float64, device=device)
+    (o, dq, dk, dv, _, _), es = _attention64(q4, k4, v4, None, live, rows, do.double().view(b, nq, heads, hd).transpose(1, 2))
+
+    def flat(t):
+        return t.transpose(1, 2).reshape(b, nq, heads * hd)
+
+    def shared(t):  # the query heads of a key head add up
+        return t.view(b, kv_heads, -1, nk, hd).sum(2).transpose(1, 2).reshape(b, nk, kv_heads * hd)
+
+    with torch.no_grad():
+        _within(F.cross_attention(q, kv, heads, kv_heads, lens), flat(o), flat(es[0]), "out without gradients")
+    if not grads:
+        return
+    ql, kl = q.clone().requires_grad_(), kv.clone().requires_grad_()
+    out = F.cross_attention(ql, kl, heads, kv_heads, lens)
+    gq, gkv = torch.autograd.grad(out, [ql, kl], do)
+    _within(out, flat(o), flat(es[0]), "out")
+    _within(gq, flat(dq), flat(es[1]), "dq")
+    w = kv_heads * hd
+    _within(gkv[..., :w], shared(dk), shared(es[2]), "dk")
+    _within(gkv[..., w:], shared(dv), shared(es[3]), "dv")
+    return out, gq, gkv
+
+
+def _check_norm(device, shape, per_sample, post, scale, seed=0, only=None):
+    g = torch.Generator().manual_seed(seed)
+    d = shape[-1]
+    x, y = _rand(g, *shape, std=2.0, device=device), _rand(g, *shape, device=device)
+    du, dn = _rand(g, *shape, std=0.1, device=device), _rand(g, *shape, std=0.1, device=device)
+    gate = _rand(g, *((shape[0], d) if per_sample else (d,)), std=0.5, dtype=torch.float32, device=device)
+    ps = [1 + _rand(g, d, std=0.2, dtype=torch.float32, device=device) if i % 2 == 0 else _rand(g, d, dtype=torch.float32, device=device)
+          for i in range(4 if post else 2)]
+    leaves = [t.clone().requires_grad_() for t in (x, y, gate, *ps)]
+    new, normed = F.gated_residual_norm(*leaves[:5], 1e-6, *(leaves[5:] if post else ()), residual_scale=scale)
+    with torch.no_grad():
+        again = F.gated_residual_norm(x, y, gate, *ps[:2], 1e-6, *(ps[2:] if post else ()), residual_scale=scale)
+    assert torch.equal(again[0], new) and torch.equal(again[1], normed)
+    w64 = [t.detach().double().requires_grad_() for t in leaves]
+    X, Y, G, W, Bi = w64[:5]
+    z = torch.nn.functional.layer_norm(Y, (d,), w64[5], w64[6], 1e-6) if post else Y
+    Gb = G.view(shape[0], *[1] * (len(shape) - 2), d) if per_sample else G
+    u = scale * X + Gb * z
+    n = torch.nn.functional.layer_norm(u, (d,), W, Bi, 1e-6)
+    outs, gs = (new, normed), (du, dn)
+    if only is not None:
+        outs, gs, u_n, g64 = (outs[only],), (gs[only],), ((u, n)[only],), (gs[only].double(),)
+    else:
+        u_n, g64 = (u, n), (du.double(), dn.double())
+    got = torch.autograd.grad(outs, leaves, gs, allow_unused=True)
+    want = torch.autograd.grad(u_n, w64, g64, allow_unused=True)
+    # one rounding of each bf16 output; 32-bit work on rows of d terms is off by some 2^-24 * sqrt(d) of the row's largest
+    # value, times 1 / deviation where a norm divides by it: 2^-17 of the row's largest output covers widths up to 2048
+    for name, a, b in (("x_new", new, u), ("normed", normed, n)):
+        b = b.detach()
+        _within(a, b, U * b.abs() + 2.0 ** -17 * b.abs().amax(-1, keepdim=True), name)
+    names = ("dx", "dbranch", "dgate", "dweight", "dbias", "dpost_weight", "dpost_bias")
+    rows = math.prod(shape[:-1])
+    for i, (name, a, b) in enumerate(zip(names, got, want)):
+        if b is None or a is None:
+            assert b is None or not b.abs().max() > 0, name
+            assert a is None or not a.abs().max() > 0, name
+            continue
+        if i < 2:
+            _within(a, b, U * b.abs() + 2.0 ** -16 * b.abs().amax(-1, keepdim=True), name)
+        else:  # sums over the rows in 32 bits of terms whose own error is 2^-17 of the largest
+            _within(a, b, 2.0 ** -17 * b.abs().max() + 2.0 ** -17 * math.sqrt(rows) * 0.2 + TINY, name)
+
+
+def _grid(side):
+    return pdt.nn.grid_position_buckets(side, side, prefix=1)
+
+
+def _log(n, far=16, buckets=8):
+    return pdt.nn.log_position_buckets(n, buckets, far)
+
+
+# ------------------------------------------------------------------------------------------------- on the CPU
+def test_grid_position_buckets():
+    q, k, of = pdt.nn.grid_position_buckets(3, 2, prefix=1)
+    assert of.tolist() == list(range(5 * 3 + 3))
+    b = of[(q[:, None] - k[None]).clamp(0, of.numel() - 1).long()]
+    yx = [(i // 2, i % 2) for i in range(6)]
+    seen = {}
+    for i, (yi, xi) in enumerate(yx):
+        for j, (yj, xj) in enumerate(yx):
+            seen.setdefault(int(b[i + 1, j + 1]), set()).add((yi - yj, xi - xj))
+    assert len(seen) == 15 and all(len(v) == 1 for v in seen.values())
+    prefix = {int(b[0, 0])}, set(b[0, 1:].tolist()), set(b[1:, 0].tolist())
+    assert all(len(s) == 1 for s in prefix) and len(set.union(*prefix, set(seen))) == 18
+
+
+def test_log_position_buckets():
+    q, k, of = pdt.nn.log_position_buckets(300, 32, 128)
+    b = of[(q[:, None] - k[None]).clamp(0, of.numel() - 1).long()]
+    assert b[10, 10] == 0 and b[10, 3] == 7 and b[10, 11] == 17 and b[299, 0] == 15 and b[0, 299] == 31
+    assert b.min() == 0 and b.max() == 31 and (torch.diff(b[299].flip(0)[:200]) >= 0).all()
+    q, k, of = pdt.nn.log_position_buckets(40, 32, 128, bidirectional=False)
+    b = of[(q[:, None] - k[None]).clamp(0, of.numel() - 1).long()]
+    assert (b.triu() == 0).all() and b[20, 5] == 15 and b[39, 0] > 16
+
+
+CPU_REL = [dict(b=2, codes=_grid(3), heads=2, hd=8), dict(b=4, codes=_log(17), heads=3, hd=4, lengths=[17, 9, 1, 0], poison=True)]
+
+
+@pytest.mark.parametrize("case", CPU_REL)
+def test_rel_bias_attention_oracle(case):
+    _check_rel(_dev("cpu"), **case)
+
+
+@pytest.mark.parametrize("case", [dict(b=2, nq=5, nk=7, heads=4, kv_heads=2, hd=8),
+                                  dict(b=3, nq=1, nk=9, heads=3, kv_heads=1, hd=4, lengths=[9, 4, 0], poison=True)])
+def test_cross_attention_oracle(case):
+    _check_cross(_dev("cpu"), **case)
+
+
+@pytest.mark.parametrize("per_sample,post", [(False, True), (True, False), (True, True)])
+def test_gated_residual_norm_oracle(per_sample, post):
+    _check_norm(_dev("cpu"), (3, 5, 20), per_sample, post, 0.5)
+
+
+def test_gradients_against_differences():
+    """Central differences in 64 bits through the oracle's formulas."""
+    g = torch.Generator().manual_seed(3)
+
+    def r(*s):
+        return torch.randn(*s, generator=g, dtype=torch.float64).requires_grad_()
+
+    qc, kc, of = _grid(2)
+    lens = torch.tensor([5, 3])
+    assert torch.autograd.gradcheck(lambda a, t: F.rel_bias_attention(a, t, qc, kc, of, 2, lens), (r(2, 5, 24), r(int(of.max()) + 1, 2)))
+    assert torch.autograd.gradcheck(lambda a, b: F.cross_attention(a, b, 4, 2, lens), (r(2, 3, 16), r(2, 6, 16)))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_refusals(device):
+    dev = _dev(device)
+    qc, kc, of = (t.to(dev) for t in _grid(2))
+    qkv, table = torch.zeros(2, 5, 96, dtype=torch.bfloat16, device=dev), torch.zeros(12, 1, device=dev)
+
+    def rel(qkv=qkv, table=table, qc=qc, kc=kc, of=of, heads=1, lens=None):
+        return F.rel_bias_attention(qkv, table, qc, kc, of, heads, lens)
+
+    assert rel().shape == (2, 5, 32)
+    lens = torch.tensor([5, 2], device=dev)
+    assert rel(lens=lens).shape == (2, 5, 32)
+    for bad in (dict(qkv=qkv[0]), dict(heads=5), dict(heads=0), dict(table=table[:, 0]), dict(table=table.expand(12, 3)), dict(qc=qc[:4]),
+                dict(kc=kc[None]), dict(of=of[:0]), dict(qc=qc.float()), dict(lens=lens[:1]), dict(lens=lens.float())):
+        with pytest.raises(ValueError):
+            rel(**bad)
+    q, kv = torch.zeros(2, 3, 64, dtype=torch.bfloat16, device=dev), torch.zeros(2, 7, 64, dtype=torch.bfloat16, device=dev)
+    assert F.cross_attention(q, kv, 2, 1).shape == q.shape
+    for bad in ((q, kv, 2, 3), (q, kv, 0, 1), (q, kv, 2, 2), (q[:1], kv, 2, 1), (q[0], kv[0], 2, 1), (q.float(), kv, 2, 1),
+                (q, kv, 2, 1, lens[:1]), (q, kv, 3, 1)):
+        with pytest.raises(ValueError):
+            F.cross_attention(*bad)
+    x, v = torch.zeros(2, 3, 8, dtype=torch.bfloat16, device=dev), torch.ones(8, device=dev)
+    assert F.gated_residual_norm(x, x, v, v, v)[0].shape == x.shape
+    for bad in ((x, x[:1], v, v, v), (x, x.float(), v, v, v), (x, x, v[:4], v, v), (x, x, v.expand(3, 8), v, v), (x, x, v, v[:4], v),
+                (x, x, v, v, v, 1e-6, v), (x, x, v, v, v, 1e-6, v, v[:1])):
+        with pytest.raises(ValueError):
+            F.gated_residual_norm(*bad)
+    if device == "cuda":
+        for bad in (dict(lens=lens.cpu()), dict(table=table.cpu()), dict(of=of.cpu())):
+            with pytest.raises(ValueError):
+                rel(**bad)
+
+
+# ------------------------------------------------------------------------------------------------- on the GPU
+REL = [
+    dict(b=1, codes=_log(1), heads=1, hd=64), dict(b=2, codes=_log(2), heads=2, hd=32), dict(b=3, codes=_grid(2), heads=3, hd=128),
+    dict(b=2, codes=_log(31), heads=2, hd=64), dict(b=2, codes=_log(32), heads=1, hd=32), dict(b=2, codes=_log(33), heads=1, hd=128),
+    dict(b=2, codes=_log(63), heads=3, hd=64), dict(b=1, codes=_log(64), heads=2, hd=64), dict(b=2, codes=_log(65), heads=2, hd=128),
+    dict(b=2, codes=_log(129, 200, 32), heads=2, hd=64), dict(b=3, codes=_grid(14), heads=3, hd=64), dict(b=2, codes=_grid(15), heads=2, hd=64),
+    dict(b=300, codes=_grid(4), heads=2, hd=64), dict(b=2, codes=_grid(24), heads=2, hd=64), dict(b=1, codes=_grid(17), heads=2, hd=32),
+    dict(b=5, codes=_grid(14), heads=2, hd=64, lengths=[197, 0, 1, 64, 130], poison=True),
+    dict(b=4, codes=_log(300, 64, 32), heads=2, hd=128, lengths=[300, 2, 0, 257], poison=True),
+    dict(b=4, codes=_log(100, 20, 8), heads=3, hd=32, lengths=[33, 100, 96, 1], poison=True),
+    dict(b=1, codes=_log(2049, 128, 32), heads=1, hd=64), dict(b=2, codes=_log(1100, 2000, 32), heads=1, hd=128, lengths=[1100, 700]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", REL, ids=lambda c: f"b{c['b']}-n{c['codes'][0].numel()}-h{c['heads']}x{c['hd']}{'-ragged' if 'lengths' in c else ''}")
+def test_rel_bias_attention(case):
+    before = dict(F.fallback_counts)
+    _check_rel(_dev("cuda"), **case)
+    assert dict(F.fallback_counts) == before
+
+
+@gpu
+def test_rel_bias_forbidden_lowest_and_unnamed_entries():
+    """-inf entries forbid pairs (a row may lose every key), the lowest finite value beats nothing but itself, and an entry
+    that names no bucket adds nothing and gets no gradient."""
+    dev = _dev("cuda")
+    n, heads, hd = 70, 2, 64
+    qc, kc = torch.arange(n) + n, torch.arange(n)
+    of = torch.zeros(2 * n + 1, dtype=torch.int64)
+    of[:n] = 1                      # keys after the query
+    of[n + 5] = 2
+    of[n + 9], of[n + 11] = -1, 77  # no such buckets
+    table = torch.tensor([[0.3, -0.2], [-math.inf, 1.0], [torch.finfo(torch.float32).min, 0.5]])
+    out, dqkv, dtable = _check_rel_inf(dev, (qc, kc, of), heads, hd, table)
+    assert dtable[1, 0] == 0
+    # every key forbidden: zeros, and no gradients
+    gone = torch.full((1, heads), -math.inf)
+    g = torch.Generator().manual_seed(5)
+    qkv = _rand(g, 1, n, 3 * heads * hd, device=dev).requires_grad_()
+    t = gone.to(dev).requires_grad_()
+    zero = torch.zeros_like(of).to(dev)
+    o = F.rel_bias_attention(qkv, t, qc.to(dev), kc.to(dev), zero, heads)
+    gs = torch.autograd.grad(o, [qkv, t], torch.ones_like(o))
+    assert not o.any() and not gs[0].any() and not gs[1].any()
+    # every key at the lowest value: as without a bias
+    low = torch.full((1, heads), torch.finfo(torch.float32).min).to(dev)
+    none = torch.zeros((1, heads)).to(dev)
+    with torch.no_grad():
+        a = F.rel_bias_attention(qkv, low, qc.to(dev), kc.to(dev), zero, heads)
+    v = qkv.detach()[..., 2 * heads * hd:].double().mean(1, keepdim=True)
+    assert (a.double() - v).abs().max() < 2 * U * qkv.detach().abs().max()  # equal weights: absorbed scores
+    assert torch.isfinite(F.rel_bias_attention(qkv, none, qc.to(dev), kc.to(dev), zero, heads)).all()
+
+
+def _check_rel_inf(dev, codes, heads, hd, table):
+    """`_check_rel` with -inf and lowest entries in the table: the 64-bit form takes them as they are (head 0, buckets 1 and 2)."""
+    return _check_rel(dev, 2, codes, heads, hd, table=table)
+
+
+CROSS = [
+    dict(b=1, nq=1, nk=1, heads=1, kv_heads=1, hd=64), dict(b=2, nq=1, nk=33, heads=4, kv_heads=2, hd=32),
+    dict(b=2, nq=3, nk=64, heads=8, kv_heads=1, hd=128), dict(b=3, nq=7, nk=31, heads=2, kv_heads=2, hd=64),
+    dict(b=2, nq=33, nk=100, heads=2, kv_heads=1, hd=64), dict(b=2, nq=130, nk=65, heads=6, kv_heads=2, hd=32),
+    dict(b=1, nq=64, nk=1000, heads=2, kv_heads=1, hd=128), dict(b=1, nq=1, nk=3000, heads=2, kv_heads=2, hd=64),
+    dict(b=1, nq=1, nk=5001, heads=8, kv_heads=2, hd=128), dict(b=1, nq=600, nk=40, heads=3, kv_heads=1, hd=64),
+    dict(b=4, nq=5, nk=500, heads=3, kv_heads=1, hd=64, lengths=[500, 0, 1, 77], poison=True),
+    dict(b=3, nq=50, nk=300, heads=4, kv_heads=4, hd=32, lengths=[64, 300, 0], poison=True),
+    dict(b=2, nq=1, nk=4000, heads=4, kv_heads=1, hd=128, lengths=[17, 4000], poison=True),
+    dict(b=70, nq=1, nk=197, heads=12, kv_heads=12, hd=64), dict(b=2, nq=11, nk=45, heads=9, kv_heads=3, hd=32, lengths=[45, 1]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", CROSS, ids=lambda c: f"b{c['b']}-{c['nq']}x{c['nk']}-h{c['heads']}of{c['kv_heads']}x{c['hd']}{'-ragged' if 'lengths' in c else ''}")
+def test_cross_attention(case):
+    before = dict(F.fallback_counts)
+    _check_cross(_dev("cuda"), **case)
+    assert dict(F.fallback_counts) == before
+
+
+NORM = [((1, 1, 4), False, True, 1.0), ((3, 5, 36), True, True, 0.5), ((2, 197, 192), False, True, 1.0), ((7, 768), True, False, 1.0),
+        ((4, 33, 1024), True, False, 0.5), ((5, 3, 11, 260), True, True, 0.9), ((2, 9, 2048), False, True, 1.0), ((2, 65, 1300), True, True, 1.0),
+        ((1, 2100, 64), True, False, 1.0), ((1300, 2, 40), True, True, 1.0), ((3, 700, 516), False, False, 1.0)]
+
+
+@gpu
+@pytest.mark.parametrize("case", NORM, ids=str)
+def test_gated_residual_norm(case):
+    before = dict(F.fallback_counts)
+    _check_norm(_dev("cuda"), *case)
+    assert dict(F.fallback_counts) == before
+
+
+@gpu
+@pytest.mark.parametrize("only", [0, 1])
+def test_gated_residual_norm_with_one_gradient(only):
+    _check_norm(_dev("cuda"), (2, 37, 128), True, True, 1.0, only=only)
+
+
+@gpu
+def test_empty_inputs():
+    dev = _dev("cuda")
+    qc, kc, of = (t.to(dev) for t in _log(5))
+    t = torch.ones(8, 2, device=dev, requires_grad=True)
+    e = torch.zeros(0, 5, 192, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    o = F.rel_bias_attention(e, t, qc, kc, of, 2)
+    g = torch.autograd.grad(o, [e, t], torch.zeros_like(o))
+    assert o.shape == (0, 5, 64) and g[0].shape == e.shape and not g[1].any()
+    e = torch.zeros(2, 0, 192, dtype=torch.bfloat16, device=dev)
+    assert F.rel_bias_attention(e, t.detach(), qc[:0], kc[:0], of, 2).shape == (2, 0, 64)
+    q = torch.ones(2, 3, 64, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    kv = torch.zeros(2, 0, 128, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    o = F.cross_attention(q, kv, 2)
+    gq, gkv = torch.autograd.grad(o, [q, kv], torch.ones_like(o))
+    assert not o.any() and not gq.any() and gkv.shape == kv.shape
+    kv = torch.ones(2, 9, 128, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    o = F.cross_attention(q[:, :0], kv, 2)
+    assert o.shape == (2, 0, 64) and not torch.autograd.grad(o, kv, torch.ones_like(o))[0].any()
+    x = torch.zeros(0, 3, 64, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    v = torch.ones(64, device=dev, requires_grad=True)
+    a, b = F.gated_residual_norm(x, x, v, v, v)
+    assert a.shape == x.shape and not torch.autograd.grad(b, v, torch.zeros_like(b))[0].any()
+
+
+@gpu
+def test_views_other_types_and_alignment():
+    """Rows inside a wider tensor, an expanded batch, misaligned slices, int64 codes and lengths, a bf16 table."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(1)
+    wide = _rand(g, 2, 50, 64 + 192 + 64, device=dev)
+    qc, kc, of = (t.to(dev) for t in _log(50))
+    table = _rand(g, 8, 1, dtype=torch.float32, device=dev)
+    view = wide[:, :, 64:256]
+    args = (table, qc, kc, of, 1)
+    with torch.no_grad():
+        want = F.rel_bias_attention(view.contiguous(), *args)
+        assert torch.equal(F.rel_bias_attention(view, *args), want)
+        assert torch.equal(F.rel_bias_attention(wide[:, :, 63:255], *args), F.rel_bias_attention(wide[:, :, 63:255].contiguous(), *args))
+        assert torch.equal(F.rel_bias_attention(view.transpose(0, 1).contiguous().transpose(0, 1), *args), want)
+        assert torch.equal(F.rel_bias_attention(view, table, qc.long(), kc.long(), of.long(), 1, torch.tensor([50, 50], device=dev)), want)
+        lens = torch.tensor([9, 50, 3], dtype=torch.int32, device=dev)[1:]
+        a = F.rel_bias_attention(view, *args, lens)
+        assert torch.equal(a, F.rel_bias_attention(view, *args, lens.clone()))
+        one = view[:1].expand(2, -1, -1)
+        assert torch.equal(F.rel_bias_attention(one, *args)[1], want[0])
+        q, kv = wide[:, :7, :128], wide[:, :, 64:320]
+        want = F.cross_attention(q.contiguous(), kv.contiguous(), 2)
+        assert torch.equal(F.cross_attention(q, kv, 2), want)
+        assert torch.equal(F.cross_attention(q[:, ::2], kv[:, ::3], 2), F.cross_attention(q[:, ::2].contiguous(), kv[:, ::3].contiguous(), 2))
+        x = wide[:, :, 3:71]
+        v = _rand(g, 69, dtype=torch.float32, device=dev)[1:]
+        a = F.gated_residual_norm(x, x, v, v, v)
+        b = F.gated_residual_norm(x.contiguous(), x.contiguous(), v.clone(), v.clone(), v.clone())
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    t = table.bfloat16().requires_grad_()
+    o = F.rel_bias_attention(view, t, qc, kc, of, 1)
+    (gt,) = torch.autograd.grad(o, t, torch.ones_like(o))
+    assert gt.dtype == torch.bfloat16
+    # gradients of views and of broadcast inputs
+    base = wide.clone().requires_grad_()
+    o = F.rel_bias_attention(base[:, :, 64:256], *args)
+    (gb,) = torch.autograd.grad(o, base, torch.ones_like(o).expand_as(o))
+    leaf = view.clone().requires_grad_()
+    (gl,) = torch.autograd.grad(F.rel_bias_attention(leaf, *args), leaf, torch.ones_like(o))
+    assert torch.equal(gb[:, :, 64:256], gl) and not gb[:, :, :64].any() and not gb[:, :, 256:].any()
+
+
+@gpu
+def test_types_without_a_kernel_are_counted():
+    dev = _dev("cuda")
+    before = sum(F.fallback_counts.values())
+    q, kv = torch.randn(2, 3, 64, device=dev), torch.randn(2, 5, 128, device=dev)
+    F.cross_attention(q, kv, 1)
+    F.cross_attention(q.bfloat16(), kv.bfloat16(), 4)  # head_dim 16
+    F.gated_residual_norm(q, q, q[0, 0], q[0, 0], q[0, 0])
+    qc, kc, of = (t.to(dev) for t in pdt.nn.grid_position_buckets(33, 33))
+    F.rel_bias_attention(torch.zeros(1, qc.numel(), 96, dtype=torch.bfloat16, device=dev), torch.zeros(int(of.max()) + 1, 1, device=dev), qc, kc, of, 1)
+    assert sum(F.fallback_counts.values()) == before + 4
+
+
+def _chain(dev, seed):
+    """The operators as a model uses them: self attention with positions, a block end, cross attention, a block end."""
+    g = torch.Generator().manual_seed(seed)
+    b, n, m, heads, hd = 3, 50, 70, 2, 64
+    d = heads * hd
+    qc, kc, of = (t.to(dev) for t in _grid(7))
+    p = dict(qkv=_rand(g, b, n, 3 * d, device=dev), table=_rand(g, int(of.max()) + 1, heads, dtype=torch.float32, device=dev),
+             x=_rand(g, b, n, d, device=dev), kv=_rand(g, b, m, 2 * d, device=dev), g1=_rand(g, d, dtype=torch.float32, device=dev),
+             g2=_rand(g, b, d, dtype=torch.float32, device=dev), w=1 + _rand(g, d, std=0.1, dtype=torch.float32, device=dev),
+             bias=_rand(g, d, dtype=torch.float32, device=dev))
+    lens = torch.tensor([70, 33, 0], dtype=torch.int32, device=dev)
+
+    def step(p):
+        y = F.rel_bias_attention(p["qkv"], p["table"], qc, kc, of, heads)
+        x, h = F.gated_residual_norm(p["x"], y, p["g1"], p["w"], p["bias"], 1e-6, p["w"], p["bias"])
+        y = F.cross_attention(h, p["kv"], heads, None, lens)
+        x, h = F.gated_residual_norm(x, y, p["g2"], p["w"], p["bias"])
+        return [h, *torch.autograd.grad([x, h], list(p.values()), [torch.ones_like(x), torch.ones_like(h)])]
+
+    return {k: v.requires_grad_() for k, v in p.items()}, step
+
+
+@gpu
+def test_chain_against_the_oracle_and_bit_for_bit():
+    dev = _dev("cuda")
+    p, step = _chain(dev, 0)
+    a, b = step(p), step(p)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    from pytorch_distributed_training_amd import ops
+    ops.set_force_reference(True)
+    try:
+        want = step(p)
+    finally:
+        ops.set_force_reference(False)
+    for x, y in zip(a, want):  # a chain of four operators with a handful of roundings each: 2^-8 * 8 in the 2-norm
+        assert (x.double() - y.double()).norm() <= 8 * U * y.double().norm()
+
+
+@gpu
+def test_captured_and_replayed_chain():
+    dev = _dev("cuda")
+    p, step = _chain(dev, 1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(p)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(p)
+        graphs.append((graph, outs))
+    for seed in range(3):
+        fresh, _ = _chain(dev, 10 + seed)
+        with torch.no_grad():
+            for k in p:
+                p[k].copy_(fresh[k])
+        want = [t.clone() for t in step(p)]
+        for graph, outs in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, outs in graphs:
+            assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+@gpu
+def test_two_streams_at_once():
+    dev = _dev("cuda")
+    jobs = [_chain(dev, 20 + i) for i in range(2)]
+    want = [[t.clone() for t in step(p)] for p, step in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [None, None]
+    for _ in range(5):
+        for i, (s, (p, step)) in enumerate(zip(streams, jobs)):
+            with torch.cuda.stream(s):
+                got[i] = step(p)
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert all(torch.equal(a, b) for a, b in zip(x, y))
+
+
+@gpu
+def test_keys_past_32_bit_offsets():
+    """A cache of more than 2^32 bytes for one sequence: the last keys are read, and nothing behind the length."""
+    dev = _dev("cuda")
+    heads, hd, n = 8, 128, 1_100_003
+    kv = torch.zeros(1, n, 2 * heads * hd, dtype=torch.bfloat16, device=dev)
+    assert kv.numel() * 2 > 2 ** 32
+    q = torch.ones(1, 1, heads * hd, dtype=torch.bfloat16, device=dev)
+    kv[0, n - 2, :heads * hd] = 2.0  # score 2 * 128 / sqrt(128) = 22.6: e^22.6 = 6.6e9 against 1.1e6 others
+    kv[0, n - 2, heads * hd:] = 3.0
+    kv[0, n - 1] = math.nan
+    lens = torch.tensor([n - 1], dtype=torch.int32, device=dev)
+    share = 1 / (1 + (n - 2) * math.exp(-2 * 128 / math.sqrt(128)))
+    with torch.no_grad():
+        out = F.cross_attention(q, kv, heads, None, lens)
+        wide = F.cross_attention(q.expand(1, 40, -1), kv, heads, None, lens)  # the kernel for more rows
+    for o in (out, wide):
+        assert (o.double() - 3 * share).abs().max() <= 3 * (2 * U + SLACK)
