@@ -131,7 +131,7 @@ Tensor ext_bwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, const Ten
     w.q = ext_plan_bwd(BH, a.M, a.Sk);
     w.kv = ext_plan_bwd(BH, a.Sk, a.M);
     check_grid(a, w.q); check_grid(a, w.kv);
-    Tensor dsum = at::empty({BH, a.Mp}, f32), pq, pk, pv, slab, mid;
+    Tensor dsum = at::empty({BH, a.Mp}, f32), pq, pk, pv;
     w.dsum = dsum.data_ptr<float>();
     if (w.q.splits > 1) {
         pq = at::empty({BH * w.q.splits * a.M * hd}, f32);
@@ -143,17 +143,13 @@ Tensor ext_bwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, const Ten
         w.part_k = pk.data_ptr<float>();
         w.part_v = pv.data_ptr<float>();
     }
-    const int per_head = w.q.tiles * w.q.splits;
-    if (dtable.defined()) {
-        slab = at::empty({BH * per_head, a.Rp}, f32);
-        w.slab = slab.data_ptr<float>();
-    }
     launch_ext_bwd(a, w, (int)hd, stream_of(q));
     if (dtable.defined() && NB > 0) {
-        const int chunks = bias_grad_chunks(a.B * per_head);
-        mid = at::empty({chunks, (long)heads, a.Rp}, f32);
-        launch_bias_grad(w.slab, mid.data_ptr<float>(), bucket_of->data_ptr<int>(), dtable.data_ptr<float>(), a.R, a.Rp, (int)NB,
-                         (int)heads, a.B, per_head, chunks, stream_of(q));
+        const RelPlan p = rel_plan(a.B, a.Hkv, a.Sk);
+        Tensor dense = at::empty({p.dense}, f32), slab = at::empty({(long)heads * p.rows, a.Rp}, f32),
+               mid = at::empty({p.mid, (long)heads, a.Rp}, f32);
+        launch_rel_bias_grad(a, w, (int)hd, p, dense.data_ptr<float>(), slab.data_ptr<float>(), mid.data_ptr<float>(),
+                             bucket_of->data_ptr<int>(), dtable.data_ptr<float>(), (int)NB, stream_of(q));
     }
     return dtable;
 }

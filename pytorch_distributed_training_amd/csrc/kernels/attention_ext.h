@@ -6,7 +6,7 @@
 
 namespace pdt {
 
-constexpr int kExtMaxEntries = 4096;  // entries of a relative-position table a head keeps in LDS, five times in the backward
+constexpr int kExtMaxEntries = 4096;  // entries of a relative-position table a head keeps in LDS
 
 // rows of a [B, rows, heads, hd] tensor: element strides, and the division of a row by the heads that share a key head
 struct ExtView {
@@ -34,7 +34,7 @@ struct ExtBwd {
     const float* stat;
     float* dsum;
     void *dq, *dk, *dv;
-    float *part_q, *part_k, *part_v, *slab;
+    float *part_q, *part_k, *part_v;
     ExtPlan q, kv;
 };
 
@@ -45,8 +45,19 @@ void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, void*
 void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s);
 void launch_bias_tables(const float* table, const int* bucket_of, const int* q_codes, const int* k_codes, float* tab, int* q4,
                         int* k4, int R, int Rp, int NB, int H, int S, int Sp, float inv_scale, hipStream_t s);
-int bias_grad_chunks(int rows);
-void launch_bias_grad(const float* slab, float* mid, const int* bucket_of, float* dtable, int R, int Rp, int NB, int H, int B,
-                      int per_head, int chunks, hipStream_t s);
+// the bias table's gradient: after launch_ext_bwd (which leaves D in dsum)
+struct RelBlocks {
+    int h0, heads, q0, qblocks, kblocks;  // of this launch: heads, blocks of 128 queries; blocks of 128 keys of all
+    int chunks, slab_rows;                // parts of the batch; rows of a head in the slab of entries
+};
+struct RelPlan {
+    int heads, qblocks, chunks;  // of a launch
+    int parts, rows, mid;        // ranges of key tiles; slab rows per head; partial rows of the slab's sum
+    long dense;                  // floats: sums of dS by pair
+};
+RelPlan rel_plan(int B, int H, int S);
+// dense [plan.dense], slab [H][plan.rows][Rp], mid [plan.mid][H][Rp]
+void launch_rel_bias_grad(const ExtArgs& a, const ExtBwd& w, int hd, const RelPlan& p, float* dense, float* slab, float* mid,
+                          const int* bucket_of, float* dtable, int NB, hipStream_t s);
 
 }  // namespace pdt

@@ -22,8 +22,9 @@
 //    length are sent out of range and arrive as zeros, so whatever they hold (NaN, infinities) is never multiplied.
 //  * Few rows: the streamed axis is cut into `splits`, each with its own workgroup and an fp32 partial that a small kernel
 //    joins in a fixed order.
-//  * No atomics in memory: the bias gradient is added up in a histogram per WAVE in LDS (program order), the waves and the
-//    workgroups are summed in a fixed order.
+//  * No atomics in memory: the bias gradient sums dS over the batch in registers first (a kernel of its own, which walks over
+//    the batch with a block of pairs fixed), then the pairs by entry in a histogram per WAVE in LDS (program order), then waves
+//    and workgroups in a fixed order.
 #include <cmath>
 
 #include "attn_tile.h"
@@ -544,24 +545,22 @@ __device__ __forceinline__ void store_acc32(const f32x16* t, float* dst, int hal
         }
 }
 
-// Row owner: dQ, D for the key owner (written by split 0) and the histogram of dS over the table's entries.  A softmax over
-// one key is constant, so with len = 1 dS is zero, and is set so (as a difference of two rounded numbers it would not be).
+// Row owner: dQ, and D for the key owner (written by split 0).  A softmax over one key is constant, so with len = 1 dS is
+// zero, and is set so (as a difference of two rounded numbers it would not be).
 template <int HD, bool BIAS>
 __global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ out_lo,
                                                    const bf16* __restrict__ dout, const float* __restrict__ stat,
-                                                   float* __restrict__ dsum, bf16* __restrict__ dq, float* __restrict__ part,
-                                                   float* __restrict__ slab, int tiles, int splits) {
+                                                   float* __restrict__ dsum, bf16* __restrict__ dq, float* __restrict__ part, int tiles,
+                                                   int splits) {
     using G = AttnGeo<HD>;
     constexpr int IMG = 64 * G::ROWBYTES;
-    extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][K, V], [2][codes 1 KiB], table [Rt], histograms [4][Rt]
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][K, V], [2][codes 1 KiB], table
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Job j = job_of(a, tiles, splits);
     const uint32_t lds0 = lds_address(smem);
     char* codes = smem + 4 * IMG;
     char* tab = smem + 4 * IMG + 2048;
-    const int Rt = (a.Rp + 255) & ~255;
-    char* hist = tab + (long)Rt * 4 * (1 + wave);
     const int r = j.tile * 128 + wave * 32 + l31;
     const bool live = r < j.rows;
     const int nb = (j.len + 63) >> 6, per = (nb + splits - 1) / splits;
@@ -586,13 +585,10 @@ __global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __rest
         if (BIAS && wave == 0) dma_words(lds0 + 4 * IMG + buf * 1024, a.k_codes4 + kb * 64, lane);
     };
     if (any) issue(kb0, 0);
-    if (BIAS) {
-        if (any) {
-            const i32x4 rsrc = uniform_rsrc(a.tab + (long)j.hkv * a.Rp, (uint32_t)a.Rp * 4u);
-            for (int p = wave; p * 256 < a.Rp; p += 4)
-                lds_dma16(rsrc, (uint32_t)(p * 1024 + lane * 16), (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + 4 * IMG + 2048 + p * 1024)));
-        }
-        for (int i = lane; i < Rt; i += 64) reinterpret_cast<float*>(hist)[i] = 0.f;
+    if (BIAS && any) {
+        const i32x4 rsrc = uniform_rsrc(a.tab + (long)j.hkv * a.Rp, (uint32_t)a.Rp * 4u);
+        for (int p = wave; p * 256 < a.Rp; p += 4)
+            lds_dma16(rsrc, (uint32_t)(p * 1024 + lane * 16), (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + 4 * IMG + 2048 + p * 1024)));
     }
     // own rows, and D from them
     bf16x8 qf[G::STEPS], gf[G::STEPS];
@@ -629,16 +625,12 @@ __global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __rest
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
                 f32x16 sc, dp;
-                int at[16];
                 if (BIAS) {
 #pragma unroll
                     for (int jj = 0; jj < 4; ++jj) {
                         const i32x4 kc = *reinterpret_cast<const i32x4*>(codes + buf * 1024 + (kt * 32 + 8 * jj + 4 * half) * 4);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            at[4 * jj + e] = bias_at(qc, kc[e], top4);
-                            sc[4 * jj + e] = *reinterpret_cast<const float*>(tab + at[4 * jj + e]) - mq;
-                        }
+                        for (int e = 0; e < 4; ++e) sc[4 * jj + e] = *reinterpret_cast<const float*>(tab + bias_at(qc, kc[e], top4)) - mq;
                     }
                 }
 #pragma unroll
@@ -658,11 +650,6 @@ __global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __rest
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, -lq)) * keep;
-                if (BIAS && slab) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        __hip_atomic_fetch_add(reinterpret_cast<float*>(hist + at[i]), dp[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                }
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
                     const bf16x8 ds = acc_to_a(dp, blk);
@@ -673,24 +660,177 @@ __global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __rest
             }
         }
     }
-    if (BIAS && slab) {
-        __syncthreads();
-        float* dst = slab + (((long)j.bh * tiles + j.tile) * splits + j.split) * a.Rp;
-        for (int i = tid; i < a.Rp; i += 256) {
-            float s = 0.f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) s += reinterpret_cast<const float*>(tab)[(long)Rt * (1 + w) + i];
-            dst[i] = s;
-        }
-    }
     if (r >= a.M) return;
     if (splits > 1) store_acc32<HD>(acc, part + (((long)j.bh * splits + j.split) * a.M + r) * HD, half);
     else store_acc<HD>(acc, dq + (long)j.b * a.dqv.bs + row_offset(a.dqv, r, j.hkv, a.G, HD), a.scale, half);
 }
 
+// dS summed over a part of the batch, for 128 queries x 128 keys of a head a workgroup (a wave: 32 queries, four tiles of 32
+// keys).  The bias of the block and the sums stay in registers while the batch streams through, so a pair costs two
+// multiply-adds and an exponential per sequence; written in register order, [tile][4][64 lanes] x 4 floats.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __restrict__ dout, const float* __restrict__ stat,
+                                                      const float* __restrict__ dsum, float* __restrict__ dense, RelBlocks w) {
+    using G = AttnGeo<HD>;
+    constexpr int IMG = 128 * G::ROWBYTES;  // as two blocks of 64 rows
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // K, V of one sequence, twice where it fits; before that the table
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int l = xcd_order((int)blockIdx.x, (int)gridDim.x);
+    const int kb = l % w.kblocks;
+    l /= w.kblocks;
+    const int qb = l % w.qblocks + w.q0;
+    l /= w.qblocks;
+    const int hl = l % w.heads, h = hl + w.h0, ch = l / w.heads;
+    const int per = (a.B + w.chunks - 1) / w.chunks, b0 = ch * per, b1 = b0 + per < a.B ? b0 + per : a.B;
+    const uint32_t lds0 = lds_address(smem);
+    const int q = qb * 128 + wave * 32 + l31, krs = (int)a.kv.rs;
+
+    // the block's bias (minus nothing yet): the table through LDS
+    f32x16 bias[4], acc[4];
+    {
+        const i32x4 rsrc = uniform_rsrc(a.tab + (long)h * a.Rp, (uint32_t)a.Rp * 4u);
+        for (int p = wave; p * 256 < a.Rp; p += 4)
+            lds_dma16(rsrc, (uint32_t)(p * 1024 + lane * 16), (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + p * 1024)));
+        const int qc = q < a.Sk ? a.q_codes4[q] : 0, top4 = (a.R - 1) * 4;
+        dma_barrier();
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = kb * 128 + kt * 32 + acc_row(i, half);
+                const int kc = key < a.Sk ? a.k_codes4[key] : 0;
+                bias[kt][i] = *reinterpret_cast<const float*>(smem + bias_at(qc, kc, top4));
+                acc[kt][i] = 0.f;
+            }
+        dma_barrier();
+    }
+    for (int b = b0; b < b1; ++b) {
+        int len = a.Sk;
+        if (a.lens) {
+            len = a.lens[b];
+            len = __builtin_amdgcn_readfirstlane(len < 0 ? 0 : len > a.Sk ? a.Sk : len);
+        }
+        if (len <= 1 || kb * 128 >= len || qb * 128 >= len) continue;  // (one key: dS is zero)
+        const long kvb = (long)b * a.kv.bs + (long)h * HD + (long)kb * 128 * krs;
+        auto off = [&](int row) { return row * krs; };
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int left = len - kb * 128 - s * 64, valid = left < 0 ? 0 : left < 64 ? left : 64;
+            const uint32_t bytes = valid ? (uint32_t)(valid - 1) * (uint32_t)krs * 2u + G::ROWBYTES : 0u;
+            dma_block<HD, 4>(lds0 + s * (IMG / 2), a.k + kvb + (long)s * 64 * krs, bytes, valid, wave, lane, off);
+            dma_block<HD, 4>(lds0 + IMG + s * (IMG / 2), a.v + kvb + (long)s * 64 * krs, bytes, valid, wave, lane, off);
+        }
+        const bool live = q < len;
+        bf16x8 qf[G::STEPS], gf[G::STEPS];
+        own_frags<HD>(qf, a.q + (long)b * a.qv.bs + (long)(live ? q : 0) * a.qv.rs + (long)h * HD, live, half);
+        own_frags<HD>(gf, dout + (long)b * a.o.bs + (long)(live ? q : 0) * a.o.rs + (long)h * HD, live, half);
+        const long sr = ((long)b * a.Hkv + h) * a.Mp + (live ? q : 0);
+        const float mq = live ? stat[sr] : 0.f, lq = live ? stat[a.stat_n + sr] : kInf, d = live ? dsum[sr] : 0.f;
+        dma_barrier();
+        if (qb * 128 + wave * 32 < len) {
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                if (kb * 128 + kt * 32 < len) {
+                    const char* Ks = smem + (kt >> 1) * (IMG / 2);
+                    const char* Vs = Ks + IMG;
+                    f32x16 sc, dp;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        sc[i] = bias[kt][i] - mq;
+                        dp[i] = -d;
+                    }
+#pragma unroll
+                    for (int s = 0; s < G::STEPS; ++s) {
+                        sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::rows(Ks, (kt & 1) * 32 + l31, s, half), qf[s], sc, 0, 0, 0);
+                        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::rows(Vs, (kt & 1) * 32 + l31, s, half), gf[s], dp, 0, 0, 0);
+                    }
+                    if (kb * 128 + kt * 32 + 32 > len) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (kb * 128 + kt * 32 + acc_row(i, half) >= len) sc[i] = -kInf;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[kt][i] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[i], a.c, -lq)), dp[i], acc[kt][i]);
+                }
+            }
+        }
+        dma_barrier();
+    }
+    const int nkt = w.kblocks * 4;
+    const long row = ((long)ch * w.heads + hl) * (w.qblocks * 4) + (qb - w.q0) * 4 + wave;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+        float* dst = dense + (row * nkt + kb * 4 + kt) * 1024 + lane * 4;
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+            f32x4 t;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = acc[kt][4 * jj + e];
+            *reinterpret_cast<f32x4*>(dst + jj * 256) = t;
+        }
+    }
+}
+
+// The pairs' sums by entry: a workgroup takes a tile row (32 queries) of a head and one of `parts` ranges of its key tiles; its
+// waves take every fourth tile, each with a histogram of its own.  LDS float adds run at some 200 cycles an instruction
+// here, which is why the batch is summed first; a tile whose pairs all fall on one entry (far positions) costs one add.
+__global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __restrict__ dense, float* __restrict__ slab, RelBlocks w,
+                                                     int parts) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // [4][Rp] floats
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int part = (int)blockIdx.x % parts, rest = (int)blockIdx.x / parts, nqt = w.qblocks * 4, nkt = w.kblocks * 4;
+    const int qt = rest % nqt, hl = rest / nqt;
+    float* hist = reinterpret_cast<float*>(smem) + (long)wave * a.Rp;
+    for (int i = lane; i < a.Rp; i += 64) hist[i] = 0.f;
+    const int q = (w.q0 * 4 + qt) * 32 + l31, top4 = (a.R - 1) * 4;
+    const int qc = q < a.Sk ? a.q_codes4[q] : 0;
+    const int live_t = (a.Sk + 31) / 32, per = (live_t + parts - 1) / parts;
+    const int t1 = (part + 1) * per < live_t ? (part + 1) * per : live_t;
+    for (int kt = part * per + wave; kt < t1; kt += 4) {
+        float v[16];
+        int at[16], lo = 0x7fffffff, hi = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int key = kt * 32 + acc_row(i, half);
+            at[i] = bias_at(qc, key < a.Sk ? a.k_codes4[key] : 0, top4);
+            lo = at[i] < lo ? at[i] : lo;
+            hi = at[i] > hi ? at[i] : hi;
+            v[i] = 0.f;
+        }
+        for (int ch = 0; ch < w.chunks; ++ch) {
+            const float* src = dense + ((((long)ch * w.heads + hl) * nqt + qt) * nkt + kt) * 1024 + lane * 4;
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+                const f32x4 t = *reinterpret_cast<const f32x4*>(src + jj * 256);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * jj + e] += t[e];
+            }
+        }
+        const int one = __builtin_amdgcn_readfirstlane(lo);
+        if (__all(lo == hi && lo == one)) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s += v[i];
+            s = wave_sum(s);
+            if (lane == 0) hist[one >> 2] += s;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                __hip_atomic_fetch_add(reinterpret_cast<float*>(reinterpret_cast<char*>(hist) + at[i]), v[i], __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+    }
+    __syncthreads();
+    float* dst = slab + ((long)(hl + w.h0) * w.slab_rows + (long)(w.q0 * 4 + qt) * parts + part) * a.Rp;
+    const float* all = reinterpret_cast<const float*>(smem);
+    for (int i = tid; i < a.Rp; i += 256) dst[i] = all[i] + all[a.Rp + i] + all[2 * a.Rp + i] + all[3 * a.Rp + i];
+}
+
 // Key owner: dK and dV of 128 keys a workgroup; the rows of all G heads stream through.
 template <int HD, bool BIAS>
-__global__ __launch_bounds__(256) void k_ext_bwd_kv(ExtArgs a, const bf16* __restrict__ dout, const float* __restrict__ stat,
+__global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                     const float* __restrict__ dsum, bf16* __restrict__ dk, bf16* __restrict__ dv,
                                                     float* __restrict__ part_k, float* __restrict__ part_v, int tiles, int splits) {
     using G = AttnGeo<HD>;
@@ -851,18 +991,15 @@ __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ t
     (w < Sp ? q4 : k4)[at] = c * 4;
 }
 
-// mid[chunk][h][r] = sum of the slab rows of head h in this chunk, in order
-__global__ __launch_bounds__(256) void k_bias_slab(const float* __restrict__ slab, float* __restrict__ mid, int Rp, int H, int B,
-                                                   int per_head /* tiles * splits */, int chunks) {
+// mid[chunk][h][r] = sum of this chunk's slab rows [H][rows][Rp] of head h, in order
+__global__ __launch_bounds__(256) void k_bias_slab(const float* __restrict__ slab, float* __restrict__ mid, int Rp, int H, int rows,
+                                                   int chunks) {
     const int r = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, ch = blockIdx.z;
     if (r >= Rp) return;
-    const int rows = B * per_head, per = (rows + chunks - 1) / chunks;
-    const int i0 = ch * per, i1 = i0 + per < rows ? i0 + per : rows;
+    const int per = (rows + chunks - 1) / chunks, i0 = ch * per, i1 = i0 + per < rows ? i0 + per : rows;
     float s = 0.f;
-    for (int i = i0; i < i1; ++i) {
-        const int b = i / per_head, t = i - b * per_head;
-        s += slab[((long)(b * H + h) * per_head + t) * Rp + r];
-    }
+#pragma unroll 4
+    for (int i = i0; i < i1; ++i) s += slab[((long)h * rows + i) * Rp + r];
     mid[((long)ch * H + h) * Rp + r] = s;
 }
 
@@ -933,12 +1070,12 @@ template <int HD>
 void bwd(const ExtArgs& a, const ExtBwd& w, hipStream_t s) {
     const ExtPlan &pq = w.q, &pk = w.kv;
     const dim3 gq((unsigned)((long)a.B * a.Hkv * pq.tiles * pq.splits)), gk((unsigned)((long)a.B * a.Hkv * pk.tiles * pk.splits));
-    const size_t lq = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + 5 * table_bytes(a);
+    const size_t lq = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + table_bytes(a);
     const size_t lk = (size_t)4 * 64 * HD * 2 + 8192 + table_bytes(a);
 #define PDT_EXT_BWD(BIAS)                                                                                                  \
     allow_lds(&k_ext_bwd_q<HD, BIAS>, lq);                                                                                 \
     hipLaunchKernelGGL((k_ext_bwd_q<HD, BIAS>), gq, dim3(256), lq, s, a, (const bf16*)w.out, (const bf16*)w.out_lo,        \
-                       (const bf16*)w.dout, w.stat, w.dsum, (bf16*)w.dq, w.part_q, w.slab, pq.tiles, pq.splits);           \
+                       (const bf16*)w.dout, w.stat, w.dsum, (bf16*)w.dq, w.part_q, pq.tiles, pq.splits);                   \
     allow_lds(&k_ext_bwd_kv<HD, BIAS>, lk);                                                                                \
     hipLaunchKernelGGL((k_ext_bwd_kv<HD, BIAS>), gk, dim3(256), lk, s, a, (const bf16*)w.dout, w.stat, (const float*)w.dsum, \
                        (bf16*)w.dk, (bf16*)w.dv, w.part_k, w.part_v, pk.tiles, pk.splits);
@@ -1007,12 +1144,62 @@ void launch_bias_tables(const float* table, const int* bucket_of, const int* q_c
     hipLaunchKernelGGL(k_bias_tables, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, table, bucket_of, q_codes, k_codes,
                        tab, q4, k4, R, Rp, NB, H, S, Sp, inv_scale, total);
 }
-int bias_grad_chunks(int rows) { return rows < 32 ? 1 : rows < 32 * 32 ? (rows + 31) / 32 : 32; }
-void launch_bias_grad(const float* slab, float* mid, const int* bucket_of, float* dtable, int R, int Rp, int NB, int H, int B,
-                      int per_head, int chunks, hipStream_t s) {
-    hipLaunchKernelGGL(k_bias_slab, dim3((Rp + 255) / 256, H, chunks), dim3(256), 0, s, slab, mid, Rp, H, B, per_head, chunks);
-    hipLaunchKernelGGL(k_bias_buckets, dim3((NB + 255) / 256, H), dim3(256), 0, s, (const float*)mid, bucket_of, dtable, R, Rp, NB, H,
-                       chunks);
+// Head groups and query blocks of a dense sum of at most 1 GiB; the batch in parts, so that about 1024 workgroups run
+RelPlan rel_plan(int B, int H, int S) {
+    RelPlan p;
+    const long blocks = (S + 127) / 128, row_block = blocks * 4 * blocks * 4 * 4096;  // bytes of a head
+    const long most = 1L << 30;
+    p.heads = (int)(row_block >= most ? 1 : most / row_block < H ? most / row_block : H);
+    p.qblocks = (int)(row_block <= most ? blocks : most / (row_block / blocks) > 0 ? most / (row_block / blocks) : 1);
+    const long groups = (long)p.heads * p.qblocks * blocks;
+    long c = (1024 + groups - 1) / groups;
+    const long room = most / (p.heads * p.qblocks * (row_block / blocks));
+    c = c < B / 4 ? c : B / 4;
+    c = c < room ? c : room;
+    p.chunks = (int)(c < 1 ? 1 : c);
+    // ranges of key tiles, so that the histograms' adds are spread over the CUs
+    const long rows = (long)H * blocks * 4;
+    const long tiles = (S + 31) / 32;
+    long q = (1024 + rows - 1) / rows;
+    q = q < (tiles + 3) / 4 ? q : (tiles + 3) / 4;
+    p.parts = (int)(q < 1 ? 1 : q);
+    p.rows = (int)(blocks * 4 * p.parts);
+    p.dense = (long)p.chunks * p.heads * p.qblocks * (row_block / blocks) / 4;
+    p.mid = p.rows < 32 ? 1 : p.rows < 32 * 32 ? (p.rows + 31) / 32 : 32;
+    return p;
+}
+template <int HD>
+static void rel_dbias(const ExtArgs& a, const ExtBwd& x, float* dense, const RelBlocks& w, hipStream_t s) {
+    const size_t tab = (size_t)((a.Rp + 255) & ~255) * 4, stage = (size_t)2 * 128 * HD * 2, lds = tab > stage ? tab : stage;
+    allow_lds(&k_rel_dbias<HD>, lds);
+    hipLaunchKernelGGL((k_rel_dbias<HD>), dim3((unsigned)(w.kblocks * w.qblocks * w.heads * w.chunks)), dim3(256), lds, s, a,
+                       (const bf16*)x.dout, x.stat, (const float*)x.dsum, dense, w);
+}
+void launch_rel_bias_grad(const ExtArgs& a, const ExtBwd& x, int hd, const RelPlan& p, float* dense, float* slab, float* mid,
+                          const int* bucket_of, float* dtable, int NB, hipStream_t s) {
+    const int blocks = (a.Sk + 127) / 128;
+    for (int h0 = 0; h0 < a.Hkv; h0 += p.heads)
+        for (int q0 = 0; q0 < blocks; q0 += p.qblocks) {
+            RelBlocks w;
+            w.h0 = h0;
+            w.heads = a.Hkv - h0 < p.heads ? a.Hkv - h0 : p.heads;
+            w.q0 = q0;
+            w.qblocks = blocks - q0 < p.qblocks ? blocks - q0 : p.qblocks;
+            w.kblocks = blocks;
+            w.chunks = p.chunks;
+            w.slab_rows = p.rows;
+            if (hd == 32) rel_dbias<32>(a, x, dense, w, s);
+            else if (hd == 64) rel_dbias<64>(a, x, dense, w, s);
+            else rel_dbias<128>(a, x, dense, w, s);
+            const size_t lds = (size_t)4 * a.Rp * 4;
+            allow_lds(&k_rel_entries, lds);
+            hipLaunchKernelGGL(k_rel_entries, dim3((unsigned)(w.heads * w.qblocks * 4 * p.parts)), dim3(256), lds, s, a,
+                               (const float*)dense, slab, w, p.parts);
+        }
+    hipLaunchKernelGGL(k_bias_slab, dim3((a.Rp + 255) / 256, a.Hkv, p.mid), dim3(256), 0, s, (const float*)slab, mid, a.Rp, a.Hkv, p.rows,
+                       p.mid);
+    hipLaunchKernelGGL(k_bias_buckets, dim3((NB + 255) / 256, a.Hkv), dim3(256), 0, s, (const float*)mid, bucket_of, dtable, a.R, a.Rp, NB,
+                       a.Hkv, p.mid);
 }
 
 }  // namespace pdt
