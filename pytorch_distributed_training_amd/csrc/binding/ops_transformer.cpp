@@ -72,7 +72,7 @@ void check_grid(const ExtArgs& a, const ExtPlan& p) {
     TORCH_CHECK((long)a.B * a.Hkv < (1L << 30) / std::max(1, p.tiles * p.splits), "attention: more than 2^30 workgroups");
 }
 void set_tables(ExtArgs& a, const Tensor& tab, const Tensor& codes, int64_t R) {
-    const long Sp = (a.Sk + 63) / 64 * 64, Rp = (R + 3) / 4 * 4;
+    const long Sp = (a.Sk + 127) / 128 * 128, Rp = (R + 3) / 4 * 4;
     TORCH_CHECK(R >= 1 && R <= kExtMaxEntries, "rel_bias_attention: ", R, " entries (1 to ", kExtMaxEntries, ")");
     TORCH_CHECK(tab.sizes() == at::IntArrayRef({(long)a.Hkv, Rp}) && codes.sizes() == at::IntArrayRef({2, Sp}), "bias tables: shape");
     a.tab = tab.data_ptr<float>();
@@ -173,7 +173,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> rel_bias_attention_fwd(const 
     check_dense(k_codes, {S}, at::kInt, qkv, "k_codes");
     check_dense(bucket_of, {R}, at::kInt, qkv, "bucket_of");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(qkv.device());
-    const long Rp = (R + 3) / 4 * 4, Sp = (S + 63) / 64 * 64;
+    const long Rp = (R + 3) / 4 * 4, Sp = (S + 127) / 128 * 128;
     Tensor tab = at::empty({heads, Rp}, table.options()), codes = at::empty({2, Sp}, q_codes.options());
     launch_bias_tables(table.data_ptr<float>(), bucket_of.data_ptr<int>(), q_codes.data_ptr<int>(), k_codes.data_ptr<int>(),
                        tab.data_ptr<float>(), codes.data_ptr<int>(), codes.data_ptr<int>() + Sp, (int)R, (int)Rp, (int)NB, (int)heads,

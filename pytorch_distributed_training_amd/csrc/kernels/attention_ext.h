@@ -22,7 +22,7 @@ struct ExtArgs {
     int R, Rp;
     int self;                     // rows past lens[b] are dead too
     int B, Hkv, G, Sq, Sk, M, Mp; // M = Sq * G rows per key head, Mp = M rounded up to 64
-    long stat_n;                  // B * Hkv * Mp: the statistics are [2][stat_n], m and log2 l
+    long stat_n;                  // B * Hkv * Mp: the statistics are [2][stat_n], -m and -log2 l
     float c, scale;               // log2(e) / sqrt(hd), 1 / sqrt(hd)
 };
 struct ExtPlan {
@@ -32,7 +32,7 @@ struct ExtPlan {
 struct ExtBwd {
     const void *out, *out_lo, *dout;
     const float* stat;
-    float* dsum;
+    float* dsum;  // -D
     void *dq, *dk, *dv;
     float *part_q, *part_k, *part_v;
     ExtPlan q, kv;

@@ -15,7 +15,7 @@
 //  * Scores are produced TRANSPOSED in the passes that own rows (lane = row, registers = keys) and straight in the pass that
 //    owns keys (lane = key, registers = rows); the second product is transposed as well (V^T P^T, K^T dS^T, ...), so that
 //    running maximum, sums, rescaling and the stores (four neighbouring channels a lane) are all per lane.
-//  * The statistics that the backward gets are m (in units of q . k) and log2 l apart.  Where a bias of -1e9 holds for a whole
+//  * The statistics that the backward gets are -m (in units of q . k) and -log2 l apart.  Where a bias of -1e9 holds for a whole
 //    row, their sum would not leave a bit of l, and 2^(c s - sum), a difference of two numbers rounded at 1e9, is anything.
 //    The backward's scores start at bias - m, so that no large number is left to round.
 //  * The axis that streams comes by LDS-DMA in blocks of 64 rows, two buffers, one barrier a block; rows past the valid
@@ -74,10 +74,15 @@ __device__ __forceinline__ void dma_words(uint32_t img, const void* base, int la
     lds_dma16(uniform_rsrc(base, 256u), lane < 16 ? (uint32_t)lane * 16u : kOOB, (uint32_t)__builtin_amdgcn_readfirstlane((int)img));
 }
 
-__device__ __forceinline__ int bias_at(int qc4, int kc4, int top4) {
-    const int d = qc4 - kc4;
-    return d < 0 ? 0 : d > top4 ? top4 : d;
+// LDS address of a pair's bias: clamp(q code - k code) in bytes, `lo` and `hi` the addresses of the table's first and last
+// entry and `lo` already in the query's code (two instructions an element; a clamp of unknown bounds compiles to four)
+__device__ __forceinline__ int bias_at(int qc4, int kc4, int lo, int hi) {
+    int d = qc4 - kc4;
+    asm("v_med3_i32 %0, %0, %1, %2" : "+v"(d) : "v"(lo), "s"(hi));
+    return d;
 }
+typedef const float __attribute__((address_space(3))) * lds_cfloat_ptr;
+__device__ __forceinline__ float lds_float(int addr) { return *(lds_cfloat_ptr)(uintptr_t)(uint32_t)addr; }
 
 __device__ __forceinline__ long row_offset(const ExtView& v, int r, int hkv, int G, int HD) {
     const int q = (int)fdiv((uint32_t)r, v.g);
@@ -107,11 +112,11 @@ __device__ __forceinline__ Job job_of(const ExtArgs& a, int tiles, int splits) {
     return j;
 }
 
-// the row's statistics; where nothing was attended to, log2 l = +inf makes every P of the backward zero.  Where l was summed
+// the row's statistics; where nothing was attended to, -log2 l = -inf makes every P of the backward zero.  Where l was summed
 // from 2^(c s + base) with base = -c m rounded, `rounding` = c m + base goes into log2 l
 __device__ __forceinline__ void put_stat(const ExtArgs& a, float* stat, long at, bool some, float m, float l, float rounding) {
-    stat[at] = some ? m : 0.f;
-    stat[a.stat_n + at] = some ? __builtin_amdgcn_logf(l) - rounding : kInf;
+    stat[at] = some ? -m : 0.f;
+    stat[a.stat_n + at] = some ? rounding - __builtin_amdgcn_logf(l) : -kInf;
 }
 
 template <int HD>
@@ -130,7 +135,7 @@ __device__ __forceinline__ void own_frags(bf16x8* f, const bf16* p, bool live, i
 // HL: P and O as two bf16 each (value and remainder), so that the backward's D = dO . O, and with it the fp32 gradient of
 // the bias table, does not carry the rounding of P and O to 8 bits of mantissa.
 template <int HD, bool BIAS, bool HL>
-__global__ __launch_bounds__(256) void k_ext_fwd(ExtArgs a, bf16* __restrict__ out, bf16* __restrict__ out_lo,
+__global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict__ out, bf16* __restrict__ out_lo,
                                                  float* __restrict__ stat, float* __restrict__ part, float* __restrict__ part_ml,
                                                  int tiles, int splits) {
     using G = AttnGeo<HD>;
@@ -141,7 +146,7 @@ __global__ __launch_bounds__(256) void k_ext_fwd(ExtArgs a, bf16* __restrict__ o
     const Job j = job_of(a, tiles, splits);
     const uint32_t lds0 = lds_address(smem);
     char* codes = smem + 4 * IMG;
-    const float* tab = reinterpret_cast<const float*>(smem + 4 * IMG + 2048);
+    const int tab = (int)lds0 + 4 * IMG + 2048;
     const int r = j.tile * 128 + wave * 32 + l31;
     const bool live = r < j.rows;
     const long orow = r < a.M ? (long)j.b * a.o.bs + row_offset(a.o, r, j.hkv, a.G, HD) : 0;
@@ -178,7 +183,7 @@ __global__ __launch_bounds__(256) void k_ext_fwd(ExtArgs a, bf16* __restrict__ o
         }
         bf16x8 bq[G::STEPS];
         own_frags<HD>(bq, a.q + (long)j.b * a.qv.bs + row_offset(a.qv, live ? r : 0, j.hkv, a.G, HD), live, half);
-        const int qc = BIAS && live ? a.q_codes4[r] : 0, top4 = (a.R - 1) * 4;
+        const int qc = tab + (BIAS && live ? a.q_codes4[r] : 0), top = tab + (a.R - 1) * 4;
 
         for (int kb = kb0; kb < kb1; ++kb) {
             const int buf = (kb - kb0) & 1;
@@ -195,8 +200,7 @@ __global__ __launch_bounds__(256) void k_ext_fwd(ExtArgs a, bf16* __restrict__ o
                     for (int jj = 0; jj < 4; ++jj) {
                         const i32x4 kc = *reinterpret_cast<const i32x4*>(codes + buf * 1024 + (kt * 32 + 8 * jj + 4 * half) * 4);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            st[kt][4 * jj + e] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(tab) + bias_at(qc, kc[e], top4));
+                        for (int e = 0; e < 4; ++e) st[kt][4 * jj + e] = lds_float(bias_at(qc, kc[e], tab, top));
                     }
                 } else {
 #pragma unroll
@@ -214,12 +218,10 @@ __global__ __launch_bounds__(256) void k_ext_fwd(ExtArgs a, bf16* __restrict__ o
                 for (int i = 0; i < 16; ++i) mb = fmaxf(mb, st[kt][i]);
             }
             mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
-            // (with a bias, s - m is taken before the product: a mask of -1e9 over a whole row leaves P in [0, 1]; without one
-            // scores are small enough for one multiply-add.  Every key so far forbidden: m counts as 0, all P are 0)
-            const float top = mb == -kInf ? 0.f : mb;
-            base = BIAS ? -top : -top * a.c;
+            const float mx = mb == -kInf ? 0.f : mb;  // (every key so far forbidden: m counts as 0, all P are 0)
+            base = -mx * a.c;
             if (__any(mb > m)) {
-                const float alpha = __builtin_amdgcn_exp2f(BIAS ? (m + base) * a.c : fmaf(m, a.c, base));
+                const float alpha = __builtin_amdgcn_exp2f((m - mx) * a.c);
                 l *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < G::DT; ++dt)
@@ -227,23 +229,35 @@ __global__ __launch_bounds__(256) void k_ext_fwd(ExtArgs a, bf16* __restrict__ o
                     for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
                 m = mb;
             }
+            // one multiply-add a score, but for a bias of, say, -1e9 over a whole row: its product leaves nothing of the scores
+            if (BIAS && !__all(fabsf(mx) < 65536.f)) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) st[kt][i] -= mx;
+                base = 0.f;
+            }
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
                 float part_l = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    st[kt][i] = __builtin_amdgcn_exp2f(BIAS ? (st[kt][i] + base) * a.c : fmaf(st[kt][i], a.c, base));
+                    st[kt][i] = __builtin_amdgcn_exp2f(fmaf(st[kt][i], a.c, base));
                     part_l += st[kt][i];
                 }
                 l += part_l;
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
-                    const bf16x8 p = acc_to_a(st[kt], blk);
-                    bf16x8 plo;
-                    if (HL) {
+                    u32x4 hi, lo;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) plo[i] = (bf16)(st[kt][8 * blk + i] - (float)p[i]);
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = st[kt][8 * blk + 2 * i], y = st[kt][8 * blk + 2 * i + 1];
+                        hi[i] = pack_bf16(x, y);
+                        if (HL) lo[i] = pack_bf16(x - __uint_as_float(hi[i] << 16), y - __uint_as_float(hi[i] & 0xffff0000u));
                     }
+                    const bf16x8 p = __builtin_bit_cast(bf16x8, hi);
+                    bf16x8 plo;
+                    if (HL) plo = __builtin_bit_cast(bf16x8, lo);
 #pragma unroll
                     for (int dt = 0; dt < G::DT; ++dt) {
                         const bf16x8 vt = G::cols(Vs, kt * 32 + blk * 16, dt * 32, lane);
@@ -275,7 +289,7 @@ __global__ __launch_bounds__(256) void k_ext_fwd(ExtArgs a, bf16* __restrict__ o
         return;
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    if (stat && half == 0 && r < a.Mp) put_stat(a, stat, (long)j.bh * a.Mp + r, live && (l > 0.f || l != l), m, l, BIAS ? 0.f : fmaf(m, a.c, base));
+    if (stat && half == 0 && r < a.Mp) put_stat(a, stat, (long)j.bh * a.Mp + r, live && (l > 0.f || l != l), m, l, BIAS && base == 0.f ? 0.f : fmaf(m, a.c, base));
     if (r < a.M) {
 #pragma unroll
         for (int dt = 0; dt < G::DT; ++dt)
@@ -298,7 +312,7 @@ __global__ __launch_bounds__(256) void k_ext_fwd(ExtArgs a, bf16* __restrict__ o
 // every fourth tile of 32 keys each, through an LDS ring of their own (no barrier until the join): the kernel is a stream over
 // K and V, 16 to 64 KiB of it in flight per workgroup.
 template <int HD>
-__global__ __launch_bounds__(256) void k_ext_fwd_few(ExtArgs a, bf16* __restrict__ out, float* __restrict__ stat,
+__global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restrict__ out, float* __restrict__ stat,
                                                      float* __restrict__ part, float* __restrict__ part_ml, int splits) {
     using G = AttnGeo<HD>;
     constexpr int TIMG = 32 * G::ROWBYTES, STAGE = 2 * TIMG, RPP = 1024 / G::ROWBYTES, NP = 32 / RPP;
@@ -548,7 +562,7 @@ __device__ __forceinline__ void store_acc32(const f32x16* t, float* dst, int hal
 // Row owner: dQ, and D for the key owner (written by split 0).  A softmax over one key is constant, so with len = 1 dS is
 // zero, and is set so (as a difference of two rounded numbers it would not be).
 template <int HD, bool BIAS>
-__global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ out_lo,
+__global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ out_lo,
                                                    const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                    float* __restrict__ dsum, bf16* __restrict__ dq, float* __restrict__ part, int tiles,
                                                    int splits) {
@@ -560,7 +574,7 @@ __global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __rest
     const Job j = job_of(a, tiles, splits);
     const uint32_t lds0 = lds_address(smem);
     char* codes = smem + 4 * IMG;
-    char* tab = smem + 4 * IMG + 2048;
+    const int tab = (int)lds0 + 4 * IMG + 2048;
     const int r = j.tile * 128 + wave * 32 + l31;
     const bool live = r < j.rows;
     const int nb = (j.len + 63) >> 6, per = (nb + splits - 1) / splits;
@@ -610,10 +624,10 @@ __global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __rest
             }
         d += __shfl_xor(d, 32, 64);
     }
-    if (j.split == 0 && half == 0 && r < a.Mp) dsum[(long)j.bh * a.Mp + r] = live ? d : 0.f;
-    const float mq = live ? stat[(long)j.bh * a.Mp + r] : 0.f, lq = live ? stat[a.stat_n + (long)j.bh * a.Mp + r] : kInf;
-    const int qc = BIAS && live ? a.q_codes4[r] : 0, top4 = (a.R - 1) * 4;
-    const float keep = j.len > 1 ? 1.f : 0.f;
+    if (j.split == 0 && half == 0 && r < a.Mp) dsum[(long)j.bh * a.Mp + r] = live ? -d : 0.f;
+    const float mq = live ? stat[(long)j.bh * a.Mp + r] : 0.f;
+    const float lq = live && j.len > 1 ? stat[a.stat_n + (long)j.bh * a.Mp + r] : -kInf;
+    const int qc = tab + (BIAS && live ? a.q_codes4[r] : 0), top = tab + (a.R - 1) * 4;
 
     if (any) {
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -630,12 +644,12 @@ __global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __rest
                     for (int jj = 0; jj < 4; ++jj) {
                         const i32x4 kc = *reinterpret_cast<const i32x4*>(codes + buf * 1024 + (kt * 32 + 8 * jj + 4 * half) * 4);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[4 * jj + e] = *reinterpret_cast<const float*>(tab + bias_at(qc, kc[e], top4)) - mq;
+                        for (int e = 0; e < 4; ++e) sc[4 * jj + e] = lds_float(bias_at(qc, kc[e], tab, top)) + mq;
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    if (!BIAS) sc[i] = -mq;
+                    if (!BIAS) sc[i] = mq;
                     dp[i] = -d;
                 }
 #pragma unroll
@@ -649,7 +663,7 @@ __global__ __launch_bounds__(256) void k_ext_bwd_q(ExtArgs a, const bf16* __rest
                         if (kb * 64 + kt * 32 + acc_row(i, half) >= j.len) sc[i] = -kInf;
                 }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, -lq)) * keep;
+                for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lq));
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
                     const bf16x8 ds = acc_to_a(dp, blk);
@@ -692,16 +706,18 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
         const i32x4 rsrc = uniform_rsrc(a.tab + (long)h * a.Rp, (uint32_t)a.Rp * 4u);
         for (int p = wave; p * 256 < a.Rp; p += 4)
             lds_dma16(rsrc, (uint32_t)(p * 1024 + lane * 16), (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + p * 1024)));
-        const int qc = q < a.Sk ? a.q_codes4[q] : 0, top4 = (a.R - 1) * 4;
+        const int qc = (int)lds0 + (q < a.Sk ? a.q_codes4[q] : 0), top = (int)lds0 + (a.R - 1) * 4;
         dma_barrier();
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = kb * 128 + kt * 32 + acc_row(i, half);
-                const int kc = key < a.Sk ? a.k_codes4[key] : 0;
-                bias[kt][i] = *reinterpret_cast<const float*>(smem + bias_at(qc, kc, top4));
-                acc[kt][i] = 0.f;
+            for (int jj = 0; jj < 4; ++jj) {
+                const i32x4 kc = *reinterpret_cast<const i32x4*>(a.k_codes4 + kb * 128 + kt * 32 + 8 * jj + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    bias[kt][4 * jj + e] = lds_float(bias_at(qc, kc[e], (int)lds0, top));
+                    acc[kt][4 * jj + e] = 0.f;
+                }
             }
         dma_barrier();
     }
@@ -726,7 +742,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
         own_frags<HD>(qf, a.q + (long)b * a.qv.bs + (long)(live ? q : 0) * a.qv.rs + (long)h * HD, live, half);
         own_frags<HD>(gf, dout + (long)b * a.o.bs + (long)(live ? q : 0) * a.o.rs + (long)h * HD, live, half);
         const long sr = ((long)b * a.Hkv + h) * a.Mp + (live ? q : 0);
-        const float mq = live ? stat[sr] : 0.f, lq = live ? stat[a.stat_n + sr] : kInf, d = live ? dsum[sr] : 0.f;
+        const float mq = live ? stat[sr] : 0.f, lq = live ? stat[a.stat_n + sr] : -kInf, d = live ? dsum[sr] : 0.f;
         dma_barrier();
         if (qb * 128 + wave * 32 < len) {
 #pragma unroll
@@ -737,8 +753,8 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
                     f32x16 sc, dp;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        sc[i] = bias[kt][i] - mq;
-                        dp[i] = -d;
+                        sc[i] = bias[kt][i] + mq;
+                        dp[i] = d;
                     }
 #pragma unroll
                     for (int s = 0; s < G::STEPS; ++s) {
@@ -751,7 +767,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
                             if (kb * 128 + kt * 32 + acc_row(i, half) >= len) sc[i] = -kInf;
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[kt][i] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[i], a.c, -lq)), dp[i], acc[kt][i]);
+                    for (int i = 0; i < 16; ++i) acc[kt][i] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lq)), dp[i], acc[kt][i]);
                 }
             }
         }
@@ -783,21 +799,26 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
     const int part = (int)blockIdx.x % parts, rest = (int)blockIdx.x / parts, nqt = w.qblocks * 4, nkt = w.kblocks * 4;
     const int qt = rest % nqt, hl = rest / nqt;
     float* hist = reinterpret_cast<float*>(smem) + (long)wave * a.Rp;
+    const int base = (int)lds_address(hist), top = base + (a.R - 1) * 4;
     for (int i = lane; i < a.Rp; i += 64) hist[i] = 0.f;
-    const int q = (w.q0 * 4 + qt) * 32 + l31, top4 = (a.R - 1) * 4;
-    const int qc = q < a.Sk ? a.q_codes4[q] : 0;
+    const int q = (w.q0 * 4 + qt) * 32 + l31;
+    const int qc = base + (q < a.Sk ? a.q_codes4[q] : 0);
     const int live_t = (a.Sk + 31) / 32, per = (live_t + parts - 1) / parts;
     const int t1 = (part + 1) * per < live_t ? (part + 1) * per : live_t;
     for (int kt = part * per + wave; kt < t1; kt += 4) {
         float v[16];
         int at[16], lo = 0x7fffffff, hi = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int key = kt * 32 + acc_row(i, half);
-            at[i] = bias_at(qc, key < a.Sk ? a.k_codes4[key] : 0, top4);
-            lo = at[i] < lo ? at[i] : lo;
-            hi = at[i] > hi ? at[i] : hi;
-            v[i] = 0.f;
+        for (int jj = 0; jj < 4; ++jj) {
+            const i32x4 kc = *reinterpret_cast<const i32x4*>(a.k_codes4 + kt * 32 + 8 * jj + 4 * half);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * jj + e;
+                at[i] = bias_at(qc, kc[e], base, top) - base;
+                lo = at[i] < lo ? at[i] : lo;
+                hi = at[i] > hi ? at[i] : hi;
+                v[i] = 0.f;
+            }
         }
         for (int ch = 0; ch < w.chunks; ++ch) {
             const float* src = dense + ((((long)ch * w.heads + hl) * nqt + qt) * nkt + kt) * 1024 + lane * 4;
@@ -835,13 +856,13 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
                                                     float* __restrict__ part_k, float* __restrict__ part_v, int tiles, int splits) {
     using G = AttnGeo<HD>;
     constexpr int IMG = 64 * G::ROWBYTES;
-    extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][Q, dO], [2][log2 l, D, codes, m: 1 KiB each], table
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][Q, dO], [2][-log2 l, -D, codes, -m: 1 KiB each], table
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Job j = job_of(a, tiles, splits);
     const uint32_t lds0 = lds_address(smem);
     char* stat_s = smem + 4 * IMG;
-    char* tab = stat_s + 2 * 4096;
+    const int tab = (int)lds0 + 4 * IMG + 8192;
     const int key = j.tile * 128 + wave * 32 + l31;
     const bool live = key < j.len;
     const int nb = (j.rows + 63) >> 6, per = (nb + splits - 1) / splits;
@@ -893,8 +914,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
         const long ko = (long)j.b * a.kv.bs + (long)(live ? key : 0) * a.kv.rs + (long)j.hkv * HD;
         own_frags<HD>(kf, a.k + ko, live, half);
         own_frags<HD>(vf, a.v + ko, live, half);
-        const int kc = BIAS && live ? a.k_codes4[key] : 0, top4 = (a.R - 1) * 4;
-        const float keep = j.len > 1 ? 1.f : 0.f;
+        const int kc = (BIAS && live ? a.k_codes4[key] : 0) - tab, top = tab + (a.R - 1) * 4;
 
         for (int rb = rb0; rb < rb1; ++rb) {
             const int buf = (rb - rb0) & 1;
@@ -916,8 +936,8 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
                     if (BIAS) qc = *reinterpret_cast<const i32x4*>(st + 2048 + w);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        sc[4 * jj + e] = BIAS ? *reinterpret_cast<const float*>(tab + bias_at(qc[e], kc, top4)) - mr[e] : -mr[e];
-                        dp[4 * jj + e] = -dr[e];
+                        sc[4 * jj + e] = BIAS ? lds_float(bias_at(qc[e], kc, tab, top)) + mr[e] : mr[e];
+                        dp[4 * jj + e] = dr[e];
                     }
                 }
 #pragma unroll
@@ -925,12 +945,12 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
                     sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::rows(Qs, rt * 32 + l31, s, half), kf[s], sc, 0, 0, 0);
                     dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::rows(Gs, rt * 32 + l31, s, half), vf[s], dp, 0, 0, 0);
                 }
-                // (no mask: a dead key is a lane of its own whose results are not stored; rows past the end have log2 l = +inf)
+                // (no mask: a dead key is a lane of its own whose results are not stored; rows past the end have -log2 l = -inf)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, -lr[i >> 2][i & 3]));
+                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lr[i >> 2][i & 3]));
                     sc[i] = p;
-                    dp[i] *= p * keep;
+                    dp[i] *= p;
                 }
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
@@ -945,15 +965,13 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
         }
     }
     if (key >= a.Sk) return;
-    if (!live) {
 #pragma unroll
-        for (int dt = 0; dt < G::DT; ++dt)
+    for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                ak[dt][i] = 0.f;
-                av[dt][i] = 0.f;
-            }
-    }
+        for (int i = 0; i < 16; ++i) {
+            if (!live) av[dt][i] = 0.f;
+            if (!live || j.len <= 1) ak[dt][i] = 0.f;
+        }
     if (splits > 1) {
         const long at = (((long)j.bh * splits + j.split) * a.Sk + key) * HD;
         store_acc32<HD>(ak, part_k + at, half);
@@ -967,7 +985,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
 
 // ------------------------------------------------------------------------------------------------------- bias tables
 // tab[h][r] = table[bucket_of[r]][h] * sqrt(hd) (the scores are scaled after the bias is added), zero where the entry names no
-// bucket; byte offsets of the position codes, padded with zeros to a multiple of 64
+// bucket; byte offsets of the position codes, padded with zeros to a multiple of 128
 __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ table, const int* __restrict__ bucket_of,
                                                      const int* __restrict__ q_codes, const int* __restrict__ k_codes,
                                                      float* __restrict__ tab, int* __restrict__ q4, int* __restrict__ k4, int R,
@@ -1003,30 +1021,34 @@ __global__ __launch_bounds__(256) void k_bias_slab(const float* __restrict__ sla
     mid[((long)ch * H + h) * Rp + r] = s;
 }
 
-// dtable[n][h] = sum over the entries r of bucket n: the head's entries and their buckets in LDS, one thread per bucket
+// dtable[n][h] = sum over the entries r of bucket n: the head's entries and their buckets in LDS, a lane per bucket, each of the
+// four waves over a quarter of the entries (any number of entries may share a bucket, in any order)
 __global__ __launch_bounds__(256) void k_bias_buckets(const float* __restrict__ mid, const int* __restrict__ bucket_of,
                                                       float* __restrict__ dtable, int R, int Rp, int NB, int H, int chunks) {
     __shared__ __attribute__((aligned(16))) float sums[kExtMaxEntries];
     __shared__ __attribute__((aligned(16))) int of[kExtMaxEntries];
-    const int h = blockIdx.y;
+    __shared__ float red[4][64];
+    const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int r = threadIdx.x; r < Rp; r += 256) {
         float s = 0.f;
+#pragma unroll 4
         for (int c = 0; c < chunks; ++c) s += mid[((long)c * H + h) * Rp + r];
         sums[r] = s;
         of[r] = r < R ? bucket_of[r] : -1;
     }
     __syncthreads();
-    const int n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= NB) return;
+    const int n = blockIdx.x * 64 + lane, quads = Rp >> 2, per = (quads + 3) >> 2;
     float s = 0.f;
-    for (int r = 0; r < Rp; r += 4) {
-        const i32x4 o = *reinterpret_cast<const i32x4*>(of + r);
-        const f32x4 v = *reinterpret_cast<const f32x4*>(sums + r);
+#pragma unroll 4
+    for (int i = wave * per; i < (wave + 1) * per && i < quads; ++i) {
+        const i32x4 o = *reinterpret_cast<const i32x4*>(of + 4 * i);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(sums + 4 * i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (o[e] == n) s += v[e];
+        for (int e = 0; e < 4; ++e) s += o[e] == n ? v[e] : 0.f;
     }
-    dtable[(long)n * H + h] = s;
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && n < NB) dtable[(long)n * H + h] = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
 }
 
 template <typename K>
@@ -1198,7 +1220,7 @@ void launch_rel_bias_grad(const ExtArgs& a, const ExtBwd& x, int hd, const RelPl
         }
     hipLaunchKernelGGL(k_bias_slab, dim3((a.Rp + 255) / 256, a.Hkv, p.mid), dim3(256), 0, s, (const float*)slab, mid, a.Rp, a.Hkv, p.rows,
                        p.mid);
-    hipLaunchKernelGGL(k_bias_buckets, dim3((NB + 255) / 256, a.Hkv), dim3(256), 0, s, (const float*)mid, bucket_of, dtable, a.R, a.Rp, NB,
+    hipLaunchKernelGGL(k_bias_buckets, dim3((NB + 63) / 64, a.Hkv), dim3(256), 0, s, (const float*)mid, bucket_of, dtable, a.R, a.Rp, NB,
                        a.Hkv, p.mid);
 }
 
