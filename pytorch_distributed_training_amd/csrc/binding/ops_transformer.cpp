@@ -89,7 +89,7 @@ std::tuple<Tensor, Tensor, Tensor> ext_fwd(ExtArgs& a, const Tensor& q, int64_t 
     if (lo) out_lo = at::empty_like(out);
     if (out.numel() == 0) return {out, stat, out_lo};
     const long BH = (long)a.B * a.Hkv;
-    const ExtPlan p = ext_plan_fwd(BH, a.M, a.Sk, a.tab != nullptr);
+    const ExtPlan p = ext_plan_fwd(BH, a.M, a.Sk, a.tab == nullptr && !lo);
     check_grid(a, p);
     Tensor part, ml;
     if (p.splits > 1) {
@@ -128,8 +128,7 @@ Tensor ext_bwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, const Ten
     w.stat = stat.data_ptr<float>();
     w.dq = dq.data_ptr(); w.dk = dk.data_ptr(); w.dv = dv.data_ptr();
     a.dqv = view_of(dq, a.G); a.dkv = view_of(dk, 1);
-    w.q = ext_plan_bwd(BH, a.M, a.Sk);
-    w.kv = ext_plan_bwd(BH, a.Sk, a.M);
+    ext_plan_bwd(BH, a.M, a.Sk, a.tab != nullptr, w.q, w.kv);
     check_grid(a, w.q); check_grid(a, w.kv);
     Tensor dsum = at::empty({BH, a.Mp}, f32), pq, pk, pv;
     w.dsum = dsum.data_ptr<float>();
@@ -214,23 +213,24 @@ long cross_head_dim(const Tensor& q, const Tensor& kv, int64_t heads, int64_t kv
     TORCH_CHECK(q.size(0) == kv.size(0), "cross_attention: batches ", q.size(0), " and ", kv.size(0));
     return q.size(2) / heads;
 }
-// q [B, Sq, H hd], kv [B, Sk, 2 Hkv hd] (keys | values) -> out [B, Sq, H hd], stat (with `grad`)
-std::tuple<Tensor, Tensor> cross_attention_fwd(const Tensor& q, const Tensor& kv, int64_t heads, int64_t kv_heads, const OptTensor& lens,
+// q [B, Sq, H hd], kv [B, Sk, 2 Hkv hd] (keys | values) -> out [B, Sq, H hd], stat (with `grad`), out_lo (with `grad` and at most
+// kExtFewKeys keys: dS = P (dP - D) is then a small difference, and D of an output rounded to bf16 costs it half of its
+// precision; with more keys out is small against V and so is its rounding)
+std::tuple<Tensor, Tensor, Tensor> cross_attention_fwd(const Tensor& q, const Tensor& kv, int64_t heads, int64_t kv_heads, const OptTensor& lens,
                                                bool grad) {
     const long hd = cross_head_dim(q, kv, heads, kv_heads), W = kv_heads * hd;
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
     ExtArgs a = ext_args(q, kv.narrow(2, 0, W), kv.narrow(2, W, W), heads, kv_heads, lens, hd, false);
-    auto [out, stat, lo] = ext_fwd(a, q, heads, hd, grad, false);
-    return {out, stat};
+    return ext_fwd(a, q, heads, hd, grad, grad && a.Sk <= kExtFewKeys);
 }
-std::tuple<Tensor, Tensor> cross_attention_bwd(const Tensor& dout, const Tensor& q, const Tensor& kv, const Tensor& out, const Tensor& stat,
-                                               int64_t heads, int64_t kv_heads, const OptTensor& lens) {
+std::tuple<Tensor, Tensor> cross_attention_bwd(const Tensor& dout, const Tensor& q, const Tensor& kv, const Tensor& out, const OptTensor& out_lo,
+                                               const Tensor& stat, int64_t heads, int64_t kv_heads, const OptTensor& lens) {
     const long hd = cross_head_dim(q, kv, heads, kv_heads), W = kv_heads * hd;
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
     ExtArgs a = ext_args(q, kv.narrow(2, 0, W), kv.narrow(2, W, W), heads, kv_heads, lens, hd, false);
     Tensor dq = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
     Tensor dkv = at::empty(kv.sizes(), kv.options().memory_format(at::MemoryFormat::Contiguous));
-    ext_bwd(a, q, heads, hd, dout, out, OptTensor(), stat, dq, dkv.narrow(2, 0, W), dkv.narrow(2, W, W), OptTensor(), 0);
+    ext_bwd(a, q, heads, hd, dout, out, out_lo, stat, dq, dkv.narrow(2, 0, W), dkv.narrow(2, W, W), OptTensor(), 0);
     return {dq, dkv};
 }
 

@@ -38,8 +38,9 @@ struct ExtBwd {
     ExtPlan q, kv;
 };
 
-ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool bias);
-ExtPlan ext_plan_bwd(long BH, int own, int other);  // workgroups own tiles of `own`, `other` streams
+constexpr int kExtFewKeys = 64;  // up to that many keys a training forward keeps the remainder of its output (see cross_attention_fwd)
+ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool streams);
+void ext_plan_bwd(long BH, int M, int Sk, bool bias, ExtPlan& q, ExtPlan& kv);  // of the row owner and the key owner
 void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, void* out_lo, float* stat, float* part, float* part_ml,
                     hipStream_t s);
 void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s);

@@ -69,6 +69,20 @@ __device__ __forceinline__ void dma_block(uint32_t img, const bf16* base, uint32
         }
     }
 }
+// rows [r0, r0 + 32) -> LDS image, by one wave; rows >= valid arrive as zeros
+template <int HD>
+__device__ __forceinline__ void dma_tile(uint32_t img, const bf16* base, int rs, int valid, int lane) {
+    using G = AttnGeo<HD>;
+    constexpr int RPP = 1024 / G::ROWBYTES, NP = 32 / RPP;
+    const i32x4 rsrc = uniform_rsrc(base, (uint32_t)(valid - 1) * (uint32_t)rs * 2u + G::ROWBYTES);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        const int row = p * RPP + lane / G::NCH;
+        const int x = ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) & (G::NCH - 1);
+        const uint32_t o = row < valid ? (uint32_t)(row * rs) * 2u + (uint32_t)(((lane % G::NCH) ^ x) << 4) : kOOB;
+        lds_dma16(rsrc, o, (uint32_t)__builtin_amdgcn_readfirstlane((int)(img + p * 1024)));
+    }
+}
 // 64 consecutive 4-byte values -> LDS (the image takes 1 KiB: lanes 16.. write zeros)
 __device__ __forceinline__ void dma_words(uint32_t img, const void* base, int lane) {
     lds_dma16(uniform_rsrc(base, 256u), lane < 16 ? (uint32_t)lane * 16u : kOOB, (uint32_t)__builtin_amdgcn_readfirstlane((int)img));
@@ -336,17 +350,9 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
 
     auto issue = [&](int t, int buf) {
         const int valid = j.len - t * 32 < 32 ? j.len - t * 32 : 32;
-        const uint32_t bytes = (uint32_t)(valid - 1) * (uint32_t)krs * 2u + G::ROWBYTES;
         const long at = (long)t * 32 * krs;
-        const i32x4 rk = uniform_rsrc(kbase + at, bytes), rv = uniform_rsrc(vbase + at, bytes);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            const int row = p * RPP + lane / G::NCH;
-            const int x = ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) & (G::NCH - 1);
-            const uint32_t o = row < valid ? (uint32_t)(row * krs) * 2u + (uint32_t)(((lane % G::NCH) ^ x) << 4) : kOOB;
-            lds_dma16(rk, o, (uint32_t)__builtin_amdgcn_readfirstlane((int)(ring_lds + buf * STAGE + p * 1024)));
-            lds_dma16(rv, o, (uint32_t)__builtin_amdgcn_readfirstlane((int)(ring_lds + buf * STAGE + TIMG + p * 1024)));
-        }
+        dma_tile<HD>(ring_lds + buf * STAGE, kbase + at, krs, valid, lane);
+        dma_tile<HD>(ring_lds + buf * STAGE + TIMG, vbase + at, krs, valid, lane);
     };
     f32x16 o[G::DT];
 #pragma unroll
@@ -478,8 +484,10 @@ __global__ __launch_bounds__(256) void k_ext_join(ExtArgs a, const float* __rest
     const int b = bh / a.Hkv, hkv = bh - b * a.Hkv;
     float mx = -kInf, sum = 0.f;
     const long at0 = (long)bh * splits * a.M + r;
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) mx = fmaxf(mx, part_ml[2 * (at0 + (long)s * a.M)]);
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) {
         const long at = at0 + (long)s * a.M;
         const float ms = part_ml[2 * at], f = ms == -kInf ? 0.f : __builtin_amdgcn_exp2f((ms - mx) * a.c);
@@ -520,6 +528,7 @@ __global__ __launch_bounds__(256) void k_ext_sum(const float* __restrict__ part,
     const int bh = (int)(row / rows), r = (int)(row - (long)bh * rows);
     const int b = bh / Hkv, hkv = bh - b * Hkv;
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
     for (int s = 0; s < splits; ++s) {
         const f32x4 u = *reinterpret_cast<const f32x4*>(part + (((long)bh * splits + s) * rows + r) * HD + d);
 #pragma unroll
@@ -557,6 +566,32 @@ __device__ __forceinline__ void store_acc32(const f32x16* t, float* dst, int hal
             for (int e = 0; e < 4; ++e) w[e] = t[dt][4 * jj + e];
             *reinterpret_cast<f32x4*>(dst + dt * 32 + 8 * jj + 4 * half) = w;
         }
+}
+
+// The same 32 rows (lane = row) through a tile image in LDS, so that a store writes whole rows, 16 B a lane: 8-byte pieces of 32
+// rows at a time cost the pass over single queries a quarter of its time.  One wave, its own image.
+template <int HD>
+__device__ __forceinline__ void store_tile(const f32x16* t, char* img, bf16* dst, int rs, int valid, float scale, int lane) {
+    using G = AttnGeo<HD>;
+    constexpr int RPP = 1024 / G::ROWBYTES, NP = 32 / RPP;
+    const int half = lane >> 5, l31 = lane & 31;
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+            bf16x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = (bf16)(t[dt][4 * jj + e] * scale);
+            *reinterpret_cast<bf16x4*>(img + G::swz(l31, dt * 4 + jj) + half * 8) = w;
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        const int row = p * RPP + lane / G::NCH;
+        const int x = ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) & (G::NCH - 1);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(img + p * 1024 + lane * 16);
+        if (row < valid) *reinterpret_cast<u32x4*>(dst + (long)row * rs + ((lane % G::NCH) ^ x) * 8) = v;
+    }
 }
 
 // Row owner: dQ, and D for the key owner (written by split 0).  A softmax over one key is constant, so with len = 1 dS is
@@ -613,13 +648,13 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
         own_frags<HD>(gf, dout + ro, live, half);
         bf16x8 of[G::STEPS], ol[G::STEPS];
         own_frags<HD>(of, out + ro, live, half);
-        if (BIAS && out_lo) own_frags<HD>(ol, out_lo + ro, live, half);
+        if (out_lo) own_frags<HD>(ol, out_lo + ro, live, half);
 #pragma unroll
         for (int s = 0; s < G::STEPS; ++s)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 float v = (float)of[s][k];
-                if (BIAS && out_lo) v += (float)ol[s][k];
+                if (out_lo) v += (float)ol[s][k];
                 d += v * (float)gf[s][k];
             }
         d += __shfl_xor(d, 32, 64);
@@ -679,6 +714,211 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
     else store_acc<HD>(acc, dq + (long)j.b * a.dqv.bs + row_offset(a.dqv, r, j.hkv, a.G, HD), a.scale, half);
 }
 
+// Few rows (at most 32 for a key head: an attention pooling head's query): everything in one pass over K and V.  A wave takes
+// every fourth tile of 32 keys through a ring of its own, makes the tile's scores in both orientations (two small products; the
+// pass is bound by the stream of K, V, dK and dV), stores dK and dV of its keys and keeps its part of dQ, which the four
+// waves join at the end.
+template <int HD>
+__global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_few(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ out_lo,
+                                                        const bf16* __restrict__ dout, const float* __restrict__ stat,
+                                                        bf16* __restrict__ dq, bf16* __restrict__ dk, bf16* __restrict__ dv,
+                                                        float* __restrict__ part, int splits) {
+    using G = AttnGeo<HD>;
+    constexpr int TIMG = 32 * G::ROWBYTES, STAGE = 2 * TIMG, NP = TIMG / 1024;
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // [4 waves][2 stages][K, V], Q image, dO image, [3][32] floats
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Job j = job_of(a, 1, splits);
+    char* ring = smem + wave * 2 * STAGE;
+    const uint32_t ring_lds = lds_address(ring);
+    char* Qs = smem + 8 * STAGE;
+    char* Gs = Qs + TIMG;
+    float* st = reinterpret_cast<float*>(Gs + TIMG);  // -m, -log2 l, -D
+    const bool live = l31 < a.M;
+    const int nt = (j.len + 31) >> 5, all = (a.Sk + 31) >> 5, per = (all + splits - 1) / splits;
+    const int t0 = j.split * per, t1 = t0 + per < all ? t0 + per : all;
+    const bf16* kbase = a.k + (long)j.b * a.kv.bs + (long)j.hkv * HD;
+    const bf16* vbase = a.v + (long)j.b * a.kv.bs + (long)j.hkv * HD;
+    const int krs = (int)a.kv.rs;
+    auto issue = [&](int t, int buf) {
+        const int valid = j.len - t * 32 < 32 ? j.len - t * 32 : 32;
+        const long at = (long)t * 32 * krs;
+        dma_tile<HD>(ring_lds + buf * STAGE, kbase + at, krs, valid, lane);
+        dma_tile<HD>(ring_lds + buf * STAGE + TIMG, vbase + at, krs, valid, lane);
+    };
+    if (t0 + wave < t1 && t0 + wave < nt) issue(t0 + wave, 0);
+    // the rows as operands of both orientations (lane = row), their images for the products over rows, and D
+    bf16x8 qf[G::STEPS], gf[G::STEPS];
+    float mq, lq, d = 0.f;
+    {
+        const long ro = row_offset(a.o, live ? l31 : 0, j.hkv, a.G, HD) + (long)j.b * a.o.bs;
+        own_frags<HD>(qf, a.q + (long)j.b * a.qv.bs + row_offset(a.qv, live ? l31 : 0, j.hkv, a.G, HD), live, half);
+        own_frags<HD>(gf, dout + ro, live, half);
+        bf16x8 of[G::STEPS], ol[G::STEPS];
+        own_frags<HD>(of, out + ro, live, half);
+        if (out_lo) own_frags<HD>(ol, out_lo + ro, live, half);
+#pragma unroll
+        for (int s = 0; s < G::STEPS; ++s)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                float v = (float)of[s][k];
+                if (out_lo) v += (float)ol[s][k];
+                d -= v * (float)gf[s][k];
+            }
+        d += __shfl_xor(d, 32, 64);
+        const long sr = (long)j.bh * a.Mp + l31;
+        mq = live ? stat[sr] : 0.f;
+        lq = live ? stat[a.stat_n + sr] : -kInf;
+        if (wave == 0) {
+#pragma unroll
+            for (int s = 0; s < G::STEPS; ++s) {
+                *reinterpret_cast<bf16x8*>(Qs + G::swz(l31, 2 * s + half)) = qf[s];
+                *reinterpret_cast<bf16x8*>(Gs + G::swz(l31, 2 * s + half)) = gf[s];
+            }
+            if (half == 0) {
+                st[l31] = mq;
+                st[32 + l31] = lq;
+                st[64 + l31] = d;
+            }
+        }
+        if (j.len <= 1) lq = -kInf;  // (dS of one key is zero; P for dV comes from the other orientation)
+    }
+    __syncthreads();
+    f32x16 acc[G::DT];
+#pragma unroll
+    for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+    int buf = 0;
+    for (int t = t0 + wave; t < t1; t += 4) {
+        const int key = t * 32 + l31;
+        const long at = (long)j.b * a.dkv.bs + (long)t * 32 * a.dkv.rs + (long)j.hkv * HD;
+        const int rows = a.Sk - t * 32 < 32 ? a.Sk - t * 32 : 32;
+        if (t >= nt) {  // past the valid keys: zeros
+            const u32x4 z = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const int row = p * (32 / NP) + lane / G::NCH;
+                if (row < rows) {
+                    *reinterpret_cast<u32x4*>(dk + at + (long)row * a.dkv.rs + (lane % G::NCH) * 8) = z;
+                    *reinterpret_cast<u32x4*>(dv + at + (long)row * a.dkv.rs + (lane % G::NCH) * 8) = z;
+                }
+            }
+            continue;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other stage has been read
+        if (t + 4 < t1 && t + 4 < nt) {
+            issue(t + 4, buf ^ 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NP) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const char* Ks = ring + buf * STAGE;
+        const char* Vs = Ks + TIMG;
+        buf ^= 1;  // (this tile's stage is buf ^ 1 from here)
+        bf16x8 kf[G::STEPS], vf[G::STEPS];
+#pragma unroll
+        for (int s = 0; s < G::STEPS; ++s) {
+            kf[s] = G::rows(Ks, l31, s, half);
+            vf[s] = G::rows(Vs, l31, s, half);
+        }
+        {  // lane = row, registers = keys: dQ
+            f32x16 sc, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sc[i] = mq;
+                dp[i] = d;
+            }
+#pragma unroll
+            for (int s = 0; s < G::STEPS; ++s) {
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[s], qf[s], sc, 0, 0, 0);
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[s], gf[s], dp, 0, 0, 0);
+            }
+            if ((t + 1) * 32 > j.len) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (t * 32 + acc_row(i, half) >= j.len) sc[i] = -kInf;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lq));
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+                const bf16x8 ds = acc_to_a(dp, blk);
+#pragma unroll
+                for (int dt = 0; dt < G::DT; ++dt)
+                    acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Ks, blk * 16, dt * 32, lane), ds, acc[dt], 0, 0, 0);
+            }
+        }
+        {  // lane = key, registers = rows: dK, dV
+            f32x16 sc, dp, o[G::DT];
+            f32x4 lr[4];
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+                const f32x4 mr = *reinterpret_cast<const f32x4*>(st + 8 * jj + 4 * half);
+                lr[jj] = *reinterpret_cast<const f32x4*>(st + 32 + 8 * jj + 4 * half);
+                const f32x4 dr = *reinterpret_cast<const f32x4*>(st + 64 + 8 * jj + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[4 * jj + e] = mr[e];
+                    dp[4 * jj + e] = dr[e];
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < G::STEPS; ++s) {
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[s], kf[s], sc, 0, 0, 0);
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gf[s], vf[s], dp, 0, 0, 0);
+            }
+            const bool key_live = key < j.len;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sc[i] = key_live ? __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lr[i >> 2][i & 3])) : 0.f;
+                dp[i] = key_live && j.len > 1 ? dp[i] * sc[i] : 0.f;
+            }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const char* img = g ? Qs : Gs;
+#pragma unroll
+                for (int dt = 0; dt < G::DT; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk) {
+                    const bf16x8 x = acc_to_a(g ? dp : sc, blk);
+#pragma unroll
+                    for (int dt = 0; dt < G::DT; ++dt)
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(img, blk * 16, dt * 32, lane), x, o[dt], 0, 0, 0);
+                }
+                // (the tile's own images are free: its rows are in registers, its columns were read for dQ)
+                store_tile<HD>(o, ring + (buf ^ 1) * STAGE + (g ? 0 : TIMG), (g ? dk : dv) + at, (int)a.dkv.rs, rows, g ? a.scale : 1.f, lane);
+            }
+        }
+    }
+    // the waves' parts of dQ through their rings
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    float* mine = reinterpret_cast<float*>(ring);
+    static_assert(2 * STAGE >= 32 * HD * 4, "the join uses the ring");
+    store_acc32<HD>(acc, mine + l31 * HD, half);
+    __syncthreads();
+    for (int i = tid; i < a.M * (HD / 4); i += 256) {
+        const int r = i / (HD / 4), c = i % (HD / 4) * 4;
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem + w * 2 * STAGE) + r * HD + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += u[e];
+        }
+        if (splits > 1) {
+            *reinterpret_cast<f32x4*>(part + (((long)j.bh * splits + j.split) * a.M + r) * HD + c) = s;
+        } else {
+            bf16x4 w4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w4[e] = (bf16)(s[e] * a.scale);
+            *reinterpret_cast<bf16x4*>(dq + (long)j.b * a.dqv.bs + row_offset(a.dqv, r, j.hkv, a.G, HD) + c) = w4;
+        }
+    }
+}
+
 // dS summed over a part of the batch, for 128 queries x 128 keys of a head a workgroup (a wave: 32 queries, four tiles of 32
 // keys).  The bias of the block and the sums stay in registers while the batch streams through, so a pair costs two
 // multiply-adds and an exponential per sequence; written in register order, [tile][4][64 lanes] x 4 floats.
@@ -706,7 +946,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
         const i32x4 rsrc = uniform_rsrc(a.tab + (long)h * a.Rp, (uint32_t)a.Rp * 4u);
         for (int p = wave; p * 256 < a.Rp; p += 4)
             lds_dma16(rsrc, (uint32_t)(p * 1024 + lane * 16), (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + p * 1024)));
-        const int qc = (int)lds0 + (q < a.Sk ? a.q_codes4[q] : 0), top = (int)lds0 + (a.R - 1) * 4;
+        const int qc = (int)lds0 + a.q_codes4[q], top = (int)lds0 + (a.R - 1) * 4;
         dma_barrier();
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
@@ -789,8 +1029,8 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
 }
 
 // The pairs' sums by entry: a workgroup takes a tile row (32 queries) of a head and one of `parts` ranges of its key tiles; its
-// waves take every fourth tile, each with a histogram of its own.  LDS float adds run at some 200 cycles an instruction
-// here, which is why the batch is summed first; a tile whose pairs all fall on one entry (far positions) costs one add.
+// waves take every fourth tile, each with a histogram of its own.  LDS float adds take a cycle a lane, and many times that where
+// lanes meet on one address: the batch is summed first, and pairs past either end of the table are summed in registers.
 __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __restrict__ dense, float* __restrict__ slab, RelBlocks w,
                                                      int parts) {
     extern __shared__ __attribute__((aligned(16))) char smem[];  // [4][Rp] floats
@@ -802,46 +1042,44 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
     const int base = (int)lds_address(hist), top = base + (a.R - 1) * 4;
     for (int i = lane; i < a.Rp; i += 64) hist[i] = 0.f;
     const int q = (w.q0 * 4 + qt) * 32 + l31;
-    const int qc = base + (q < a.Sk ? a.q_codes4[q] : 0);
+    const int qc = base + a.q_codes4[q];
     const int live_t = (a.Sk + 31) / 32, per = (live_t + parts - 1) / parts;
     const int t1 = (part + 1) * per < live_t ? (part + 1) * per : live_t;
+    float ends[2] = {0.f, 0.f};
     for (int kt = part * per + wave; kt < t1; kt += 4) {
         float v[16];
-        int at[16], lo = 0x7fffffff, hi = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.f;
+        const float* src = dense + (((long)hl * nqt + qt) * nkt + kt) * 1024 + lane * 4;
+        const long step = (long)w.heads * nqt * nkt * 1024;
+#pragma unroll 4
+        for (int ch = 0; ch < w.chunks; ++ch) {
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+                const f32x4 t = *reinterpret_cast<const f32x4*>(src + ch * step + jj * 256);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * jj + e] += t[e];
+            }
+        }
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
             const i32x4 kc = *reinterpret_cast<const i32x4*>(a.k_codes4 + kt * 32 + 8 * jj + 4 * half);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int i = 4 * jj + e;
-                at[i] = bias_at(qc, kc[e], base, top) - base;
-                lo = at[i] < lo ? at[i] : lo;
-                hi = at[i] > hi ? at[i] : hi;
-                v[i] = 0.f;
+                const int at = bias_at(qc, kc[e], base, top);
+                const float x = v[4 * jj + e];
+                ends[0] += at == base ? x : 0.f;
+                ends[1] += at == top && top != base ? x : 0.f;
+                if (at != base && at != top)
+                    __hip_atomic_fetch_add(reinterpret_cast<float*>(reinterpret_cast<char*>(hist) + (at - base)), x, __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_WORKGROUP);
             }
         }
-        for (int ch = 0; ch < w.chunks; ++ch) {
-            const float* src = dense + ((((long)ch * w.heads + hl) * nqt + qt) * nkt + kt) * 1024 + lane * 4;
+    }
 #pragma unroll
-            for (int jj = 0; jj < 4; ++jj) {
-                const f32x4 t = *reinterpret_cast<const f32x4*>(src + jj * 256);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * jj + e] += t[e];
-            }
-        }
-        const int one = __builtin_amdgcn_readfirstlane(lo);
-        if (__all(lo == hi && lo == one)) {
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s += v[i];
-            s = wave_sum(s);
-            if (lane == 0) hist[one >> 2] += s;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                __hip_atomic_fetch_add(reinterpret_cast<float*>(reinterpret_cast<char*>(hist) + at[i]), v[i], __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
+    for (int i = 0; i < 2; ++i) {
+        ends[i] = wave_sum(ends[i]);
+        if (lane == 0) hist[i * (a.R - 1)] += ends[i];
     }
     __syncthreads();
     float* dst = slab + ((long)(hl + w.h0) * w.slab_rows + (long)(w.q0 * 4 + qt) * parts + part) * a.Rp;
@@ -985,7 +1223,8 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
 
 // ------------------------------------------------------------------------------------------------------- bias tables
 // tab[h][r] = table[bucket_of[r]][h] * sqrt(hd) (the scores are scaled after the bias is added), zero where the entry names no
-// bucket; byte offsets of the position codes, padded with zeros to a multiple of 128
+// bucket; byte offsets of the position codes, padded with the last one to a multiple of 128 (what is past the end then falls
+// on an entry that its neighbours use)
 __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ table, const int* __restrict__ bucket_of,
                                                      const int* __restrict__ q_codes, const int* __restrict__ k_codes,
                                                      float* __restrict__ tab, int* __restrict__ q4, int* __restrict__ k4, int R,
@@ -1004,7 +1243,7 @@ __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ t
     const long w = i - (long)H * Rp;
     const int at = (int)(w % Sp);
     const int* src = w < Sp ? q_codes : k_codes;
-    int c = at < S ? src[at] : 0;
+    int c = src[at < S ? at : S - 1];
     c = c < -(1 << 28) ? -(1 << 28) : c > (1 << 28) - 1 ? (1 << 28) - 1 : c;  // differences of the byte offsets fit 32 bits
     (w < Sp ? q4 : k4)[at] = c * 4;
 }
@@ -1076,6 +1315,8 @@ void fwd(const ExtArgs& a, const ExtPlan& p, void* out, void* out_lo, float* sta
             PDT_EXT_FWD(true, true)
         } else if (a.tab) {
             PDT_EXT_FWD(true, false)
+        } else if (out_lo) {
+            PDT_EXT_FWD(false, true)
         } else {
             PDT_EXT_FWD(false, false)
         }
@@ -1092,6 +1333,12 @@ template <int HD>
 void bwd(const ExtArgs& a, const ExtBwd& w, hipStream_t s) {
     const ExtPlan &pq = w.q, &pk = w.kv;
     const dim3 gq((unsigned)((long)a.B * a.Hkv * pq.tiles * pq.splits)), gk((unsigned)((long)a.B * a.Hkv * pk.tiles * pk.splits));
+    if (pq.few) {
+        const size_t lds = (size_t)(16 + 2) * 32 * HD * 2 + 3 * 32 * sizeof(float);
+        allow_lds(&k_ext_bwd_few<HD>, lds);
+        hipLaunchKernelGGL((k_ext_bwd_few<HD>), gq, dim3(256), lds, s, a, (const bf16*)w.out, (const bf16*)w.out_lo, (const bf16*)w.dout,
+                           w.stat, (bf16*)w.dq, (bf16*)w.dk, (bf16*)w.dv, w.part_q, pq.splits);
+    } else {
     const size_t lq = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + table_bytes(a);
     const size_t lk = (size_t)4 * 64 * HD * 2 + 8192 + table_bytes(a);
 #define PDT_EXT_BWD(BIAS)                                                                                                  \
@@ -1107,6 +1354,7 @@ void bwd(const ExtArgs& a, const ExtBwd& w, hipStream_t s) {
         PDT_EXT_BWD(false)
     }
 #undef PDT_EXT_BWD
+    }
     const long BH = (long)a.B * a.Hkv;
     if (pq.splits > 1) {
         const long total = BH * a.M * (HD / 4);
@@ -1134,19 +1382,25 @@ int splits_for(long groups, long blocks, long least) {
 
 }  // namespace
 
-ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool bias) {
+ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool streams /* a plain forward: no bias, no remainder kept */) {
     ExtPlan p;
-    p.few = !bias && M <= 32;
+    p.few = streams && M <= 32;
     p.tiles = p.few ? 1 : (M + 127) / 128;
     p.splits = p.few ? splits_for(BH, (Sk + 31) / 32, 8) : splits_for(BH * p.tiles, (Sk + 63) / 64, 4);
     return p;
 }
-ExtPlan ext_plan_bwd(long BH, int own, int other) {
-    ExtPlan p;
-    p.few = false;
-    p.tiles = (own + 127) / 128;
-    p.splits = splits_for(BH * p.tiles, (other + 63) / 64, 4);
-    return p;
+void ext_plan_bwd(long BH, int M, int Sk, bool bias, ExtPlan& q, ExtPlan& kv) {
+    q.few = kv.few = !bias && M <= 32;
+    if (q.few) {  // one kernel
+        q.tiles = 1;
+        q.splits = splits_for(BH, (Sk + 31) / 32, 8);
+        kv.tiles = kv.splits = 0;
+        return;
+    }
+    q.tiles = (M + 127) / 128;
+    q.splits = splits_for(BH * q.tiles, (Sk + 63) / 64, 4);
+    kv.tiles = (Sk + 127) / 128;
+    kv.splits = splits_for(BH * kv.tiles, (M + 63) / 64, 4);
 }
 
 void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, void* out_lo, float* stat, float* part, float* part_ml,

@@ -631,17 +631,17 @@ def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, leng
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, kv, heads, kv_heads, lengths, be):
-        out, lse = be.cross_attention_fwd(q, kv, heads, kv_heads, lengths, True)
-        ctx.save_for_backward(q, kv, out, lse, lengths)
+        out, lse, lo = be.cross_attention_fwd(q, kv, heads, kv_heads, lengths, True)
+        ctx.save_for_backward(q, kv, out, lo, lse, lengths)
         ctx.cfg = (be, heads, kv_heads)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, kv, out, lse, lengths = ctx.saved_tensors
+        q, kv, out, lo, lse, lengths = ctx.saved_tensors
         be, heads, kv_heads = ctx.cfg
-        dq, dkv = be.cross_attention_bwd(dout, q, kv, out, lse, heads, kv_heads, lengths)
+        dq, dkv = be.cross_attention_bwd(dout, q, kv, out, lo, lse, heads, kv_heads, lengths)
         return dq, dkv, None, None, None, None
 
 

@@ -309,13 +309,13 @@ def rel_bias_attention_bwd(dout, qkv, out, out_lo, lse, tab, codes, bucket_of, b
 
 
 def cross_attention_fwd(q, kv, heads: int, kv_heads: int, lengths=None, grad: bool = True):
-    """-> (out [B, Sq, H*hd], statistics for the backward, or None)"""
+    """-> (out [B, Sq, H*hd], statistics, out_lo): what the backward wants back, or None"""
     return _C.cross_attention_fwd(q, kv, heads, kv_heads, _i32(lengths), grad)
 
 
-def cross_attention_bwd(dout, q, kv, out, lse, heads: int, kv_heads: int, lengths=None):
+def cross_attention_bwd(dout, q, kv, out, out_lo, lse, heads: int, kv_heads: int, lengths=None):
     """-> (dq, dkv)"""
-    return _C.cross_attention_bwd(_al(dout), q, kv, out, lse, heads, kv_heads, _i32(lengths))
+    return _C.cross_attention_bwd(_al(dout), q, kv, out, out_lo, lse, heads, kv_heads, _i32(lengths))
 
 
 # ------------------------------------------------------------------------- gated norm (csrc/kernels/gated_norm.hip)

@@ -302,12 +302,12 @@ def _cross_rows(t, q, heads, kv_heads):
 
 
 def cross_attention_fwd(q, kv, heads: int, kv_heads: int, lengths=None, grad: bool = True):
-    """Oracle of csrc/kernels/attention_ext.hip -> (out, None)"""
+    """Oracle of csrc/kernels/attention_ext.hip -> (out, None, None)"""
     qf, k, v = _cross_parts(q, kv, heads, kv_heads, lengths)
-    return _cross_rows(torch.matmul(_ext_probs(qf, k, None, lengths), v), q, heads, kv_heads), None
+    return _cross_rows(torch.matmul(_ext_probs(qf, k, None, lengths), v), q, heads, kv_heads), None, None
 
 
-def cross_attention_bwd(dout, q, kv, out, lse, heads: int, kv_heads: int, lengths=None):
+def cross_attention_bwd(dout, q, kv, out, out_lo, lse, heads: int, kv_heads: int, lengths=None):
     b, sk = kv.shape[:2]
     qf, k, v = _cross_parts(q, kv, heads, kv_heads, lengths)
     do = _cross_parts(dout, kv, heads, kv_heads, None)[0]
