@@ -11,8 +11,9 @@
 // Bound by memory: forward 2 reads + 2 writes, backward 4 reads + 2 writes of 2 bytes per element.  x and y are what the
 // backward reads again (not u): u is recomputed in fp32, so the parameter gradients see the numbers that the forward normalised,
 // at no more traffic than a saved u would cost.  One wave holds a row in registers (4 channels a lane and piece, NP pieces of
-// 256 channels); the column sums stay in registers over all rows a wave visits, are added over the waves in LDS and over the
-// workgroups in a fixed order (no atomics).
+// 256 channels) and walks over rows with the parameters in registers (read again for every row they were 2.7 times the
+// row's own bytes) and the next row's loads in flight.  Row sums by DPP, not through LDS.  The column sums stay in registers over
+// all rows a wave visits, are added over the waves in LDS and over the workgroups in a fixed order (no atomics).
 #include "common.h"
 #include "gated_norm.h"
 
@@ -21,98 +22,133 @@ namespace {
 
 constexpr int kMaxPieces = 8;  // D <= 2048
 
-__device__ __forceinline__ void load4(float* v, const bf16* p, bool in) {
+__device__ __forceinline__ bf16x4 raw4(const bf16* p, bool in) {
     bf16x4 t = {(bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f};
     if (in) t = *reinterpret_cast<const bf16x4*>(p);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = (float)t[k];
+    return t;
 }
 __device__ __forceinline__ f32x4 par4(const float* p, bool in) {
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
     if (in) t = *reinterpret_cast<const f32x4*>(p);
     return t;
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+// sum over the 64 lanes, the same in all: pairs, quads, half rows, rows of 16, then rows into the last one
+__device__ __forceinline__ float row_sum(float v) {
+    v = dpp_add<0xB1, 0xf>(v);   // lanes ^ 1
+    v = dpp_add<0x4E, 0xf>(v);   // lanes ^ 2
+    v = dpp_add<0x141, 0xf>(v);  // mirrored within 8
+    v = dpp_add<0x140, 0xf>(v);  // mirrored within 16
+    v = dpp_add<0x142, 0xa>(v);  // row 0 into 1, 2 into 3
+    v = dpp_add<0x143, 0xc>(v);  // rows 0 and 1 into 2 and 3
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
 
 template <int NP, bool POST>
-__global__ __launch_bounds__(256) void k_gn_fwd(GatedNorm p, bf16* __restrict__ u_out, bf16* __restrict__ n_out,
-                                                float* __restrict__ stats /* [4][M], or null */) {
-    const int lane = threadIdx.x & 63;
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+__global__ __launch_bounds__(256, NP <= 4 ? 4 : 2) void k_gn_fwd(GatedNorm p, bf16* __restrict__ u_out, bf16* __restrict__ n_out,
+                                                                  float* __restrict__ stats /* [2 or 4][M], or null */) {
+    const int lane = threadIdx.x & 63, D = p.D, np4 = D >> 2;
+    const long stride = (long)gridDim.x * 4;
+    long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= p.M) return;
-    const int D = p.D, np4 = D >> 2;
     const float inv_d = 1.f / (float)D;
-    const float* gate = p.gate + (p.per_sample ? row / p.T * D : 0);
-    float x[NP][4], y[NP][4];
-    float s = 0.f;
+    f32x4 ga[NP], w[NP], b[NP], pw[POST ? NP : 1], pb[POST ? NP : 1];
+    bf16x4 xn[NP], yn[NP];
+    auto fetch = [&](long r) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int c = lane + 64 * j;
+            xn[j] = raw4(p.x + r * D + 4 * c, c < np4);
+            yn[j] = raw4(p.y + r * D + 4 * c, c < np4);
+        }
+    };
+    fetch(row);
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
         const int c = lane + 64 * j;
-        load4(x[j], p.x + row * D + 4 * c, c < np4);
-        load4(y[j], p.y + row * D + 4 * c, c < np4);
+        w[j] = par4(p.w + 4 * c, c < np4);
+        b[j] = par4(p.b + 4 * c, c < np4);
+        if (POST) {
+            pw[j] = par4(p.pw + 4 * c, c < np4);
+            pb[j] = par4(p.pb + 4 * c, c < np4);
+        }
     }
-    if (POST) {
-#pragma unroll
-        for (int j = 0; j < NP; ++j)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s += y[j][k];
-        const float mean = wave_sum(s) * inv_d;
-        float q = 0.f;
+    long sample = -1;
+    for (; row < p.M; row += stride) {
+        float x[NP][4], y[NP][4];
 #pragma unroll
         for (int j = 0; j < NP; ++j)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float d = lane + 64 * j < np4 ? y[j][k] - mean : 0.f;
-                q += d * d;
+                x[j][k] = (float)xn[j][k];
+                y[j][k] = (float)yn[j][k];
             }
-        const float rstd = rsqrtf(wave_sum(q) * inv_d + p.eps);
+        if (row + stride < p.M) fetch(row + stride);
+        const long own = p.per_sample ? row / p.T : 0;
+        if (own != sample) {
+            sample = own;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) ga[j] = par4(p.gate + own * D + 4 * (lane + 64 * j), lane + 64 * j < np4);
+        }
+        float s = 0.f, q = 0.f;
+        if (POST) {
+#pragma unroll
+            for (int j = 0; j < NP; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s += y[j][k];
+            const float mean = row_sum(s) * inv_d;
+#pragma unroll
+            for (int j = 0; j < NP; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float d = lane + 64 * j < np4 ? y[j][k] - mean : 0.f;
+                    q += d * d;
+                }
+            const float rstd = rsqrtf(row_sum(q) * inv_d + p.eps);
+#pragma unroll
+            for (int j = 0; j < NP; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[j][k] = (y[j][k] - mean) * rstd * pw[j][k] + pb[j][k];
+            if (stats && lane == 0) {
+                stats[2 * p.M + row] = mean;
+                stats[3 * p.M + row] = rstd;
+            }
+        }
+        s = q = 0.f;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-            const bool in = lane + 64 * j < np4;
-            const f32x4 w = par4(p.pw + 4 * (lane + 64 * j), in), b = par4(p.pb + 4 * (lane + 64 * j), in);
+            bf16x4 o;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[j][k] = (y[j][k] - mean) * rstd * w[k] + b[k];
+            for (int k = 0; k < 4; ++k) {
+                x[j][k] = p.a * x[j][k] + ga[j][k] * y[j][k];
+                s += x[j][k];
+                o[k] = (bf16)x[j][k];
+            }
+            if (lane + 64 * j < np4) *reinterpret_cast<bf16x4*>(u_out + row * D + 4 * (lane + 64 * j)) = o;
+        }
+        const float mean = row_sum(s) * inv_d;
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float d = lane + 64 * j < np4 ? x[j][k] - mean : 0.f;
+                q += d * d;
+            }
+        const float rstd = rsqrtf(row_sum(q) * inv_d + p.eps);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            bf16x4 o;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = (bf16)((x[j][k] - mean) * rstd * w[j][k] + b[j][k]);
+            if (lane + 64 * j < np4) *reinterpret_cast<bf16x4*>(n_out + row * D + 4 * (lane + 64 * j)) = o;
         }
         if (stats && lane == 0) {
-            stats[2 * p.M + row] = mean;
-            stats[3 * p.M + row] = rstd;
+            stats[row] = mean;
+            stats[p.M + row] = rstd;
         }
-    }
-    s = 0.f;
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const bool in = lane + 64 * j < np4;
-        const f32x4 g = par4(gate + 4 * (lane + 64 * j), in);
-        bf16x4 o;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            x[j][k] = p.a * x[j][k] + g[k] * y[j][k];
-            s += x[j][k];
-            o[k] = (bf16)x[j][k];
-        }
-        if (in) *reinterpret_cast<bf16x4*>(u_out + row * D + 4 * (lane + 64 * j)) = o;
-    }
-    const float mean = wave_sum(s) * inv_d;
-    float q = 0.f;
-#pragma unroll
-    for (int j = 0; j < NP; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float d = lane + 64 * j < np4 ? x[j][k] - mean : 0.f;
-            q += d * d;
-        }
-    const float rstd = rsqrtf(wave_sum(q) * inv_d + p.eps);
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int c = lane + 64 * j;
-        const f32x4 w = par4(p.w + 4 * c, c < np4), b = par4(p.b + 4 * c, c < np4);
-        bf16x4 o;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = (bf16)((x[j][k] - mean) * rstd * w[k] + b[k]);
-        if (c < np4) *reinterpret_cast<bf16x4*>(n_out + row * D + 4 * c) = o;
-    }
-    if (stats && lane == 0) {
-        stats[row] = mean;
-        stats[p.M + row] = rstd;
     }
 }
 
@@ -151,117 +187,115 @@ __device__ __forceinline__ void column_sum(float (&v)[NP][4], float* red, float*
 // A unit is one of `chunks` parts of a sample's rows; a workgroup takes the units blockIdx.x, + gridDim.x, ...  The gate's sums
 // leave after every unit (to gate_part + unit * gate_stride), the others at the end (slab [gridDim.x][srow]: db, dw, dpb, dpw).
 template <int NP, bool POST>
-__global__ __launch_bounds__(256) void k_gn_bwd(GatedNorm p, const bf16* __restrict__ du, const bf16* __restrict__ dn,
-                                                const float* __restrict__ stats, bf16* __restrict__ dx, bf16* __restrict__ dy,
-                                                float* __restrict__ gate_part, long gate_stride, float* __restrict__ slab, int srow,
-                                                int chunks, long units) {
+__global__ __launch_bounds__(256, NP <= (POST ? 4 : 6) ? 2 : 1) void k_gn_bwd(
+    GatedNorm p, const bf16* __restrict__ du, const bf16* __restrict__ dn, const float* __restrict__ stats, bf16* __restrict__ dx,
+    bf16* __restrict__ dy, float* __restrict__ gate_part, long gate_stride, float* __restrict__ slab, int srow, int chunks, long units) {
     extern __shared__ __attribute__((aligned(16))) float red[];  // [3][NP * 256]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int D = p.D, np4 = D >> 2;
     const float inv_d = 1.f / (float)D;
     float sg[NP][4], sw[NP][4], sb[NP][4], spw[POST ? NP : 1][4], spb[POST ? NP : 1][4];
+    f32x4 ga[NP], w[NP], pw[POST ? NP : 1], pb[POST ? NP : 1];
 #pragma unroll
-    for (int j = 0; j < NP; ++j)
+    for (int j = 0; j < NP; ++j) {
+        const int c = lane + 64 * j;
+        w[j] = par4(p.w + 4 * c, c < np4);
+        if (POST) {
+            pw[j] = par4(p.pw + 4 * c, c < np4);
+            pb[j] = par4(p.pb + 4 * c, c < np4);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             sg[j][k] = sw[j][k] = sb[j][k] = 0.f;
             if (POST) spw[j][k] = spb[j][k] = 0.f;
         }
+    }
     const long rows = p.per_sample ? p.T : p.M, per = (rows + chunks - 1) / chunks;
     for (long unit = blockIdx.x; unit < units; unit += gridDim.x) {
         const long b = unit / chunks, ch = unit - b * chunks;
         const long r0 = b * rows + ch * per, r1 = r0 + per < (b + 1) * rows ? r0 + per : (b + 1) * rows;
         const float* gate = p.gate + (p.per_sample ? b * D : 0);
-        for (long row = r0 + wave; row < r1; row += 4) {
-            float x[NP][4], y[NP][4], g[NP][4], d[NP][4];
+        bf16x4 xn[NP], yn[NP], gn[NP], en[NP];
+        f32x4 st;
+        auto fetch = [&](long r) {
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
                 const int c = lane + 64 * j;
                 const bool in = c < np4;
-                load4(x[j], p.x + row * D + 4 * c, in);
-                load4(y[j], p.y + row * D + 4 * c, in);
-                load4(d[j], dn + row * D + 4 * c, in && dn);
-                load4(g[j], du + row * D + 4 * c, in && du);
+                xn[j] = raw4(p.x + r * D + 4 * c, in);
+                yn[j] = raw4(p.y + r * D + 4 * c, in);
+                en[j] = raw4(dn + r * D + 4 * c, in && dn);
+                gn[j] = raw4(du + r * D + 4 * c, in && du);
             }
-            const float mu = stats[row], ru = stats[p.M + row];
-            float my = 0.f, ry = 1.f;
+            st[0] = stats[r];
+            st[1] = stats[p.M + r];
             if (POST) {
-                my = stats[2 * p.M + row];
-                ry = stats[3 * p.M + row];
+                st[2] = stats[2 * p.M + r];
+                st[3] = stats[3 * p.M + r];
             }
-            // x <- uh, y <- yh (or y), s1 / s2: sums of dn w and dn w uh
-            float s1 = 0.f, s2 = 0.f;
+        };
+        if (r0 + wave < r1) fetch(r0 + wave);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) ga[j] = par4(gate + 4 * (lane + 64 * j), lane + 64 * j < np4);
+        for (long row = r0 + wave; row < r1; row += 4) {
+            float x[NP][4], y[NP][4];  // uh; yh, or y
+            bf16x4 e[NP], g[NP];
+            const float mu = st[0], ru = st[1], my = st[2], ry = st[3];
+            float s1 = 0.f, s2 = 0.f;  // sums of dn w and dn w uh
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
-                const int c = lane + 64 * j;
-                const bool in = c < np4;
-                const f32x4 ga = par4(gate + 4 * c, in), w = par4(p.w + 4 * c, in);
-                f32x4 pw = {1.f, 1.f, 1.f, 1.f}, pb = {0.f, 0.f, 0.f, 0.f};
-                if (POST) {
-                    pw = par4(p.pw + 4 * c, in);
-                    pb = par4(p.pb + 4 * c, in);
-                }
+                e[j] = en[j];
+                g[j] = gn[j];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    float z = y[j][k];
-                    if (POST) {
-                        y[j][k] = (y[j][k] - my) * ry;
-                        z = y[j][k] * pw[k] + pb[k];
-                    }
-                    x[j][k] = in ? (p.a * x[j][k] + ga[k] * z - mu) * ru : 0.f;
-                    sw[j][k] += d[j][k] * x[j][k];
-                    sb[j][k] += d[j][k];
-                    const float t = d[j][k] * w[k];
+                    float z = (float)yn[j][k];
+                    if (POST) z = (z - my) * ry;
+                    y[j][k] = z;
+                    if (POST) z = z * pw[j][k] + pb[j][k];
+                    x[j][k] = (p.a * (float)xn[j][k] + ga[j][k] * z - mu) * ru;
+                    const float d = (float)en[j][k];  // (zero past the end, and so is all that follows from it)
+                    sw[j][k] += d * x[j][k];
+                    sb[j][k] += d;
+                    const float t = d * w[j][k];
                     s1 += t;
                     s2 += t * x[j][k];
                 }
             }
-            s1 = wave_sum(s1) * inv_d;
-            s2 = wave_sum(s2) * inv_d;
+            if (row + 4 < r1) fetch(row + 4);
+            s1 = row_sum(s1) * inv_d;
+            s2 = row_sum(s2) * inv_d;
             float s3 = 0.f, s4 = 0.f;
+            float dz[NP][4];
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
-                const int c = lane + 64 * j;
-                const bool in = c < np4;
-                const f32x4 ga = par4(gate + 4 * c, in), w = par4(p.w + 4 * c, in);
-                f32x4 pw = {1.f, 1.f, 1.f, 1.f}, pb = {0.f, 0.f, 0.f, 0.f};
-                if (POST) {
-                    pw = par4(p.pw + 4 * c, in);
-                    pb = par4(p.pb + 4 * c, in);
-                }
+                const bool in = lane + 64 * j < np4;
                 bf16x4 o;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float gk = in ? g[j][k] + ru * (d[j][k] * w[k] - s1 - x[j][k] * s2) : 0.f;
+                    const float gk = in ? (float)g[j][k] + ru * ((float)e[j][k] * w[j][k] - s1 - x[j][k] * s2) : 0.f;
                     o[k] = (bf16)(p.a * gk);
-                    const float z = POST ? y[j][k] * pw[k] + pb[k] : y[j][k];
-                    sg[j][k] += gk * z;
-                    const float dz = gk * ga[k];
-                    g[j][k] = dz;
+                    sg[j][k] += gk * (POST ? y[j][k] * pw[j][k] + pb[j][k] : y[j][k]);
+                    dz[j][k] = gk * ga[j][k];
                     if (POST) {
-                        spw[j][k] += dz * y[j][k];
-                        spb[j][k] += dz;
-                        const float t = dz * pw[k];
+                        spw[j][k] += dz[j][k] * y[j][k];
+                        spb[j][k] += dz[j][k];
+                        const float t = dz[j][k] * pw[j][k];
                         s3 += t;
                         s4 += t * y[j][k];
                     }
                 }
-                if (in) *reinterpret_cast<bf16x4*>(dx + row * D + 4 * c) = o;
+                if (in) *reinterpret_cast<bf16x4*>(dx + row * D + 4 * (lane + 64 * j)) = o;
             }
             if (POST) {
-                s3 = wave_sum(s3) * inv_d;
-                s4 = wave_sum(s4) * inv_d;
+                s3 = row_sum(s3) * inv_d;
+                s4 = row_sum(s4) * inv_d;
             }
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
-                const int c = lane + 64 * j;
-                const bool in = c < np4;
-                f32x4 pw = {1.f, 1.f, 1.f, 1.f};
-                if (POST) pw = par4(p.pw + 4 * c, in);
                 bf16x4 o;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o[k] = (bf16)(POST ? ry * (g[j][k] * pw[k] - s3 - y[j][k] * s4) : g[j][k]);
-                if (in) *reinterpret_cast<bf16x4*>(dy + row * D + 4 * c) = o;
+                for (int k = 0; k < 4; ++k) o[k] = (bf16)(POST ? ry * (dz[j][k] * pw[j][k] - s3 - y[j][k] * s4) : dz[j][k]);
+                if (lane + 64 * j < np4) *reinterpret_cast<bf16x4*>(dy + row * D + 4 * (lane + 64 * j)) = o;
             }
         }
         column_sum<NP>(sg, red, gate_part + unit * gate_stride, lane, wave, np4);
@@ -304,7 +338,8 @@ bool gated_norm_dim_ok(long D) { return D >= 4 && D % 4 == 0 && D <= kMaxPieces 
     }
 
 void launch_gated_norm_fwd(const GatedNorm& p, void* u, void* n, float* stats, hipStream_t s) {
-    const unsigned grid = (unsigned)((p.M + 3) / 4);
+    const long full = (p.M + 3) / 4;
+    const unsigned grid = (unsigned)(full < 1024 ? full : 1024);  // (4 per CU walk over the rows)
     PDT_GN_DISPATCH(p.D, {
         if (p.pw) hipLaunchKernelGGL((k_gn_fwd<NP, true>), dim3(grid), dim3(256), 0, s, p, (bf16*)u, (bf16*)n, stats);
         else hipLaunchKernelGGL((k_gn_fwd<NP, false>), dim3(grid), dim3(256), 0, s, p, (bf16*)u, (bf16*)n, stats);
@@ -312,15 +347,15 @@ void launch_gated_norm_fwd(const GatedNorm& p, void* u, void* n, float* stats, h
 }
 
 GatedNormPlan gated_norm_plan(long B, long T, long M, bool per_sample) {
-    // about 1024 workgroups (4 per CU) of at least 8 rows
+    // about 512 workgroups (2 per CU) of at least 8 rows: at 1024 their partial sums were a quarter of the kernel's traffic
     GatedNormPlan q;
     const long samples = per_sample ? B : 1, rows = per_sample ? T : M;
-    long c = (1024 + samples - 1) / samples;
+    long c = (512 + samples - 1) / samples;
     if (c > (rows + 7) / 8) c = (rows + 7) / 8;
     if (per_sample && c > 256) c = 256;  // (k_gate_sum walks over a sample's chunks)
     q.chunks = (int)(c < 1 ? 1 : c);
     q.units = samples * q.chunks;
-    q.blocks = (int)(q.units < 1024 ? q.units : 1024);
+    q.blocks = (int)(q.units < 512 ? q.units : 512);
     return q;
 }
 

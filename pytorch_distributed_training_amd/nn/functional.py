@@ -676,28 +676,6 @@ def cross_attention(q, kv, heads: int, kv_heads: int | None = None, lengths=None
     return _CrossAttentionFn.apply(q, kv, heads, kv_heads, lengths, be)
 
 
-class _GatedResidualNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, branch, gate, weight, bias, post_weight, post_bias, eps, scale, be):
-        ps = [None if t is None else t.float().contiguous() for t in (gate, weight, bias, post_weight, post_bias)]
-        new, normed, stats = be.gated_norm_fwd(x, branch, *ps, eps, scale, True)
-        ctx.save_for_backward(x, branch, *ps, stats)
-        ctx.cfg = (be, eps, scale, [None if t is None else t.dtype for t in (gate, weight, bias, post_weight, post_bias)])
-        ctx.set_materialize_grads(False)
-        return new, normed
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dnew, dnormed):
-        if dnew is None and dnormed is None:
-            return (None,) * 10
-        x, branch, *ps, stats = ctx.saved_tensors
-        be, eps, scale, dts = ctx.cfg
-        dx, dy, *dps = be.gated_norm_bwd(dnew, dnormed, x, branch, *ps, stats, eps, scale)
-        dps += [None] * (5 - len(dps))
-        return (dx, dy, *(None if t is None else t.to(dt) for t, dt in zip(dps, dts)), None, None, None)
-
-
 def gated_residual_norm(x, branch, gate, weight, bias, eps: float = 1e-6, post_weight=None, post_bias=None,
                         residual_scale: float = 1.0):
     """The end of a residual block and the norm of the next one, in one pass -> ``(x_new, normed)``:
@@ -725,11 +703,7 @@ def gated_residual_norm(x, branch, gate, weight, bias, eps: float = 1e-6, post_w
         if why is not None:
             _note_fallback("gated_residual_norm", why)
             be = reference
-    x, branch = x.contiguous(), branch.contiguous()
-    if not _wants_grad(x, branch, gate, weight, bias, post_weight, post_bias):
-        ps = [None if t is None else t.float().contiguous() for t in (gate, weight, bias, post_weight, post_bias)]
-        return be.gated_norm_fwd(x, branch, *ps, float(eps), float(residual_scale), False)[:2]
-    return _GatedResidualNormFn.apply(x, branch, gate, weight, bias, post_weight, post_bias, float(eps), float(residual_scale), be)
+    return be.gated_residual_norm(x, branch, gate, weight, bias, float(eps), post_weight, post_bias, float(residual_scale))
 
 
 # ------------------------------------------------------------------- linear

@@ -319,15 +319,9 @@ def cross_attention_bwd(dout, q, kv, out, out_lo, lse, heads: int, kv_heads: int
 
 
 # ------------------------------------------------------------------------- gated norm (csrc/kernels/gated_norm.hip)
-def gated_norm_fwd(x, branch, gate, weight, bias, post_weight, post_bias, eps: float, scale: float, grad: bool = True):
-    """-> (x_new, normed, statistics for the backward, or None); parameters fp32"""
-    return _C.gated_norm_fwd(_al(x), _al(branch), _al(gate), _al(weight), _al(bias), _al(post_weight), _al(post_bias), eps, scale, grad)
-
-
-def gated_norm_bwd(dnew, dnormed, x, branch, gate, weight, bias, post_weight, post_bias, stats, eps: float, scale: float):
-    """-> [dx, dbranch, dgate, dweight, dbias (, dpost_weight, dpost_bias)]; a gradient that is None counts as zeros"""
-    return _C.gated_norm_bwd(_al(dnew), _al(dnormed), _al(x), _al(branch), _al(gate), _al(weight), _al(bias), _al(post_weight),
-                             _al(post_bias), stats, eps, scale)
+def gated_residual_norm(x, branch, gate, weight, bias, eps: float, post_weight, post_bias, scale: float):
+    """-> (x_new, normed), differentiable (the autograd node is in the extension)"""
+    return _C.gated_residual_norm(x, branch, gate, weight, bias, post_weight, post_bias, eps, scale)
 
 
 # ------------------------------------------------------------------- linear

@@ -334,14 +334,15 @@ def _gated_parts(x, branch, gate, post_weight, post_bias, eps, scale):
     return g, yh, yr, z, scale * xf + g * z
 
 
-def gated_norm_fwd(x, branch, gate, weight, bias, post_weight, post_bias, eps: float, scale: float, grad: bool = True):
-    """Oracle of csrc/kernels/gated_norm.hip -> (x_new, normed, None)"""
+def gated_norm_fwd(x, branch, gate, weight, bias, post_weight, post_bias, eps: float, scale: float):
+    """Oracle of csrc/kernels/gated_norm.hip -> (x_new, normed)"""
     new = _gated_parts(x, branch, gate, post_weight, post_bias, eps, scale)[4]
     normed = _normalise(new, eps)[0] * weight.to(new.dtype) + bias.to(new.dtype)
-    return new.to(x.dtype), normed.to(x.dtype), None
+    return new.to(x.dtype), normed.to(x.dtype)
 
 
-def gated_norm_bwd(dnew, dnormed, x, branch, gate, weight, bias, post_weight, post_bias, stats, eps: float, scale: float):
+def gated_norm_bwd(dnew, dnormed, x, branch, gate, weight, bias, post_weight, post_bias, eps: float, scale: float):
+    """-> [dx, dbranch, dgate, dweight, dbias (, dpost_weight, dpost_bias)]; a gradient that is None counts as zeros"""
     g, yh, yr, z, new = _gated_parts(x, branch, gate, post_weight, post_bias, eps, scale)
     f = new.dtype
     nh, nr = _normalise(new, eps)
@@ -359,6 +360,29 @@ def gated_norm_bwd(dnew, dnormed, x, branch, gate, weight, bias, post_weight, po
     grads = [(scale * du).to(x.dtype), dy.to(x.dtype), (du * z).sum(rows if gate.dim() == 1 else rows[1:]), (dn * nh).sum(rows),
              dn.sum(rows)]
     return grads if post_weight is None else grads + [(dz * yh).sum(rows), dz.sum(rows)]
+
+
+class GatedResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, gate, weight, bias, post_weight, post_bias, eps, scale):
+        ctx.save_for_backward(x, branch, gate, weight, bias, post_weight, post_bias)
+        ctx.cfg = (eps, scale)
+        ctx.set_materialize_grads(False)
+        return gated_norm_fwd(x, branch, gate, weight, bias, post_weight, post_bias, eps, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dnew, dnormed):
+        if dnew is None and dnormed is None:
+            return (None,) * 9
+        saved = ctx.saved_tensors
+        d = gated_norm_bwd(dnew, dnormed, *saved, *ctx.cfg)
+        d += [None] * (7 - len(d))
+        return (*(None if t is None else t.to(s.dtype) for t, s in zip(d, saved)), None, None)
+
+
+def gated_residual_norm(x, branch, gate, weight, bias, eps: float, post_weight, post_bias, scale: float):
+    return GatedResidualNorm.apply(x, branch, gate, weight, bias, post_weight, post_bias, eps, scale)
 
 
 # ---------------------------------------------------------------- pools ----
