@@ -48,7 +48,7 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 template <int NP, bool POST>
-__global__ __launch_bounds__(256, NP <= 4 ? 4 : 2) void k_gn_fwd(GatedNorm p, bf16* __restrict__ u_out, bf16* __restrict__ n_out,
+__global__ __launch_bounds__(256, NP <= 3 ? 4 : NP == 4 ? 3 : NP < 8 ? 2 : 1) void k_gn_fwd(GatedNorm p, bf16* __restrict__ u_out, bf16* __restrict__ n_out,
                                                                   float* __restrict__ stats /* [2 or 4][M], or null */) {
     const int lane = threadIdx.x & 63, D = p.D, np4 = D >> 2;
     const long stride = (long)gridDim.x * 4;
@@ -190,20 +190,25 @@ template <int NP, bool POST>
 __global__ __launch_bounds__(256, NP <= (POST ? 4 : 6) ? 2 : 1) void k_gn_bwd(
     GatedNorm p, const bf16* __restrict__ du, const bf16* __restrict__ dn, const float* __restrict__ stats, bf16* __restrict__ dx,
     bf16* __restrict__ dy, float* __restrict__ gate_part, long gate_stride, float* __restrict__ slab, int srow, int chunks, long units) {
-    extern __shared__ __attribute__((aligned(16))) float red[];  // [3][NP * 256]
+    constexpr int DP = NP * 256;
+    extern __shared__ __attribute__((aligned(16))) float red[];  // [3][DP] for the column sums, then the parameters, [4][DP]
+    f32x4* wl = reinterpret_cast<f32x4*>(red + 3 * DP);  // (in registers they left no room for a second wave; zeros past D)
+    f32x4* gl = wl + DP / 4;
+    f32x4* pwl = gl + DP / 4;
+    f32x4* pbl = pwl + DP / 4;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int D = p.D, np4 = D >> 2;
     const float inv_d = 1.f / (float)D;
     float sg[NP][4], sw[NP][4], sb[NP][4], spw[POST ? NP : 1][4], spb[POST ? NP : 1][4];
-    f32x4 ga[NP], w[NP], pw[POST ? NP : 1], pb[POST ? NP : 1];
+    for (int c = threadIdx.x; c < DP / 4; c += 256) {
+        wl[c] = par4(p.w + 4 * c, c < np4);
+        if (POST) {
+            pwl[c] = par4(p.pw + 4 * c, c < np4);
+            pbl[c] = par4(p.pb + 4 * c, c < np4);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        const int c = lane + 64 * j;
-        w[j] = par4(p.w + 4 * c, c < np4);
-        if (POST) {
-            pw[j] = par4(p.pw + 4 * c, c < np4);
-            pb[j] = par4(p.pb + 4 * c, c < np4);
-        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             sg[j][k] = sw[j][k] = sb[j][k] = 0.f;
@@ -235,9 +240,10 @@ __global__ __launch_bounds__(256, NP <= (POST ? 4 : 6) ? 2 : 1) void k_gn_bwd(
             }
         };
         if (r0 + wave < r1) fetch(r0 + wave);
-#pragma unroll
-        for (int j = 0; j < NP; ++j) ga[j] = par4(gate + 4 * (lane + 64 * j), lane + 64 * j < np4);
+        for (int c = threadIdx.x; c < DP / 4; c += 256) gl[c] = par4(gate + 4 * c, c < np4);
+        __syncthreads();
         for (long row = r0 + wave; row < r1; row += 4) {
+            asm volatile("" ::: "memory");  // (the parameters are read here, not kept across rows)
             float x[NP][4], y[NP][4];  // uh; yh, or y
             bf16x4 e[NP], g[NP];
             const float mu = st[0], ru = st[1], my = st[2], ry = st[3];
@@ -246,17 +252,23 @@ __global__ __launch_bounds__(256, NP <= (POST ? 4 : 6) ? 2 : 1) void k_gn_bwd(
             for (int j = 0; j < NP; ++j) {
                 e[j] = en[j];
                 g[j] = gn[j];
+                const f32x4 ga = gl[lane + 64 * j], w = wl[lane + 64 * j];
+                f32x4 pw, pb;
+                if (POST) {
+                    pw = pwl[lane + 64 * j];
+                    pb = pbl[lane + 64 * j];
+                }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     float z = (float)yn[j][k];
                     if (POST) z = (z - my) * ry;
                     y[j][k] = z;
-                    if (POST) z = z * pw[j][k] + pb[j][k];
-                    x[j][k] = (p.a * (float)xn[j][k] + ga[j][k] * z - mu) * ru;
+                    if (POST) z = z * pw[k] + pb[k];
+                    x[j][k] = (p.a * (float)xn[j][k] + ga[k] * z - mu) * ru;
                     const float d = (float)en[j][k];  // (zero past the end, and so is all that follows from it)
                     sw[j][k] += d * x[j][k];
                     sb[j][k] += d;
-                    const float t = d * w[j][k];
+                    const float t = d * w[k];
                     s1 += t;
                     s2 += t * x[j][k];
                 }
@@ -264,22 +276,29 @@ __global__ __launch_bounds__(256, NP <= (POST ? 4 : 6) ? 2 : 1) void k_gn_bwd(
             if (row + 4 < r1) fetch(row + 4);
             s1 = row_sum(s1) * inv_d;
             s2 = row_sum(s2) * inv_d;
+            asm volatile("" ::: "memory");
             float s3 = 0.f, s4 = 0.f;
             float dz[NP][4];
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
                 const bool in = lane + 64 * j < np4;
+                const f32x4 ga = gl[lane + 64 * j], w = wl[lane + 64 * j];
+                f32x4 pw, pb;
+                if (POST) {
+                    pw = pwl[lane + 64 * j];
+                    pb = pbl[lane + 64 * j];
+                }
                 bf16x4 o;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float gk = in ? (float)g[j][k] + ru * ((float)e[j][k] * w[j][k] - s1 - x[j][k] * s2) : 0.f;
+                    const float gk = in ? (float)g[j][k] + ru * ((float)e[j][k] * w[k] - s1 - x[j][k] * s2) : 0.f;
                     o[k] = (bf16)(p.a * gk);
-                    sg[j][k] += gk * (POST ? y[j][k] * pw[j][k] + pb[j][k] : y[j][k]);
-                    dz[j][k] = gk * ga[j][k];
+                    sg[j][k] += gk * (POST ? y[j][k] * pw[k] + pb[k] : y[j][k]);
+                    dz[j][k] = gk * ga[k];
                     if (POST) {
                         spw[j][k] += dz[j][k] * y[j][k];
                         spb[j][k] += dz[j][k];
-                        const float t = dz[j][k] * pw[j][k];
+                        const float t = dz[j][k] * pw[k];
                         s3 += t;
                         s4 += t * y[j][k];
                     }
@@ -289,12 +308,15 @@ __global__ __launch_bounds__(256, NP <= (POST ? 4 : 6) ? 2 : 1) void k_gn_bwd(
             if (POST) {
                 s3 = row_sum(s3) * inv_d;
                 s4 = row_sum(s4) * inv_d;
+                asm volatile("" ::: "memory");
             }
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
+                f32x4 pw;
+                if (POST) pw = pwl[lane + 64 * j];
                 bf16x4 o;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o[k] = (bf16)(POST ? ry * (dz[j][k] * pw[j][k] - s3 - y[j][k] * s4) : dz[j][k]);
+                for (int k = 0; k < 4; ++k) o[k] = (bf16)(POST ? ry * (dz[j][k] * pw[k] - s3 - y[j][k] * s4) : dz[j][k]);
                 if (lane + 64 * j < np4) *reinterpret_cast<bf16x4*>(dy + row * D + 4 * (lane + 64 * j)) = o;
             }
         }
@@ -362,7 +384,7 @@ GatedNormPlan gated_norm_plan(long B, long T, long M, bool per_sample) {
 void launch_gated_norm_bwd(const GatedNorm& p, const GatedNormPlan& q, const void* du, const void* dn, const float* stats, void* dx,
                            void* dy, float* gate_part, long gate_stride, float* slab, int srow, hipStream_t s) {
     PDT_GN_DISPATCH(p.D, {
-        const size_t lds = (size_t)3 * NP * 256 * sizeof(float);
+        const size_t lds = (size_t)7 * NP * 256 * sizeof(float);
         if (p.pw)
             hipLaunchKernelGGL((k_gn_bwd<NP, true>), dim3(q.blocks), dim3(256), lds, s, p, (const bf16*)du, (const bf16*)dn, stats,
                                (bf16*)dx, (bf16*)dy, gate_part, gate_stride, slab, srow, q.chunks, q.units);
