@@ -187,7 +187,7 @@ __device__ __forceinline__ void column_sum(float (&v)[NP][4], float* red, float*
 // A unit is one of `chunks` parts of a sample's rows; a workgroup takes the units blockIdx.x, + gridDim.x, ...  The gate's sums
 // leave after every unit (to gate_part + unit * gate_stride), the others at the end (slab [gridDim.x][srow]: db, dw, dpb, dpw).
 template <int NP, bool POST>
-__global__ __launch_bounds__(256, NP <= (POST ? 4 : 6) ? 2 : 1) void k_gn_bwd(
+__global__ __launch_bounds__(256, NP <= (POST ? 3 : 4) ? 2 : 1) void k_gn_bwd(
     GatedNorm p, const bf16* __restrict__ du, const bf16* __restrict__ dn, const float* __restrict__ stats, bf16* __restrict__ dx,
     bf16* __restrict__ dy, float* __restrict__ gate_part, long gate_stride, float* __restrict__ slab, int srow, int chunks, long units) {
     constexpr int DP = NP * 256;
