@@ -81,29 +81,28 @@ void set_tables(ExtArgs& a, const Tensor& tab, const Tensor& codes, int64_t R) {
     a.R = (int)R; a.Rp = (int)Rp;
 }
 
-// -> out, stat (with `grad`), out_lo (with `lo`)
-std::tuple<Tensor, Tensor, Tensor> ext_fwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, bool grad, bool lo) {
-    Tensor out = at::empty({a.B, a.Sq, heads * hd}, q.options().memory_format(at::MemoryFormat::Contiguous)), stat, out_lo;
+// -> out, stat (with `grad`)
+std::tuple<Tensor, Tensor> ext_fwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, bool grad) {
+    Tensor out = at::empty({a.B, a.Sq, heads * hd}, q.options().memory_format(at::MemoryFormat::Contiguous)), stat;
     const auto f32 = q.options().dtype(at::kFloat);
     if (grad) stat = at::empty({2, (long)a.B * a.Hkv, a.Mp}, f32);
-    if (lo) out_lo = at::empty_like(out);
-    if (out.numel() == 0) return {out, stat, out_lo};
+    if (out.numel() == 0) return {out, stat};
     const long BH = (long)a.B * a.Hkv;
-    const ExtPlan p = ext_plan_fwd(BH, a.M, a.Sk, a.tab == nullptr && !lo);
+    const ExtPlan p = ext_plan_fwd(BH, a.M, a.Sk, a.tab != nullptr);
     check_grid(a, p);
     Tensor part, ml;
     if (p.splits > 1) {
         part = at::empty({BH * p.splits * a.M * hd}, f32);
         ml = at::empty({BH * p.splits * a.M * 2}, f32);
     }
-    launch_ext_fwd(a, p, (int)hd, out.data_ptr(), lo ? out_lo.data_ptr() : nullptr, grad ? stat.data_ptr<float>() : nullptr,
+    launch_ext_fwd(a, p, (int)hd, out.data_ptr(), grad ? stat.data_ptr<float>() : nullptr,
                    part.defined() ? part.data_ptr<float>() : nullptr, ml.defined() ? ml.data_ptr<float>() : nullptr, stream_of(q));
-    return {out, stat, out_lo};
+    return {out, stat};
 }
 
 // dq / dk / dv: views to fill; -> dtable [NB, H] when bucket_of is given
-Tensor ext_bwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, const Tensor& dout, const Tensor& out, const OptTensor& out_lo,
-               const Tensor& stat, Tensor dq, Tensor dk, Tensor dv, const OptTensor& bucket_of, int64_t NB) {
+Tensor ext_bwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, const Tensor& dout, const Tensor& out, const Tensor& stat,
+               Tensor dq, Tensor dk, Tensor dv, const OptTensor& bucket_of, int64_t NB) {
     const long width = heads * hd, BH = (long)a.B * a.Hkv;
     check_dense(dout, {a.B, a.Sq, width}, at::kBFloat16, q, "dout");
     check_dense(out, {a.B, a.Sq, width}, at::kBFloat16, q, "out");
@@ -121,16 +120,12 @@ Tensor ext_bwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, const Ten
     }
     ExtBwd w{};
     w.out = out.data_ptr(); w.dout = dout.data_ptr();
-    if (given(out_lo)) {
-        check_dense(*out_lo, {a.B, a.Sq, width}, at::kBFloat16, q, "out_lo");
-        w.out_lo = out_lo->data_ptr();
-    }
     w.stat = stat.data_ptr<float>();
     w.dq = dq.data_ptr(); w.dk = dk.data_ptr(); w.dv = dv.data_ptr();
     a.dqv = view_of(dq, a.G); a.dkv = view_of(dk, 1);
     ext_plan_bwd(BH, a.M, a.Sk, a.tab != nullptr, w.q, w.kv);
     check_grid(a, w.q); check_grid(a, w.kv);
-    Tensor dsum = at::empty({BH, a.Mp}, f32), pq, pk, pv;
+    Tensor dsum = at::empty({w.q.few ? 1 : w.q.splits, BH, a.Mp}, f32), pq, pk, pv;
     w.dsum = dsum.data_ptr<float>();
     if (w.q.splits > 1) {
         pq = at::empty({BH * w.q.splits * a.M * hd}, f32);
@@ -160,10 +155,10 @@ long packed_head_dim(const Tensor& qkv, int64_t heads) {
     return qkv.size(2) / (3 * heads);
 }
 
-// -> out, stat, out_lo, tab [H, Rp], codes [2, Sp]; stat with `grad`, out_lo with `lo`
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> rel_bias_attention_fwd(const Tensor& qkv, const Tensor& table, const Tensor& q_codes,
-                                                                          const Tensor& k_codes, const Tensor& bucket_of, int64_t heads,
-                                                                          const OptTensor& lens, bool grad, bool lo) {
+// -> out, stat (with `grad`), tab [H, Rp], codes [2, Sp]
+std::tuple<Tensor, Tensor, Tensor, Tensor> rel_bias_attention_fwd(const Tensor& qkv, const Tensor& table, const Tensor& q_codes,
+                                                                  const Tensor& k_codes, const Tensor& bucket_of, int64_t heads,
+                                                                  const OptTensor& lens, bool grad) {
     const long hd = packed_head_dim(qkv, heads), D = heads * hd, S = qkv.size(1), R = bucket_of.size(0), NB = table.size(0);
     TORCH_CHECK(R >= 1 && R <= kExtMaxEntries, "rel_bias_attention: ", R, " entries (1 to ", kExtMaxEntries, ")");
     TORCH_CHECK(NB < (1L << 30) && S < (1L << 30), "rel_bias_attention: sizes below 2^30");
@@ -180,13 +175,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> rel_bias_attention_fwd(const 
     const Tensor q = qkv.narrow(2, 0, D), k = qkv.narrow(2, D, D), v = qkv.narrow(2, 2 * D, D);
     ExtArgs a = ext_args(q, k, v, heads, heads, lens, hd, true);
     set_tables(a, tab, codes, R);
-    auto [out, stat, out_lo] = ext_fwd(a, q, heads, hd, grad, lo);
-    return {out, stat, out_lo, tab, codes};
+    auto [out, stat] = ext_fwd(a, q, heads, hd, grad);
+    return {out, stat, tab, codes};
 }
 
 // -> dqkv [B, S, 3 H hd], dtable [NB, H] fp32 (undefined without `want_table`)
-std::tuple<Tensor, Tensor> rel_bias_attention_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out, const OptTensor& out_lo,
-                                                  const Tensor& stat, const Tensor& tab, const Tensor& codes, const Tensor& bucket_of,
+std::tuple<Tensor, Tensor> rel_bias_attention_bwd(const Tensor& dout, const Tensor& qkv, const Tensor& out, const Tensor& stat,
+                                                  const Tensor& tab, const Tensor& codes, const Tensor& bucket_of,
                                                   int64_t NB, int64_t heads, const OptTensor& lens, bool want_table) {
     const long hd = packed_head_dim(qkv, heads), D = heads * hd;
     TORCH_CHECK(NB >= 0 && NB < (1L << 30), "rel_bias_attention: ", NB, " buckets");
@@ -198,7 +193,7 @@ std::tuple<Tensor, Tensor> rel_bias_attention_bwd(const Tensor& dout, const Tens
     ExtArgs a = ext_args(q, k, v, heads, heads, lens, hd, true);
     set_tables(a, tab, codes, bucket_of.size(0));
     Tensor dqkv = at::empty({qkv.size(0), qkv.size(1), 3 * D}, qkv.options().memory_format(at::MemoryFormat::Contiguous));
-    Tensor dtable = ext_bwd(a, q, heads, hd, dout, out, out_lo, stat, dqkv.narrow(2, 0, D), dqkv.narrow(2, D, D), dqkv.narrow(2, 2 * D, D),
+    Tensor dtable = ext_bwd(a, q, heads, hd, dout, out, stat, dqkv.narrow(2, 0, D), dqkv.narrow(2, D, D), dqkv.narrow(2, 2 * D, D),
                             want_table ? OptTensor(bucket_of) : OptTensor(), NB);
     return {dqkv, dtable};
 }
@@ -213,24 +208,22 @@ long cross_head_dim(const Tensor& q, const Tensor& kv, int64_t heads, int64_t kv
     TORCH_CHECK(q.size(0) == kv.size(0), "cross_attention: batches ", q.size(0), " and ", kv.size(0));
     return q.size(2) / heads;
 }
-// q [B, Sq, H hd], kv [B, Sk, 2 Hkv hd] (keys | values) -> out [B, Sq, H hd], stat (with `grad`), out_lo (with `grad` and at most
-// kExtFewKeys keys: dS = P (dP - D) is then a small difference, and D of an output rounded to bf16 costs it half of its
-// precision; with more keys out is small against V and so is its rounding)
-std::tuple<Tensor, Tensor, Tensor> cross_attention_fwd(const Tensor& q, const Tensor& kv, int64_t heads, int64_t kv_heads, const OptTensor& lens,
+// q [B, Sq, H hd], kv [B, Sk, 2 Hkv hd] (keys | values) -> out [B, Sq, H hd], stat (with `grad`)
+std::tuple<Tensor, Tensor> cross_attention_fwd(const Tensor& q, const Tensor& kv, int64_t heads, int64_t kv_heads, const OptTensor& lens,
                                                bool grad) {
     const long hd = cross_head_dim(q, kv, heads, kv_heads), W = kv_heads * hd;
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
     ExtArgs a = ext_args(q, kv.narrow(2, 0, W), kv.narrow(2, W, W), heads, kv_heads, lens, hd, false);
-    return ext_fwd(a, q, heads, hd, grad, grad && a.Sk <= kExtFewKeys);
+    return ext_fwd(a, q, heads, hd, grad);
 }
-std::tuple<Tensor, Tensor> cross_attention_bwd(const Tensor& dout, const Tensor& q, const Tensor& kv, const Tensor& out, const OptTensor& out_lo,
-                                               const Tensor& stat, int64_t heads, int64_t kv_heads, const OptTensor& lens) {
+std::tuple<Tensor, Tensor> cross_attention_bwd(const Tensor& dout, const Tensor& q, const Tensor& kv, const Tensor& out, const Tensor& stat,
+                                               int64_t heads, int64_t kv_heads, const OptTensor& lens) {
     const long hd = cross_head_dim(q, kv, heads, kv_heads), W = kv_heads * hd;
     c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
     ExtArgs a = ext_args(q, kv.narrow(2, 0, W), kv.narrow(2, W, W), heads, kv_heads, lens, hd, false);
     Tensor dq = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
     Tensor dkv = at::empty(kv.sizes(), kv.options().memory_format(at::MemoryFormat::Contiguous));
-    ext_bwd(a, q, heads, hd, dout, out, out_lo, stat, dq, dkv.narrow(2, 0, W), dkv.narrow(2, W, W), OptTensor(), 0);
+    ext_bwd(a, q, heads, hd, dout, out, stat, dq, dkv.narrow(2, 0, W), dkv.narrow(2, W, W), OptTensor(), 0);
     return {dq, dkv};
 }
 

@@ -15,7 +15,7 @@ struct ExtView {
 };
 struct ExtArgs {
     const __bf16 *q, *k, *v;
-    ExtView qv, kv, o, dqv, dkv;  // k and v share strides; `o` holds for out, out_lo and dout
+    ExtView qv, kv, o, dqv, dkv;  // k and v share strides; `o` holds for out and dout
     const int* lens;              // [B] valid keys, or null
     const float* tab;             // [H][Rp] bias per code difference, times sqrt(hd), or null
     const int *q_codes4, *k_codes4;
@@ -30,18 +30,17 @@ struct ExtPlan {
     int tiles, splits;
 };
 struct ExtBwd {
-    const void *out, *out_lo, *dout;
+    const void *out, *dout;
     const float* stat;
-    float* dsum;  // -D
+    float* dsum;  // [splits of the row owner][stat_n]: -D, in the end in the first
     void *dq, *dk, *dv;
     float *part_q, *part_k, *part_v;
     ExtPlan q, kv;
 };
 
-constexpr int kExtFewKeys = 64;  // up to that many keys a training forward keeps the remainder of its output (see cross_attention_fwd)
-ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool streams);
+ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool bias);
 void ext_plan_bwd(long BH, int M, int Sk, bool bias, ExtPlan& q, ExtPlan& kv);  // of the row owner and the key owner
-void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, void* out_lo, float* stat, float* part, float* part_ml,
+void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, float* stat, float* part, float* part_ml,
                     hipStream_t s);
 void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s);
 void launch_bias_tables(const float* table, const int* bucket_of, const int* q_codes, const int* k_codes, float* tab, int* q4,

@@ -146,11 +146,8 @@ __device__ __forceinline__ void own_frags(bf16x8* f, const bf16* p, bool live, i
 
 // ------------------------------------------------------------------------------------------------------- forward
 // One sweep with a running maximum.  4 waves own 32 rows each; keys in blocks of 64.
-// HL: P and O as two bf16 each (value and remainder), so that the backward's D = dO . O, and with it the fp32 gradient of
-// the bias table, does not carry the rounding of P and O to 8 bits of mantissa.
-template <int HD, bool BIAS, bool HL>
-__global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict__ out, bf16* __restrict__ out_lo,
-                                                 float* __restrict__ stat, float* __restrict__ part, float* __restrict__ part_ml,
+template <int HD, bool BIAS>
+__global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict__ out, float* __restrict__ stat, float* __restrict__ part, float* __restrict__ part_ml,
                                                  int tiles, int splits) {
     using G = AttnGeo<HD>;
     constexpr int IMG = 64 * G::ROWBYTES;
@@ -262,22 +259,10 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
                 l += part_l;
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
-                    u32x4 hi, lo;
+                    const bf16x8 p = acc_to_a(st[kt], blk);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = st[kt][8 * blk + 2 * i], y = st[kt][8 * blk + 2 * i + 1];
-                        hi[i] = pack_bf16(x, y);
-                        if (HL) lo[i] = pack_bf16(x - __uint_as_float(hi[i] << 16), y - __uint_as_float(hi[i] & 0xffff0000u));
-                    }
-                    const bf16x8 p = __builtin_bit_cast(bf16x8, hi);
-                    bf16x8 plo;
-                    if (HL) plo = __builtin_bit_cast(bf16x8, lo);
-#pragma unroll
-                    for (int dt = 0; dt < G::DT; ++dt) {
-                        const bf16x8 vt = G::cols(Vs, kt * 32 + blk * 16, dt * 32, lane);
-                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, p, o[dt], 0, 0, 0);
-                        if (HL) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, plo, o[dt], 0, 0, 0);
-                    }
+                    for (int dt = 0; dt < G::DT; ++dt)
+                        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Vs, kt * 32 + blk * 16, dt * 32, lane), p, o[dt], 0, 0, 0);
                 }
             }
         }
@@ -309,15 +294,10 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
         for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
             for (int jj = 0; jj < 4; ++jj) {
-                bf16x4 t, tl;
+                bf16x4 t;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = live ? o[dt][4 * jj + e] * inv : 0.f;
-                    t[e] = (bf16)v;
-                    tl[e] = (bf16)(v - (float)t[e]);
-                }
+                for (int e = 0; e < 4; ++e) t[e] = (bf16)(live ? o[dt][4 * jj + e] * inv : 0.f);
                 *reinterpret_cast<bf16x4*>(out + orow + dt * 32 + 8 * jj + 4 * half) = t;
-                if (HL) *reinterpret_cast<bf16x4*>(out_lo + orow + dt * 32 + 8 * jj + 4 * half) = tl;
             }
     }
 }
@@ -472,8 +452,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
 // where this takes 5)
 template <int HD>
 __global__ __launch_bounds__(256) void k_ext_join(ExtArgs a, const float* __restrict__ part, const float* __restrict__ part_ml,
-                                                  bf16* __restrict__ out, bf16* __restrict__ out_lo, float* __restrict__ stat,
-                                                  int splits) {
+                                                  bf16* __restrict__ out, float* __restrict__ stat, int splits) {
     constexpr int W = HD / 4, NG = 256 / W;
     __shared__ __attribute__((aligned(16))) float red[NG][HD + 4];
     const int bh = (int)blockIdx.x / a.M, r = (int)blockIdx.x - bh * a.M;
@@ -518,15 +497,10 @@ __global__ __launch_bounds__(256) void k_ext_join(ExtArgs a, const float* __rest
     const bool some = (sum > 0.f || sum != sum) && r < rows;
     const float inv = some ? 1.f / sum : 0.f;
     const long o = (long)b * a.o.bs + row_offset(a.o, r, hkv, a.G, HD) + d;
-    bf16x4 w4, lo;
+    bf16x4 w4;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float v = some ? t[e] * inv : 0.f;
-        w4[e] = (bf16)v;
-        lo[e] = (bf16)(v - (float)w4[e]);
-    }
+    for (int e = 0; e < 4; ++e) w4[e] = (bf16)(some ? t[e] * inv : 0.f);
     *reinterpret_cast<bf16x4*>(out + o) = w4;
-    if (out_lo) *reinterpret_cast<bf16x4*>(out_lo + o) = lo;
     if (stat && d == 0) put_stat(a, stat, (long)bh * a.Mp + r, some, mx, sum, 0.f);
 }
 
@@ -608,11 +582,13 @@ __device__ __forceinline__ void store_tile(const f32x16* t, char* img, bf16* dst
     }
 }
 
-// Row owner: dQ, and D for the key owner (written by split 0).  A softmax over one key is constant, so with len = 1 dS is
-// zero, and is set so (as a difference of two rounded numbers it would not be).
-template <int HD, bool BIAS>
-__global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ out_lo,
-                                                   const bf16* __restrict__ dout, const float* __restrict__ stat,
+// Row owner: dQ, and D for what follows.  dO . O carries the rounding of P and O to bf16, and the sum of a row's
+// P (dP - dO . O) is exactly what it is off by (as a row's P add up to 1): added, D is good to 32 bits, which the fp32 gradient of
+// the bias table needs; that sum costs an add a score, keeping O's remainder in the forward cost it a quarter of its time.
+// Where all keys are in one block dS is corrected too: with few keys P (dP - D) is a small difference.  A softmax over one key is
+// constant, so with len = 1 dS is zero, and is set so (as a difference of two rounded numbers it would not be).
+template <int HD, bool BIAS, bool ONE /* all keys in one block of 64 */>
+__global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                    float* __restrict__ dsum, bf16* __restrict__ dq, float* __restrict__ part, int tiles,
                                                    int splits) {
     using G = AttnGeo<HD>;
@@ -655,25 +631,19 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
     }
     // own rows, and D from them
     bf16x8 qf[G::STEPS], gf[G::STEPS];
-    float d = 0.f;
+    float d = 0.f, delta = 0.f;
     {
         const long ro = row_offset(a.o, live ? r : 0, j.hkv, a.G, HD) + (long)j.b * a.o.bs;
         own_frags<HD>(qf, a.q + (long)j.b * a.qv.bs + row_offset(a.qv, live ? r : 0, j.hkv, a.G, HD), live, half);
         own_frags<HD>(gf, dout + ro, live, half);
-        bf16x8 of[G::STEPS], ol[G::STEPS];
+        bf16x8 of[G::STEPS];
         own_frags<HD>(of, out + ro, live, half);
-        if (out_lo) own_frags<HD>(ol, out_lo + ro, live, half);
 #pragma unroll
         for (int s = 0; s < G::STEPS; ++s)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                float v = (float)of[s][k];
-                if (out_lo) v += (float)ol[s][k];
-                d += v * (float)gf[s][k];
-            }
+            for (int k = 0; k < 8; ++k) d += (float)of[s][k] * (float)gf[s][k];
         d += __shfl_xor(d, 32, 64);
     }
-    if (j.split == 0 && half == 0 && r < a.Mp) dsum[(long)j.bh * a.Mp + r] = live ? -d : 0.f;
     const float mq = live ? stat[(long)j.bh * a.Mp + r] : 0.f;
     const float lq = live && j.len > 1 ? stat[a.stat_n + (long)j.bh * a.Mp + r] : -kInf;
     const int qc = tab + (BIAS && live ? a.q_codes4[r] : 0), top = tab + (a.R - 1) * 4;
@@ -685,6 +655,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
             if (kb + 1 < kb1) issue(kb + 1, buf ^ 1);
             const char* Ks = smem + buf * 2 * IMG;
             const char* Vs = Ks + IMG;
+            f32x16 ds[2], pr[2];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
                 f32x16 sc, dp;
@@ -711,18 +682,37 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
                     for (int i = 0; i < 16; ++i)
                         if (kb * 64 + kt * 32 + acc_row(i, half) >= j.len) sc[i] = -kInf;
                 }
+                float off = 0.f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) dp[i] *= __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lq));
+                for (int i = 0; i < 16; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lq));
+                    if (ONE) pr[kt][i] = p;
+                    ds[kt][i] = dp[i] * p;
+                    off += ds[kt][i];
+                }
+                delta += off;
+            }
+            if (ONE) {
+                const float off = delta + __shfl_xor(delta, 32, 64);
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) ds[kt][i] = fmaf(-off, pr[kt][i], ds[kt][i]);
+            }
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
-                    const bf16x8 ds = acc_to_a(dp, blk);
+                    const bf16x8 x = acc_to_a(ds[kt], blk);
 #pragma unroll
                     for (int dt = 0; dt < G::DT; ++dt)
-                        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Ks, kt * 32 + blk * 16, dt * 32, lane), ds, acc[dt], 0, 0, 0);
+                        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Ks, kt * 32 + blk * 16, dt * 32, lane), x, acc[dt], 0, 0, 0);
                 }
-            }
         }
     }
+    delta += __shfl_xor(delta, 32, 64);
+    // -D of this split's keys: the first split has dO . O too, the sum over the splits is made where there is more than one
+    if (half == 0 && r < a.Mp) dsum[((long)j.split * a.B * a.Hkv + j.bh) * a.Mp + r] = live ? -(delta + (j.split == 0 ? d : 0.f)) : 0.f;
     if (r >= a.M) return;
     if (splits > 1) store_acc32<HD>(acc, part + (((long)j.bh * splits + j.split) * a.M + r) * HD, half);
     else store_acc<HD>(acc, dq + (long)j.b * a.dqv.bs + row_offset(a.dqv, r, j.hkv, a.G, HD), a.scale, half);
@@ -733,8 +723,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
 // pass is bound by the stream of K, V, dK and dV), stores dK and dV of its keys and keeps its part of dQ, which the four
 // waves join at the end.
 template <int HD>
-__global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_few(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ out_lo,
-                                                        const bf16* __restrict__ dout, const float* __restrict__ stat,
+__global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_few(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                         bf16* __restrict__ dq, bf16* __restrict__ dk, bf16* __restrict__ dv,
                                                         float* __restrict__ part, int splits) {
     using G = AttnGeo<HD>;
@@ -768,17 +757,12 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_few(ExtArgs a,
         const long ro = row_offset(a.o, live ? l31 : 0, j.hkv, a.G, HD) + (long)j.b * a.o.bs;
         own_frags<HD>(qf, a.q + (long)j.b * a.qv.bs + row_offset(a.qv, live ? l31 : 0, j.hkv, a.G, HD), live, half);
         own_frags<HD>(gf, dout + ro, live, half);
-        bf16x8 of[G::STEPS], ol[G::STEPS];
+        bf16x8 of[G::STEPS];
         own_frags<HD>(of, out + ro, live, half);
-        if (out_lo) own_frags<HD>(ol, out_lo + ro, live, half);
 #pragma unroll
         for (int s = 0; s < G::STEPS; ++s)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                float v = (float)of[s][k];
-                if (out_lo) v += (float)ol[s][k];
-                d -= v * (float)gf[s][k];
-            }
+            for (int k = 0; k < 8; ++k) d -= (float)of[s][k] * (float)gf[s][k];
         d += __shfl_xor(d, 32, 64);
         const long sr = (long)j.bh * a.Mp + l31;
         mq = live ? stat[sr] : 0.f;
@@ -931,6 +915,15 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_few(ExtArgs a,
             *reinterpret_cast<bf16x4*>(dq + (long)j.b * a.dqv.bs + row_offset(a.dqv, r, j.hkv, a.G, HD) + c) = w4;
         }
     }
+}
+
+// dsum[0] <- the sum of the splits' parts of -D, in order
+__global__ __launch_bounds__(256) void k_ext_dsum(float* __restrict__ dsum, long n, int splits) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float s = dsum[i];
+    for (int k = 1; k < splits; ++k) s += dsum[k * n + i];
+    dsum[i] = s;
 }
 
 // dS summed over a part of the batch, for 128 queries x 128 keys of a head a workgroup (a wave: 32 queries, four tiles of 32
@@ -1313,7 +1306,7 @@ void allow_lds(K kern, size_t bytes) {
 size_t table_bytes(const ExtArgs& a) { return a.tab ? (size_t)((a.Rp + 255) & ~255) * 4 : 0; }
 
 template <int HD>
-void fwd(const ExtArgs& a, const ExtPlan& p, void* out, void* out_lo, float* stat, float* part, float* part_ml, hipStream_t s) {
+void fwd(const ExtArgs& a, const ExtPlan& p, void* out, float* stat, float* part, float* part_ml, hipStream_t s) {
     const unsigned grid = (unsigned)((long)a.B * a.Hkv * p.tiles * p.splits);
     if (p.few) {
         const size_t lds = (size_t)16 * 32 * HD * 2 + 4 * 32 * 2 * sizeof(float);
@@ -1321,24 +1314,19 @@ void fwd(const ExtArgs& a, const ExtPlan& p, void* out, void* out_lo, float* sta
         hipLaunchKernelGGL((k_ext_fwd_few<HD>), dim3(grid), dim3(256), lds, s, a, (bf16*)out, stat, part, part_ml, p.splits);
     } else {
         const size_t lds = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + table_bytes(a);
-#define PDT_EXT_FWD(BIAS, HL)                                                                                             \
-    allow_lds(&k_ext_fwd<HD, BIAS, HL>, lds);                                                                             \
-    hipLaunchKernelGGL((k_ext_fwd<HD, BIAS, HL>), dim3(grid), dim3(256), lds, s, a, (bf16*)out, (bf16*)out_lo, stat, part, \
-                       part_ml, p.tiles, p.splits);
-        if (a.tab && out_lo) {
-            PDT_EXT_FWD(true, true)
-        } else if (a.tab) {
-            PDT_EXT_FWD(true, false)
-        } else if (out_lo) {
-            PDT_EXT_FWD(false, true)
+#define PDT_EXT_FWD(BIAS)                                                                                               \
+    allow_lds(&k_ext_fwd<HD, BIAS>, lds);                                                                              \
+    hipLaunchKernelGGL((k_ext_fwd<HD, BIAS>), dim3(grid), dim3(256), lds, s, a, (bf16*)out, stat, part, part_ml, p.tiles, p.splits);
+        if (a.tab) {
+            PDT_EXT_FWD(true)
         } else {
-            PDT_EXT_FWD(false, false)
+            PDT_EXT_FWD(false)
         }
 #undef PDT_EXT_FWD
     }
     if (p.splits > 1) {
         hipLaunchKernelGGL((k_ext_join<HD>), dim3((unsigned)((long)a.B * a.Hkv * a.M)), dim3(256), 0, s, a, (const float*)part,
-                           (const float*)part_ml, (bf16*)out, (bf16*)out_lo, stat, p.splits);
+                           (const float*)part_ml, (bf16*)out, stat, p.splits);
     }
 }
 
@@ -1349,24 +1337,37 @@ void bwd(const ExtArgs& a, const ExtBwd& w, hipStream_t s) {
     if (pq.few) {
         const size_t lds = (size_t)(16 + 2) * 32 * HD * 2 + 3 * 32 * sizeof(float);
         allow_lds(&k_ext_bwd_few<HD>, lds);
-        hipLaunchKernelGGL((k_ext_bwd_few<HD>), gq, dim3(256), lds, s, a, (const bf16*)w.out, (const bf16*)w.out_lo, (const bf16*)w.dout,
-                           w.stat, (bf16*)w.dq, (bf16*)w.dk, (bf16*)w.dv, w.part_q, pq.splits);
+        hipLaunchKernelGGL((k_ext_bwd_few<HD>), gq, dim3(256), lds, s, a, (const bf16*)w.out, (const bf16*)w.dout, w.stat, (bf16*)w.dq, (bf16*)w.dk, (bf16*)w.dv, w.part_q, pq.splits);
     } else {
-    const size_t lq = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + table_bytes(a);
-    const size_t lk = (size_t)4 * 64 * HD * 2 + 8192 + table_bytes(a);
-#define PDT_EXT_BWD(BIAS)                                                                                                  \
-    allow_lds(&k_ext_bwd_q<HD, BIAS>, lq);                                                                                 \
-    hipLaunchKernelGGL((k_ext_bwd_q<HD, BIAS>), gq, dim3(256), lq, s, a, (const bf16*)w.out, (const bf16*)w.out_lo,        \
-                       (const bf16*)w.dout, w.stat, w.dsum, (bf16*)w.dq, w.part_q, pq.tiles, pq.splits);                   \
-    allow_lds(&k_ext_bwd_kv<HD, BIAS>, lk);                                                                                \
+        const size_t lq = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + table_bytes(a);
+        const size_t lk = (size_t)4 * 64 * HD * 2 + 8192 + table_bytes(a);
+        const long n = a.stat_n;
+#define PDT_EXT_BWD_Q(BIAS, ONE)                                                                                          \
+    allow_lds(&k_ext_bwd_q<HD, BIAS, ONE>, lq);                                                                           \
+    hipLaunchKernelGGL((k_ext_bwd_q<HD, BIAS, ONE>), gq, dim3(256), lq, s, a, (const bf16*)w.out, (const bf16*)w.dout, w.stat, \
+                       w.dsum, (bf16*)w.dq, w.part_q, pq.tiles, pq.splits);
+#define PDT_EXT_BWD_KV(BIAS)                                                                                              \
+    allow_lds(&k_ext_bwd_kv<HD, BIAS>, lk);                                                                               \
     hipLaunchKernelGGL((k_ext_bwd_kv<HD, BIAS>), gk, dim3(256), lk, s, a, (const bf16*)w.dout, w.stat, (const float*)w.dsum, \
                        (bf16*)w.dk, (bf16*)w.dv, w.part_k, w.part_v, pk.tiles, pk.splits);
-    if (a.tab) {
-        PDT_EXT_BWD(true)
-    } else {
-        PDT_EXT_BWD(false)
-    }
-#undef PDT_EXT_BWD
+        const bool one = a.Sk <= 64;
+        if (a.tab && one) {
+            PDT_EXT_BWD_Q(true, true)
+        } else if (a.tab) {
+            PDT_EXT_BWD_Q(true, false)
+        } else if (one) {
+            PDT_EXT_BWD_Q(false, true)
+        } else {
+            PDT_EXT_BWD_Q(false, false)
+        }
+        if (pq.splits > 1) hipLaunchKernelGGL(k_ext_dsum, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, w.dsum, n, pq.splits);
+        if (a.tab) {
+            PDT_EXT_BWD_KV(true)
+        } else {
+            PDT_EXT_BWD_KV(false)
+        }
+#undef PDT_EXT_BWD_Q
+#undef PDT_EXT_BWD_KV
     }
     const long BH = (long)a.B * a.Hkv;
     if (pq.splits > 1) {
@@ -1395,15 +1396,15 @@ int splits_for(long groups, long blocks, long least) {
 
 }  // namespace
 
-ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool streams /* a plain forward: no bias, no remainder kept */) {
+ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool bias) {
     ExtPlan p;
-    p.few = streams && M <= 32;
+    p.few = !bias && M <= 32;
     p.tiles = p.few ? 1 : (M + 127) / 128;
     p.splits = p.few ? splits_for(BH, (Sk + 31) / 32, 8) : splits_for(BH * p.tiles, (Sk + 63) / 64, 4);
     return p;
 }
 void ext_plan_bwd(long BH, int M, int Sk, bool bias, ExtPlan& q, ExtPlan& kv) {
-    q.few = kv.few = !bias && M <= 32;
+    q.few = kv.few = !bias && M <= 32 && Sk > 64;  // (few keys want D exact: the row owner)
     if (q.few) {  // one kernel
         q.tiles = 1;
         q.splits = splits_for(BH, (Sk + 31) / 32, 8);
@@ -1416,11 +1417,11 @@ void ext_plan_bwd(long BH, int M, int Sk, bool bias, ExtPlan& q, ExtPlan& kv) {
     kv.splits = splits_for(BH * kv.tiles, (M + 63) / 64, 4);
 }
 
-void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, void* out_lo, float* stat, float* part, float* part_ml,
+void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, float* stat, float* part, float* part_ml,
                     hipStream_t s) {
-    if (hd == 32) fwd<32>(a, p, out, out_lo, stat, part, part_ml, s);
-    else if (hd == 64) fwd<64>(a, p, out, out_lo, stat, part, part_ml, s);
-    else fwd<128>(a, p, out, out_lo, stat, part, part_ml, s);
+    if (hd == 32) fwd<32>(a, p, out, stat, part, part_ml, s);
+    else if (hd == 64) fwd<64>(a, p, out, stat, part, part_ml, s);
+    else fwd<128>(a, p, out, stat, part, part_ml, s);
 }
 void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s) {
     if (hd == 32) bwd<32>(a, w, s);

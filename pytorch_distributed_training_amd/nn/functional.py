@@ -565,24 +565,19 @@ def _check_lengths(lengths, like, op: str) -> None:
 
 
 class _RelBiasAttentionFn(torch.autograd.Function):
-    """The bias table's gradient is fp32 and summed without atomics; for it the forward also keeps the part of its output that
-    bf16 drops (``out_lo``), which the backward adds to D = dO . O."""
-
     @staticmethod
     def forward(ctx, qkv, table, q_codes, k_codes, bucket_of, heads, lengths, be):
-        want_table = ctx.needs_input_grad[1]
-        out, lse, lo, tab, codes = be.rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, True,
-                                                             want_table)
-        ctx.save_for_backward(qkv, out, lo, lse, tab, codes, bucket_of, lengths)
+        out, lse, tab, codes = be.rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, True)
+        ctx.save_for_backward(qkv, out, lse, tab, codes, bucket_of, lengths)
         ctx.cfg = (be, heads, table.shape[0], table.dtype)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qkv, out, lo, lse, tab, codes, bucket_of, lengths = ctx.saved_tensors
+        qkv, out, lse, tab, codes, bucket_of, lengths = ctx.saved_tensors
         be, heads, buckets, tdt = ctx.cfg
-        dqkv, dtable = be.rel_bias_attention_bwd(dout, qkv, out, lo, lse, tab, codes, bucket_of, buckets, heads, lengths,
+        dqkv, dtable = be.rel_bias_attention_bwd(dout, qkv, out, lse, tab, codes, bucket_of, buckets, heads, lengths,
                                                  ctx.needs_input_grad[1])
         return dqkv, (None if dtable is None else dtable.to(tdt)), None, None, None, None, None, None
 
@@ -624,24 +619,24 @@ def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, leng
             be = reference
     qkv = _rows3(qkv)
     if not _wants_grad(qkv, table):
-        return be.rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, False, False)[0]
+        return be.rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, False)[0]
     return _RelBiasAttentionFn.apply(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, be)
 
 
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, kv, heads, kv_heads, lengths, be):
-        out, lse, lo = be.cross_attention_fwd(q, kv, heads, kv_heads, lengths, True)
-        ctx.save_for_backward(q, kv, out, lo, lse, lengths)
+        out, lse = be.cross_attention_fwd(q, kv, heads, kv_heads, lengths, True)
+        ctx.save_for_backward(q, kv, out, lse, lengths)
         ctx.cfg = (be, heads, kv_heads)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, kv, out, lo, lse, lengths = ctx.saved_tensors
+        q, kv, out, lse, lengths = ctx.saved_tensors
         be, heads, kv_heads = ctx.cfg
-        dq, dkv = be.cross_attention_bwd(dout, q, kv, out, lo, lse, heads, kv_heads, lengths)
+        dq, dkv = be.cross_attention_bwd(dout, q, kv, out, lse, heads, kv_heads, lengths)
         return dq, dkv, None, None, None, None
 
 

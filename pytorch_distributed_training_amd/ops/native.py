@@ -293,29 +293,27 @@ def rel_bias_attention_unsupported_reason(qkv, heads: int, bucket_of):
     return None
 
 
-def rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None, grad: bool = True,
-                           want_table: bool = True):
-    """-> (out [B, S, D], stat, out_lo, tab, codes): what ``rel_bias_attention_bwd`` wants back, the statistics with ``grad``,
-    ``out_lo`` with ``want_table``"""
+def rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None, grad: bool = True):
+    """-> (out [B, S, D], statistics for the backward or None, tab, codes)"""
     return _C.rel_bias_attention_fwd(qkv, _f32(table), _i32(q_codes), _i32(k_codes), _i32(bucket_of), heads, _i32(lengths),
-                                     grad, want_table)
+                                     grad)
 
 
-def rel_bias_attention_bwd(dout, qkv, out, out_lo, lse, tab, codes, bucket_of, buckets: int, heads: int, lengths=None,
+def rel_bias_attention_bwd(dout, qkv, out, lse, tab, codes, bucket_of, buckets: int, heads: int, lengths=None,
                            want_table: bool = True):
     """-> (dqkv, dtable [buckets, heads] fp32, or None)"""
-    return _C.rel_bias_attention_bwd(_al(dout), qkv, out, out_lo, lse, tab, codes, _i32(bucket_of), buckets, heads,
+    return _C.rel_bias_attention_bwd(_al(dout), qkv, out, lse, tab, codes, _i32(bucket_of), buckets, heads,
                                      _i32(lengths), want_table)
 
 
 def cross_attention_fwd(q, kv, heads: int, kv_heads: int, lengths=None, grad: bool = True):
-    """-> (out [B, Sq, H*hd], statistics, out_lo): what the backward wants back, or None"""
+    """-> (out [B, Sq, H*hd], statistics for the backward or None)"""
     return _C.cross_attention_fwd(q, kv, heads, kv_heads, _i32(lengths), grad)
 
 
-def cross_attention_bwd(dout, q, kv, out, out_lo, lse, heads: int, kv_heads: int, lengths=None):
+def cross_attention_bwd(dout, q, kv, out, lse, heads: int, kv_heads: int, lengths=None):
     """-> (dq, dkv)"""
-    return _C.cross_attention_bwd(_al(dout), q, kv, out, out_lo, lse, heads, kv_heads, _i32(lengths))
+    return _C.cross_attention_bwd(_al(dout), q, kv, out, lse, heads, kv_heads, _i32(lengths))
 
 
 # ------------------------------------------------------------------------- gated norm (csrc/kernels/gated_norm.hip)

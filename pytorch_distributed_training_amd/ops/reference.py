@@ -258,17 +258,16 @@ def _rel_probs(q, k, table, bucket, lengths):
     return p, real
 
 
-def rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None, grad: bool = True,
-                           want_table: bool = True):
-    """Oracle of csrc/kernels/attention_ext.hip -> (out, None, None, table, codes)"""
+def rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None, grad: bool = True):
+    """Oracle of csrc/kernels/attention_ext.hip -> (out, None, table, codes)"""
     b, s, w = qkv.shape
     q, k, v = _rel_parts(qkv, heads, lengths)
     p, _ = _rel_probs(q, k, table, _rel_buckets(q_codes, k_codes, bucket_of), lengths)
     out = torch.matmul(p, v).transpose(1, 2).reshape(b, s, w // 3).to(qkv.dtype)
-    return out, None, None, table, torch.stack([q_codes, k_codes])
+    return out, None, table, torch.stack([q_codes, k_codes])
 
 
-def rel_bias_attention_bwd(dout, qkv, out, out_lo, lse, tab, codes, bucket_of, buckets: int, heads: int, lengths=None,
+def rel_bias_attention_bwd(dout, qkv, out, lse, tab, codes, bucket_of, buckets: int, heads: int, lengths=None,
                            want_table: bool = True):
     b, s, w = qkv.shape
     q, k, v = _rel_parts(qkv, heads, lengths)
@@ -302,12 +301,12 @@ def _cross_rows(t, q, heads, kv_heads):
 
 
 def cross_attention_fwd(q, kv, heads: int, kv_heads: int, lengths=None, grad: bool = True):
-    """Oracle of csrc/kernels/attention_ext.hip -> (out, None, None)"""
+    """Oracle of csrc/kernels/attention_ext.hip -> (out, None)"""
     qf, k, v = _cross_parts(q, kv, heads, kv_heads, lengths)
-    return _cross_rows(torch.matmul(_ext_probs(qf, k, None, lengths), v), q, heads, kv_heads), None, None
+    return _cross_rows(torch.matmul(_ext_probs(qf, k, None, lengths), v), q, heads, kv_heads), None
 
 
-def cross_attention_bwd(dout, q, kv, out, out_lo, lse, heads: int, kv_heads: int, lengths=None):
+def cross_attention_bwd(dout, q, kv, out, lse, heads: int, kv_heads: int, lengths=None):
     b, sk = kv.shape[:2]
     qf, k, v = _cross_parts(q, kv, heads, kv_heads, lengths)
     do = _cross_parts(dout, kv, heads, kv_heads, None)[0]
