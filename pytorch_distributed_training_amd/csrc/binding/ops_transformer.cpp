@@ -141,7 +141,7 @@ Tensor ext_bwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, const Ten
     if (dtable.defined() && NB > 0) {
         const RelPlan p = rel_plan(a.B, a.Hkv, a.Sk);
         Tensor dense = at::empty({p.dense}, f32), slab = at::empty({(long)heads * p.rows, a.Rp}, f32),
-               mid = at::empty({p.mid, (long)heads, a.Rp}, f32);
+               mid = at::empty({(long)heads, a.Rp}, f32);
         launch_rel_bias_grad(a, w, (int)hd, p, dense.data_ptr<float>(), slab.data_ptr<float>(), mid.data_ptr<float>(),
                              bucket_of->data_ptr<int>(), dtable.data_ptr<float>(), (int)NB, stream_of(q));
     }

@@ -52,11 +52,11 @@ struct RelBlocks {
 };
 struct RelPlan {
     int heads, qblocks, chunks;  // of a launch
-    int parts, rows, mid;        // ranges of key tiles; slab rows per head; partial rows of the slab's sum
+    int parts, rows;             // ranges of key tiles; slab rows per head
     long dense;                  // floats: sums of dS by pair
 };
 RelPlan rel_plan(int B, int H, int S);
-// dense [plan.dense], slab [H][plan.rows][Rp], mid [plan.mid][H][Rp]
+// dense [plan.dense], slab [H][plan.rows][Rp], mid [H][Rp]
 void launch_rel_bias_grad(const ExtArgs& a, const ExtBwd& w, int hd, const RelPlan& p, float* dense, float* slab, float* mid,
                           const int* bucket_of, float* dtable, int NB, hipStream_t s);
 

@@ -113,9 +113,12 @@ __device__ __forceinline__ Job job_of(const ExtArgs& a, int tiles, int splits) {
     j.split = l % splits;
     l /= splits;
     j.tile = l % tiles;
-    j.bh = l / tiles;
-    j.b = j.bh / a.Hkv;
-    j.hkv = j.bh - j.b * a.Hkv;
+    l /= tiles;
+    // heads outside, the batch inside: an XCD gets sequences of all lengths (with the batch outside the XCDs of the long ones
+    // worked twice as long as the rest on a padded batch), and its head's bias table stays in its cache
+    j.hkv = l / a.B;
+    j.b = l - j.hkv * a.B;
+    j.bh = j.b * a.Hkv + j.hkv;
     int len = a.Sk;
     if (a.lens) {
         len = a.lens[j.b];
@@ -200,12 +203,19 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
             const int buf = (kb - kb0) & 1;
             dma_barrier();
             if (kb + 1 < kb1) issue(kb + 1, buf ^ 1);
+            if (j.tile * 128 + wave * 32 >= j.rows) continue;  // (this wave has no rows: it helps with the staging)
             const char* Ks = smem + buf * 2 * IMG;
             const char* Vs = Ks + IMG;
+            const bool both = kb * 64 + 32 < j.len;  // whether the second tile has keys
             f32x16 st[2];
             float mb = m;
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
+                if (kt == 1 && !both) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) st[1][i] = -kInf;
+                    break;
+                }
                 if (BIAS) {
 #pragma unroll
                     for (int jj = 0; jj < 4; ++jj) {
@@ -250,6 +260,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
             }
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
+                if (kt == 1 && !both) break;
                 float part_l = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -585,8 +596,9 @@ __device__ __forceinline__ void store_tile(const f32x16* t, char* img, bf16* dst
 // Row owner: dQ, and D for what follows.  dO . O carries the rounding of P and O to bf16, and the sum of a row's
 // P (dP - dO . O) is exactly what it is off by (as a row's P add up to 1): added, D is good to 32 bits, which the fp32 gradient of
 // the bias table needs; that sum costs an add a score, keeping O's remainder in the forward cost it a quarter of its time.
-// Where all keys are in one block dS is corrected too: with few keys P (dP - D) is a small difference.  A softmax over one key is
-// constant, so with len = 1 dS is zero, and is set so (as a difference of two rounded numbers it would not be).
+// Where all keys are in one block dS is corrected too: with few keys P (dP - D) is a small difference.  Without a bias and with
+// more keys O is small against V, its rounding against dP, and nothing is added.  A softmax over one key is constant, so with
+// len = 1 dS is zero, and is set so (as a difference of two rounded numbers it would not be).
 template <int HD, bool BIAS, bool ONE /* all keys in one block of 64 */>
 __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                    float* __restrict__ dsum, bf16* __restrict__ dq, float* __restrict__ part, int tiles,
@@ -653,11 +665,23 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
             const int buf = (kb - kb0) & 1;
             dma_barrier();
             if (kb + 1 < kb1) issue(kb + 1, buf ^ 1);
+            if (j.tile * 128 + wave * 32 >= j.rows) continue;
             const char* Ks = smem + buf * 2 * IMG;
             const char* Vs = Ks + IMG;
-            f32x16 ds[2], pr[2];
+            const bool both = kb * 64 + 32 < j.len;
+            f32x16 ds[ONE ? 2 : 1], pr[ONE ? 2 : 1];
+            auto product = [&](const f32x16& x, int kt) {
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk) {
+                    const bf16x8 d8 = acc_to_a(x, blk);
+#pragma unroll
+                    for (int dt = 0; dt < G::DT; ++dt)
+                        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Ks, kt * 32 + blk * 16, dt * 32, lane), d8, acc[dt], 0, 0, 0);
+                }
+            };
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
+                if (!ONE && kt == 1 && !both) break;
                 f32x16 sc, dp;
                 if (BIAS) {
 #pragma unroll
@@ -687,27 +711,22 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
                 for (int i = 0; i < 16; ++i) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lq));
                     if (ONE) pr[kt][i] = p;
-                    ds[kt][i] = dp[i] * p;
-                    off += ds[kt][i];
+                    dp[i] *= p;
+                    if (BIAS || ONE) off += dp[i];
                 }
                 delta += off;
+                if (ONE) ds[kt] = dp;
+                else product(dp, kt);
             }
             if (ONE) {
                 const float off = delta + __shfl_xor(delta, 32, 64);
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
+                for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) ds[kt][i] = fmaf(-off, pr[kt][i], ds[kt][i]);
-            }
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int blk = 0; blk < 2; ++blk) {
-                    const bf16x8 x = acc_to_a(ds[kt], blk);
-#pragma unroll
-                    for (int dt = 0; dt < G::DT; ++dt)
-                        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Ks, kt * 32 + blk * 16, dt * 32, lane), x, acc[dt], 0, 0, 0);
+                    product(ds[kt], kt);
                 }
+            }
         }
     }
     delta += __shfl_xor(delta, 32, 64);
@@ -934,7 +953,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
                                                       const float* __restrict__ dsum, float* __restrict__ dense, RelBlocks w) {
     using G = AttnGeo<HD>;
     constexpr int IMG = 128 * G::ROWBYTES;  // as two blocks of 64 rows
-    extern __shared__ __attribute__((aligned(16))) char smem[];  // K, V of one sequence, twice where it fits; before that the table
+    extern __shared__ __attribute__((aligned(16))) char smem[];  // K, V of one sequence; before that the table
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int l = xcd_order((int)blockIdx.x, (int)gridDim.x);
@@ -1068,18 +1087,30 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
                 for (int e = 0; e < 4; ++e) v[4 * jj + e] += t[e];
             }
         }
+        int at[16];
+        bool end = false;
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
             const i32x4 kc = *reinterpret_cast<const i32x4*>(a.k_codes4 + kt * 32 + 8 * jj + 4 * half);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int at = bias_at(qc, kc[e], base, top);
-                const float x = v[4 * jj + e];
-                ends[0] += at == base ? x : 0.f;
-                ends[1] += at == top && top != base ? x : 0.f;
-                if (at != base && at != top)
-                    __hip_atomic_fetch_add(reinterpret_cast<float*>(reinterpret_cast<char*>(hist) + (at - base)), x, __ATOMIC_RELAXED,
-                                           __HIP_MEMORY_SCOPE_WORKGROUP);
+                at[4 * jj + e] = bias_at(qc, kc[e], base, top);
+                end |= at[4 * jj + e] == base || at[4 * jj + e] == top;
+            }
+        }
+        auto add = [&](int i) {
+            __hip_atomic_fetch_add(reinterpret_cast<float*>(reinterpret_cast<char*>(hist) + (at[i] - base)), v[i], __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_WORKGROUP);
+        };
+        if (!__any(end)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) add(i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                ends[0] += at[i] == base ? v[i] : 0.f;
+                ends[1] += at[i] == top && top != base ? v[i] : 0.f;
+                if (at[i] != base && at[i] != top) add(i);
             }
         }
     }
@@ -1165,11 +1196,13 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
             const int buf = (rb - rb0) & 1;
             dma_barrier();
             if (rb + 1 < rb1) issue(rb + 1, buf ^ 1);
+            if (j.tile * 128 + wave * 32 >= j.len) continue;
             const char* Qs = smem + buf * 2 * IMG;
             const char* Gs = Qs + IMG;
             const char* st = stat_s + buf * 4096;
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
+                if (rt == 1 && rb * 64 + 32 >= j.rows) break;
                 f32x16 sc, dp;
                 f32x4 lr[4];
 #pragma unroll
@@ -1255,33 +1288,34 @@ __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ t
     (w < Sp ? q4 : k4)[at] = c * 4;
 }
 
-// mid[chunk][h][r] = sum of this chunk's slab rows [H][rows][Rp] of head h, in order
-__global__ __launch_bounds__(256) void k_bias_slab(const float* __restrict__ slab, float* __restrict__ mid, int Rp, int H, int rows,
-                                                   int chunks) {
-    const int r = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, ch = blockIdx.z;
-    if (r >= Rp) return;
-    const int per = (rows + chunks - 1) / chunks, i0 = ch * per, i1 = i0 + per < rows ? i0 + per : rows;
+// sums[h][r] = sum of the slab rows [H][rows][Rp] of head h: 64 entries a workgroup, each of its four waves every fourth row
+__global__ __launch_bounds__(256) void k_bias_slab(const float* __restrict__ slab, float* __restrict__ sums, int Rp, int rows) {
+    __shared__ float red[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x * 64 + lane, h = blockIdx.y;
     float s = 0.f;
-#pragma unroll 4
-    for (int i = i0; i < i1; ++i) s += slab[((long)h * rows + i) * Rp + r];
-    mid[((long)ch * H + h) * Rp + r] = s;
+    if (r < Rp) {
+#pragma unroll 8
+        for (int i = wave; i < rows; i += 4) s += slab[((long)h * rows + i) * Rp + r];
+    }
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && r < Rp) sums[(long)h * Rp + r] = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
 }
 
 // dtable[n][h] = sum over the entries r of bucket n: the head's entries and their buckets in LDS, a lane per bucket, each of the
 // four waves over a quarter of the entries (any number of entries may share a bucket, in any order)
 __global__ __launch_bounds__(256) void k_bias_buckets(const float* __restrict__ mid, const int* __restrict__ bucket_of,
-                                                      float* __restrict__ dtable, int R, int Rp, int NB, int H, int chunks) {
+                                                      float* __restrict__ dtable, int R, int Rp, int NB, int H) {
     __shared__ __attribute__((aligned(16))) float sums[kExtMaxEntries];
     __shared__ __attribute__((aligned(16))) int of[kExtMaxEntries];
     __shared__ float red[4][64];
     const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll 8
     for (int r = threadIdx.x; r < Rp; r += 256) {
-        float s = 0.f;
-#pragma unroll 4
-        for (int c = 0; c < chunks; ++c) s += mid[((long)c * H + h) * Rp + r];
-        sums[r] = s;
-        of[r] = r < R ? bucket_of[r] : -1;
+        sums[r] = mid[(long)h * Rp + r];
+        of[r] = bucket_of[r < R ? r : R - 1];
     }
+    for (int r = R + (int)threadIdx.x; r < Rp; r += 256) sums[r] = 0.f;
     __syncthreads();
     const int n = blockIdx.x * 64 + lane, quads = Rp >> 2, per = (quads + 3) >> 2;
     float s = 0.f;
@@ -1434,7 +1468,7 @@ void launch_bias_tables(const float* table, const int* bucket_of, const int* q_c
     hipLaunchKernelGGL(k_bias_tables, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, table, bucket_of, q_codes, k_codes,
                        tab, q4, k4, R, Rp, NB, H, S, Sp, inv_scale, total);
 }
-// Head groups and query blocks of a dense sum of at most 1 GiB; the batch in parts, so that about 1024 workgroups run
+// Head groups and query blocks of a dense sum of at most 1 GiB; the batch in parts
 RelPlan rel_plan(int B, int H, int S) {
     RelPlan p;
     const long blocks = (S + 127) / 128, row_block = blocks * 4 * blocks * 4 * 4096;  // bytes of a head
@@ -1442,7 +1476,9 @@ RelPlan rel_plan(int B, int H, int S) {
     p.heads = (int)(row_block >= most ? 1 : most / row_block < H ? most / row_block : H);
     p.qblocks = (int)(row_block <= most ? blocks : most / (row_block / blocks) > 0 ? most / (row_block / blocks) : 1);
     const long groups = (long)p.heads * p.qblocks * blocks;
-    long c = (1024 + groups - 1) / groups;
+    // the fewest parts that keep the two workgroups a CU holds (512) busy for nine tenths of the last round's end
+    long c = 1;
+    while (c < 16 && groups * c * 10 < 9 * 512 * ((groups * c + 511) / 512)) ++c;
     const long room = most / (p.heads * p.qblocks * (row_block / blocks));
     c = c < B / 4 ? c : B / 4;
     c = c < room ? c : room;
@@ -1455,7 +1491,6 @@ RelPlan rel_plan(int B, int H, int S) {
     p.parts = (int)(q < 1 ? 1 : q);
     p.rows = (int)(blocks * 4 * p.parts);
     p.dense = (long)p.chunks * p.heads * p.qblocks * (row_block / blocks) / 4;
-    p.mid = p.rows < 32 ? 1 : p.rows < 32 * 32 ? (p.rows + 31) / 32 : 32;
     return p;
 }
 template <int HD>
@@ -1486,10 +1521,9 @@ void launch_rel_bias_grad(const ExtArgs& a, const ExtBwd& x, int hd, const RelPl
             hipLaunchKernelGGL(k_rel_entries, dim3((unsigned)(w.heads * w.qblocks * 4 * p.parts)), dim3(256), lds, s, a,
                                (const float*)dense, slab, w, p.parts);
         }
-    hipLaunchKernelGGL(k_bias_slab, dim3((a.Rp + 255) / 256, a.Hkv, p.mid), dim3(256), 0, s, (const float*)slab, mid, a.Rp, a.Hkv, p.rows,
-                       p.mid);
+    hipLaunchKernelGGL(k_bias_slab, dim3((a.Rp + 63) / 64, a.Hkv), dim3(256), 0, s, (const float*)slab, mid, a.Rp, p.rows);
     hipLaunchKernelGGL(k_bias_buckets, dim3((NB + 63) / 64, a.Hkv), dim3(256), 0, s, (const float*)mid, bucket_of, dtable, a.R, a.Rp, NB,
-                       a.Hkv, p.mid);
+                       a.Hkv);
 }
 
 }  // namespace pdt
