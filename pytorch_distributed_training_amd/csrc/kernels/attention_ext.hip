@@ -1202,7 +1202,8 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
             const char* st = stat_s + buf * 4096;
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
-                if (rt == 1 && rb * 64 + 32 >= j.rows) break;
+                // (one wave a SIMD at head_dim 128 lives on the two tiles' overlap: 172 us with, 203 us cut by this branch)
+                if (HD <= 64 && rt == 1 && rb * 64 + 32 >= j.rows) break;
                 f32x16 sc, dp;
                 f32x4 lr[4];
 #pragma unroll
