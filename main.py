@@ -51,6 +51,10 @@ def get_parser() -> argparse.ArgumentParser:
     p.add_argument("--model", default="resnet50",
                    choices=["resnet18", "resnet34", "resnet50", "resnet101", "resnet152", "vit_b_16", "vit_ti_16", "vit_s_16", "vit_l_16",
                             "vit_tiny_test"])
+    p.add_argument("--rel_pos_bias", action="store_true", help="ViT: learned relative position bias in every layer's attention")
+    p.add_argument("--layer_scale", default=None, type=float, help="ViT: learned gate per channel on every branch, started here")
+    p.add_argument("--post_norm", action="store_true", help="ViT: LayerNorm on every branch before its gate (with --layer_scale)")
+    p.add_argument("--attention_pool", action="store_true", help="ViT: pool by one learned query instead of the class token")
     p.add_argument("--dataset", default="cifar100",
                    choices=["cifar100", "synthetic-cifar", "synthetic-cifar10", "synthetic-imagenet"])
     p.add_argument("--data_root", default="dataset", type=str)
@@ -90,8 +94,26 @@ def get_parser() -> argparse.ArgumentParser:
     return p
 
 
+def model_options(args) -> dict:
+    o = {}
+    if args.rel_pos_bias:
+        o["rel_pos_bias"] = True
+    if args.layer_scale is not None:
+        o["layer_scale"] = args.layer_scale
+    if args.post_norm:
+        o["post_norm"] = True
+    if args.attention_pool:
+        o["pool"] = "attention"
+    if o and not args.model.startswith("vit"):
+        raise SystemExit(f"--rel_pos_bias / --layer_scale / --post_norm / --attention_pool: not for --model {args.model}")
+    if args.post_norm and args.layer_scale is None:
+        raise SystemExit("--post_norm goes with --layer_scale")
+    return o
+
+
 def main(argv=None) -> int:
     args = get_parser().parse_args(argv)
+    vit_options = model_options(args)
     if args.grad_comm is not None:
         os.environ["PDT_GRAD_COMM"] = args.grad_comm  # (read when the reducer is built)
     batch_size, job_id, epochs = args.batch_size, args.JobID, args.epochs
@@ -134,7 +156,7 @@ def main(argv=None) -> int:
             # the torch profiler's one cycle (wait 2 + warmup 2 + active 6) ends at step 10: capture after it, so
             # that the trace shows real kernels and no collection is active while the stream is being captured
             graph_warmup=12 if args.profile == "torch" else 3,
-            image_size=trainset.sample_shape[1]))
+            image_size=trainset.sample_shape[1], model_options=vit_options))
         if maybe_graph:
             use_graph = engine.cfg.graph = engine.device_only_step()
         start_epoch, global_step, resume_batches = 0, 0, 0

@@ -43,6 +43,7 @@ class EngineConfig:
     reducer: str | None = None
     seed: int | None = None
     image_size: int | None = None
+    model_options: dict | None = None  # further arguments of the model (ViT: rel_pos_bias, layer_scale, post_norm, pool)
     # capture forward + backward + optimizer of the steady-state step in one hipGraph (launch-bound shapes:
     # the CIFAR-shaped reference config issues ~550 kernels of a few microseconds each per step)
     graph: bool = False
@@ -106,7 +107,7 @@ class Engine:
         kw = {}
         if cfg.image_size is not None and cfg.model.startswith("vit"):
             kw["image_size"] = cfg.image_size
-        net = build_model(cfg.model, cfg.num_classes, **kw)
+        net = build_model(cfg.model, cfg.num_classes, **kw, **(cfg.model_options or {}))
         # reference order: criterion + optimizer BEFORE .cuda() / SyncBN conversion / DDP (main.py:79-83)
         self.criterion = pnn.CrossEntropyLoss()
         self.optimizer = build_optimizer(cfg.optimizer, net.parameters(), cfg.lr, cfg.momentum, cfg.weight_decay)

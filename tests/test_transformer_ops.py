@@ -298,6 +298,100 @@ def test_refusals(device):
                 rel(**bad)
 
 
+OPTIONS = dict(rel_pos_bias=True, layer_scale=0.5, post_norm=True, pool="attention")
+
+
+def test_vit_options_leave_the_plain_model_alone():
+    from pytorch_distributed_training_amd.models import build_model
+
+    plain, more = build_model("vit_tiny_test"), build_model("vit_tiny_test", **OPTIONS)
+    assert set(plain.state_dict()) < set(more.state_dict())
+    new = sorted(set(more.state_dict()) - set(plain.state_dict()))
+    assert "encoder.layers.encoder_layer_0.self_attention.relative_position_bias_table" in new and "pool.query" in new
+    assert not any("codes" in k or "bucket" in k for k in more.state_dict())
+    for bad in (dict(pool="mean"), dict(post_norm=True)):
+        with pytest.raises(ValueError):
+            build_model("vit_tiny_test", **bad)
+
+
+def _vit_gradients(model, x, y):
+    loss = torch.nn.functional.cross_entropy(model(x).float(), y)
+    return loss.detach(), torch.autograd.grad(loss, list(model.parameters()))
+
+
+@pytest.mark.parametrize("options", [OPTIONS, dict(rel_pos_bias=True), dict(layer_scale=0.1), dict(pool="attention"), dict(OPTIONS, dropout=0.2)], ids=str)
+def test_vit_with_options_has_every_gradient(options):
+    from pytorch_distributed_training_amd.models import build_model
+
+    torch.manual_seed(0)
+    m = build_model("vit_tiny_test", num_classes=10, **options)
+    for p in m.parameters():  # (the head and the tables start at zero)
+        torch.nn.init.normal_(p, std=0.1)
+    loss, gs = _vit_gradients(m, torch.rand(3, 3, 32, 32), torch.tensor([1, 2, 3]))
+    assert torch.isfinite(loss)
+    for (name, _), g in zip(m.named_parameters(), gs):
+        assert torch.isfinite(g).all() and g.abs().max() > 0, name
+
+
+@gpu
+def test_vit_with_options_against_the_oracle():
+    """Logits and every gradient of a model with all options, kernels against the fp32 formulas on the same bf16 activations."""
+    from pytorch_distributed_training_amd import ops
+    from pytorch_distributed_training_amd.models import build_model
+
+    dev = _dev("cuda")
+    torch.manual_seed(0)
+    m = build_model("vit_ti_16", num_classes=16, image_size=112, **OPTIONS).to(dev)
+    for n, p in m.named_parameters():
+        if n.endswith("bias_table") or n.startswith("heads"):
+            torch.nn.init.normal_(p, std=0.1)
+    g = torch.Generator().manual_seed(1)
+    x = torch.rand(4, 3, 112, 112, generator=g).to(dev).to(torch.bfloat16).contiguous(memory_format=torch.channels_last)
+    y = torch.randint(0, 16, (4,), generator=g).to(dev)
+    before = dict(F.fallback_counts)
+    loss, gs = _vit_gradients(m, x, y)
+    assert dict(F.fallback_counts) == before
+    ops.set_force_reference(True)
+    try:
+        want, ws = _vit_gradients(m, x, y)
+    finally:
+        ops.set_force_reference(False)
+    assert abs(loss - want) <= 16 * U * abs(want)
+    true = _vit_gradients(m, x.float(), y)[1]  # the same formulas in 32 bits throughout
+    for (name, _), a, b, c in zip(m.named_parameters(), gs, ws, true):
+        # Twelve layers of some ten roundings each, each off by U at most and by U / sqrt(3) in the mean square, add up to
+        # sqrt(120 / 3) U of a gradient's norm where they meet at random.  Where the gradient itself is a small difference
+        # (pool.query: the sum over the keys of P (dP - D) k, whose P (dP - D) add up to zero) the same roundings are
+        # (sum P |dP| |k|) / |sum P (dP - D) k| times as large against its norm, for the kernels and the oracle alike.  So the
+        # kernels are held to the oracle's own error: they round P and dS too, 12 roundings a layer for 10, which is
+        # sqrt(1.2) = 1.1 times its error, and two independent errors' norms of this many terms differ by less than that again.
+        size, off, oracle = c.double().norm(), (a.double() - c.double()).norm(), (b.double() - c.double()).norm()
+        assert off <= 2 * max(oracle, math.sqrt(40) * U * size / 2) + 1e-12, (name, off, oracle, size)
+
+
+@gpu
+def test_engine_trains_a_vit_with_options():
+    from pytorch_distributed_training_amd import dist as pdist
+    from pytorch_distributed_training_amd.engine import Engine, EngineConfig
+
+    import os
+
+    _dev("cuda")
+    os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
+    os.environ.setdefault("MASTER_PORT", "29541")
+    pdist.init_process_group(backend="rccl", local_rank=0)
+    eng = Engine(EngineConfig(model="vit_tiny_test", num_classes=10, optimizer="adamw", lr=1e-3, sync_bn=False, seed=0,
+                              model_options=OPTIONS))
+    g = torch.Generator().manual_seed(0)
+    x, y = torch.rand(8, 3, 32, 32, generator=g).cuda(), torch.randint(0, 10, (8,), generator=g).cuda()
+    before = dict(F.fallback_counts)
+    start = [p.detach().clone() for p in eng.net.parameters()]
+    losses = [float(eng.train_step(x, y)) for _ in range(3)]
+    assert all(math.isfinite(v) for v in losses)
+    assert all(not torch.equal(a, b) for a, b in zip(start, eng.net.parameters()))
+    assert dict(F.fallback_counts) == before
+
+
 # ------------------------------------------------------------------------------------------------- on the GPU
 REL = [
     dict(b=1, codes=_log(1), heads=1, hd=64), dict(b=2, codes=_log(2), heads=2, hd=32), dict(b=3, codes=_grid(2), heads=3, hd=128),
