@@ -91,7 +91,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = True) ->
     common_defs = ["-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DHIPBLAS_V2", "-DTORCH_EXTENSION_NAME=_C",
                    "-D_GLIBCXX_USE_CXX11_ABI=1", "-DTORCH_API_INCLUDE_EXTENSION_H"]
     hip_flags = ["hipcc", f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffast-math", "-fno-gpu-rdc",
-                 "-Wno-unused-result"]
+                 "-Wno-unused-result", *NO_PACKED_FP32]
     cpp_flags = ["hipcc", "-O2", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Wno-unused-value", "-Wno-deprecated-declarations",
                  *common_defs, *[f"-I{p}" for p in inc], f"-I{py_inc}"]
     tasks = []
@@ -103,8 +103,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = True) ->
         obj = os.path.join(BUILD, rel.replace("/", "_") + ".o")
         objs.append(obj)
         is_hip = rel.endswith(".hip")
-        flags = [*hip_flags, *NO_PACKED_FP32] if rel in ("kernels/attention_ext.hip", "kernels/gated_norm.hip") else (
-            hip_flags if is_hip else cpp_flags)
+        flags = hip_flags if is_hip else cpp_flags
         if rel in NAN_AWARE:
             flags = [*flags, "-fno-finite-math-only"]
         stamp = digest + "|" + " ".join(flags)
