@@ -74,10 +74,12 @@ void check_grid(const ExtArgs& a, const ExtPlan& p) {
 void set_tables(ExtArgs& a, const Tensor& tab, const Tensor& codes, int64_t R) {
     const long Sp = (a.Sk + 127) / 128 * 128, Rp = (R + 3) / 4 * 4;
     TORCH_CHECK(R >= 1 && R <= kExtMaxEntries, "rel_bias_attention: ", R, " entries (1 to ", kExtMaxEntries, ")");
-    TORCH_CHECK(tab.sizes() == at::IntArrayRef({(long)a.Hkv, Rp}) && codes.sizes() == at::IntArrayRef({2, Sp}), "bias tables: shape");
+    TORCH_CHECK(tab.sizes() == at::IntArrayRef({(long)a.Hkv, Rp}) && codes.sizes() == at::IntArrayRef({2 * Sp + Sp / 8}), "bias tables: shape");
     a.tab = tab.data_ptr<float>();
     a.q_codes4 = codes.data_ptr<int>();
     a.k_codes4 = codes.data_ptr<int>() + Sp;
+    a.q_range = reinterpret_cast<const int2*>(codes.data_ptr<int>() + 2 * Sp);
+    a.k_range = a.q_range + Sp / 32;
     a.R = (int)R; a.Rp = (int)Rp;
 }
 
@@ -155,7 +157,7 @@ long packed_head_dim(const Tensor& qkv, int64_t heads) {
     return qkv.size(2) / (3 * heads);
 }
 
-// -> out, stat (with `grad`), tab [H, Rp], codes [2, Sp]
+// -> out, stat (with `grad`), tab [H, Rp], codes
 std::tuple<Tensor, Tensor, Tensor, Tensor> rel_bias_attention_fwd(const Tensor& qkv, const Tensor& table, const Tensor& q_codes,
                                                                   const Tensor& k_codes, const Tensor& bucket_of, int64_t heads,
                                                                   const OptTensor& lens, bool grad) {
@@ -168,9 +170,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rel_bias_attention_fwd(const Tensor& 
     check_dense(bucket_of, {R}, at::kInt, qkv, "bucket_of");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(qkv.device());
     const long Rp = (R + 3) / 4 * 4, Sp = (S + 127) / 128 * 128;
-    Tensor tab = at::empty({heads, Rp}, table.options()), codes = at::empty({2, Sp}, q_codes.options());
+    Tensor tab = at::empty({heads, Rp}, table.options()), codes = at::empty({2 * Sp + Sp / 8}, q_codes.options());
     launch_bias_tables(table.data_ptr<float>(), bucket_of.data_ptr<int>(), q_codes.data_ptr<int>(), k_codes.data_ptr<int>(),
-                       tab.data_ptr<float>(), codes.data_ptr<int>(), codes.data_ptr<int>() + Sp, (int)R, (int)Rp, (int)NB, (int)heads,
+                       tab.data_ptr<float>(), codes.data_ptr<int>(), (int)R, (int)Rp, (int)NB, (int)heads,
                        (int)S, (int)Sp, (float)std::sqrt((double)hd), stream_of(qkv));
     const Tensor q = qkv.narrow(2, 0, D), k = qkv.narrow(2, D, D), v = qkv.narrow(2, 2 * D, D);
     ExtArgs a = ext_args(q, k, v, heads, heads, lens, hd, true);

@@ -18,7 +18,8 @@ struct ExtArgs {
     ExtView qv, kv, o, dqv, dkv;  // k and v share strides; `o` holds for out and dout
     const int* lens;              // [B] valid keys, or null
     const float* tab;             // [H][Rp] bias per code difference, times sqrt(hd), or null
-    const int *q_codes4, *k_codes4;
+    const int *q_codes4, *k_codes4;  // byte offsets, padded to a multiple of 128
+    const int2 *q_range, *k_range;   // smallest and largest of each 32
     int R, Rp;
     int self;                     // rows past lens[b] are dead too
     int B, Hkv, G, Sq, Sk, M, Mp; // M = Sq * G rows per key head, Mp = M rounded up to 64
@@ -43,8 +44,8 @@ void ext_plan_bwd(long BH, int M, int Sk, bool bias, ExtPlan& q, ExtPlan& kv);  
 void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, float* stat, float* part, float* part_ml,
                     hipStream_t s);
 void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s);
-void launch_bias_tables(const float* table, const int* bucket_of, const int* q_codes, const int* k_codes, float* tab, int* q4,
-                        int* k4, int R, int Rp, int NB, int H, int S, int Sp, float inv_scale, hipStream_t s);
+// codes [2 Sp + 4 Sp / 32]
+void launch_bias_tables(const float* table, const int* bucket_of, const int* q_codes, const int* k_codes, float* tab, int* codes, int R, int Rp, int NB, int H, int S, int Sp, float inv_scale, hipStream_t s);
 // the bias table's gradient: after launch_ext_bwd (which leaves D in dsum)
 struct RelBlocks {
     int h0, heads, q0, qblocks, kblocks;  // of this launch: heads, blocks of 128 queries; blocks of 128 keys of all

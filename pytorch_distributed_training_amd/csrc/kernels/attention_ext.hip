@@ -98,6 +98,52 @@ __device__ __forceinline__ int bias_at(int qc4, int kc4, int lo, int hi) {
 typedef const float __attribute__((address_space(3))) * lds_cfloat_ptr;
 __device__ __forceinline__ float lds_float(int addr) { return *(lds_cfloat_ptr)(uintptr_t)(uint32_t)addr; }
 
+// The one table address that all pairs of 32 queries and 32 keys fall on, or -1: from the smallest and largest code of each side.
+// Positions further apart than the table reaches share an entry, so on long sequences most tiles need no histogram.  (In the
+// attention kernels the test cost more than the gather that it would have saved: 56 -> 67 us forward at 197 tokens.)
+__device__ __forceinline__ int one_entry(const ExtArgs& a, int qt, int kt, int lo, int hi) {
+    const int2 q = a.q_range[qt], k = a.k_range[kt];
+    int x = lo + q.x - k.y, y = lo + q.y - k.x;
+    x = x < lo ? lo : x > hi ? hi : x;
+    y = y < lo ? lo : y > hi ? hi : y;
+    return x == y ? x : -1;
+}
+// The scores' start: bias (+ add) of 16 pairs of a lane whose own code is `mine` and the others' codes lie in LDS at `codes`
+__device__ __forceinline__ void gather_bias(f32x16& st, const char* codes, int half, int mine, int lo, int hi, float add) {
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+        const i32x4 c = *reinterpret_cast<const i32x4*>(codes + (8 * jj + 4 * half) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[4 * jj + e] = lds_float(bias_at(mine, c[e], lo, hi)) + add;
+    }
+}
+// v[i] of the pairs at table addresses at[i] into a wave's own histogram.  LDS float adds take a cycle a lane, and many times
+// that where lanes meet on one address: pairs at either end of the table are summed in registers (ends), and a lane whose
+// neighbour's next key falls on the same entry (positions in a row) takes that sum over, so that a diagonal of four costs one
+// lane's add instead of four.
+__device__ __forceinline__ void add_tile(char* hist, const int (&at)[16], float (&v)[16], int base, int top, float (&ends)[2]) {
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+#pragma unroll
+        for (int e = 3; e > 0; --e) {  // lane l + 1's pair (4 jj + e) joins lane l's (4 jj + e - 1)
+            const int i = 4 * jj + e;
+            const float from = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v[i]), 0x130, 0xf, 0xf, true));
+            const int there = __builtin_amdgcn_update_dpp(-1, at[i], 0x130, 0xf, 0xf, false);
+            const bool takes = there == at[i - 1];
+            v[i - 1] += takes ? from : 0.f;
+            const bool gone = __builtin_amdgcn_update_dpp(0, (int)takes, 0x138, 0xf, 0xf, true) != 0;
+            v[i] = gone ? 0.f : v[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        ends[0] += at[i] == base ? v[i] : 0.f;
+        ends[1] += at[i] == top && top != base ? v[i] : 0.f;
+        if (at[i] != base && at[i] != top && v[i] != 0.f)
+            __hip_atomic_fetch_add(reinterpret_cast<float*>(hist + (at[i] - base)), v[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+}
+
 __device__ __forceinline__ long row_offset(const ExtView& v, int r, int hkv, int G, int HD) {
     const int q = (int)fdiv((uint32_t)r, v.g);
     return (long)q * v.rs + (long)(hkv * G + (r - q * G)) * HD;
@@ -217,12 +263,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
                     break;
                 }
                 if (BIAS) {
-#pragma unroll
-                    for (int jj = 0; jj < 4; ++jj) {
-                        const i32x4 kc = *reinterpret_cast<const i32x4*>(codes + buf * 1024 + (kt * 32 + 8 * jj + 4 * half) * 4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) st[kt][4 * jj + e] = lds_float(bias_at(qc, kc[e], tab, top));
-                    }
+                    gather_bias(st[kt], codes + buf * 1024 + kt * 128, half, qc, tab, top, 0.f);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
@@ -683,14 +724,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
             for (int kt = 0; kt < 2; ++kt) {
                 if (!ONE && kt == 1 && !both) break;
                 f32x16 sc, dp;
-                if (BIAS) {
-#pragma unroll
-                    for (int jj = 0; jj < 4; ++jj) {
-                        const i32x4 kc = *reinterpret_cast<const i32x4*>(codes + buf * 1024 + (kt * 32 + 8 * jj + 4 * half) * 4);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[4 * jj + e] = lds_float(bias_at(qc, kc[e], tab, top)) + mq;
-                    }
-                }
+                if (BIAS) gather_bias(sc, codes + buf * 1024 + kt * 128, half, qc, tab, top, mq);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     if (!BIAS) sc[i] = mq;
@@ -1044,6 +1078,14 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
         float* dst = dense + (row * nkt + kb * 4 + kt) * 1024 + lane * 4;
+        if (one_entry(a, qb * 4 + wave, kb * 4 + kt, 0, (a.R - 1) * 4) >= 0) {  // one number
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s += acc[kt][i];
+            s = row_sum(s);
+            if (lane == 0) dst[0] = s;
+            continue;
+        }
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
             f32x4 t;
@@ -1055,8 +1097,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
 }
 
 // The pairs' sums by entry: a workgroup takes a tile row (32 queries) of a head and one of `parts` ranges of its key tiles; its
-// waves take every fourth tile, each with a histogram of its own.  LDS float adds take a cycle a lane, and many times that where
-// lanes meet on one address: the batch is summed first, and pairs past either end of the table are summed in registers.
+// waves take every fourth tile, each with a histogram of its own.
 __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __restrict__ dense, float* __restrict__ slab, RelBlocks w,
                                                      int parts) {
     extern __shared__ __attribute__((aligned(16))) char smem[];  // [4][Rp] floats
@@ -1073,11 +1114,20 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
     const int t1 = (part + 1) * per < live_t ? (part + 1) * per : live_t;
     float ends[2] = {0.f, 0.f};
     for (int kt = part * per + wave; kt < t1; kt += 4) {
+        const float* src = dense + (((long)hl * nqt + qt) * nkt + kt) * 1024 + lane * 4;
+        const long step = (long)w.heads * nqt * nkt * 1024;
+        const int one = one_entry(a, w.q0 * 4 + qt, kt, base, top);
+        if (one >= 0) {
+            if (lane == 0) {
+                float s = 0.f;
+                for (int ch = 0; ch < w.chunks; ++ch) s += src[ch * step];
+                hist[(one - base) >> 2] += s;
+            }
+            continue;
+        }
         float v[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = 0.f;
-        const float* src = dense + (((long)hl * nqt + qt) * nkt + kt) * 1024 + lane * 4;
-        const long step = (long)w.heads * nqt * nkt * 1024;
 #pragma unroll 4
         for (int ch = 0; ch < w.chunks; ++ch) {
 #pragma unroll
@@ -1088,35 +1138,17 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
             }
         }
         int at[16];
-        bool end = false;
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
             const i32x4 kc = *reinterpret_cast<const i32x4*>(a.k_codes4 + kt * 32 + 8 * jj + 4 * half);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                at[4 * jj + e] = bias_at(qc, kc[e], base, top);
-                end |= at[4 * jj + e] == base || at[4 * jj + e] == top;
-            }
+            for (int e = 0; e < 4; ++e) at[4 * jj + e] = bias_at(qc, kc[e], base, top);
         }
-        auto add = [&](int i) {
-            __hip_atomic_fetch_add(reinterpret_cast<float*>(reinterpret_cast<char*>(hist) + (at[i] - base)), v[i], __ATOMIC_RELAXED,
-                                   __HIP_MEMORY_SCOPE_WORKGROUP);
-        };
-        if (!__any(end)) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) add(i);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                ends[0] += at[i] == base ? v[i] : 0.f;
-                ends[1] += at[i] == top && top != base ? v[i] : 0.f;
-                if (at[i] != base && at[i] != top) add(i);
-            }
-        }
+        add_tile(reinterpret_cast<char*>(hist), at, v, base, top, ends);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        ends[i] = wave_sum(ends[i]);
+        ends[i] = row_sum(ends[i]);
         if (lane == 0) hist[i * (a.R - 1)] += ends[i];
     }
     __syncthreads();
@@ -1268,7 +1300,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
 // on an entry that its neighbours use)
 __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ table, const int* __restrict__ bucket_of,
                                                      const int* __restrict__ q_codes, const int* __restrict__ k_codes,
-                                                     float* __restrict__ tab, int* __restrict__ q4, int* __restrict__ k4, int R,
+                                                     float* __restrict__ tab, int* __restrict__ codes /* q4 [Sp], k4 [Sp], ranges of 32 */, int R,
                                                      int Rp, int NB, int H, int S, int Sp, float inv_scale, long total) {
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
     if (i >= total) return;
@@ -1282,11 +1314,25 @@ __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ t
         return;
     }
     const long w = i - (long)H * Rp;
-    const int at = (int)(w % Sp);
-    const int* src = w < Sp ? q_codes : k_codes;
-    int c = src[at < S ? at : S - 1];
-    c = c < -(1 << 28) ? -(1 << 28) : c > (1 << 28) - 1 ? (1 << 28) - 1 : c;  // differences of the byte offsets fit 32 bits
-    (w < Sp ? q4 : k4)[at] = c * 4;
+    auto code4 = [&](long x) {  // x < 2 Sp
+        const int at = (int)(x % Sp);
+        int c = (x < Sp ? q_codes : k_codes)[at < S ? at : S - 1];
+        c = c < -(1 << 27) ? -(1 << 27) : c > (1 << 27) - 1 ? (1 << 27) - 1 : c;  // byte offsets' differences and an LDS address fit 32 bits
+        return c * 4;
+    };
+    if (w < 2L * Sp) {
+        codes[w] = code4(w);
+        return;
+    }
+    int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+    const long r = w - 2L * Sp;
+    for (int e = 0; e < 32; ++e) {
+        const int c = code4(r * 32 + e);
+        lo = c < lo ? c : lo;
+        hi = c > hi ? c : hi;
+    }
+    codes[2L * Sp + 2 * r] = lo;
+    codes[2L * Sp + 2 * r + 1] = hi;
 }
 
 // sums[h][r] = sum of the slab rows [H][rows][Rp] of head h: 64 entries a workgroup, each of its four waves every fourth row
@@ -1377,8 +1423,8 @@ void bwd(const ExtArgs& a, const ExtBwd& w, hipStream_t s) {
         const size_t lq = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + table_bytes(a);
         const size_t lk = (size_t)4 * 64 * HD * 2 + 8192 + table_bytes(a);
         const long n = a.stat_n;
-#define PDT_EXT_BWD_Q(BIAS, ONE)                                                                                          \
-    allow_lds(&k_ext_bwd_q<HD, BIAS, ONE>, lq);                                                                           \
+#define PDT_EXT_BWD_Q(BIAS, ONE)                                                                                    \
+    allow_lds(&k_ext_bwd_q<HD, BIAS, ONE>, lq);                                                                     \
     hipLaunchKernelGGL((k_ext_bwd_q<HD, BIAS, ONE>), gq, dim3(256), lq, s, a, (const bf16*)w.out, (const bf16*)w.dout, w.stat, \
                        w.dsum, (bf16*)w.dq, w.part_q, pq.tiles, pq.splits);
 #define PDT_EXT_BWD_KV(BIAS)                                                                                              \
@@ -1463,11 +1509,10 @@ void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s) {
     else if (hd == 64) bwd<64>(a, w, s);
     else bwd<128>(a, w, s);
 }
-void launch_bias_tables(const float* table, const int* bucket_of, const int* q_codes, const int* k_codes, float* tab, int* q4,
-                        int* k4, int R, int Rp, int NB, int H, int S, int Sp, float inv_scale, hipStream_t s) {
-    const long total = (long)H * Rp + 2L * Sp;
+void launch_bias_tables(const float* table, const int* bucket_of, const int* q_codes, const int* k_codes, float* tab, int* codes, int R, int Rp, int NB, int H, int S, int Sp, float inv_scale, hipStream_t s) {
+    const long total = (long)H * Rp + 2L * Sp + 2L * Sp / 32;
     hipLaunchKernelGGL(k_bias_tables, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, table, bucket_of, q_codes, k_codes,
-                       tab, q4, k4, R, Rp, NB, H, S, Sp, inv_scale, total);
+                       tab, codes, R, Rp, NB, H, S, Sp, inv_scale, total);
 }
 // Head groups and query blocks of a dense sum of at most 1 GiB; the batch in parts
 RelPlan rel_plan(int B, int H, int S) {

@@ -24,6 +24,21 @@ __device__ __forceinline__ bf16x8 acc_to_a(const f32x16& t, int blk) {
 }
 __device__ __forceinline__ int acc_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+// sum over the 64 lanes, the same in all, without LDS: pairs, quads, half rows, rows of 16, then rows into the last one
+__device__ __forceinline__ float row_sum(float v) {
+    v = dpp_add<0xB1, 0xf>(v);   // lanes ^ 1
+    v = dpp_add<0x4E, 0xf>(v);   // lanes ^ 2
+    v = dpp_add<0x141, 0xf>(v);  // mirrored within 8
+    v = dpp_add<0x140, 0xf>(v);  // mirrored within 16
+    v = dpp_add<0x142, 0xa>(v);  // row 0 into 1, 2 into 3
+    v = dpp_add<0x143, 0xc>(v);  // rows 0 and 1 into 2 and 3
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 template <int HDT>
 struct AttnGeo {
     static constexpr int ROWBYTES = HDT * 2, NCH = HDT / 8, STEPS = HDT / 16, DT = HDT / 32;

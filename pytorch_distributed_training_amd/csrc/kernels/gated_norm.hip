@@ -14,7 +14,7 @@
 // 256 channels) and walks over rows with the parameters in registers (read again for every row they were 2.7 times the
 // row's own bytes) and the next row's loads in flight.  Row sums by DPP, not through LDS.  The column sums stay in registers over
 // all rows a wave visits, are added over the waves in LDS and over the workgroups in a fixed order (no atomics).
-#include "common.h"
+#include "attn_tile.h"
 #include "gated_norm.h"
 
 namespace pdt {
@@ -32,21 +32,6 @@ __device__ __forceinline__ f32x4 par4(const float* p, bool in) {
     if (in) t = *reinterpret_cast<const f32x4*>(p);
     return t;
 }
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp_add(float v) {
-    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
-}
-// sum over the 64 lanes, the same in all: pairs, quads, half rows, rows of 16, then rows into the last one
-__device__ __forceinline__ float row_sum(float v) {
-    v = dpp_add<0xB1, 0xf>(v);   // lanes ^ 1
-    v = dpp_add<0x4E, 0xf>(v);   // lanes ^ 2
-    v = dpp_add<0x141, 0xf>(v);  // mirrored within 8
-    v = dpp_add<0x140, 0xf>(v);  // mirrored within 16
-    v = dpp_add<0x142, 0xa>(v);  // row 0 into 1, 2 into 3
-    v = dpp_add<0x143, 0xc>(v);  // rows 0 and 1 into 2 and 3
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-}
-
 template <int NP, bool POST>
 __global__ __launch_bounds__(256, NP <= 3 ? 4 : NP == 4 ? 3 : NP < 8 ? 2 : 1) void k_gn_fwd(GatedNorm p, bf16* __restrict__ u_out, bf16* __restrict__ n_out,
                                                                   float* __restrict__ stats /* [2 or 4][M], or null */) {

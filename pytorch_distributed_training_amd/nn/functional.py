@@ -588,7 +588,7 @@ def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, leng
 
     The bias of query ``i`` and key ``j`` in head ``h`` is ``table[bucket, h]`` (``table`` ``[buckets, heads]``, learned) with
     ``bucket = bucket_of[clamp(q_codes[i] - k_codes[j], 0, len(bucket_of) - 1)]``; ``nn.grid_position_buckets`` and
-    ``nn.log_position_buckets`` make the three integer tensors (codes below 2^28 in magnitude).  An entry of ``bucket_of``
+    ``nn.log_position_buckets`` make the three integer tensors (codes below 2^27 in magnitude).  An entry of ``bucket_of``
     outside the table means no bias; a table entry of ``-inf`` forbids the pair.
 
     ``lengths`` (``[B]`` integers, on the device of ``qkv``): sequence ``b`` is its first ``lengths[b]`` tokens; the rows behind

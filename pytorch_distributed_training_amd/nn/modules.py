@@ -156,7 +156,7 @@ def grid_position_buckets(height: int, width: int, prefix: int = 1):
         raise ValueError(f"grid_position_buckets: {height} x {width} cells, {prefix} prefix tokens")
     w = 2 * width - 1
     top = (height - 1) * w + width - 1
-    if 4 * top + 3 >= 1 << 28:
+    if 4 * top + 3 >= 1 << 27:
         raise ValueError(f"grid_position_buckets: {height} x {width} cells are too many")
     cell = (torch.arange(height)[:, None] * w + torch.arange(width)[None, :]).reshape(-1)
     q = torch.cat([torch.full((prefix,), 4 * top + 3), cell + top + 1])
