@@ -1228,13 +1228,14 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
             const int buf = (rb - rb0) & 1;
             dma_barrier();
             if (rb + 1 < rb1) issue(rb + 1, buf ^ 1);
-            if (j.tile * 128 + wave * 32 >= j.len) continue;
+            // (a wave without keys helps with the staging.  head_dim 128 has one wave a SIMD and lives on the overlap of its two
+            // row tiles: 170 us on four sequences of up to 2047, 203 us with this branch or the next one)
+            if (HD <= 64 && j.tile * 128 + wave * 32 >= j.len) continue;
             const char* Qs = smem + buf * 2 * IMG;
             const char* Gs = Qs + IMG;
             const char* st = stat_s + buf * 4096;
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
-                // (one wave a SIMD at head_dim 128 lives on the two tiles' overlap: 172 us with, 203 us cut by this branch)
                 if (HD <= 64 && rt == 1 && rb * 64 + 32 >= j.rows) break;
                 f32x16 sc, dp;
                 f32x4 lr[4];
