@@ -4,6 +4,7 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -21,6 +22,23 @@ using OptTensor = c10::optional<Tensor>;
 
 hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// A backward pass that is captured while an eager graph of the same leaves lives accumulates on the eager graph's stream: the
+// engine would wait for a stream outside the capture, in a thread whose exception ends the process.  Refused at the forward.
+void check_capture(const std::vector<OptTensor>& leaves) {
+    if (!at::GradMode::is_enabled() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const OptTensor& t : leaves) {
+        if (!given(t) || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!node || !node->stream()) continue;
+        const hipStream_t s = c10::hip::HIPStreamMasqueradingAsCUDA(c10::hip::HIPStreamMasqueradingAsCUDA::UNCHECKED, *node->stream()).stream();
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (s) (void)hipStreamIsCapturing(s, &status);
+        TORCH_CHECK(status == hipStreamCaptureStatusActive,
+                    "a forward pass with gradients is being captured while an eager graph of the same parameters lives on another stream: "
+                    "release that graph's outputs first");
+    }
+}
 
 void check_same_device(const Tensor& t, const Tensor& like, const char* name) {
     TORCH_CHECK(t.device() == like.device(), name, ": expected on ", like.device(), ", got ", t.device());
@@ -68,8 +86,10 @@ ExtArgs ext_args(const Tensor& q, const Tensor& k, const Tensor& v, int64_t head
     a.c = (float)(1.4426950408889634 / std::sqrt((double)hd));
     return a;
 }
+// a launch has fewer than 2^32 threads: 2^24 workgroups of 256
 void check_grid(const ExtArgs& a, const ExtPlan& p) {
-    TORCH_CHECK((long)a.B * a.Hkv < (1L << 30) / std::max(1, p.tiles * p.splits), "attention: more than 2^30 workgroups");
+    TORCH_CHECK((long)a.B * a.Hkv < (1L << 24) / std::max(1, p.tiles * p.splits), "attention: ", a.B, " sequences of ", a.Hkv,
+                " key heads are more workgroups than a launch has (2^24)");
 }
 void set_tables(ExtArgs& a, const Tensor& tab, const Tensor& codes, int64_t R) {
     const long Sp = (a.Sk + 127) / 128 * 128, Rp = (R + 3) / 4 * 4;
@@ -163,7 +183,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rel_bias_attention_fwd(const Tensor& 
                                                                   const OptTensor& lens, bool grad) {
     const long hd = packed_head_dim(qkv, heads), D = heads * hd, S = qkv.size(1), R = bucket_of.size(0), NB = table.size(0);
     TORCH_CHECK(R >= 1 && R <= kExtMaxEntries, "rel_bias_attention: ", R, " entries (1 to ", kExtMaxEntries, ")");
-    TORCH_CHECK(NB < (1L << 30) && S < (1L << 30), "rel_bias_attention: sizes below 2^30");
+    TORCH_CHECK(NB < (1L << 24) && S < (1L << 30) && heads < 65536, "rel_bias_attention: ", NB, " buckets, ", S, " positions, ", heads,
+                " heads (below 2^24, 2^30 and 2^16)");
     check_dense(table, {NB, heads}, at::kFloat, qkv, "table");
     check_dense(q_codes, {S}, at::kInt, qkv, "q_codes");
     check_dense(k_codes, {S}, at::kInt, qkv, "k_codes");
@@ -186,7 +207,7 @@ std::tuple<Tensor, Tensor> rel_bias_attention_bwd(const Tensor& dout, const Tens
                                                   const Tensor& tab, const Tensor& codes, const Tensor& bucket_of,
                                                   int64_t NB, int64_t heads, const OptTensor& lens, bool want_table) {
     const long hd = packed_head_dim(qkv, heads), D = heads * hd;
-    TORCH_CHECK(NB >= 0 && NB < (1L << 30), "rel_bias_attention: ", NB, " buckets");
+    TORCH_CHECK(NB >= 0 && NB < (1L << 24) && heads < 65536, "rel_bias_attention: ", NB, " buckets, ", heads, " heads");
     check_same_device(tab, qkv, "tab"); check_same_device(codes, qkv, "codes");
     TORCH_CHECK(tab.scalar_type() == at::kFloat && tab.is_contiguous() && codes.scalar_type() == at::kInt && codes.is_contiguous(),
                 "bias tables: as the forward made them");
@@ -298,7 +319,7 @@ std::vector<Tensor> gated_norm_bwd(const OptTensor& du, const OptTensor& dn, con
     float* gp = slab.data_ptr<float>() + cols * D;
     long gstride = srow;
     if (p.per_sample) {
-        TORCH_CHECK(x.size(0) < (1L << 31) / ((D + 63) / 64), "gated_residual_norm: ", x.size(0), " samples");
+        TORCH_CHECK(x.size(0) < (1L << 24) / ((D + 63) / 64), "gated_residual_norm: ", x.size(0), " samples");
         gate_part = q.chunks > 1 ? at::empty({q.units, D}, w.options()) : dgate;
         gp = gate_part.data_ptr<float>();
         gstride = D;
@@ -374,6 +395,7 @@ std::tuple<Tensor, Tensor> gated_residual_norm(const Tensor& x, const Tensor& y,
                                             given(pw) ? opt(param32(*pw)) : pw, given(pb) ? opt(param32(*pb)) : pb, eps, scale, false);
         return {u, n};
     }
+    check_capture({x, y, gate, w, b, pw, pb});
     const auto r = GatedNormFn::apply(x, y, gate, w, b, pw, pb, eps, scale);
     return {r[0], r[1]};
 }
@@ -385,6 +407,7 @@ void bind_transformer_ops(pybind11::module& m) {
     m.def("rel_bias_attention_bwd", &rel_bias_attention_bwd);
     m.def("cross_attention_fwd", &cross_attention_fwd);
     m.def("cross_attention_bwd", &cross_attention_bwd);
+    m.def("check_capture", &check_capture);
     m.def("gated_residual_norm", &gated_residual_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
     m.attr("rel_bias_max_entries") = kExtMaxEntries;
 }

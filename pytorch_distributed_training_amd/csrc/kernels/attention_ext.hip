@@ -25,7 +25,8 @@
 //  * No atomics in memory: the bias gradient sums dS over the batch in registers first (a kernel of its own, which walks over
 //    the batch with a block of pairs fixed), then the pairs by entry in a histogram per WAVE in LDS (program order), then waves
 //    and workgroups in a fixed order.
-#include <cmath>
+#include <stdexcept>
+#include <string>
 
 #include "attn_tile.h"
 #include "attention_ext.h"
@@ -1381,8 +1382,9 @@ __global__ __launch_bounds__(256) void k_bias_buckets(const float* __restrict__ 
 
 template <typename K>
 void allow_lds(K kern, size_t bytes) {
-    if (bytes > 65536)
-        PDT_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (bytes <= 65536) return;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) throw std::runtime_error(std::string("attention: ") + hipGetErrorString(e));  // (an exception of the call)
 }
 
 size_t table_bytes(const ExtArgs& a) { return a.tab ? (size_t)((a.Rp + 255) & ~255) * 4 : 0; }

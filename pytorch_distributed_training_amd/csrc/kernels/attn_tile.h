@@ -10,11 +10,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 typedef bf16x4 __attribute__((address_space(3))) * lds_bf16x4_ptr;
 
-// two floats -> two bf16 in one word (round to nearest even)
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    const f32x2 v = {a, b};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-}
 // accumulator tile regs [8*blk, 8*blk+8) -> bf16 A operand
 __device__ __forceinline__ bf16x8 acc_to_a(const f32x16& t, int blk) {
     bf16x8 a;

@@ -617,8 +617,11 @@ def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, leng
         if why is not None:
             _note_fallback("rel_bias_attention", why)
             be = reference
+    grad = _wants_grad(qkv, table)
+    if grad and be is not reference:
+        be.check_capture(qkv, table)
     qkv = _rows3(qkv)
-    if not _wants_grad(qkv, table):
+    if not grad:
         return be.rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, False)[0]
     return _RelBiasAttentionFn.apply(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, be)
 
@@ -665,8 +668,11 @@ def cross_attention(q, kv, heads: int, kv_heads: int | None = None, lengths=None
         if why is not None:
             _note_fallback("cross_attention", why)
             be = reference
+    grad = _wants_grad(q, kv)
+    if grad and be is not reference:
+        be.check_capture(q, kv)
     q, kv = _rows3(q), _rows3(kv)
-    if not _wants_grad(q, kv):
+    if not grad:
         return be.cross_attention_fwd(q, kv, heads, kv_heads, lengths, False)[0]
     return _CrossAttentionFn.apply(q, kv, heads, kv_heads, lengths, be)
 

@@ -268,11 +268,16 @@ def _al(t):
 
 
 def _i32(t):
-    return None if t is None else _al(t if t.dtype == torch.int32 else t.to(torch.int32))
+    return None if t is None else _al(t if t.dtype == torch.int32 else t.clamp(-(2 ** 31), 2 ** 31 - 1).to(torch.int32))
 
 
 def _f32(t):
     return _al(t if t.dtype == torch.float32 else t.float())
+
+
+def check_capture(*leaves):
+    """raises where a captured backward pass would meet an eager graph of the same leaves on another stream"""
+    _C.check_capture(leaves)
 
 
 def cross_attention_unsupported_reason(q, heads: int):

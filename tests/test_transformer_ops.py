@@ -674,3 +674,94 @@ def test_keys_past_32_bit_offsets():
         wide = F.cross_attention(q.expand(1, 40, -1), kv, heads, None, lens)  # the kernel for more rows
     for o in (out, wide):
         assert (o.double() - 3 * share).abs().max() <= 3 * (2 * U + SLACK)
+
+
+@gpu
+def test_lengths_and_buckets_outside_their_range():
+    """Counts below zero are none and counts past the end all, in 64 bits too; a bucket past 32 bits is no bucket."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(2)
+    q, kv = _rand(g, 4, 3, 64, device=dev), _rand(g, 4, 40, 128, device=dev)
+    want = torch.tensor([0, 40, 40, 7], dtype=torch.int32, device=dev)
+    qc, kc, of = (t.to(dev) for t in _log(40))
+    qkv, table = _rand(g, 4, 40, 192, device=dev), _rand(g, 8, 1, dtype=torch.float32, device=dev)
+    far = of.long()
+    far[5] += 2 ** 32  # an entry of bucket_of[5] in its lower half
+    none = of.clone()
+    none[5] = -1
+    for lens in (torch.tensor([-3, 41, 2 ** 31 - 1, 7], dtype=torch.int32, device=dev),
+                 torch.tensor([-(2 ** 33) - 1, 2 ** 32, 2 ** 32 + 3, 7], device=dev)):
+        a, b = q.clone().requires_grad_(), q.clone().requires_grad_()
+        x, y = F.cross_attention(a, kv, 1, None, lens), F.cross_attention(b, kv, 1, None, want)
+        assert torch.equal(x, y)
+        assert torch.equal(*(torch.autograd.grad(o, t, torch.ones_like(o))[0] for o, t in ((x, a), (y, b))))
+        a, b = table.clone().requires_grad_(), table.clone().requires_grad_()
+        x, y = F.rel_bias_attention(qkv, a, qc, kc, far, 1, lens), F.rel_bias_attention(qkv, b, qc, kc, none, 1, want)
+        assert torch.equal(x, y)
+        assert torch.equal(*(torch.autograd.grad(o, t, torch.ones_like(o))[0] for o, t in ((x, a), (y, b))))
+
+
+@gpu
+def test_more_sequences_than_a_launch_has_workgroups():
+    dev = _dev("cuda")
+    n = 1 << 24
+    q, kv = (torch.zeros(1, 1, w, dtype=torch.bfloat16, device=dev).expand(n, -1, -1) for w in (32, 64))
+    with pytest.raises(RuntimeError, match="workgroups"):
+        F.cross_attention(q, kv, 1)
+    qc, kc, of = (t.to(dev) for t in _log(1))
+    table = torch.zeros(8, 1, device=dev)
+    with pytest.raises(RuntimeError, match="workgroups"):
+        F.rel_bias_attention(torch.zeros(1, 1, 96, dtype=torch.bfloat16, device=dev).expand(n, -1, -1), table, qc, kc, of, 1)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_gradients_twice_and_of_gradients(device):
+    """A graph that is kept gives the same gradients again; gradients of gradients are refused."""
+    dev = _dev(device)
+    g = torch.Generator().manual_seed(7)
+    qc, kc, of = (t.to(dev) for t in _log(9))
+    qkv, q, kv = (_rand(g, 2, 9, w, device=dev).requires_grad_() for w in (192, 64, 128))
+    table, gate = (_rand(g, *s, dtype=torch.float32, device=dev).requires_grad_() for s in ((8, 1), (64,)))
+    one = torch.ones(64, device=dev)
+    for call, leaves in ((lambda: F.rel_bias_attention(qkv, table, qc, kc, of, 1), [qkv, table]),
+                         (lambda: F.cross_attention(q, kv, 1), [q, kv]),
+                         (lambda: F.gated_residual_norm(q, q * 0.5, gate, one, one)[1], [q, gate])):
+        out = call()
+        w = torch.ones_like(out)
+        w[:, ::2] = 0.5
+        a = torch.autograd.grad(out, leaves, w, retain_graph=True)
+        b = torch.autograd.grad(out, leaves, w, retain_graph=True)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+        with pytest.raises(RuntimeError):
+            c = torch.autograd.grad(out, leaves, w, create_graph=True)
+            torch.autograd.grad(c[0].float().sum(), leaves)
+
+
+@gpu
+def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
+    """The forward says so: the backward would end the process.  Released, the capture works."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(8)
+    qc, kc, of = (t.to(dev) for t in _log(9))
+    table, q, gate = (_rand(g, *s, dtype=t, device=dev).requires_grad_()
+                      for s, t in (((8, 1), torch.float32), ((2, 9, 64), torch.bfloat16), ((64,), torch.float32)))
+    qkv, kv, x = (_rand(g, 2, 9, w, device=dev) for w in (192, 128, 64))
+    one = torch.ones(64, device=dev)
+    for call, leaf in ((lambda: F.rel_bias_attention(qkv, table, qc, kc, of, 1), table), (lambda: F.cross_attention(q, kv, 1), q),
+                       (lambda: F.gated_residual_norm(x, x, gate, one, one)[0], gate)):
+        alive = call()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                one * 2
+                call()
+        want = torch.autograd.grad(alive, leaf, torch.ones_like(alive))[0]
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+            (got,) = torch.autograd.grad(out, leaf, torch.ones_like(out))
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
