@@ -8,6 +8,8 @@
 #include <torch/extension.h>
 
 #include <cmath>
+#include <initializer_list>
+#include <limits>
 
 #include "../kernels/attention_ext.h"
 #include "../kernels/gated_norm.h"
@@ -23,12 +25,37 @@ using OptTensor = c10::optional<Tensor>;
 hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 
+// The operators are differentiable calls with their nodes in C++: with Python functions a backward spent 20 to 50 us more on the
+// interpreter (lock, unpacking of saved tensors), more than its kernels take on small inputs.  A call whose operands the kernels
+// do not take (or that nobody should make) returns nothing: the Python side has the words for why.
+Tensor dense16(const Tensor& t) {  // contiguous and 16-B aligned, by a copy where it is not
+    if (!t.defined()) return t;
+    Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+Tensor param32(const Tensor& t) { return t.defined() ? dense16(t.scalar_type() == at::kFloat ? t : t.to(at::kFloat)) : t; }
+Tensor int32(const Tensor& t) {
+    if (!t.defined() || t.scalar_type() == at::kInt) return dense16(t);
+    return t.clamp(std::numeric_limits<int32_t>::min(), std::numeric_limits<int32_t>::max()).to(at::kInt);
+}
+bool is_index(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : ts)
+        if (t->defined() && t->requires_grad()) return true;
+    return false;
+}
+void no_second_backward(const char* op) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the backward pass cannot be differentiated again");
+}
+
 // A backward pass that is captured while an eager graph of the same leaves lives accumulates on the eager graph's stream: the
 // engine would wait for a stream outside the capture, in a thread whose exception ends the process.  Refused at the forward.
-void check_capture(const std::vector<OptTensor>& leaves) {
-    if (!at::GradMode::is_enabled() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    for (const OptTensor& t : leaves) {
-        if (!given(t) || !t->requires_grad() || !t->is_leaf()) continue;
+void check_capture(std::initializer_list<const Tensor*> leaves) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const Tensor* t : leaves) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
         if (!node || !node->stream()) continue;
         const hipStream_t s = c10::hip::HIPStreamMasqueradingAsCUDA(c10::hip::HIPStreamMasqueradingAsCUDA::UNCHECKED, *node->stream()).stream();
@@ -51,6 +78,21 @@ void check_rows(const Tensor& t, const char* name) {
     TORCH_CHECK(t.size(1) < 2 || (t.stride(1) % 8 == 0 && t.stride(1) >= t.size(2) && t.stride(1) < (1L << 23)), name,
                 ": row stride ", t.stride(1));
     TORCH_CHECK(t.size(0) < 2 || (t.stride(0) % 8 == 0 && t.stride(0) >= 0), name, ": batch stride ", t.stride(0));
+}
+// `t` where its rows are as check_rows wants them, else a copy
+Tensor rows3(const Tensor& t) {
+    const bool ok = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                    (t.size(1) < 2 || (t.stride(1) % 8 == 0 && t.stride(1) >= t.size(2) && t.stride(1) < (1L << 23))) &&
+                    (t.size(0) < 2 || t.stride(0) % 8 == 0);
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+bool lengths_fit(const OptTensor& lens, const Tensor& like) {
+    return !given(lens) || (lens->dim() == 1 && lens->size(0) == like.size(0) && is_index(*lens) && lens->device() == like.device());
+}
+bool attention_dim_ok(int64_t width, int64_t parts) {
+    if (parts < 1 || width % parts) return false;
+    const int64_t hd = width / parts;
+    return hd == 32 || hd == 64 || hd == 128;
 }
 void check_dense(const Tensor& t, at::IntArrayRef shape, at::ScalarType type, const Tensor& like, const char* name) {
     TORCH_CHECK(t.scalar_type() == type && t.is_contiguous() && t.sizes() == shape, name, ": expected contiguous ", type, " ", shape,
@@ -221,6 +263,48 @@ std::tuple<Tensor, Tensor> rel_bias_attention_bwd(const Tensor& dout, const Tens
     return {dqkv, dtable};
 }
 
+struct RelBiasFn : torch::autograd::Function<RelBiasFn> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& qkv_, const Tensor& table_, const Tensor& q_codes,
+                          const Tensor& k_codes, const Tensor& bucket_of_, const OptTensor& lens_, int64_t heads) {
+        const Tensor qkv = rows3(qkv_), bucket_of = int32(bucket_of_), lens = given(lens_) ? int32(*lens_) : Tensor();
+        auto [out, stat, tab, codes] = rel_bias_attention_fwd(qkv, param32(table_), int32(q_codes), int32(k_codes), bucket_of, heads, opt(lens), true);
+        ctx->save_for_backward({qkv, out, stat, tab, codes, bucket_of, lens});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["heads"] = heads;
+        ctx->saved_data["buckets"] = table_.size(0);
+        ctx->saved_data["type"] = (int64_t)table_.scalar_type();
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        no_second_backward("rel_bias_attention");
+        torch::autograd::variable_list r(7);
+        if (!g[0].defined()) return r;
+        const auto s = ctx->get_saved_variables();
+        auto [dqkv, dtable] = rel_bias_attention_bwd(dense16(g[0]), s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["buckets"].toInt(),
+                                                     ctx->saved_data["heads"].toInt(), opt(s[6]), ctx->needs_input_grad(1));
+        r[0] = dqkv;
+        if (dtable.defined()) r[1] = dtable.to((at::ScalarType)ctx->saved_data["type"].toInt());
+        return r;
+    }
+};
+OptTensor rel_bias_attention(const Tensor& qkv, const Tensor& table, const Tensor& q_codes, const Tensor& k_codes, const Tensor& bucket_of,
+                             int64_t heads, const OptTensor& lens) {
+    if (!qkv.is_cuda() || qkv.scalar_type() != at::kBFloat16 || qkv.dim() != 3 || heads < 1 || !attention_dim_ok(qkv.size(2), 3 * heads) ||
+        table.dim() != 2 || table.size(1) != heads || !at::isFloatingType(table.scalar_type()) || bucket_of.dim() != 1 ||
+        bucket_of.size(0) < 1 || bucket_of.size(0) > kExtMaxEntries || !lengths_fit(lens, qkv))
+        return {};
+    for (const Tensor* t : {&q_codes, &k_codes})
+        if (t->dim() != 1 || t->size(0) != qkv.size(1)) return {};
+    for (const Tensor* t : {&q_codes, &k_codes, &bucket_of})
+        if (!is_index(*t) || t->device() != qkv.device()) return {};
+    if (table.device() != qkv.device()) return {};
+    if (!wants_grad({&qkv, &table}))
+        return std::get<0>(rel_bias_attention_fwd(rows3(qkv), param32(table), int32(q_codes), int32(k_codes), int32(bucket_of), heads,
+                                                  given(lens) ? opt(int32(*lens)) : lens, false));
+    check_capture({&qkv, &table});
+    return RelBiasFn::apply(qkv, table, q_codes, k_codes, bucket_of, lens, heads);
+}
+
 // ------------------------------------------------------------------------------------------- cross attention
 long cross_head_dim(const Tensor& q, const Tensor& kv, int64_t heads, int64_t kv_heads) {
     check_rows(q, "q"); check_rows(kv, "kv");
@@ -248,6 +332,40 @@ std::tuple<Tensor, Tensor> cross_attention_bwd(const Tensor& dout, const Tensor&
     Tensor dkv = at::empty(kv.sizes(), kv.options().memory_format(at::MemoryFormat::Contiguous));
     ext_bwd(a, q, heads, hd, dout, out, stat, dq, dkv.narrow(2, 0, W), dkv.narrow(2, W, W), OptTensor(), 0);
     return {dq, dkv};
+}
+
+struct CrossFn : torch::autograd::Function<CrossFn> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& q_, const Tensor& kv_, const OptTensor& lens_, int64_t heads,
+                          int64_t kv_heads) {
+        const Tensor q = rows3(q_), kv = rows3(kv_), lens = given(lens_) ? int32(*lens_) : Tensor();
+        auto [out, stat] = cross_attention_fwd(q, kv, heads, kv_heads, opt(lens), true);
+        ctx->save_for_backward({q, kv, out, stat, lens});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["heads"] = heads;
+        ctx->saved_data["kv_heads"] = kv_heads;
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        no_second_backward("cross_attention");
+        torch::autograd::variable_list r(5);
+        if (!g[0].defined()) return r;
+        const auto s = ctx->get_saved_variables();
+        auto [dq, dkv] = cross_attention_bwd(dense16(g[0]), s[0], s[1], s[2], s[3], ctx->saved_data["heads"].toInt(),
+                                             ctx->saved_data["kv_heads"].toInt(), opt(s[4]));
+        r[0] = dq;
+        r[1] = dkv;
+        return r;
+    }
+};
+OptTensor cross_attention(const Tensor& q, const Tensor& kv, int64_t heads, int64_t kv_heads, const OptTensor& lens) {
+    if (!q.is_cuda() || q.scalar_type() != at::kBFloat16 || kv.scalar_type() != at::kBFloat16 || q.dim() != 3 || kv.dim() != 3 || heads < 1 ||
+        kv_heads < 1 || heads % kv_heads || !attention_dim_ok(q.size(2), heads) || kv.size(2) != 2 * kv_heads * (q.size(2) / heads) ||
+        q.size(0) != kv.size(0) || q.device() != kv.device() || !lengths_fit(lens, q))
+        return {};
+    if (!wants_grad({&q, &kv}))
+        return std::get<0>(cross_attention_fwd(rows3(q), rows3(kv), heads, kv_heads, given(lens) ? opt(int32(*lens)) : lens, false));
+    check_capture({&q, &kv});
+    return CrossFn::apply(q, kv, lens, heads, kv_heads);
 }
 
 // ---------------------------------------------------------------------------------------- gated residual norm
@@ -344,16 +462,6 @@ std::vector<Tensor> gated_norm_bwd(const OptTensor& du, const OptTensor& dn, con
     return r;
 }
 
-// ---- as one differentiable call, in C++: with a Python function the backward spent some 50 us on the interpreter (lock, unpacking
-// of nine tensors), more than its kernels take on a [64 * 197, 768] activation
-Tensor dense16(const Tensor& t) {  // contiguous and 16-B aligned, by a copy where it is not
-    if (!t.defined()) return t;
-    Tensor c = t.contiguous();
-    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
-}
-Tensor param32(const Tensor& t) { return t.defined() ? dense16(t.scalar_type() == at::kFloat ? t : t.to(at::kFloat)) : t; }
-OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
-
 struct GatedNormFn : torch::autograd::Function<GatedNormFn> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x_, const Tensor& y_, const Tensor& gate_,
                                                   const Tensor& w_, const Tensor& b_, const OptTensor& pw_, const OptTensor& pb_, double eps,
@@ -371,7 +479,7 @@ struct GatedNormFn : torch::autograd::Function<GatedNormFn> {
         return {u, n};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
-        TORCH_CHECK(!at::GradMode::is_enabled(), "gated_residual_norm: the backward pass cannot be differentiated again");
+        no_second_backward("gated_residual_norm");
         torch::autograd::variable_list r(9);
         if (!g[0].defined() && !g[1].defined()) return r;
         const auto s = ctx->get_saved_variables();
@@ -385,30 +493,36 @@ struct GatedNormFn : torch::autograd::Function<GatedNormFn> {
         return r;
     }
 };
-std::tuple<Tensor, Tensor> gated_residual_norm(const Tensor& x, const Tensor& y, const Tensor& gate, const Tensor& w, const Tensor& b,
-                                               const OptTensor& pw, const OptTensor& pb, double eps, double scale) {
-    bool grad = false;
-    if (at::GradMode::is_enabled())
-        for (const Tensor* t : {&x, &y, &gate, &w, &b, given(pw) ? &*pw : &w, given(pb) ? &*pb : &b}) grad |= t->requires_grad();
-    if (!grad) {
-        auto [u, n, stats] = gated_norm_fwd(dense16(x), dense16(y), param32(gate), param32(w), param32(b),
-                                            given(pw) ? opt(param32(*pw)) : pw, given(pb) ? opt(param32(*pb)) : pb, eps, scale, false);
-        return {u, n};
+c10::optional<std::tuple<Tensor, Tensor>> gated_residual_norm(const Tensor& x, const Tensor& y, const Tensor& gate, const Tensor& w,
+                                                              const Tensor& b, const OptTensor& pw_, const OptTensor& pb_, double eps,
+                                                              double scale) {
+    const Tensor pw = given(pw_) ? *pw_ : Tensor(), pb = given(pb_) ? *pb_ : Tensor();
+    if (!x.is_cuda() || x.scalar_type() != at::kBFloat16 || x.dim() < 2 || !gated_norm_dim_ok(x.size(-1)) || y.scalar_type() != x.scalar_type() ||
+        y.sizes() != x.sizes() || y.device() != x.device() || pw.defined() != pb.defined())
+        return {};
+    const int64_t D = x.size(-1);
+    if (gate.sizes() != at::IntArrayRef({D}) && gate.sizes() != at::IntArrayRef({x.size(0), D})) return {};
+    for (const Tensor* t : {&gate, &w, &b, &pw, &pb}) {
+        if (!t->defined()) continue;
+        if (t->device() != x.device() || !at::isFloatingType(t->scalar_type()) || (t != &gate && t->sizes() != at::IntArrayRef({D}))) return {};
     }
-    check_capture({x, y, gate, w, b, pw, pb});
-    const auto r = GatedNormFn::apply(x, y, gate, w, b, pw, pb, eps, scale);
-    return {r[0], r[1]};
+    if (!wants_grad({&x, &y, &gate, &w, &b, &pw, &pb})) {
+        auto [u, n, stats] = gated_norm_fwd(dense16(x), dense16(y), param32(gate), param32(w), param32(b), opt(param32(pw)),
+                                            opt(param32(pb)), eps, scale, false);
+        return std::make_tuple(u, n);
+    }
+    check_capture({&x, &y, &gate, &w, &b, &pw, &pb});
+    const auto r = GatedNormFn::apply(x, y, gate, w, b, pw_, pb_, eps, scale);
+    return std::make_tuple(r[0], r[1]);
 }
 
 }  // namespace
 
 void bind_transformer_ops(pybind11::module& m) {
-    m.def("rel_bias_attention_fwd", &rel_bias_attention_fwd);
-    m.def("rel_bias_attention_bwd", &rel_bias_attention_bwd);
-    m.def("cross_attention_fwd", &cross_attention_fwd);
-    m.def("cross_attention_bwd", &cross_attention_bwd);
-    m.def("check_capture", &check_capture);
-    m.def("gated_residual_norm", &gated_residual_norm, pybind11::call_guard<pybind11::gil_scoped_release>());
+    using release = pybind11::call_guard<pybind11::gil_scoped_release>;
+    m.def("rel_bias_attention", &rel_bias_attention, release());
+    m.def("cross_attention", &cross_attention, release());
+    m.def("gated_residual_norm", &gated_residual_norm, release());
     m.attr("rel_bias_max_entries") = kExtMaxEntries;
 }
 

@@ -544,17 +544,6 @@ def layer_norm(x, weight, bias, eps: float = 1e-5, with_skip: bool = False):
 
 
 # ------------------------------------------------- attention with relative positions, cross attention, gated norms
-def _rows3(t):
-    """``t`` [B, rows, width] with contiguous, 16-B aligned, non-overlapping rows (a copy only where it has none)"""
-    ok = (t.stride(2) == 1 and t.data_ptr() % 16 == 0 and (t.shape[1] < 2 or (t.stride(1) % 8 == 0 and t.stride(1) >= t.shape[2]
-          and t.stride(1) < (1 << 23))) and (t.shape[0] < 2 or t.stride(0) % 8 == 0))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
-
-
-def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
-
-
 def _check_lengths(lengths, like, op: str) -> None:
     if lengths is None:
         return
@@ -565,21 +554,22 @@ def _check_lengths(lengths, like, op: str) -> None:
 
 
 class _RelBiasAttentionFn(torch.autograd.Function):
+    """The oracle's node (the kernels' is csrc/binding/ops_transformer.cpp)"""
+
     @staticmethod
-    def forward(ctx, qkv, table, q_codes, k_codes, bucket_of, heads, lengths, be):
-        out, lse, tab, codes = be.rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, True)
-        ctx.save_for_backward(qkv, out, lse, tab, codes, bucket_of, lengths)
-        ctx.cfg = (be, heads, table.shape[0], table.dtype)
+    def forward(ctx, qkv, table, q_codes, k_codes, bucket_of, heads, lengths):
+        out = reference.rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads, lengths)
+        ctx.save_for_backward(qkv, table, q_codes, k_codes, bucket_of, lengths)
+        ctx.heads = heads
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        qkv, out, lse, tab, codes, bucket_of, lengths = ctx.saved_tensors
-        be, heads, buckets, tdt = ctx.cfg
-        dqkv, dtable = be.rel_bias_attention_bwd(dout, qkv, out, lse, tab, codes, bucket_of, buckets, heads, lengths,
-                                                 ctx.needs_input_grad[1])
-        return dqkv, (None if dtable is None else dtable.to(tdt)), None, None, None, None, None, None
+        qkv, table, q_codes, k_codes, bucket_of, lengths = ctx.saved_tensors
+        dqkv, dtable = reference.rel_bias_attention_bwd(dout, qkv, table, q_codes, k_codes, bucket_of, ctx.heads, lengths,
+                                                        ctx.needs_input_grad[1])
+        return dqkv, (None if dtable is None else dtable.to(table.dtype)), None, None, None, None, None
 
 
 def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None):
@@ -596,6 +586,11 @@ def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, leng
     On bf16 GPU tensors with head_dim 32 / 64 / 128 and at most 4096 entries the HIP kernels of csrc/kernels/attention_ext.hip run;
     the PyTorch oracle elsewhere."""
     heads = int(heads)
+    be = backend_for(qkv)
+    if be is not reference:
+        out = be.rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads, lengths)
+        if out is not None:
+            return out
     if qkv.dim() != 3 or heads < 1 or qkv.shape[2] % (3 * heads):
         raise ValueError(f"rel_bias_attention: qkv {tuple(qkv.shape)} is not [B, S, 3 * {heads} * head_dim]")
     if table.dim() != 2 or table.shape[1] != heads:
@@ -611,36 +606,26 @@ def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, leng
         if name != "table" and t.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"rel_bias_attention: {name} must be integers, got {t.dtype}")
     _check_lengths(lengths, qkv, "rel_bias_attention")
-    be = backend_for(qkv)
     if be is not reference:
-        why = be.rel_bias_attention_unsupported_reason(qkv, heads, bucket_of)
-        if why is not None:
-            _note_fallback("rel_bias_attention", why)
-            be = reference
-    grad = _wants_grad(qkv, table)
-    if grad and be is not reference:
-        be.check_capture(qkv, table)
-    qkv = _rows3(qkv)
-    if not grad:
-        return be.rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, False)[0]
-    return _RelBiasAttentionFn.apply(qkv, table, q_codes, k_codes, bucket_of, heads, lengths, be)
+        _note_fallback("rel_bias_attention", be.rel_bias_attention_unsupported_reason(qkv, table, heads, bucket_of))
+    return _RelBiasAttentionFn.apply(qkv, table, q_codes, k_codes, bucket_of, heads, lengths)
 
 
 class _CrossAttentionFn(torch.autograd.Function):
+    """The oracle's node"""
+
     @staticmethod
-    def forward(ctx, q, kv, heads, kv_heads, lengths, be):
-        out, lse = be.cross_attention_fwd(q, kv, heads, kv_heads, lengths, True)
-        ctx.save_for_backward(q, kv, out, lse, lengths)
-        ctx.cfg = (be, heads, kv_heads)
-        return out
+    def forward(ctx, q, kv, heads, kv_heads, lengths):
+        ctx.save_for_backward(q, kv, lengths)
+        ctx.cfg = (heads, kv_heads)
+        return reference.cross_attention_fwd(q, kv, heads, kv_heads, lengths)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, kv, out, lse, lengths = ctx.saved_tensors
-        be, heads, kv_heads = ctx.cfg
-        dq, dkv = be.cross_attention_bwd(dout, q, kv, out, lse, heads, kv_heads, lengths)
-        return dq, dkv, None, None, None, None
+        q, kv, lengths = ctx.saved_tensors
+        dq, dkv = reference.cross_attention_bwd(dout, q, kv, *ctx.cfg, lengths)
+        return dq, dkv, None, None, None
 
 
 def cross_attention(q, kv, heads: int, kv_heads: int | None = None, lengths=None):
@@ -654,6 +639,11 @@ def cross_attention(q, kv, heads: int, kv_heads: int | None = None, lengths=None
     32 / 64 / 128, the PyTorch oracle elsewhere."""
     heads = int(heads)
     kv_heads = heads if kv_heads is None else int(kv_heads)
+    be = backend_for(q)
+    if be is not reference:
+        out = be.cross_attention(q, kv, heads, kv_heads, lengths)
+        if out is not None:
+            return out
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"cross_attention: {heads} heads over {kv_heads} key heads")
     if q.dim() != 3 or kv.dim() != 3 or q.shape[0] != kv.shape[0] or q.shape[2] % heads or (
@@ -662,19 +652,9 @@ def cross_attention(q, kv, heads: int, kv_heads: int | None = None, lengths=None
     if q.device != kv.device or q.dtype != kv.dtype:
         raise ValueError(f"cross_attention: q is {q.dtype} on {q.device}, kv {kv.dtype} on {kv.device}")
     _check_lengths(lengths, q, "cross_attention")
-    be = backend_for(q)
     if be is not reference:
-        why = be.cross_attention_unsupported_reason(q, heads)
-        if why is not None:
-            _note_fallback("cross_attention", why)
-            be = reference
-    grad = _wants_grad(q, kv)
-    if grad and be is not reference:
-        be.check_capture(q, kv)
-    q, kv = _rows3(q), _rows3(kv)
-    if not grad:
-        return be.cross_attention_fwd(q, kv, heads, kv_heads, lengths, False)[0]
-    return _CrossAttentionFn.apply(q, kv, heads, kv_heads, lengths, be)
+        _note_fallback("cross_attention", be.cross_attention_unsupported_reason(q, heads))
+    return _CrossAttentionFn.apply(q, kv, heads, kv_heads, lengths)
 
 
 def gated_residual_norm(x, branch, gate, weight, bias, eps: float = 1e-6, post_weight=None, post_bias=None,
@@ -685,6 +665,12 @@ def gated_residual_norm(x, branch, gate, weight, bias, eps: float = 1e-6, post_w
     ``[D]`` (layer scale) or ``[B, D]``, one for each entry of the first dimension.  ``normed`` is taken of ``x_new`` before
     that is rounded to the stream's type.  HIP kernel (csrc/kernels/gated_norm.hip) on bf16 GPU tensors, widths that are
     multiples of 4 up to 2048; fp32 PyTorch oracle elsewhere."""
+    eps, residual_scale = float(eps), float(residual_scale)
+    be = backend_for(x)
+    if be is not reference:
+        out = be.gated_residual_norm(x, branch, gate, weight, bias, eps, post_weight, post_bias, residual_scale)
+        if out is not None:
+            return out
     d = x.shape[-1] if x.dim() else 0
     if x.dim() < 2 or x.shape != branch.shape or x.dtype != branch.dtype:
         raise ValueError(f"gated_residual_norm: x {tuple(x.shape)} {x.dtype}, branch {tuple(branch.shape)} {branch.dtype}")
@@ -698,13 +684,9 @@ def gated_residual_norm(x, branch, gate, weight, bias, eps: float = 1e-6, post_w
             raise ValueError(f"gated_residual_norm: {name} is on {t.device}, x on {x.device}")
         if t is not None and name not in ("branch", "gate") and tuple(t.shape) != (d,):
             raise ValueError(f"gated_residual_norm: {name} {tuple(t.shape)} for width {d}")
-    be = backend_for(x)
     if be is not reference:
-        why = be.layernorm_unsupported_reason(x)
-        if why is not None:
-            _note_fallback("gated_residual_norm", why)
-            be = reference
-    return be.gated_residual_norm(x, branch, gate, weight, bias, float(eps), post_weight, post_bias, float(residual_scale))
+        _note_fallback("gated_residual_norm", be.layernorm_unsupported_reason(x) or f"parameters in {gate.dtype}, {weight.dtype}")
+    return reference.gated_residual_norm(x, branch, gate, weight, bias, eps, post_weight, post_bias, residual_scale)
 
 
 # ------------------------------------------------------------------- linear

@@ -259,71 +259,37 @@ def layernorm_bwd(dy, x, mean, rstd, gamma, addend=None):
 
 
 # -------------------------------- attention with relative positions, cross attention (csrc/kernels/attention_ext.hip)
-def _al(t):
-    """dense and 16-B aligned (a copy only where it is not: a slice that starts at an odd element)"""
-    if t is None:
-        return None
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _i32(t):
-    return None if t is None else _al(t if t.dtype == torch.int32 else t.clamp(-(2 ** 31), 2 ** 31 - 1).to(torch.int32))
-
-
-def _f32(t):
-    return _al(t if t.dtype == torch.float32 else t.float())
-
-
-def check_capture(*leaves):
-    """raises where a captured backward pass would meet an eager graph of the same leaves on another stream"""
-    _C.check_capture(leaves)
-
-
 def cross_attention_unsupported_reason(q, heads: int):
     if q.dtype != _BF16:
         return f"dtype {q.dtype} (native attention is bf16)"
     if q.shape[2] // heads not in (32, 64, 128):
         return f"head_dim {q.shape[2] // heads} (native attention: head_dim 32, 64 or 128)"
-    return None
+    raise RuntimeError("cross_attention: the kernels refused operands that they have")
 
 
-def rel_bias_attention_unsupported_reason(qkv, heads: int, bucket_of):
+def rel_bias_attention_unsupported_reason(qkv, table, heads: int, bucket_of):
     if qkv.dtype != _BF16:
         return f"dtype {qkv.dtype} (native attention is bf16)"
     if qkv.shape[2] // (3 * heads) not in (32, 64, 128):
         return f"head_dim {qkv.shape[2] // (3 * heads)} (native attention: head_dim 32, 64 or 128)"
     if bucket_of.shape[0] > _C.rel_bias_max_entries:
         return f"{bucket_of.shape[0]} relative positions (native: up to {_C.rel_bias_max_entries})"
-    return None
+    return f"a table in {table.dtype}"
 
 
-def rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None, grad: bool = True):
-    """-> (out [B, S, D], statistics for the backward or None, tab, codes)"""
-    return _C.rel_bias_attention_fwd(qkv, _f32(table), _i32(q_codes), _i32(k_codes), _i32(bucket_of), heads, _i32(lengths),
-                                     grad)
+def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths):
+    """-> out [B, S, D], differentiable (the autograd nodes are in the extension), or None for operands without a kernel"""
+    return _C.rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads, lengths)
 
 
-def rel_bias_attention_bwd(dout, qkv, out, lse, tab, codes, bucket_of, buckets: int, heads: int, lengths=None,
-                           want_table: bool = True):
-    """-> (dqkv, dtable [buckets, heads] fp32, or None)"""
-    return _C.rel_bias_attention_bwd(_al(dout), qkv, out, lse, tab, codes, _i32(bucket_of), buckets, heads,
-                                     _i32(lengths), want_table)
-
-
-def cross_attention_fwd(q, kv, heads: int, kv_heads: int, lengths=None, grad: bool = True):
-    """-> (out [B, Sq, H*hd], statistics for the backward or None)"""
-    return _C.cross_attention_fwd(q, kv, heads, kv_heads, _i32(lengths), grad)
-
-
-def cross_attention_bwd(dout, q, kv, out, lse, heads: int, kv_heads: int, lengths=None):
-    """-> (dq, dkv)"""
-    return _C.cross_attention_bwd(_al(dout), q, kv, out, lse, heads, kv_heads, _i32(lengths))
+def cross_attention(q, kv, heads: int, kv_heads: int, lengths):
+    """-> out [B, Sq, H*hd], differentiable, or None for operands without a kernel"""
+    return _C.cross_attention(q, kv, heads, kv_heads, lengths)
 
 
 # ------------------------------------------------------------------------- gated norm (csrc/kernels/gated_norm.hip)
 def gated_residual_norm(x, branch, gate, weight, bias, eps: float, post_weight, post_bias, scale: float):
-    """-> (x_new, normed), differentiable (the autograd node is in the extension)"""
+    """-> (x_new, normed), differentiable, or None for operands without a kernel"""
     return _C.gated_residual_norm(x, branch, gate, weight, bias, post_weight, post_bias, eps, scale)
 
 

@@ -258,21 +258,20 @@ def _rel_probs(q, k, table, bucket, lengths):
     return p, real
 
 
-def rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None, grad: bool = True):
-    """Oracle of csrc/kernels/attention_ext.hip -> (out, None, table, codes)"""
+def rel_bias_attention_fwd(qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None):
+    """Oracle of csrc/kernels/attention_ext.hip -> out"""
     b, s, w = qkv.shape
     q, k, v = _rel_parts(qkv, heads, lengths)
     p, _ = _rel_probs(q, k, table, _rel_buckets(q_codes, k_codes, bucket_of), lengths)
-    out = torch.matmul(p, v).transpose(1, 2).reshape(b, s, w // 3).to(qkv.dtype)
-    return out, None, table, torch.stack([q_codes, k_codes])
+    return torch.matmul(p, v).transpose(1, 2).reshape(b, s, w // 3).to(qkv.dtype)
 
 
-def rel_bias_attention_bwd(dout, qkv, out, lse, tab, codes, bucket_of, buckets: int, heads: int, lengths=None,
-                           want_table: bool = True):
+def rel_bias_attention_bwd(dout, qkv, table, q_codes, k_codes, bucket_of, heads: int, lengths=None, want_table: bool = True):
+    """-> (dqkv, dtable, or None)"""
     b, s, w = qkv.shape
     q, k, v = _rel_parts(qkv, heads, lengths)
-    bucket = _rel_buckets(codes[0], codes[1], bucket_of)
-    p, real = _rel_probs(q, k, tab, bucket, lengths)
+    bucket, buckets = _rel_buckets(q_codes, k_codes, bucket_of), table.shape[0]
+    p, real = _rel_probs(q, k, table, bucket, lengths)
     do = _no_dead_rows(dout.to(q.dtype).view(b, s, heads, -1).transpose(1, 2), lengths)
     dq, dk, dv, ds = _ext_grads(do, q, k, v, p)
     dqkv = torch.stack([dq, dk, dv]).permute(1, 3, 0, 2, 4).reshape(b, s, w).to(qkv.dtype)
@@ -300,13 +299,14 @@ def _cross_rows(t, q, heads, kv_heads):
     return t.view(b, kv_heads, heads // kv_heads, sq, w // heads).permute(0, 3, 1, 2, 4).reshape(b, sq, w).to(q.dtype)
 
 
-def cross_attention_fwd(q, kv, heads: int, kv_heads: int, lengths=None, grad: bool = True):
-    """Oracle of csrc/kernels/attention_ext.hip -> (out, None)"""
+def cross_attention_fwd(q, kv, heads: int, kv_heads: int, lengths=None):
+    """Oracle of csrc/kernels/attention_ext.hip -> out"""
     qf, k, v = _cross_parts(q, kv, heads, kv_heads, lengths)
-    return _cross_rows(torch.matmul(_ext_probs(qf, k, None, lengths), v), q, heads, kv_heads), None
+    return _cross_rows(torch.matmul(_ext_probs(qf, k, None, lengths), v), q, heads, kv_heads)
 
 
-def cross_attention_bwd(dout, q, kv, out, lse, heads: int, kv_heads: int, lengths=None):
+def cross_attention_bwd(dout, q, kv, heads: int, kv_heads: int, lengths=None):
+    """-> (dq, dkv)"""
     b, sk = kv.shape[:2]
     qf, k, v = _cross_parts(q, kv, heads, kv_heads, lengths)
     do = _cross_parts(dout, kv, heads, kv_heads, None)[0]
