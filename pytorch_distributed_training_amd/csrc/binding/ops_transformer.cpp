@@ -13,7 +13,6 @@
 
 #include "../kernels/attention_ext.h"
 #include "../kernels/gated_norm.h"
-#include "../kernels/kernels.h"
 #include "binding.h"
 
 namespace pdt {
@@ -203,7 +202,7 @@ Tensor ext_bwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, const Ten
     }
     launch_ext_bwd(a, w, (int)hd, stream_of(q));
     if (dtable.defined() && NB > 0) {
-        const RelPlan p = rel_plan(a.B, a.Hkv, a.Sk);
+        const RelPlan p = rel_plan(a.B, a.Hkv, a.Sk, (int)hd);
         Tensor dense = at::empty({p.dense}, f32), slab = at::empty({(long)heads * p.rows, a.Rp}, f32),
                mid = at::empty({(long)heads, a.Rp}, f32);
         launch_rel_bias_grad(a, w, (int)hd, p, dense.data_ptr<float>(), slab.data_ptr<float>(), mid.data_ptr<float>(),
@@ -421,43 +420,33 @@ std::vector<Tensor> gated_norm_bwd(const OptTensor& du, const OptTensor& dn, con
     check_dense(stats, {post ? 4 : 2, p.M}, at::kFloat, x, "stats");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     const long D = p.D;
-    Tensor dx = at::empty_like(x), dy = at::empty_like(x), dgate = at::empty(gate.sizes(), gate.options());
+    Tensor dx = at::empty_like(x), dy = at::empty_like(x);
     const int cols = post ? 4 : 2;
     if (p.M == 0) {
         Tensor z = at::zeros({cols, D}, w.options());
-        dgate.zero_();
-        std::vector<Tensor> r = {dx, dy, dgate, z[1], z[0]};
+        std::vector<Tensor> r = {dx, dy, at::zeros(gate.sizes(), gate.options()), z[1], z[0]};
         if (post) { r.push_back(z[3]); r.push_back(z[2]); }
         return r;
     }
     const GatedNormPlan q = gated_norm_plan(x.size(0), p.T, p.M, p.per_sample);
     // without a gate per sample a workgroup has one unit: its gate sums are one more column block of the slab
-    const int srow = (int)((cols + (p.per_sample ? 0 : 1)) * D);
-    Tensor slab = at::empty({q.blocks, srow}, w.options()), gate_part;
-    float* gp = slab.data_ptr<float>() + cols * D;
-    long gstride = srow;
-    if (p.per_sample) {
-        TORCH_CHECK(x.size(0) < (1L << 24) / ((D + 63) / 64), "gated_residual_norm: ", x.size(0), " samples");
-        gate_part = q.chunks > 1 ? at::empty({q.units, D}, w.options()) : dgate;
-        gp = gate_part.data_ptr<float>();
-        gstride = D;
-    }
+    const int groups = cols + (p.per_sample ? 0 : 1), srow = (int)(groups * D);
+    const bool parts = p.per_sample && q.chunks > 1;
+    TORCH_CHECK(!p.per_sample || x.size(0) < (1L << 24) / ((D + 63) / 64), "gated_residual_norm: ", x.size(0), " samples");
+    Tensor work = at::empty({(long)q.blocks * srow + (parts ? q.units * D : 0)}, w.options());
+    float* slab = work.data_ptr<float>();
+    Tensor sums = q.blocks == 1 ? work.narrow(0, 0, srow).view({groups, D}) : at::empty({groups, D}, w.options());
+    Tensor dgate = p.per_sample ? at::empty(gate.sizes(), gate.options()) : Tensor();
+    float* gp = !p.per_sample ? slab + cols * D : parts ? slab + (long)q.blocks * srow : dgate.data_ptr<float>();
     launch_gated_norm_bwd(p, q, given(du) ? du->data_ptr() : nullptr, given(dn) ? dn->data_ptr() : nullptr, stats.data_ptr<float>(),
-                          dx.data_ptr(), dy.data_ptr(), gp, gstride, slab.data_ptr<float>(), srow, stream_of(x));
-    if (p.per_sample && q.chunks > 1)
-        launch_gate_sum(gp, dgate.data_ptr<float>(), x.size(0), p.D, q.chunks, stream_of(x));
-    Tensor sums;
-    if (q.blocks == 1) {
-        sums = slab.view({srow});
-    } else {
-        sums = at::empty({srow}, w.options());
-        Tensor tmp = at::empty({kReduceChunks, srow}, w.options());
-        launch_reduce_slab(slab.data_ptr<float>(), q.blocks, srow, srow, sums.data_ptr<float>(), tmp.data_ptr<float>(), stream_of(x));
-    } 
-    std::vector<Tensor> r = {dx, dy, p.per_sample ? dgate : sums.narrow(0, cols * D, D), sums.narrow(0, D, D), sums.narrow(0, 0, D)};
+                          dx.data_ptr(), dy.data_ptr(), gp, p.per_sample ? D : srow, slab, srow, stream_of(x));
+    if (parts) launch_gate_sum(gp, dgate.data_ptr<float>(), x.size(0), p.D, q.chunks, stream_of(x));
+    if (q.blocks > 1) launch_gated_norm_sum(slab, sums.data_ptr<float>(), q.blocks, srow, stream_of(x));
+    const std::vector<Tensor> c = sums.unbind(0);  // db, dw[, dpb, dpw][, dgate]
+    std::vector<Tensor> r = {dx, dy, p.per_sample ? dgate : c[cols], c[1], c[0]};
     if (post) {
-        r.push_back(sums.narrow(0, 3 * D, D));
-        r.push_back(sums.narrow(0, 2 * D, D));
+        r.push_back(c[3]);
+        r.push_back(c[2]);
     }
     return r;
 }

@@ -56,7 +56,7 @@ struct RelPlan {
     int parts, rows;             // ranges of key tiles; slab rows per head
     long dense;                  // floats: sums of dS by pair
 };
-RelPlan rel_plan(int B, int H, int S);
+RelPlan rel_plan(int B, int H, int S, int hd);
 // dense [plan.dense], slab [H][plan.rows][Rp], mid [H][Rp]
 void launch_rel_bias_grad(const ExtArgs& a, const ExtBwd& w, int hd, const RelPlan& p, float* dense, float* slab, float* mid,
                           const int* bucket_of, float* dtable, int NB, hipStream_t s);

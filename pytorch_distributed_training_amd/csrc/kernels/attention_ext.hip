@@ -1078,6 +1078,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
     const long row = ((long)ch * w.heads + hl) * (w.qblocks * 4) + (qb - w.q0) * 4 + wave;
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
+        if (kb * 128 + kt * 32 >= a.Sk || qb * 128 + wave * 32 >= a.Sk) break;  // (tiles that are not read)
         float* dst = dense + (row * nkt + kb * 4 + kt) * 1024 + lane * 4;
         if (one_entry(a, qb * 4 + wave, kb * 4 + kt, 0, (a.R - 1) * 4) >= 0) {  // one number
             float s = 0.f;
@@ -1112,7 +1113,7 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
     const int q = (w.q0 * 4 + qt) * 32 + l31;
     const int qc = base + a.q_codes4[q];
     const int live_t = (a.Sk + 31) / 32, per = (live_t + parts - 1) / parts;
-    const int t1 = (part + 1) * per < live_t ? (part + 1) * per : live_t;
+    const int t1 = w.q0 * 4 + qt >= live_t ? 0 : (part + 1) * per < live_t ? (part + 1) * per : live_t;
     float ends[2] = {0.f, 0.f};
     for (int kt = part * per + wave; kt < t1; kt += 4) {
         const float* src = dense + (((long)hl * nqt + qt) * nkt + kt) * 1024 + lane * 4;
@@ -1351,33 +1352,30 @@ __global__ __launch_bounds__(256) void k_bias_slab(const float* __restrict__ sla
     if (wave == 0 && r < Rp) sums[(long)h * Rp + r] = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
 }
 
-// dtable[n][h] = sum over the entries r of bucket n: the head's entries and their buckets in LDS, a lane per bucket, each of the
-// four waves over a quarter of the entries (any number of entries may share a bucket, in any order)
-__global__ __launch_bounds__(256) void k_bias_buckets(const float* __restrict__ mid, const int* __restrict__ bucket_of,
+// dtable[n][h] = sum over the entries r of bucket n: a lane per bucket, a workgroup takes 64 buckets, its 16 waves every 16th 64
+// entries.  Entries lie a lane each and go round by readlane; 64 whose buckets are all in other workgroups (on a grid nearly
+// all: there an entry is a bucket) are passed over.  Any number of entries may share a bucket, in any order.
+__global__ __launch_bounds__(1024) void k_bias_buckets(const float* __restrict__ sums, const int* __restrict__ bucket_of,
                                                       float* __restrict__ dtable, int R, int Rp, int NB, int H) {
-    __shared__ __attribute__((aligned(16))) float sums[kExtMaxEntries];
-    __shared__ __attribute__((aligned(16))) int of[kExtMaxEntries];
-    __shared__ float red[4][64];
-    const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll 8
-    for (int r = threadIdx.x; r < Rp; r += 256) {
-        sums[r] = mid[(long)h * Rp + r];
-        of[r] = bucket_of[r < R ? r : R - 1];
-    }
-    for (int r = R + (int)threadIdx.x; r < Rp; r += 256) sums[r] = 0.f;
-    __syncthreads();
-    const int n = blockIdx.x * 64 + lane, quads = Rp >> 2, per = (quads + 3) >> 2;
+    __shared__ float red[16][64];
+    const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
     float s = 0.f;
-#pragma unroll 4
-    for (int i = wave * per; i < (wave + 1) * per && i < quads; ++i) {
-        const i32x4 o = *reinterpret_cast<const i32x4*>(of + 4 * i);
-        const f32x4 v = *reinterpret_cast<const f32x4*>(sums + 4 * i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s += o[e] == n ? v[e] : 0.f;
+    for (int r0 = wave * 64; r0 < R; r0 += 1024) {
+        const int r = r0 + lane, of = r < R ? bucket_of[r] - (int)blockIdx.x * 64 : -1;
+        if (!__any(of >= 0 && of < 64)) continue;
+        const float v = r < R ? sums[(long)h * Rp + r] : 0.f;
+#pragma unroll 8
+        for (int e = 0; e < 64; ++e) {
+            const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), e));
+            s += __builtin_amdgcn_readlane(of, e) == lane ? x : 0.f;
+        }
     }
     red[wave][lane] = s;
     __syncthreads();
-    if (wave == 0 && n < NB) dtable[(long)n * H + h] = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
+    if (wave > 0 || n >= NB) return;
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += red[i][lane];
+    dtable[(long)n * H + h] = s;
 }
 
 template <typename K>
@@ -1518,20 +1516,28 @@ void launch_bias_tables(const float* table, const int* bucket_of, const int* q_c
                        tab, codes, R, Rp, NB, H, S, Sp, inv_scale, total);
 }
 // Head groups and query blocks of a dense sum of at most 1 GiB; the batch in parts
-RelPlan rel_plan(int B, int H, int S) {
+RelPlan rel_plan(int B, int H, int S, int hd) {
     RelPlan p;
     const long blocks = (S + 127) / 128, row_block = blocks * 4 * blocks * 4 * 4096;  // bytes of a head
     const long most = 1L << 30;
     p.heads = (int)(row_block >= most ? 1 : most / row_block < H ? most / row_block : H);
     p.qblocks = (int)(row_block <= most ? blocks : most / (row_block / blocks) > 0 ? most / (row_block / blocks) : 1);
     const long groups = (long)p.heads * p.qblocks * blocks;
-    // the fewest parts that keep the two workgroups a CU holds (512) busy for nine tenths of the last round's end
-    long c = 1;
-    while (c < 16 && groups * c * 10 < 9 * 512 * ((groups * c + 511) / 512)) ++c;
-    const long room = most / (p.heads * p.qblocks * (row_block / blocks));
-    c = c < B / 4 ? c : B / 4;
-    c = c < room ? c : room;
-    p.chunks = (int)(c < 1 ? 1 : c);
+    // Parts of the batch: a launch runs in rounds of the 512 workgroups that the CUs hold; a round is 4 us and, per sequence of a
+    // part, 4.2 us at head_dim 64, and each part's sums are written and read once at 5 TB/s.  (128 sequences of 197 on 12 heads: 10
+    // parts in one round, where the 16 that fill the last of two rounds better took 58 us; 32 of 577 on 16 heads: one part, where
+    // five in four rounds took 145 us, 26 of them for the sums.)
+    const long part = p.heads * p.qblocks * (row_block / blocks), room = most / part, live = (S + 31) / 32;
+    const double move = 2.0 * part * live * live / (16.0 * blocks * blocks) / 5e6, step = 4.2 * hd / 64;
+    p.chunks = 1;
+    double best = 0;
+    for (int c = 1; c <= 16 && c <= B && (c == 1 || c <= room); ++c) {
+        const double t = (double)((groups * c + 511) / 512) * (4 + step * ((B + c - 1) / c)) + c * move;
+        if (c == 1 || t < best) {
+            best = t;
+            p.chunks = c;
+        }
+    }
     // ranges of key tiles, so that the histograms' adds are spread over the CUs
     const long rows = (long)H * blocks * 4;
     const long tiles = (S + 31) / 32;
@@ -1539,7 +1545,7 @@ RelPlan rel_plan(int B, int H, int S) {
     q = q < (tiles + 3) / 4 ? q : (tiles + 3) / 4;
     p.parts = (int)(q < 1 ? 1 : q);
     p.rows = (int)(blocks * 4 * p.parts);
-    p.dense = (long)p.chunks * p.heads * p.qblocks * (row_block / blocks) / 4;
+    p.dense = p.chunks * part / 4;
     return p;
 }
 template <int HD>
@@ -1571,7 +1577,7 @@ void launch_rel_bias_grad(const ExtArgs& a, const ExtBwd& x, int hd, const RelPl
                                (const float*)dense, slab, w, p.parts);
         }
     hipLaunchKernelGGL(k_bias_slab, dim3((a.Rp + 63) / 64, a.Hkv), dim3(256), 0, s, (const float*)slab, mid, a.Rp, p.rows);
-    hipLaunchKernelGGL(k_bias_buckets, dim3((NB + 63) / 64, a.Hkv), dim3(256), 0, s, (const float*)mid, bucket_of, dtable, a.R, a.Rp, NB,
+    hipLaunchKernelGGL(k_bias_buckets, dim3((NB + 63) / 64, a.Hkv), dim3(1024), 0, s, (const float*)mid, bucket_of, dtable, a.R, a.Rp, NB,
                        a.Hkv);
 }
 

@@ -23,6 +23,7 @@ void launch_gated_norm_fwd(const GatedNorm& p, void* u, void* n, float* stats, h
 GatedNormPlan gated_norm_plan(long B, long T, long M, bool per_sample);
 void launch_gated_norm_bwd(const GatedNorm& p, const GatedNormPlan& q, const void* du, const void* dn, const float* stats, void* dx,
                            void* dy, float* gate_part, long gate_stride, float* slab, int srow, hipStream_t s);
+void launch_gated_norm_sum(const float* slab, float* sums, int rows, int n, hipStream_t s);
 void launch_gate_sum(const float* part, float* dgate, long B, int D, int chunks, hipStream_t s);
 
 }  // namespace pdt

@@ -316,6 +316,30 @@ __global__ __launch_bounds__(256, NP <= (POST ? 3 : 4) ? 2 : 1) void k_gn_bwd(
     }
 }
 
+// sums[c] = sum of the slab's rows [rows][n]: a workgroup takes 32 columns (8 lanes of four), each of 32 groups of lanes every
+// 32nd row, the groups are added in order
+__global__ __launch_bounds__(256) void k_gn_sum(const float* __restrict__ slab, float* __restrict__ sums, int rows, int n) {
+    __shared__ __attribute__((aligned(16))) float red[32][32];
+    const int g = threadIdx.x >> 3, q = (threadIdx.x & 7) * 4, c = blockIdx.x * 32 + q;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (c < n) {
+#pragma unroll 8
+        for (int r = g; r < rows; r += 32) {
+            const f32x4 t = *reinterpret_cast<const f32x4*>(slab + (long)r * n + c);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] += t[k];
+        }
+    }
+    *reinterpret_cast<f32x4*>(&red[g][q]) = s;
+    __syncthreads();
+    if (threadIdx.x < 32 && blockIdx.x * 32 + threadIdx.x < (unsigned)n) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) t += red[k][threadIdx.x];
+        sums[blockIdx.x * 32 + threadIdx.x] = t;
+    }
+}
+
 // dgate[b][c] = sum of the sample's units: a wave of 64 columns takes every fourth, the four waves are added in order
 __global__ __launch_bounds__(256) void k_gate_sum(const float* __restrict__ part, float* __restrict__ dgate, int D, int chunks) {
     __shared__ float red[4][64];
@@ -377,6 +401,9 @@ void launch_gated_norm_bwd(const GatedNorm& p, const GatedNormPlan& q, const voi
             hipLaunchKernelGGL((k_gn_bwd<NP, false>), dim3(q.blocks), dim3(256), lds, s, p, (const bf16*)du, (const bf16*)dn, stats,
                                (bf16*)dx, (bf16*)dy, gate_part, gate_stride, slab, srow, q.chunks, q.units);
     });
+}
+void launch_gated_norm_sum(const float* slab, float* sums, int rows, int n, hipStream_t s) {
+    hipLaunchKernelGGL(k_gn_sum, dim3((unsigned)((n + 31) / 32)), dim3(256), 0, s, slab, sums, rows, n);
 }
 void launch_gate_sum(const float* part, float* dgate, long B, int D, int chunks, hipStream_t s) {
     hipLaunchKernelGGL(k_gate_sum, dim3((unsigned)(B * ((D + 63) / 64))), dim3(256), 0, s, part, dgate, D, chunks);
