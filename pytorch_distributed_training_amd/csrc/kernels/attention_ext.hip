@@ -376,11 +376,6 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
     const bf16* vbase = a.v + (long)j.b * a.kv.bs + (long)j.hkv * HD;
     const int krs = (int)a.kv.rs;
 
-    bf16x8 bq[G::STEPS];
-    own_frags<HD>(bq, a.q + (long)j.b * a.qv.bs + row_offset(a.qv, live ? l31 : 0, j.hkv, a.G, HD), live, half);
-#pragma unroll
-    for (int s = 0; s < G::STEPS; ++s) asm volatile("" : "+v"(bq[s])::"memory");  // the rows are here: only DMA is counted below
-
     auto issue = [&](int t, int buf) {
         const int valid = j.len - t * 32 < 32 ? j.len - t * 32 : 32;
         const long at = (long)t * 32 * krs;
@@ -394,7 +389,11 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
     float m = -kInf, l = 0.f;
     int buf = 0;
-    if (t0 + wave < t1) issue(t0 + wave, 0);
+    if (t0 + wave < t1) issue(t0 + wave, 0);  // (before the rows: 8.5 us for 9.5 on 8 x 12 heads of up to 1500 keys)
+    bf16x8 bq[G::STEPS];
+    own_frags<HD>(bq, a.q + (long)j.b * a.qv.bs + row_offset(a.qv, live ? l31 : 0, j.hkv, a.G, HD), live, half);
+#pragma unroll
+    for (int s = 0; s < G::STEPS; ++s) asm volatile("" : "+v"(bq[s])::"memory");  // the rows are here: only DMA is counted below
     for (int t = t0 + wave; t < t1; t += 4, buf ^= 1) {
         // the reads of the other stage (last tile) are done before it is written again
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
