@@ -154,17 +154,28 @@ __device__ __forceinline__ long row_offset(const ExtView& v, int r, int hkv, int
 struct Job {
     int b, hkv, bh, tile, split, len, rows;  // len: valid keys; rows: live rows (self attention: those before len)
 };
+template <bool FEW = false>
 __device__ __forceinline__ Job job_of(const ExtArgs& a, int tiles, int splits) {
     Job j;
-    int l = xcd_order((int)blockIdx.x, (int)gridDim.x);
-    j.split = l % splits;
-    l /= splits;
-    j.tile = l % tiles;
-    l /= tiles;
-    // heads outside, the batch inside: an XCD gets sequences of all lengths (with the batch outside the XCDs of the long ones
-    // worked twice as long as the rest on a padded batch), and its head's bias table stays in its cache
-    j.hkv = l / a.B;
-    j.b = l - j.hkv * a.B;
+    int l = FEW ? (int)blockIdx.x : xcd_order((int)blockIdx.x, (int)gridDim.x);
+    if (FEW) {
+        // a stream that no other workgroup reads: a token's heads at the same time, tokens in the order of memory (512 sequences of
+        // 197 keys on 12 heads: 73 us where the order below took 82)
+        j.tile = 0;
+        const int parts = l / a.Hkv;
+        j.hkv = l - parts * a.Hkv;
+        j.b = parts / splits;
+        j.split = parts - j.b * splits;
+    } else {
+        j.split = l % splits;
+        l /= splits;
+        j.tile = l % tiles;
+        l /= tiles;
+        // heads outside, the batch inside: an XCD gets sequences of all lengths (with the batch outside the XCDs of the long ones
+        // worked twice as long as the rest on a padded batch), and its head's bias table stays in its cache
+        j.hkv = l / a.B;
+        j.b = l - j.hkv * a.B;
+    }
     j.bh = j.b * a.Hkv + j.hkv;
     int len = a.Sk;
     if (a.lens) {
@@ -366,7 +377,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
     extern __shared__ __attribute__((aligned(16))) char smem[];  // [4 waves][2 stages][K tile, V tile], then [4][32][2] floats
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Job j = job_of(a, 1, splits);
+    const Job j = job_of<true>(a, 1, splits);
     char* ring = smem + wave * 2 * STAGE;
     const uint32_t ring_lds = lds_address(ring);
     const bool live = l31 < a.M;
@@ -784,7 +795,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_few(ExtArgs a,
     extern __shared__ __attribute__((aligned(16))) char smem[];  // [4 waves][2 stages][K, V], Q image, dO image, [3][32] floats
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Job j = job_of(a, 1, splits);
+    const Job j = job_of<true>(a, 1, splits);
     char* ring = smem + wave * 2 * STAGE;
     const uint32_t ring_lds = lds_address(ring);
     char* Qs = smem + 8 * STAGE;
