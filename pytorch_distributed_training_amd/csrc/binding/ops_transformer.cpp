@@ -224,8 +224,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rel_bias_attention_fwd(const Tensor& 
                                                                   const OptTensor& lens, bool grad) {
     const long hd = packed_head_dim(qkv, heads), D = heads * hd, S = qkv.size(1), R = bucket_of.size(0), NB = table.size(0);
     TORCH_CHECK(R >= 1 && R <= kExtMaxEntries, "rel_bias_attention: ", R, " entries (1 to ", kExtMaxEntries, ")");
-    TORCH_CHECK(NB < (1L << 24) && S < (1L << 30) && heads < 65536, "rel_bias_attention: ", NB, " buckets, ", S, " positions, ", heads,
-                " heads (below 2^24, 2^30 and 2^16)");
+    TORCH_CHECK(NB < (1L << 24) && S < (1L << 29) && heads < 65536, "rel_bias_attention: ", NB, " buckets, ", S, " positions, ", heads,
+                " heads (below 2^24, 2^29 and 2^16)");
     check_dense(table, {NB, heads}, at::kFloat, qkv, "table");
     check_dense(q_codes, {S}, at::kInt, qkv, "q_codes");
     check_dense(k_codes, {S}, at::kInt, qkv, "k_codes");

@@ -1314,38 +1314,29 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
 __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ table, const int* __restrict__ bucket_of,
                                                      const int* __restrict__ q_codes, const int* __restrict__ k_codes,
                                                      float* __restrict__ tab, int* __restrict__ codes /* q4 [Sp], k4 [Sp], ranges of 32 */, int R,
-                                                     int Rp, int NB, int H, int S, int Sp, float inv_scale, long total) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    if (i < (long)H * Rp) {
-        const int h = (int)(i / Rp), r = (int)(i % Rp);
-        const int n = r < R ? bucket_of[r] : -1;
+                                                     int Rp, int NB, int H, int S, int Sp, float inv_scale, int tab_blocks) {
+    if ((int)blockIdx.x < tab_blocks) {
+        const uint32_t i = blockIdx.x * 256 + threadIdx.x, h = i / (uint32_t)Rp, r = i - h * (uint32_t)Rp;
+        if (h >= (uint32_t)H) return;
+        const int n = r < (uint32_t)R ? bucket_of[r] : -1;
         float v = n >= 0 && n < NB ? table[(long)n * H + h] : 0.f;
         if (v < -kBiasFloor && v > -kInf) v = -kBiasFloor;
         if (v > kBiasFloor && v < kInf) v = kBiasFloor;
         tab[i] = v * inv_scale;
         return;
     }
-    const long w = i - (long)H * Rp;
-    auto code4 = [&](long x) {  // x < 2 Sp
-        const int at = (int)(x % Sp);
-        int c = (x < Sp ? q_codes : k_codes)[at < S ? at : S - 1];
-        c = c < -(1 << 27) ? -(1 << 27) : c > (1 << 27) - 1 ? (1 << 27) - 1 : c;  // byte offsets' differences and an LDS address fit 32 bits
-        return c * 4;
-    };
-    if (w < 2L * Sp) {
-        codes[w] = code4(w);
-        return;
+    const int w = ((int)blockIdx.x - tab_blocks) * 256 + (int)threadIdx.x, at = w < Sp ? w : w - Sp;  // (2 Sp: a multiple of 256)
+    int c = (w < Sp ? q_codes : k_codes)[at < S ? at : S - 1];
+    c = (c < -(1 << 27) ? -(1 << 27) : c > (1 << 27) - 1 ? (1 << 27) - 1 : c) * 4;  // offsets' differences and an LDS address fit 32 bits
+    codes[w] = c;
+    int lo = c, hi = c;
+#pragma unroll
+    for (int e = 1; e < 32; e *= 2) {
+        const int l = __shfl_xor(lo, e, 64), u = __shfl_xor(hi, e, 64);
+        lo = l < lo ? l : lo;
+        hi = u > hi ? u : hi;
     }
-    int lo = 0x7fffffff, hi = -0x7fffffff - 1;
-    const long r = w - 2L * Sp;
-    for (int e = 0; e < 32; ++e) {
-        const int c = code4(r * 32 + e);
-        lo = c < lo ? c : lo;
-        hi = c > hi ? c : hi;
-    }
-    codes[2L * Sp + 2 * r] = lo;
-    codes[2L * Sp + 2 * r + 1] = hi;
+    if ((threadIdx.x & 31) == 0) reinterpret_cast<int2*>(codes + 2L * Sp)[w >> 5] = {lo, hi};
 }
 
 // sums[h][r] = sum of the slab rows [H][rows][Rp] of head h: 64 entries a workgroup, each of its four waves every fourth row
@@ -1521,9 +1512,9 @@ void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s) {
     else bwd<128>(a, w, s);
 }
 void launch_bias_tables(const float* table, const int* bucket_of, const int* q_codes, const int* k_codes, float* tab, int* codes, int R, int Rp, int NB, int H, int S, int Sp, float inv_scale, hipStream_t s) {
-    const long total = (long)H * Rp + 2L * Sp + 2L * Sp / 32;
-    hipLaunchKernelGGL(k_bias_tables, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, table, bucket_of, q_codes, k_codes,
-                       tab, codes, R, Rp, NB, H, S, Sp, inv_scale, total);
+    const int tab_blocks = (int)(((long)H * Rp + 255) / 256);
+    hipLaunchKernelGGL(k_bias_tables, dim3((unsigned)(tab_blocks + 2L * Sp / 256)), dim3(256), 0, s, table, bucket_of, q_codes, k_codes,
+                       tab, codes, R, Rp, NB, H, S, Sp, inv_scale, tab_blocks);
 }
 // Head groups and query blocks of a dense sum of at most 1 GiB; the batch in parts
 RelPlan rel_plan(int B, int H, int S, int hd) {
