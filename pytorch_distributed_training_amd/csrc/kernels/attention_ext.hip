@@ -510,26 +510,29 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
         for (int r = a.M + tid; r < a.Mp; r += 256) put_stat(a, stat, (long)j.bh * a.Mp + r, false, 0.f, 0.f, 0.f);
 }
 
-// (m, l, O) of the splits -> out (and stat).  A workgroup takes a row: HD / 4 threads its channels, 1024 / HD groups of them
-// every so many-th split, added in order; the loads of a group's splits are independent (one thread over 16 splits took 11 us
-// where this takes 5)
-template <int HD>
+// (m, l, O) of the splits -> out (and stat).  HD / 4 lanes take a row's channels.  MANY: a workgroup has one row, and 1024 / HD
+// groups of lanes every so many-th split, added in order; the loads of a group's splits are independent (one thread over 16
+// splits took 11 us where this takes 5).  Else every group has a row of its own (6924 rows of two splits: 4 us for 9).
+template <int HD, bool MANY>
 __global__ __launch_bounds__(256) void k_ext_join(ExtArgs a, const float* __restrict__ part, const float* __restrict__ part_ml,
-                                                  bf16* __restrict__ out, float* __restrict__ stat, int splits) {
+                                                  bf16* __restrict__ out, float* __restrict__ stat, int splits, int rows_of_all) {
     constexpr int W = HD / 4, NG = 256 / W;
-    __shared__ __attribute__((aligned(16))) float red[NG][HD + 4];
-    const int bh = (int)blockIdx.x / a.M, r = (int)blockIdx.x - bh * a.M;
+    __shared__ __attribute__((aligned(16))) float red[MANY ? NG : 1][HD + 4];
     const int d = (int)(threadIdx.x % W) * 4, g = (int)threadIdx.x / W;
+    const int row = MANY ? (int)blockIdx.x : (int)blockIdx.x * NG + g;
+    if (!MANY && row >= rows_of_all) return;
+    const int bh = row / a.M, r = row - bh * a.M;
     const int b = bh / a.Hkv, hkv = bh - b * a.Hkv;
     const long at0 = (long)bh * splits * a.M + r;
     if (stat && r == a.M - 1)  // padding rows of the statistics
-        for (int i = a.M + (int)threadIdx.x; i < a.Mp; i += 256) put_stat(a, stat, (long)bh * a.Mp + i, false, 0.f, 0.f, 0.f);
+        for (int i = a.M + (MANY ? (int)threadIdx.x : d >> 2); i < a.Mp; i += MANY ? 256 : W)
+            put_stat(a, stat, (long)bh * a.Mp + i, false, 0.f, 0.f, 0.f);
     float mx = -kInf, sum = 0.f;
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) mx = fmaxf(mx, part_ml[2 * (at0 + (long)s * a.M)]);
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int s = g; s < splits; s += NG) {
+    for (int s = MANY ? g : 0; s < splits; s += MANY ? NG : 1) {
         const long at = at0 + (long)s * a.M;
         const float ms = part_ml[2 * at], f = ms == -kInf ? 0.f : __builtin_amdgcn_exp2f((ms - mx) * a.c);
         sum += part_ml[2 * at + 1] * f;
@@ -537,21 +540,23 @@ __global__ __launch_bounds__(256) void k_ext_join(ExtArgs a, const float* __rest
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] += u[e] * f;
     }
-    *reinterpret_cast<f32x4*>(&red[g][d]) = t;
-    if (d == 0) red[g][HD] = sum;
-    __syncthreads();
-    if (g > 0) return;
+    if (MANY) {
+        *reinterpret_cast<f32x4*>(&red[g][d]) = t;
+        if (d == 0) red[g][HD] = sum;
+        __syncthreads();
+        if (g > 0) return;
 #pragma unroll
-    for (int i = 1; i < NG; ++i) {
-        const f32x4 u = *reinterpret_cast<const f32x4*>(&red[i][d]);
-        if (i < splits) {
+        for (int i = 1; i < NG; ++i) {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(&red[i][d]);
+            if (i < splits) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] += u[e];
+                for (int e = 0; e < 4; ++e) t[e] += u[e];
+            }
         }
-    }
-    sum = 0.f;
+        sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) sum += red[i][HD];
+        for (int i = 0; i < NG; ++i) sum += red[i][HD];
+    }
     int rows = a.M;
     if (a.self && a.lens) {
         const int len = a.lens[b] < 0 ? 0 : a.lens[b];
@@ -1119,7 +1124,7 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
     const int qt = rest % nqt, hl = rest / nqt;
     float* hist = reinterpret_cast<float*>(smem) + (long)wave * a.Rp;
     const int base = (int)lds_address(hist), top = base + (a.R - 1) * 4;
-    for (int i = lane; i < a.Rp; i += 64) hist[i] = 0.f;
+    for (int i = lane * 4; i < a.Rp; i += 256) *reinterpret_cast<f32x4*>(hist + i) = f32x4{0.f, 0.f, 0.f, 0.f};  // (Rp: a multiple of 4)
     const int q = (w.q0 * 4 + qt) * 32 + l31;
     const int qc = base + a.q_codes4[q];
     const int live_t = (a.Sk + 31) / 32, per = (live_t + parts - 1) / parts;
@@ -1166,7 +1171,16 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
     __syncthreads();
     float* dst = slab + ((long)(hl + w.h0) * w.slab_rows + (long)(w.q0 * 4 + qt) * parts + part) * a.Rp;
     const float* all = reinterpret_cast<const float*>(smem);
-    for (int i = tid; i < a.Rp; i += 256) dst[i] = all[i] + all[a.Rp + i] + all[2 * a.Rp + i] + all[3 * a.Rp + i];
+    for (int i = tid * 4; i < a.Rp; i += 1024) {
+        f32x4 s = *reinterpret_cast<const f32x4*>(all + i);
+#pragma unroll
+        for (int w4 = 1; w4 < 4; ++w4) {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(all + w4 * a.Rp + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += u[e];
+        }
+        *reinterpret_cast<f32x4*>(dst + i) = s;
+    }
 }
 
 // Key owner: dK and dV of 128 keys a workgroup; the rows of all G heads stream through.
@@ -1408,8 +1422,13 @@ void fwd(const ExtArgs& a, const ExtPlan& p, void* out, float* stat, float* part
 #undef PDT_EXT_FWD
     }
     if (p.splits > 1) {
-        hipLaunchKernelGGL((k_ext_join<HD>), dim3((unsigned)((long)a.B * a.Hkv * a.M)), dim3(256), 0, s, a, (const float*)part,
-                           (const float*)part_ml, (bf16*)out, stat, p.splits);
+        const int rows = (int)((long)a.B * a.Hkv * a.M), ng = 1024 / HD;  // (a launch that is split has at most 256 tiles of 128 rows)
+        if (p.splits > 4)
+            hipLaunchKernelGGL((k_ext_join<HD, true>), dim3((unsigned)rows), dim3(256), 0, s, a, (const float*)part, (const float*)part_ml,
+                               (bf16*)out, stat, p.splits, rows);
+        else
+            hipLaunchKernelGGL((k_ext_join<HD, false>), dim3((unsigned)((rows + ng - 1) / ng)), dim3(256), 0, s, a, (const float*)part,
+                               (const float*)part_ml, (bf16*)out, stat, p.splits, rows);
     }
 }
 
@@ -1539,10 +1558,10 @@ RelPlan rel_plan(int B, int H, int S, int hd) {
             p.chunks = c;
         }
     }
-    // ranges of key tiles, so that the histograms' adds are spread over the CUs
+    // ranges of key tiles: as many workgroups as the CUs hold at once (four each where a head has 2000 entries)
     const long rows = (long)H * blocks * 4;
     const long tiles = (S + 31) / 32;
-    long q = (1024 + rows - 1) / rows;
+    long q = 1024 / rows;
     q = q < (tiles + 3) / 4 ? q : (tiles + 3) / 4;
     p.parts = (int)(q < 1 ? 1 : q);
     p.rows = (int)(blocks * 4 * p.parts);
