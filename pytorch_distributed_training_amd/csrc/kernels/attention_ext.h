@@ -6,7 +6,9 @@
 
 namespace pdt {
 
-constexpr int kExtMaxEntries = 4096;  // entries of a relative-position table a head keeps in LDS
+// entries of a relative-position table that a head keeps in LDS: 16 KiB beside 64 of keys at head_dim 128, so that a CU still holds
+// two workgroups; four histograms of the gradient are 64 KiB
+constexpr int kExtMaxEntries = 4096;
 
 // rows of a [B, rows, heads, hd] tensor: element strides, and the division of a row by the heads that share a key head
 struct ExtView {

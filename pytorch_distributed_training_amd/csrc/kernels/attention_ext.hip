@@ -206,7 +206,11 @@ __device__ __forceinline__ void own_frags(bf16x8* f, const bf16* p, bool live, i
 }
 
 // ------------------------------------------------------------------------------------------------------- forward
-// One sweep with a running maximum.  4 waves own 32 rows each; keys in blocks of 64.
+// One sweep with a running maximum. 4 waves own 32 rows each; keys in blocks of 64 (a block of 32 doubles the barriers, one of 128 halves
+// the workgroups that a CU holds). Bound by vector instructions: 117 for a tile's 8 matrix instructions at head_dim 64 (two of
+// a score's seven instructions are the bias's address), two thirds of the issue slots. 128 sequences of 197 on 12 heads of 64 with a bias:
+// 57 us; 32 of 577 on 16: 108; four of up to 2047 on 8 of 128: 88; 333 rows x 1025 keys, 16 heads on 4 key heads of 64, batch
+// 16: 37.
 template <int HD, bool BIAS>
 __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict__ out, float* __restrict__ stat, float* __restrict__ part, float* __restrict__ part_ml,
                                                  int tiles, int splits) {
@@ -368,7 +372,9 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
 
 // Few rows (at most one tile of 32 for a key head: single tokens).  The four waves of a workgroup share the rows and take
 // every fourth tile of 32 keys each, through an LDS ring of their own (no barrier until the join): the kernel is a stream over
-// K and V, 16 to 64 KiB of it in flight per workgroup.
+// K and V, 16 to 64 KiB of it in flight per workgroup, and bound by memory: 4 sequences of 65536 keys, 8 key heads of 128, four rows
+// each: 185 us, 5.8 TB/s (with the kernel above, whose waves would have one tile of rows for four: 193); 512 of 197 on 12 heads
+// of 64: 73 us, 4.2 TB/s (80 there, and the backward 275 for the 145 of its counterpart).
 template <int HD>
 __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restrict__ out, float* __restrict__ stat,
                                                      float* __restrict__ part, float* __restrict__ part_ml, int splits) {
@@ -650,12 +656,13 @@ __device__ __forceinline__ void store_tile(const f32x16* t, char* img, bf16* dst
     }
 }
 
-// Row owner: dQ, and D for what follows.  dO . O carries the rounding of P and O to bf16, and the sum of a row's
-// P (dP - dO . O) is exactly what it is off by (as a row's P add up to 1): added, D is good to 32 bits, which the fp32 gradient of
-// the bias table needs; that sum costs an add a score, keeping O's remainder in the forward cost it a quarter of its time.
-// Where all keys are in one block dS is corrected too: with few keys P (dP - D) is a small difference.  Without a bias and with
-// more keys O is small against V, its rounding against dP, and nothing is added.  A softmax over one key is constant, so with
-// len = 1 dS is zero, and is set so (as a difference of two rounded numbers it would not be).
+// Row owner: dQ, and D for what follows. Bound as the forward is, with half the vector instructions' slots and half of LDS in
+// use and three waves a SIMD: 75 us, 123, 104 and 40 at the sizes given there. dO . O carries the rounding of P and O to bf16,
+// and the sum of a row's P (dP - dO . O) is exactly what it is off by (as a row's P add up to 1): added, D is good to 32 bits,
+// which the fp32 gradient of the bias table needs; that sum costs an add a score, keeping O's remainder in the forward cost it
+// a quarter of its time. Where all keys are in one block dS is corrected too: with few keys P (dP - D) is a small difference.
+// Without a bias and with more keys O is small against V, its rounding against dP, and nothing is added. A softmax over one key
+// is constant, so with len = 1 dS is zero, and is set so (as a difference of two rounded numbers it would not be).
 template <int HD, bool BIAS, bool ONE /* all keys in one block of 64 */>
 __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                    float* __restrict__ dsum, bf16* __restrict__ dq, float* __restrict__ part, int tiles,
@@ -790,7 +797,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
 // Few rows (at most 32 for a key head: an attention pooling head's query): everything in one pass over K and V.  A wave takes
 // every fourth tile of 32 keys through a ring of its own, makes the tile's scores in both orientations (two small products; the
 // pass is bound by the stream of K, V, dK and dV), stores dK and dV of its keys and keeps its part of dQ, which the four
-// waves join at the end.
+// waves join at the end.  512 sequences of 197 keys, 12 heads of 64: 145 us, 4.3 TB/s; row owner and key owner took 275.
 template <int HD>
 __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_few(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                         bf16* __restrict__ dq, bf16* __restrict__ dk, bf16* __restrict__ dv,
@@ -997,7 +1004,10 @@ __global__ __launch_bounds__(256) void k_ext_dsum(float* __restrict__ dsum, long
 
 // dS summed over a part of the batch, for 128 queries x 128 keys of a head a workgroup (a wave: 32 queries, four tiles of 32
 // keys).  The bias of the block and the sums stay in registers while the batch streams through, so a pair costs two
-// multiply-adds and an exponential per sequence; written in register order, [tile][4][64 lanes] x 4 floats.
+// multiply-adds and an exponential per sequence; written in register order, [tile][4][64 lanes] x 4 floats.  Its bound is what the
+// blocks move from L2, 64 KiB for 128 x 128 pairs of head_dim 64, at 6 to 7 TB/s: 58 us, 137 and 118 at the sizes given at the
+// forward.  Blocks of 256 x 256 with the bias gathered for every sequence (no registers left for it) took 85 and 248, a second buffer
+// for K and V 64 and 149.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                       const float* __restrict__ dsum, float* __restrict__ dense, RelBlocks w) {
@@ -1113,8 +1123,9 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
     }
 }
 
-// The pairs' sums by entry: a workgroup takes a tile row (32 queries) of a head and one of `parts` ranges of its key tiles; its
-// waves take every fourth tile, each with a histogram of its own.
+// The pairs' sums by entry (10, 20 and 20 us there, most of it the LDS adds and the histograms' clearing): a workgroup takes a
+// tile row (32 queries) of a head and one of `parts` ranges of its key tiles; its waves take every fourth tile, each with a
+// histogram of its own.
 __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __restrict__ dense, float* __restrict__ slab, RelBlocks w,
                                                      int parts) {
     extern __shared__ __attribute__((aligned(16))) char smem[];  // [4][Rp] floats
@@ -1183,7 +1194,10 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
     }
 }
 
-// Key owner: dK and dV of 128 keys a workgroup; the rows of all G heads stream through.
+// Key owner: dK and dV of 128 keys a workgroup; the rows of all G heads stream through. Four products
+// a tile for the row owner's three, and a row's numbers (-m, -log2 l, -D, code) come from LDS for every register: 87 us, 153, 170 and 54 at the
+// sizes given at the forward, LDS and vector instructions half busy each. -D and the exponent by a matrix instruction with ones
+// instead: 99 and 67; the exponent as one number with a branch for large maxima: 101.
 template <int HD, bool BIAS>
 __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                     const float* __restrict__ dsum, bf16* __restrict__ dk, bf16* __restrict__ dv,
@@ -1488,7 +1502,10 @@ void bwd(const ExtArgs& a, const ExtBwd& w, hipStream_t s) {
 }
 
 // parts to cut `blocks` blocks of the streamed axis into, so that `groups` workgroups become about two per CU (512); a part
-// keeps at least `least` blocks
+// keeps at least `least` blocks. Cut and joined against whole: one sequence of 577 on 12 heads, training, 97 us for 112; 64
+// rows x 2000 keys on 8 heads, forward and dQ, 27 us for 72; single rows over 1500 and over 65536 keys, 11 and 190 us for 12
+// and 705. 256 or 1024 workgroups instead of 512 changed none of these by 5 %. With 300 workgroups cutting lost: five sequences
+// of 577, training, 144 us whole and 149 cut; single rows over 1500 keys on 24 x 12 heads 23 and 25.
 int splits_for(long groups, long blocks, long least) {
     if (groups >= 256 || blocks < 2 * least) return 1;
     long s = (512 + groups - 1) / groups;
@@ -1498,6 +1515,8 @@ int splits_for(long groups, long blocks, long least) {
 
 }  // namespace
 
+// Up to 32 rows, one tile of a wave, the waves share them: 32 rows x 1000 keys on 40 x 12 heads of 64, training, 71 us for 116; 8 rows
+// 67 for 113.  (With a bias they would want its table beside the rings.)
 ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool bias) {
     ExtPlan p;
     p.few = !bias && M <= 32;
@@ -1506,7 +1525,7 @@ ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool bias) {
     return p;
 }
 void ext_plan_bwd(long BH, int M, int Sk, bool bias, ExtPlan& q, ExtPlan& kv) {
-    q.few = kv.few = !bias && M <= 32 && Sk > 64;  // (few keys want D exact: the row owner)
+    q.few = kv.few = !bias && M <= 32 && Sk > 64;  // (few keys want D exact, which is the row owner's)
     if (q.few) {  // one kernel
         q.tiles = 1;
         q.splits = splits_for(BH, (Sk + 31) / 32, 8);
