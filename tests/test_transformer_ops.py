@@ -765,3 +765,107 @@ def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, want)
+
+
+ANY_CODES = [dict(n=150, entries=1, buckets=1, hd=64), dict(n=70, entries=2, buckets=3, hd=32), dict(n=150, entries=7, buckets=130, hd=64),
+             dict(n=300, entries=4096, buckets=500, hd=128), dict(n=33, entries=4095, buckets=1, hd=64), dict(n=40, entries=5, buckets=0, hd=32)]
+
+
+@gpu
+@pytest.mark.parametrize("case", ANY_CODES, ids=lambda c: f"n{c['n']}-r{c['entries']}-b{c['buckets']}x{c['hd']}")
+def test_rel_bias_any_codes(case):
+    """Codes and buckets in no order, on both sides of the table's reach, buckets that no entry names and entries without one."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(11)
+    n, r, nb = case["n"], case["entries"], case["buckets"]
+    qc, kc = (torch.randint(-r, 2 * r + 1, (n,), generator=g) for _ in range(2))
+    of = torch.randint(-1, nb + 2, (r,), generator=g)
+    table = torch.randn(nb, 3, generator=g)
+    if nb == 0:
+        qkv = _rand(g, 2, n, 9 * case["hd"], device=dev)
+        t = table.to(dev).requires_grad_()
+        out = F.rel_bias_attention(qkv, t, qc.to(dev), kc.to(dev), of.to(dev), 3)
+        (dt,) = torch.autograd.grad(out, t, torch.ones_like(out))
+        assert dt.shape == (0, 3)
+        return
+    _check_rel(dev, 3, (qc, kc, of), 3, case["hd"], lengths=[n, n // 2, 1], table=table, poison=True)
+
+
+@gpu
+def test_gradients_of_one_input_alone():
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(12)
+    qc, kc, of = (t.to(dev) for t in _grid(6))
+    qkv = _rand(g, 3, 37, 384, device=dev)
+    table = _rand(g, 2, int(of.max()) + 1, dtype=torch.float32, device=dev).t()  # (columns that are not neighbours)
+    w = _rand(g, 3, 37, 128, device=dev)
+    a, t = qkv.clone().requires_grad_(), table.clone().requires_grad_()
+    both = torch.autograd.grad(F.rel_bias_attention(a, t, qc, kc, of, 2), [a, t], w)
+    alone = (torch.autograd.grad(F.rel_bias_attention(a, table, qc, kc, of, 2), a, w)[0],
+             torch.autograd.grad(F.rel_bias_attention(qkv, t, qc, kc, of, 2), t, w)[0])
+    assert all(torch.equal(x, y) for x, y in zip(both, alone))
+    q, kv = _rand(g, 3, 5, 128, device=dev), _rand(g, 3, 300, 256, device=dev)
+    w = w[:, :5].contiguous()
+    ql, kl = q.clone().requires_grad_(), kv.clone().requires_grad_()
+    both = torch.autograd.grad(F.cross_attention(ql, kl, 2), [ql, kl], w)
+    alone = (torch.autograd.grad(F.cross_attention(ql, kv, 2), ql, w)[0], torch.autograd.grad(F.cross_attention(q, kl, 2), kl, w)[0])
+    assert all(torch.equal(x, y) for x, y in zip(both, alone))
+    # no tokens at all
+    e = torch.zeros(2, 0, 384, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    o = F.rel_bias_attention(e, t, qc[:0], kc[:0], of, 2)
+    ge, gt = torch.autograd.grad(o, [e, t], torch.zeros_like(o))
+    assert ge.shape == e.shape and not gt.any()
+
+
+@gpu
+def test_captured_answers():
+    """Kernels with more than 64 KiB of LDS, split and joined, in a graph without gradients, replayed on new inputs."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(13)
+    q, kv = _rand(g, 2, 1, 1024, device=dev), _rand(g, 2, 2000, 512, device=dev)
+    lens = torch.tensor([2000, 3], dtype=torch.int32, device=dev)
+    qc, kc, of = (t.to(dev) for t in _log(300, 64, 32))
+    qkv, table = _rand(g, 1, 300, 768, device=dev), _rand(g, 32, 2, dtype=torch.float32, device=dev)
+
+    @torch.no_grad()
+    def answer():
+        return F.cross_attention(q, kv, 8, 2, lens), F.rel_bias_attention(qkv, table, qc, kc, of, 2)
+
+    answer()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = answer()
+    for n in (3, 2000, 0, 777):
+        lens[1] = n
+        for t in (q, kv, qkv, table):
+            t.copy_(torch.randn(t.shape, generator=g).to(t.dtype))
+        want = answer()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+@gpu
+def test_captured_training_step_of_a_vit_with_options():
+    from pytorch_distributed_training_amd import dist as pdist
+    from pytorch_distributed_training_amd.engine import Engine, EngineConfig
+
+    import os
+
+    _dev("cuda")
+    os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
+    os.environ.setdefault("MASTER_PORT", "29541")
+    pdist.init_process_group(backend="rccl", local_rank=0)
+    g = torch.Generator().manual_seed(0)
+    xs = [torch.rand(8, 3, 32, 32, generator=g).cuda() for _ in range(6)]
+    ys = [torch.randint(0, 10, (8,), generator=g).cuda() for _ in range(6)]
+    runs = []
+    for graph in (False, True):
+        eng = Engine(EngineConfig(model="vit_tiny_test", num_classes=10, optimizer="adamw", lr=1e-3, sync_bn=False, seed=0, graph=graph,
+                                  model_options=OPTIONS))
+        eng.optimizer.set_capturable(True)
+        losses = [float(eng.train_step(x, y)) for x, y in zip(xs, ys)]
+        assert not graph or eng._graph is not None, eng._graph_failed
+        runs.append((losses, [p.detach().clone() for p in eng.net.parameters()]))
+    assert runs[0][0] == runs[1][0]  # the same kernels on the same numbers, sums in a fixed order
+    assert all(torch.equal(a, b) for a, b in zip(runs[0][1], runs[1][1]))
