@@ -188,8 +188,13 @@ Tensor ext_bwd(ExtArgs& a, const Tensor& q, int64_t heads, int64_t hd, const Ten
     a.dqv = view_of(dq, a.G); a.dkv = view_of(dk, 1);
     ext_plan_bwd(BH, a.M, a.Sk, a.tab != nullptr, w.q, w.kv);
     check_grid(a, w.q); check_grid(a, w.kv);
-    Tensor dsum = at::empty({w.q.few ? 1 : w.q.splits, BH, a.Mp}, f32), pq, pk, pv;
+    Tensor dsum = at::empty({w.q.few ? 1 : w.q.splits, BH, a.Mp}, f32), ends, pq, pk, pv;
     w.dsum = dsum.data_ptr<float>();
+    const long n_ends = dtable.defined() && NB > 0 ? ext_ends(a, w.q) : 0;
+    if (n_ends) {
+        ends = at::empty({n_ends}, f32);
+        w.ends = ends.data_ptr<float>();
+    }
     if (w.q.splits > 1) {
         pq = at::empty({BH * w.q.splits * a.M * hd}, f32);
         w.part_q = pq.data_ptr<float>();

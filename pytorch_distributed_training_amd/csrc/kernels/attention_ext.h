@@ -36,6 +36,7 @@ struct ExtBwd {
     const void *out, *dout;
     const float* stat;
     float* dsum;  // [splits of the row owner][stat_n]: -D, in the end in the first
+    float* ends;  // [ext_ends]: sums of dS over tiles of pairs past the table's reach, or null
     void *dq, *dk, *dv;
     float *part_q, *part_k, *part_v;
     ExtPlan q, kv;
@@ -43,6 +44,9 @@ struct ExtBwd {
 
 ExtPlan ext_plan_fwd(long BH, int M, int Sk, bool bias);
 void ext_plan_bwd(long BH, int M, int Sk, bool bias, ExtPlan& q, ExtPlan& kv);  // of the row owner and the key owner
+// Floats of ExtBwd::ends, or 0 where the row owner need not sum pairs past the table's reach: with more positions than entries there
+// are such pairs (positions in a row), with fewer (a grid) there are hardly any.  After ext_plan_bwd; with a gradient of the table.
+long ext_ends(const ExtArgs& a, const ExtPlan& q);
 void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, float* stat, float* part, float* part_ml,
                     hipStream_t s);
 void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s);
@@ -51,6 +55,7 @@ void launch_bias_tables(const float* table, const int* bucket_of, const int* q_c
 // the bias table's gradient: after launch_ext_bwd (which leaves D in dsum)
 struct RelBlocks {
     int h0, heads, q0, qblocks, kblocks;  // of this launch: heads, blocks of 128 queries; blocks of 128 keys of all
+    const float* ends;                    // of the row owner, or null
     int chunks, slab_rows;                // parts of the batch; rows of a head in the slab of entries
 };
 struct RelPlan {

@@ -109,6 +109,9 @@ __device__ __forceinline__ int one_entry(const ExtArgs& a, int qt, int kt, int l
     y = y < lo ? lo : y > hi ? hi : y;
     return x == y ? x : -1;
 }
+// Whether all pairs of 32 queries and 32 keys fall on the table's first entry (0) or on its last (1), or neither (-1).  On a long
+// sequence that is most of them, and the dQ pass, which has their dS, sums them for the table's gradient.
+__device__ __forceinline__ int far_end(int2 q, int2 k, int top) { return q.y - k.x <= 0 ? 0 : q.x - k.y >= top ? 1 : -1; }
 // The scores' start: bias (+ add) of 16 pairs of a lane whose own code is `mine` and the others' codes lie in LDS at `codes`
 __device__ __forceinline__ void gather_bias(f32x16& st, const char* codes, int half, int mine, int lo, int hi, float add) {
 #pragma unroll
@@ -657,16 +660,19 @@ __device__ __forceinline__ void store_tile(const f32x16* t, char* img, bf16* dst
 }
 
 // Row owner: dQ, and D for what follows. Bound as the forward is, with half the vector instructions' slots and half of LDS in
-// use and three waves a SIMD: 75 us, 123, 104 and 40 at the sizes given there. dO . O carries the rounding of P and O to bf16,
+// use and three waves a SIMD: 75 us, 123, 108 and 40 at the sizes given there. dO . O carries the rounding of P and O to bf16,
 // and the sum of a row's P (dP - dO . O) is exactly what it is off by (as a row's P add up to 1): added, D is good to 32 bits,
 // which the fp32 gradient of the bias table needs; that sum costs an add a score, keeping O's remainder in the forward cost it
 // a quarter of its time. Where all keys are in one block dS is corrected too: with few keys P (dP - D) is a small difference.
 // Without a bias and with more keys O is small against V, its rounding against dP, and nothing is added. A softmax over one key
 // is constant, so with len = 1 dS is zero, and is set so (as a difference of two rounded numbers it would not be).
-template <int HD, bool BIAS, bool ONE /* all keys in one block of 64 */>
+// FAR: `ends` [2][B Hkv][tiles of 32 rows] gets the sums of dS over the pairs of far_end's tiles, which the bias gradient's own passes
+// then leave out: sum P (dP - dO . O) - delta sum P, for 18 more vector instructions a tile.  Four sequences of up to 2047 with a
+// table of 257: this pass 104 -> 108 us, the sums over the batch 118 -> 41 and the entries 20 -> 13.
+template <int HD, bool BIAS, bool ONE /* all keys in one block of 64 */, bool FAR>
 __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ dout, const float* __restrict__ stat,
-                                                   float* __restrict__ dsum, bf16* __restrict__ dq, float* __restrict__ part, int tiles,
-                                                   int splits) {
+                                                   float* __restrict__ dsum, float* __restrict__ ends, bf16* __restrict__ dq,
+                                                   float* __restrict__ part, int tiles, int splits) {
     using G = AttnGeo<HD>;
     constexpr int IMG = 64 * G::ROWBYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][K, V], [2][codes 1 KiB], table
@@ -724,12 +730,20 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
     const float lq = live && j.len > 1 ? stat[a.stat_n + (long)j.bh * a.Mp + r] : -kInf;
     const int qc = tab + (BIAS && live ? a.q_codes4[r] : 0), top = tab + (a.R - 1) * 4;
 
+    uint64_t low = 0, high = 0;  // far_end of the 64 tiles of keys at hand
+    float end_off[2] = {0.f, 0.f}, end_p[2] = {0.f, 0.f};
     if (any) {
         for (int kb = kb0; kb < kb1; ++kb) {
             const int buf = (kb - kb0) & 1;
             dma_barrier();
             if (kb + 1 < kb1) issue(kb + 1, buf ^ 1);
             if (j.tile * 128 + wave * 32 >= j.rows) continue;
+            if (FAR && (kb & 31) == 0) {
+                const int kt = kb * 2 + lane;
+                const int end = kt * 32 < a.Sk ? far_end(a.q_range[j.tile * 4 + wave], a.k_range[kt], (a.R - 1) * 4) : -1;
+                low = __ballot(end == 0);
+                high = __ballot(end == 1);
+            }
             const char* Ks = smem + buf * 2 * IMG;
             const char* Vs = Ks + IMG;
             const bool both = kb * 64 + 32 < j.len;
@@ -763,15 +777,24 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
                     for (int i = 0; i < 16; ++i)
                         if (kb * 64 + kt * 32 + acc_row(i, half) >= j.len) sc[i] = -kInf;
                 }
-                float off = 0.f;
+                float off = 0.f, sum_p = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lq));
+                    if (FAR) sum_p += p;
                     if (ONE) pr[kt][i] = p;
                     dp[i] *= p;
                     if (BIAS || ONE) off += dp[i];
                 }
                 delta += off;
+                if (FAR) {
+                    const int bit = (kb & 31) * 2 + kt;
+                    const bool is_low = low >> bit & 1, is_high = high >> bit & 1;
+                    end_off[0] += is_low ? off : 0.f;
+                    end_p[0] += is_low ? sum_p : 0.f;
+                    end_off[1] += is_high ? off : 0.f;
+                    end_p[1] += is_high ? sum_p : 0.f;
+                }
                 if (ONE) ds[kt] = dp;
                 else product(dp, kt);
             }
@@ -787,6 +810,13 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
         }
     }
     delta += __shfl_xor(delta, 32, 64);
+    if (FAR) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float s = row_sum(fmaf(-delta, end_p[e], end_off[e]));
+            if (lane == 0) ends[((long)e * a.B * a.Hkv + j.bh) * tiles * 4 + j.tile * 4 + wave] = s;
+        }
+    }
     // -D of this split's keys: the first split has dO . O too, the sum over the splits is made where there is more than one
     if (half == 0 && r < a.Mp) dsum[((long)j.split * a.B * a.Hkv + j.bh) * a.Mp + r] = live ? -(delta + (j.split == 0 ? d : 0.f)) : 0.f;
     if (r >= a.M) return;
@@ -1005,7 +1035,7 @@ __global__ __launch_bounds__(256) void k_ext_dsum(float* __restrict__ dsum, long
 // dS summed over a part of the batch, for 128 queries x 128 keys of a head a workgroup (a wave: 32 queries, four tiles of 32
 // keys).  The bias of the block and the sums stay in registers while the batch streams through, so a pair costs two
 // multiply-adds and an exponential per sequence; written in register order, [tile][4][64 lanes] x 4 floats.  Its bound is what the
-// blocks move from L2, 64 KiB for 128 x 128 pairs of head_dim 64, at 6 to 7 TB/s: 58 us, 137 and 118 at the sizes given at the
+// blocks move from L2, 64 KiB for 128 x 128 pairs of head_dim 64, at 6 to 7 TB/s: 58 us, 137 and 41 at the sizes given at the
 // forward.  Blocks of 256 x 256 with the bias gathered for every sequence (no registers left for it) took 85 and 248, a second buffer
 // for K and V 64 and 149.
 template <int HD>
@@ -1025,6 +1055,10 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
     const int per = (a.B + w.chunks - 1) / w.chunks, b0 = ch * per, b1 = b0 + per < a.B ? b0 + per : a.B;
     const uint32_t lds0 = lds_address(smem);
     const int q = qb * 128 + wave * 32 + l31, krs = (int)a.kv.rs;
+    if (w.ends) {  // nothing to do where the dQ pass has all sixteen tiles (lanes 0 to 15 look at one each)
+        const int qt = qb * 4 + (lane & 3), kt = kb * 4 + (lane >> 2 & 3);
+        if (__all(qt * 32 >= a.Sk || kt * 32 >= a.Sk || far_end(a.q_range[qt], a.k_range[kt], (a.R - 1) * 4) >= 0)) return;
+    }
 
     // the block's bias (minus nothing yet): the table through LDS
     f32x16 bias[4], acc[4];
@@ -1105,6 +1139,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
     for (int kt = 0; kt < 4; ++kt) {
         if (kb * 128 + kt * 32 >= a.Sk || qb * 128 + wave * 32 >= a.Sk) break;  // (tiles that are not read)
         float* dst = dense + (row * nkt + kb * 4 + kt) * 1024 + lane * 4;
+        if (w.ends && far_end(a.q_range[qb * 4 + wave], a.k_range[kb * 4 + kt], (a.R - 1) * 4) >= 0) continue;
         if (one_entry(a, qb * 4 + wave, kb * 4 + kt, 0, (a.R - 1) * 4) >= 0) {  // one number
             float s = 0.f;
 #pragma unroll
@@ -1123,9 +1158,9 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
     }
 }
 
-// The pairs' sums by entry (10, 20 and 20 us there, most of it the LDS adds and the histograms' clearing): a workgroup takes a
-// tile row (32 queries) of a head and one of `parts` ranges of its key tiles; its waves take every fourth tile, each with a
-// histogram of its own.
+// The pairs' sums by entry (9, 20 and 13 us there, most of it the LDS adds and the histograms' clearing): a workgroup takes a
+// tile row (32 queries) of a head and one of `parts` shares of its key tiles; its waves take every (4 parts)-th tile (those near the
+// query are the ones with work where positions lie in a row), each with a histogram of its own.
 __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __restrict__ dense, float* __restrict__ slab, RelBlocks w,
                                                      int parts) {
     extern __shared__ __attribute__((aligned(16))) char smem[];  // [4][Rp] floats
@@ -1138,10 +1173,15 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
     for (int i = lane * 4; i < a.Rp; i += 256) *reinterpret_cast<f32x4*>(hist + i) = f32x4{0.f, 0.f, 0.f, 0.f};  // (Rp: a multiple of 4)
     const int q = (w.q0 * 4 + qt) * 32 + l31;
     const int qc = base + a.q_codes4[q];
-    const int live_t = (a.Sk + 31) / 32, per = (live_t + parts - 1) / parts;
-    const int t1 = w.q0 * 4 + qt >= live_t ? 0 : (part + 1) * per < live_t ? (part + 1) * per : live_t;
+    const int live_t = (a.Sk + 31) / 32, t1 = w.q0 * 4 + qt < live_t ? live_t : 0;
     float ends[2] = {0.f, 0.f};
-    for (int kt = part * per + wave; kt < t1; kt += 4) {
+    if (w.ends && part == 0 && wave == 0)
+        for (int b = lane; b < a.B; b += 64)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                ends[e] += w.ends[(((long)e * a.B + b) * a.Hkv + hl + w.h0) * (w.kblocks * 4) + w.q0 * 4 + qt];
+    for (int kt = part * 4 + wave; kt < t1; kt += 4 * parts) {
+        if (w.ends && far_end(a.q_range[w.q0 * 4 + qt], a.k_range[kt], (a.R - 1) * 4) >= 0) continue;
         const float* src = dense + (((long)hl * nqt + qt) * nkt + kt) * 1024 + lane * 4;
         const long step = (long)w.heads * nqt * nkt * 1024;
         const int one = one_entry(a, w.q0 * 4 + qt, kt, base, top);
@@ -1458,23 +1498,25 @@ void bwd(const ExtArgs& a, const ExtBwd& w, hipStream_t s) {
         const size_t lq = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + table_bytes(a);
         const size_t lk = (size_t)4 * 64 * HD * 2 + 8192 + table_bytes(a);
         const long n = a.stat_n;
-#define PDT_EXT_BWD_Q(BIAS, ONE)                                                                                    \
-    allow_lds(&k_ext_bwd_q<HD, BIAS, ONE>, lq);                                                                     \
-    hipLaunchKernelGGL((k_ext_bwd_q<HD, BIAS, ONE>), gq, dim3(256), lq, s, a, (const bf16*)w.out, (const bf16*)w.dout, w.stat, \
-                       w.dsum, (bf16*)w.dq, w.part_q, pq.tiles, pq.splits);
+#define PDT_EXT_BWD_Q(BIAS, ONE, FAR)                                                                                    \
+    allow_lds(&k_ext_bwd_q<HD, BIAS, ONE, FAR>, lq);                                                                     \
+    hipLaunchKernelGGL((k_ext_bwd_q<HD, BIAS, ONE, FAR>), gq, dim3(256), lq, s, a, (const bf16*)w.out, (const bf16*)w.dout, w.stat, \
+                       w.dsum, w.ends, (bf16*)w.dq, w.part_q, pq.tiles, pq.splits);
 #define PDT_EXT_BWD_KV(BIAS)                                                                                              \
     allow_lds(&k_ext_bwd_kv<HD, BIAS>, lk);                                                                               \
     hipLaunchKernelGGL((k_ext_bwd_kv<HD, BIAS>), gk, dim3(256), lk, s, a, (const bf16*)w.dout, w.stat, (const float*)w.dsum, \
                        (bf16*)w.dk, (bf16*)w.dv, w.part_k, w.part_v, pk.tiles, pk.splits);
         const bool one = a.Sk <= 64;
         if (a.tab && one) {
-            PDT_EXT_BWD_Q(true, true)
+            PDT_EXT_BWD_Q(true, true, false)
+        } else if (a.tab && w.ends) {
+            PDT_EXT_BWD_Q(true, false, true)
         } else if (a.tab) {
-            PDT_EXT_BWD_Q(true, false)
+            PDT_EXT_BWD_Q(true, false, false)
         } else if (one) {
-            PDT_EXT_BWD_Q(false, true)
+            PDT_EXT_BWD_Q(false, true, false)
         } else {
-            PDT_EXT_BWD_Q(false, false)
+            PDT_EXT_BWD_Q(false, false, false)
         }
         if (pq.splits > 1) hipLaunchKernelGGL(k_ext_dsum, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, w.dsum, n, pq.splits);
         if (a.tab) {
@@ -1554,6 +1596,9 @@ void launch_bias_tables(const float* table, const int* bucket_of, const int* q_c
     hipLaunchKernelGGL(k_bias_tables, dim3((unsigned)(tab_blocks + 2L * Sp / 256)), dim3(256), 0, s, table, bucket_of, q_codes, k_codes,
                        tab, codes, R, Rp, NB, H, S, Sp, inv_scale, tab_blocks);
 }
+long ext_ends(const ExtArgs& a, const ExtPlan& q) {
+    return a.tab && a.Sk > 64 && a.Sk >= a.R && q.splits == 1 ? 2L * a.B * a.Hkv * q.tiles * 4 : 0;
+}
 // Head groups and query blocks of a dense sum of at most 1 GiB; the batch in parts
 RelPlan rel_plan(int B, int H, int S, int hd) {
     RelPlan p;
@@ -1607,6 +1652,7 @@ void launch_rel_bias_grad(const ExtArgs& a, const ExtBwd& x, int hd, const RelPl
             w.kblocks = blocks;
             w.chunks = p.chunks;
             w.slab_rows = p.rows;
+            w.ends = x.ends;
             if (hd == 32) rel_dbias<32>(a, x, dense, w, s);
             else if (hd == 64) rel_dbias<64>(a, x, dense, w, s);
             else rel_dbias<128>(a, x, dense, w, s);

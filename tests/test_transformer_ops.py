@@ -573,6 +573,12 @@ def test_types_without_a_kernel_are_counted():
     assert sum(F.fallback_counts.values()) == before + 4
 
 
+@gpu
+def test_rel_bias_pairs_past_the_reach_of_the_table():
+    """More than 2048 positions in a row (the dQ pass looks at 64 tiles of keys at a time), lengths that end inside tiles."""
+    _check_rel(_dev("cuda"), 8, _log(2200, 64, 32), 2, 32, lengths=[2200, 2100, 0, 1, 700, 2177, 64, 2113], poison=True)
+
+
 def _chain(dev, seed):
     """The operators as a model uses them: self attention with positions, a block end, cross attention, a block end."""
     g = torch.Generator().manual_seed(seed)
