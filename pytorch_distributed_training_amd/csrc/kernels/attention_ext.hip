@@ -1159,8 +1159,9 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
 }
 
 // The pairs' sums by entry (9, 20 and 13 us there, most of it the LDS adds and the histograms' clearing): a workgroup takes a
-// tile row (32 queries) of a head and one of `parts` shares of its key tiles; its waves take every (4 parts)-th tile (those near the
-// query are the ones with work where positions lie in a row), each with a histogram of its own.
+// tile row (32 queries) of a head and one of `parts` shares of its key tiles, each wave with a histogram of its own.  Shares are
+// neighbouring tiles (20 us where tiles in turn took 21), but tiles in turn where the dQ pass has the far ones (13 for 18:
+// what is left lies together).
 __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __restrict__ dense, float* __restrict__ slab, RelBlocks w,
                                                      int parts) {
     extern __shared__ __attribute__((aligned(16))) char smem[];  // [4][Rp] floats
@@ -1173,14 +1174,15 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
     for (int i = lane * 4; i < a.Rp; i += 256) *reinterpret_cast<f32x4*>(hist + i) = f32x4{0.f, 0.f, 0.f, 0.f};  // (Rp: a multiple of 4)
     const int q = (w.q0 * 4 + qt) * 32 + l31;
     const int qc = base + a.q_codes4[q];
-    const int live_t = (a.Sk + 31) / 32, t1 = w.q0 * 4 + qt < live_t ? live_t : 0;
+    const int live_t = (a.Sk + 31) / 32, per = (live_t + parts - 1) / parts, last = w.ends || (part + 1) * per > live_t ? live_t : (part + 1) * per;
+    const int t1 = w.q0 * 4 + qt < live_t ? last : 0, step_t = w.ends ? 4 * parts : 4;
     float ends[2] = {0.f, 0.f};
     if (w.ends && part == 0 && wave == 0)
         for (int b = lane; b < a.B; b += 64)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
                 ends[e] += w.ends[(((long)e * a.B + b) * a.Hkv + hl + w.h0) * (w.kblocks * 4) + w.q0 * 4 + qt];
-    for (int kt = part * 4 + wave; kt < t1; kt += 4 * parts) {
+    for (int kt = (w.ends ? part * 4 : part * per) + wave; kt < t1; kt += step_t) {
         if (w.ends && far_end(a.q_range[w.q0 * 4 + qt], a.k_range[kt], (a.R - 1) * 4) >= 0) continue;
         const float* src = dense + (((long)hl * nqt + qt) * nkt + kt) * 1024 + lane * 4;
         const long step = (long)w.heads * nqt * nkt * 1024;
@@ -1424,7 +1426,8 @@ __global__ __launch_bounds__(256) void k_bias_slab(const float* __restrict__ sla
 // dtable[n][h] = sum over the entries r of bucket n: a lane per bucket, a workgroup takes 64 buckets, its 16 waves every 16th 64
 // entries.  Entries lie a lane each and go round by readlane; 64 whose buckets are all in other workgroups (on a grid nearly
 // all: there an entry is a bucket) are passed over.  Any number of entries may share a bucket, in any order.
-__global__ __launch_bounds__(1024) void k_bias_buckets(const float* __restrict__ sums, const int* __restrict__ bucket_of,
+// `rows` rows of sums a head.
+__global__ __launch_bounds__(1024) void k_bias_buckets(const float* __restrict__ slab, int rows, const int* __restrict__ bucket_of,
                                                       float* __restrict__ dtable, int R, int Rp, int NB, int H) {
     __shared__ float red[16][64];
     const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
@@ -1432,7 +1435,11 @@ __global__ __launch_bounds__(1024) void k_bias_buckets(const float* __restrict__
     for (int r0 = wave * 64; r0 < R; r0 += 1024) {
         const int r = r0 + lane, of = r < R ? bucket_of[r] - (int)blockIdx.x * 64 : -1;
         if (!__any(of >= 0 && of < 64)) continue;
-        const float v = r < R ? sums[(long)h * Rp + r] : 0.f;
+        float v = 0.f;
+        if (r < R) {
+#pragma unroll 8
+            for (int i = 0; i < rows; ++i) v += slab[((long)h * rows + i) * Rp + r];
+        }
 #pragma unroll 8
         for (int e = 0; e < 64; ++e) {
             const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), e));
@@ -1661,9 +1668,11 @@ void launch_rel_bias_grad(const ExtArgs& a, const ExtBwd& x, int hd, const RelPl
             hipLaunchKernelGGL(k_rel_entries, dim3((unsigned)(w.heads * w.qblocks * 4 * p.parts)), dim3(256), lds, s, a,
                                (const float*)dense, slab, w, p.parts);
         }
-    hipLaunchKernelGGL(k_bias_slab, dim3((a.Rp + 63) / 64, a.Hkv), dim3(256), 0, s, (const float*)slab, mid, a.Rp, p.rows);
-    hipLaunchKernelGGL(k_bias_buckets, dim3((NB + 63) / 64, a.Hkv), dim3(1024), 0, s, (const float*)mid, bucket_of, dtable, a.R, a.Rp, NB,
-                       a.Hkv);
+    // few rows of the slab are summed where they are read: 16 rows of 732 entries in 4.8 us for 9.4, but 60 of 2212 in 14.5 for 12.7
+    const bool direct = p.rows <= 32;
+    if (!direct) hipLaunchKernelGGL(k_bias_slab, dim3((a.Rp + 63) / 64, a.Hkv), dim3(256), 0, s, (const float*)slab, mid, a.Rp, p.rows);
+    hipLaunchKernelGGL(k_bias_buckets, dim3((NB + 63) / 64, a.Hkv), dim3(1024), 0, s, (const float*)(direct ? slab : mid), direct ? p.rows : 1,
+                       bucket_of, dtable, a.R, a.Rp, NB, a.Hkv);
 }
 
 }  // namespace pdt
