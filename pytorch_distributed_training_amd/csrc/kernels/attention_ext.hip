@@ -1292,7 +1292,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
             if (wave == 0) dma_words(st, lrow + rb * 64, lane);
             if (wave == 1) dma_words(st + 1024, drow + rb * 64, lane);
             if (BIAS && wave == 2) dma_words(st + 2048, a.q_codes4 + rb * 64, lane);
-            if (wave == 3) dma_words(st + 3072, mrow + rb * 64, lane);
+            if (wave == 3) dma_words(st + 3 * 1024, mrow + rb * 64, lane);
         };
         issue(rb0, 0);
         if (BIAS) {
@@ -1325,7 +1325,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
                 for (int jj = 0; jj < 4; ++jj) {
                     const int w = (rt * 32 + 8 * jj + 4 * half) * 4;
                     lr[jj] = *reinterpret_cast<const f32x4*>(st + w);
-                    const f32x4 dr = *reinterpret_cast<const f32x4*>(st + 1024 + w), mr = *reinterpret_cast<const f32x4*>(st + 3072 + w);
+                    const f32x4 dr = *reinterpret_cast<const f32x4*>(st + 1024 + w), mr = *reinterpret_cast<const f32x4*>(st + 3 * 1024 + w);
                     i32x4 qc = {0, 0, 0, 0};
                     if (BIAS) qc = *reinterpret_cast<const i32x4*>(st + 2048 + w);
 #pragma unroll
