@@ -437,7 +437,7 @@ std::vector<Tensor> gated_norm_bwd(const OptTensor& du, const OptTensor& dn, con
     // without a gate per sample a workgroup has one unit: its gate sums are one more column block of the slab
     const int groups = cols + (p.per_sample ? 0 : 1), srow = (int)(groups * D);
     const bool parts = p.per_sample && q.chunks > 1;
-    TORCH_CHECK(!p.per_sample || x.size(0) < (1L << 24) / ((D + 63) / 64), "gated_residual_norm: ", x.size(0), " samples");
+    TORCH_CHECK(!p.per_sample || x.size(0) < (1L << 23) / ((D + 63) / 64), "gated_residual_norm: ", x.size(0), " samples");
     Tensor work = at::empty({(long)q.blocks * srow + (parts ? q.units * D : 0)}, w.options());
     float* slab = work.data_ptr<float>();
     Tensor sums = q.blocks == 1 ? work.narrow(0, 0, srow).view({groups, D}) : at::empty({groups, D}, w.options());
@@ -445,8 +445,8 @@ std::vector<Tensor> gated_norm_bwd(const OptTensor& du, const OptTensor& dn, con
     float* gp = !p.per_sample ? slab + cols * D : parts ? slab + (long)q.blocks * srow : dgate.data_ptr<float>();
     launch_gated_norm_bwd(p, q, given(du) ? du->data_ptr() : nullptr, given(dn) ? dn->data_ptr() : nullptr, stats.data_ptr<float>(),
                           dx.data_ptr(), dy.data_ptr(), gp, p.per_sample ? D : srow, slab, srow, stream_of(x));
-    if (parts) launch_gate_sum(gp, dgate.data_ptr<float>(), x.size(0), p.D, q.chunks, stream_of(x));
-    if (q.blocks > 1) launch_gated_norm_sum(slab, sums.data_ptr<float>(), q.blocks, srow, stream_of(x));
+    launch_gated_norm_sums(slab, q.blocks > 1 ? sums.data_ptr<float>() : nullptr, q.blocks, srow, gp, parts ? dgate.data_ptr<float>() : nullptr,
+                           x.size(0), p.D, q.chunks, stream_of(x));
     const std::vector<Tensor> c = sums.unbind(0);  // db, dw[, dpb, dpw][, dgate]
     std::vector<Tensor> r = {dx, dy, p.per_sample ? dgate : c[cols], c[1], c[0]};
     if (post) {

@@ -1178,6 +1178,7 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
     const int t1 = w.q0 * 4 + qt < live_t ? last : 0, step_t = w.ends ? 4 * parts : 4;
     float ends[2] = {0.f, 0.f};
     if (w.ends && part == 0 && wave == 0)
+#pragma unroll 4
         for (int b = lane; b < a.B; b += 64)
 #pragma unroll
             for (int e = 0; e < 2; ++e)

@@ -23,7 +23,8 @@ void launch_gated_norm_fwd(const GatedNorm& p, void* u, void* n, float* stats, h
 GatedNormPlan gated_norm_plan(long B, long T, long M, bool per_sample);
 void launch_gated_norm_bwd(const GatedNorm& p, const GatedNormPlan& q, const void* du, const void* dn, const float* stats, void* dx,
                            void* dy, float* gate_part, long gate_stride, float* slab, int srow, hipStream_t s);
-void launch_gated_norm_sum(const float* slab, float* sums, int rows, int n, hipStream_t s);
-void launch_gate_sum(const float* part, float* dgate, long B, int D, int chunks, hipStream_t s);
+// sums [n] of the slab [rows][n] (or null), dgate [B][D] of the parts [B][chunks][D] (or null)
+void launch_gated_norm_sums(const float* slab, float* sums, int rows, int n, const float* part, float* dgate, long B, int D, int chunks,
+                            hipStream_t s);
 
 }  // namespace pdt
