@@ -582,12 +582,25 @@ __global__ __launch_bounds__(256) void k_ext_join(ExtArgs a, const float* __rest
 }
 
 // ------------------------------------------------------------------------------------------------------- backward
-// dst rows <- scale * (sum of the splits' fp32 partials, in order), or, for dead rows, what the partials hold: zeros
+// dst rows <- scale * (sum of the splits' fp32 partials, in order), or, for dead rows, what the partials hold: zeros.  One launch
+// for dQ, dK and dV, as far as they are split (a launch each: 12 us for 5 on one sequence of 577).
+struct SumJob {
+    const float* part;
+    bf16* dst;
+    ExtView v;
+    int G, rows, splits;
+    float scale;
+};
+struct SumJobs {
+    SumJob job[3];
+};
 template <int HD>
-__global__ __launch_bounds__(256) void k_ext_sum(const float* __restrict__ part, bf16* __restrict__ dst, ExtView v, int G,
-                                                 int Hkv, int rows, int splits, float scale, long total) {
+__global__ __launch_bounds__(256) void k_ext_sum(SumJobs jobs, int Hkv, long BH) {
+    const SumJob& w = jobs.job[blockIdx.y];
+    const float* part = w.part;
+    const int rows = w.rows, splits = w.splits;
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
+    if (i >= BH * rows * (HD / 4)) return;
     const int d = (int)(i % (HD / 4)) * 4;
     const long row = i / (HD / 4);
     const int bh = (int)(row / rows), r = (int)(row - (long)bh * rows);
@@ -601,8 +614,8 @@ __global__ __launch_bounds__(256) void k_ext_sum(const float* __restrict__ part,
     }
     bf16x4 w4;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w4[e] = (bf16)(t[e] * scale);
-    *reinterpret_cast<bf16x4*>(dst + (long)b * v.bs + row_offset(v, r, hkv, G, HD) + d) = w4;
+    for (int e = 0; e < 4; ++e) w4[e] = (bf16)(t[e] * w.scale);
+    *reinterpret_cast<bf16x4*>(w.dst + (long)b * w.v.bs + row_offset(w.v, r, hkv, w.G, HD) + d) = w4;
 }
 
 // a lane's accumulator columns: dst[d] for d = dt*32 + 8*jj + 4*half + e
@@ -1536,23 +1549,23 @@ void bwd(const ExtArgs& a, const ExtBwd& w, hipStream_t s) {
 #undef PDT_EXT_BWD_KV
     }
     const long BH = (long)a.B * a.Hkv;
-    if (pq.splits > 1) {
-        const long total = BH * a.M * (HD / 4);
-        hipLaunchKernelGGL((k_ext_sum<HD>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, (const float*)w.part_q,
-                           (bf16*)w.dq, a.dqv, a.G, a.Hkv, a.M, pq.splits, a.scale, total);
-    }
-    if (pk.splits > 1) {
-        const long total = BH * a.Sk * (HD / 4);
-        const dim3 g((unsigned)((total + 255) / 256));
-        hipLaunchKernelGGL((k_ext_sum<HD>), g, dim3(256), 0, s, (const float*)w.part_k, (bf16*)w.dk, a.dkv, 1, a.Hkv, a.Sk,
-                           pk.splits, a.scale, total);
-        hipLaunchKernelGGL((k_ext_sum<HD>), g, dim3(256), 0, s, (const float*)w.part_v, (bf16*)w.dv, a.dkv, 1, a.Hkv, a.Sk,
-                           pk.splits, 1.f, total);
-    }
+    SumJobs jobs{};
+    unsigned n = 0;
+    int rows = 0;
+    auto add = [&](const float* part, void* dst, const ExtView& v, int G, int m, int splits, float scale) {
+        if (splits < 2) return;
+        jobs.job[n++] = {part, (bf16*)dst, v, G, m, splits, scale};
+        rows = m > rows ? m : rows;
+    };
+    add(w.part_q, w.dq, a.dqv, a.G, a.M, pq.splits, a.scale);
+    add(w.part_k, w.dk, a.dkv, 1, a.Sk, pk.splits, a.scale);
+    add(w.part_v, w.dv, a.dkv, 1, a.Sk, pk.splits, 1.f);
+    if (n)
+        hipLaunchKernelGGL((k_ext_sum<HD>), dim3((unsigned)((BH * rows * (HD / 4) + 255) / 256), n), dim3(256), 0, s, jobs, a.Hkv, BH);
 }
 
 // parts to cut `blocks` blocks of the streamed axis into, so that `groups` workgroups become about two per CU (512); a part
-// keeps at least `least` blocks. Cut and joined against whole: one sequence of 577 on 12 heads, training, 97 us for 112; 64
+// keeps at least `least` blocks. Cut and joined against whole: one sequence of 577 on 12 heads, training, 100 us for 112; 64
 // rows x 2000 keys on 8 heads, forward and dQ, 27 us for 72; single rows over 1500 and over 65536 keys, 11 and 190 us for 12
 // and 705. 256 or 1024 workgroups instead of 512 changed none of these by 5 %. With 300 workgroups cutting lost: five sequences
 // of 577, training, 144 us whole and 149 cut; single rows over 1500 keys on 24 x 12 heads 23 and 25.
