@@ -9,7 +9,7 @@
 //   dx = a g,  dgate = sum g z,  dz = gate g,  dy = LN'(dz) (or dz),  dw = sum dn uh,  db = sum dn,  dpw = sum dz yh,  dpb = sum dz
 //
 // Bound by memory: forward 2 reads + 2 writes, backward 4 reads + 2 writes of 2 bytes per element.  64 x 577 rows of 1024, a gate
-// for each sample: 57 us (5.3 TB/s) and 95 (4.8 TB/s) + 9 for the sums; 64 x 197 rows of 768 with the norm of the branch: 19 and
+// for each sample: 57 us (5.3 TB/s) and 95 (4.8 TB/s) + 5 for the sums; 64 x 197 rows of 768 with the norm of the branch: 19 and
 // 31 + 4.  x and y are what the backward reads again (not u): u is recomputed in fp32, so the parameter gradients see the numbers that the forward normalised,
 // at no more traffic than a saved u would cost.  One wave holds a row in registers (4 channels a lane and piece, NP pieces of
 // 256 channels) and walks over rows with the parameters in registers (read again for every row they were 2.7 times the
