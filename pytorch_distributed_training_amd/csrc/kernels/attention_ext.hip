@@ -70,8 +70,8 @@ __device__ __forceinline__ void dma_block(uint32_t img, const bf16* base, uint32
         }
     }
 }
-// rows [r0, r0 + 32) -> LDS image, by one wave; rows >= valid arrive as zeros
-template <int HD>
+// rows [r0, r0 + 32) -> LDS image, by one wave; rows >= valid arrive as zeros.  STREAM: past the caches (streams_past_caches)
+template <int HD, bool STREAM>
 __device__ __forceinline__ void dma_tile(uint32_t img, const bf16* base, int rs, int valid, int lane) {
     using G = AttnGeo<HD>;
     constexpr int RPP = 1024 / G::ROWBYTES, NP = 32 / RPP;
@@ -81,7 +81,9 @@ __device__ __forceinline__ void dma_tile(uint32_t img, const bf16* base, int rs,
         const int row = p * RPP + lane / G::NCH;
         const int x = ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) & (G::NCH - 1);
         const uint32_t o = row < valid ? (uint32_t)(row * rs) * 2u + (uint32_t)(((lane % G::NCH) ^ x) << 4) : kOOB;
-        lds_dma16(rsrc, o, (uint32_t)__builtin_amdgcn_readfirstlane((int)(img + p * 1024)));
+        const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(img + p * 1024));
+        if (STREAM) lds_dma16_stream(rsrc, o, at);
+        else lds_dma16(rsrc, o, at);
     }
 }
 // 64 consecutive 4-byte values -> LDS (the image takes 1 KiB: lanes 16.. write zeros)
@@ -376,9 +378,9 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
 // Few rows (at most one tile of 32 for a key head: single tokens).  The four waves of a workgroup share the rows and take
 // every fourth tile of 32 keys each, through an LDS ring of their own (no barrier until the join): the kernel is a stream over
 // K and V, 16 to 64 KiB of it in flight per workgroup, and bound by memory: 4 sequences of 65536 keys, 8 key heads of 128, four rows
-// each: 185 us, 5.8 TB/s (with the kernel above, whose waves would have one tile of rows for four: 193); 512 of 197 on 12 heads
-// of 64: 73 us, 4.2 TB/s (80 there, and the backward 275 for the 145 of its counterpart).
-template <int HD>
+// each: 169 us, 6.4 TB/s (with the kernel above, whose waves would have one tile of rows for four: 193); 512 of 197 on 12 heads
+// of 64: 62 us, 5.0 TB/s (80 there, and the backward 275 for the 139 of its counterpart).
+template <int HD, bool STREAM>
 __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restrict__ out, float* __restrict__ stat,
                                                      float* __restrict__ part, float* __restrict__ part_ml, int splits) {
     using G = AttnGeo<HD>;
@@ -399,8 +401,8 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
     auto issue = [&](int t, int buf) {
         const int valid = j.len - t * 32 < 32 ? j.len - t * 32 : 32;
         const long at = (long)t * 32 * krs;
-        dma_tile<HD>(ring_lds + buf * STAGE, kbase + at, krs, valid, lane);
-        dma_tile<HD>(ring_lds + buf * STAGE + TIMG, vbase + at, krs, valid, lane);
+        dma_tile<HD, STREAM>(ring_lds + buf * STAGE, kbase + at, krs, valid, lane);
+        dma_tile<HD, STREAM>(ring_lds + buf * STAGE + TIMG, vbase + at, krs, valid, lane);
     };
     f32x16 o[G::DT];
 #pragma unroll
@@ -648,7 +650,7 @@ __device__ __forceinline__ void store_acc32(const f32x16* t, float* dst, int hal
 
 // The same 32 rows (lane = row) through a tile image in LDS, so that a store writes whole rows, 16 B a lane: 8-byte pieces of 32
 // rows at a time cost the pass over single queries a quarter of its time.  One wave, its own image.
-template <int HD>
+template <int HD, bool STREAM>
 __device__ __forceinline__ void store_tile(const f32x16* t, char* img, bf16* dst, int rs, int valid, float scale, int lane) {
     using G = AttnGeo<HD>;
     constexpr int RPP = 1024 / G::ROWBYTES, NP = 32 / RPP;
@@ -668,7 +670,9 @@ __device__ __forceinline__ void store_tile(const f32x16* t, char* img, bf16* dst
         const int row = p * RPP + lane / G::NCH;
         const int x = ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) & (G::NCH - 1);
         const u32x4 v = *reinterpret_cast<const u32x4*>(img + p * 1024 + lane * 16);
-        if (row < valid) *reinterpret_cast<u32x4*>(dst + (long)row * rs + ((lane % G::NCH) ^ x) * 8) = v;
+        bf16* to = dst + (long)row * rs + ((lane % G::NCH) ^ x) * 8;
+        if (row < valid && STREAM) st_stream(to, v);
+        else if (row < valid) *reinterpret_cast<u32x4*>(to) = v;
     }
 }
 
@@ -840,8 +844,8 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
 // Few rows (at most 32 for a key head: an attention pooling head's query): everything in one pass over K and V.  A wave takes
 // every fourth tile of 32 keys through a ring of its own, makes the tile's scores in both orientations (two small products; the
 // pass is bound by the stream of K, V, dK and dV), stores dK and dV of its keys and keeps its part of dQ, which the four
-// waves join at the end.  512 sequences of 197 keys, 12 heads of 64: 145 us, 4.3 TB/s; row owner and key owner took 275.
-template <int HD>
+// waves join at the end.  512 sequences of 197 keys, 12 heads of 64: 139 us, 4.5 TB/s; row owner and key owner took 275.
+template <int HD, bool STREAM>
 __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_few(ExtArgs a, const bf16* __restrict__ out, const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                         bf16* __restrict__ dq, bf16* __restrict__ dk, bf16* __restrict__ dv,
                                                         float* __restrict__ part, int splits) {
@@ -865,8 +869,8 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_few(ExtArgs a,
     auto issue = [&](int t, int buf) {
         const int valid = j.len - t * 32 < 32 ? j.len - t * 32 : 32;
         const long at = (long)t * 32 * krs;
-        dma_tile<HD>(ring_lds + buf * STAGE, kbase + at, krs, valid, lane);
-        dma_tile<HD>(ring_lds + buf * STAGE + TIMG, vbase + at, krs, valid, lane);
+        dma_tile<HD, STREAM>(ring_lds + buf * STAGE, kbase + at, krs, valid, lane);
+        dma_tile<HD, STREAM>(ring_lds + buf * STAGE + TIMG, vbase + at, krs, valid, lane);
     };
     if (t0 + wave < t1 && t0 + wave < nt) issue(t0 + wave, 0);
     // the rows as operands of both orientations (lane = row), their images for the products over rows, and D
@@ -1006,7 +1010,7 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_few(ExtArgs a,
                         o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(img, blk * 16, dt * 32, lane), x, o[dt], 0, 0, 0);
                 }
                 // (the tile's own images are free: its rows are in registers, its columns were read for dQ)
-                store_tile<HD>(o, ring + (buf ^ 1) * STAGE + (g ? 0 : TIMG), (g ? dk : dv) + at, (int)a.dkv.rs, rows, g ? a.scale : 1.f, lane);
+                store_tile<HD, STREAM>(o, ring + (buf ^ 1) * STAGE + (g ? 0 : TIMG), (g ? dk : dv) + at, (int)a.dkv.rs, rows, g ? a.scale : 1.f, lane);
             }
         }
     }
@@ -1475,6 +1479,11 @@ void allow_lds(K kern, size_t bytes) {
     if (e != hipSuccess) throw std::runtime_error(std::string("attention: ") + hipGetErrorString(e));  // (an exception of the call)
 }
 
+// Whether the passes over few rows take and leave K and V with the non-temporal hint: where K and V are more than the 256 MB that
+// lie in front of the memory.  310 MB: forward 74 -> 62 us, backward 147 -> 139; 1 GB: 185 -> 169; but 123 MB: backward 45 -> 55,
+// 110 MB: forward 24 -> 25.
+bool streams_past_caches(const ExtArgs& a, int hd) { return 4L * a.B * a.Sk * a.Hkv * hd >= 256L << 20; }
+
 size_t table_bytes(const ExtArgs& a) { return a.tab ? (size_t)((a.Rp + 255) & ~255) * 4 : 0; }
 
 template <int HD>
@@ -1482,8 +1491,9 @@ void fwd(const ExtArgs& a, const ExtPlan& p, void* out, float* stat, float* part
     const unsigned grid = (unsigned)((long)a.B * a.Hkv * p.tiles * p.splits);
     if (p.few) {
         const size_t lds = (size_t)16 * 32 * HD * 2 + 4 * 32 * 2 * sizeof(float);
-        allow_lds(&k_ext_fwd_few<HD>, lds);
-        hipLaunchKernelGGL((k_ext_fwd_few<HD>), dim3(grid), dim3(256), lds, s, a, (bf16*)out, stat, part, part_ml, p.splits);
+        const auto kern = streams_past_caches(a, HD) ? &k_ext_fwd_few<HD, true> : &k_ext_fwd_few<HD, false>;
+        allow_lds(kern, lds);
+        hipLaunchKernelGGL(kern, dim3(grid), dim3(256), lds, s, a, (bf16*)out, stat, part, part_ml, p.splits);
     } else {
         const size_t lds = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + table_bytes(a);
 #define PDT_EXT_FWD(BIAS)                                                                                               \
@@ -1513,8 +1523,9 @@ void bwd(const ExtArgs& a, const ExtBwd& w, hipStream_t s) {
     const dim3 gq((unsigned)((long)a.B * a.Hkv * pq.tiles * pq.splits)), gk((unsigned)((long)a.B * a.Hkv * pk.tiles * pk.splits));
     if (pq.few) {
         const size_t lds = (size_t)(16 + 2) * 32 * HD * 2 + 3 * 32 * sizeof(float);
-        allow_lds(&k_ext_bwd_few<HD>, lds);
-        hipLaunchKernelGGL((k_ext_bwd_few<HD>), gq, dim3(256), lds, s, a, (const bf16*)w.out, (const bf16*)w.dout, w.stat, (bf16*)w.dq, (bf16*)w.dk, (bf16*)w.dv, w.part_q, pq.splits);
+        const auto kern = streams_past_caches(a, HD) ? &k_ext_bwd_few<HD, true> : &k_ext_bwd_few<HD, false>;
+        allow_lds(kern, lds);
+        hipLaunchKernelGGL(kern, gq, dim3(256), lds, s, a, (const bf16*)w.out, (const bf16*)w.dout, w.stat, (bf16*)w.dq, (bf16*)w.dk, (bf16*)w.dv, w.part_q, pq.splits);
     } else {
         const size_t lq = (size_t)4 * 64 * HD * 2 + (a.tab ? 2048 : 0) + table_bytes(a);
         const size_t lk = (size_t)4 * 64 * HD * 2 + 8192 + table_bytes(a);
