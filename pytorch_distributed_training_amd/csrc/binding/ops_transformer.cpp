@@ -402,6 +402,7 @@ GatedNorm gated_norm_args(const Tensor& x, const Tensor& y, const Tensor& gate, 
     p.x = bf16_ptr(x); p.y = bf16_ptr(y);
     p.gate = gate.data_ptr<float>(); p.w = w.data_ptr<float>(); p.b = b.data_ptr<float>();
     p.a = (float)scale; p.eps = (float)eps;
+    p.stream = p.M * D * 2 >= 64L << 20;
     return p;
 }
 // -> u, n, stats [2 or 4, M] (with `grad`)

@@ -9,7 +9,7 @@
 //   dx = a g,  dgate = sum g z,  dz = gate g,  dy = LN'(dz) (or dz),  dw = sum dn uh,  db = sum dn,  dpw = sum dz yh,  dpb = sum dz
 //
 // Bound by memory: forward 2 reads + 2 writes, backward 4 reads + 2 writes of 2 bytes per element.  64 x 577 rows of 1024, a gate
-// for each sample: 57 us (5.3 TB/s) and 95 (4.8 TB/s) + 5 for the sums; 64 x 197 rows of 768 with the norm of the branch: 19 and
+// for each sample: 57 us (5.3 TB/s) and 85 (5.3 TB/s) + 5 for the sums; 64 x 197 rows of 768 with the norm of the branch: 19 and
 // 31 + 4.  x and y are what the backward reads again (not u): u is recomputed in fp32, so the parameter gradients see the numbers that the forward normalised,
 // at no more traffic than a saved u would cost.  One wave holds a row in registers (4 channels a lane and piece, NP pieces of
 // 256 channels) and walks over rows with the parameters in registers (read again for every row they were 2.7 times the
@@ -28,12 +28,17 @@ __device__ __forceinline__ bf16x4 raw4(const bf16* p, bool in) {
     if (in) t = *reinterpret_cast<const bf16x4*>(p);
     return t;
 }
+template <bool STREAM>
+__device__ __forceinline__ void put4(bf16* p, bf16x4 v) {
+    if (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<bf16x4*>(p));
+    else *reinterpret_cast<bf16x4*>(p) = v;
+}
 __device__ __forceinline__ f32x4 par4(const float* p, bool in) {
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
     if (in) t = *reinterpret_cast<const f32x4*>(p);
     return t;
 }
-template <int NP, bool POST>
+template <int NP, bool POST, bool STREAM>
 __global__ __launch_bounds__(256, NP <= 3 ? 4 : NP == 4 ? 3 : NP < 8 ? 2 : 1) void k_gn_fwd(GatedNorm p, bf16* __restrict__ u_out, bf16* __restrict__ n_out,
                                                                   float* __restrict__ stats /* [2 or 4][M], or null */) {
     const int lane = threadIdx.x & 63, D = p.D, np4 = D >> 2;
@@ -113,7 +118,7 @@ __global__ __launch_bounds__(256, NP <= 3 ? 4 : NP == 4 ? 3 : NP < 8 ? 2 : 1) vo
                 s += x[j][k];
                 o[k] = (bf16)x[j][k];
             }
-            if (lane + 64 * j < np4) *reinterpret_cast<bf16x4*>(u_out + row * D + 4 * (lane + 64 * j)) = o;
+            if (lane + 64 * j < np4) put4<STREAM>(u_out + row * D + 4 * (lane + 64 * j), o);
         }
         const float mean = row_sum(s) * inv_d;
 #pragma unroll
@@ -172,7 +177,7 @@ __device__ __forceinline__ void column_sum(float (&v)[NP][4], float* red, float*
 
 // A unit is one of `chunks` parts of a sample's rows; a workgroup takes the units blockIdx.x, + gridDim.x, ...  The gate's sums
 // leave after every unit (to gate_part + unit * gate_stride), the others at the end (slab [gridDim.x][srow]: db, dw, dpb, dpw).
-template <int NP, bool POST>
+template <int NP, bool POST, bool STREAM>
 __global__ __launch_bounds__(256, NP <= (POST ? 3 : 4) ? 2 : 1) void k_gn_bwd(
     GatedNorm p, const bf16* __restrict__ du, const bf16* __restrict__ dn, const float* __restrict__ stats, bf16* __restrict__ dx,
     bf16* __restrict__ dy, float* __restrict__ gate_part, long gate_stride, float* __restrict__ slab, int srow, int chunks, long units) {
@@ -289,7 +294,7 @@ __global__ __launch_bounds__(256, NP <= (POST ? 3 : 4) ? 2 : 1) void k_gn_bwd(
                         s4 += t * y[j][k];
                     }
                 }
-                if (in) *reinterpret_cast<bf16x4*>(dx + row * D + 4 * (lane + 64 * j)) = o;
+                if (in) put4<STREAM>(dx + row * D + 4 * (lane + 64 * j), o);
             }
             if (POST) {
                 s3 = row_sum(s3) * inv_d;
@@ -374,8 +379,9 @@ void launch_gated_norm_fwd(const GatedNorm& p, void* u, void* n, float* stats, h
     const long full = (p.M + 3) / 4;
     const unsigned grid = (unsigned)(full < 1024 ? full : 1024);  // (4 per CU walk over the rows)
     PDT_GN_DISPATCH(p.D, {
-        if (p.pw) hipLaunchKernelGGL((k_gn_fwd<NP, true>), dim3(grid), dim3(256), 0, s, p, (bf16*)u, (bf16*)n, stats);
-        else hipLaunchKernelGGL((k_gn_fwd<NP, false>), dim3(grid), dim3(256), 0, s, p, (bf16*)u, (bf16*)n, stats);
+        const auto kern = p.pw ? (p.stream ? &k_gn_fwd<NP, true, true> : &k_gn_fwd<NP, true, false>)
+                               : (p.stream ? &k_gn_fwd<NP, false, true> : &k_gn_fwd<NP, false, false>);
+        hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, s, p, (bf16*)u, (bf16*)n, stats);
     });
 }
 
@@ -396,12 +402,10 @@ void launch_gated_norm_bwd(const GatedNorm& p, const GatedNormPlan& q, const voi
                            void* dy, float* gate_part, long gate_stride, float* slab, int srow, hipStream_t s) {
     PDT_GN_DISPATCH(p.D, {
         const size_t lds = (size_t)7 * NP * 256 * sizeof(float);
-        if (p.pw)
-            hipLaunchKernelGGL((k_gn_bwd<NP, true>), dim3(q.blocks), dim3(256), lds, s, p, (const bf16*)du, (const bf16*)dn, stats,
-                               (bf16*)dx, (bf16*)dy, gate_part, gate_stride, slab, srow, q.chunks, q.units);
-        else
-            hipLaunchKernelGGL((k_gn_bwd<NP, false>), dim3(q.blocks), dim3(256), lds, s, p, (const bf16*)du, (const bf16*)dn, stats,
-                               (bf16*)dx, (bf16*)dy, gate_part, gate_stride, slab, srow, q.chunks, q.units);
+        const auto kern = p.pw ? (p.stream ? &k_gn_bwd<NP, true, true> : &k_gn_bwd<NP, true, false>)
+                               : (p.stream ? &k_gn_bwd<NP, false, true> : &k_gn_bwd<NP, false, false>);
+        hipLaunchKernelGGL(kern, dim3(q.blocks), dim3(256), lds, s, p, (const bf16*)du, (const bf16*)dn, stats, (bf16*)dx, (bf16*)dy,
+                           gate_part, gate_stride, slab, srow, q.chunks, q.units);
     });
 }
 void launch_gated_norm_sums(const float* slab, float* sums, int rows, int n, const float* part, float* dgate, long B, int D, int chunks,

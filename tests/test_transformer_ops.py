@@ -875,3 +875,21 @@ def test_captured_training_step_of_a_vit_with_options():
         runs.append((losses, [p.detach().clone() for p in eng.net.parameters()]))
     assert runs[0][0] == runs[1][0]  # the same kernels on the same numbers, sums in a fixed order
     assert all(torch.equal(a, b) for a, b in zip(runs[0][1], runs[1][1]))
+
+
+@gpu
+@pytest.mark.parametrize("case", [dict(b=512, nq=1, nk=197, heads=12, kv_heads=12, hd=64),
+                                  dict(b=2, nq=3, nk=40000, heads=8, kv_heads=8, hd=128, lengths=[40000, 777], poison=True)],
+                         ids=["pool", "long"])
+def test_cross_attention_past_the_caches(case):
+    """Keys and values of more than 256 MB: the variants that stream past the caches."""
+    assert 4 * case["b"] * case["nk"] * case["kv_heads"] * case["hd"] >= 256 << 20
+    _check_cross(_dev("cuda"), **case)
+
+
+@gpu
+@pytest.mark.parametrize("per_sample,post", [(True, False), (False, True)])
+def test_gated_residual_norm_past_the_caches(per_sample, post):
+    """Activations of more than 64 MB."""
+    assert 64 * 530 * 1024 * 2 >= 64 << 20
+    _check_norm(_dev("cuda"), (64, 530, 1024), per_sample, post, 0.5)
