@@ -17,7 +17,9 @@
 //    running maximum, sums, rescaling and the stores (four neighbouring channels a lane) are all per lane.
 //  * The statistics that the backward gets are -m (in units of q . k) and -log2 l apart.  Where a bias of -1e9 holds for a whole
 //    row, their sum would not leave a bit of l, and 2^(c s - sum), a difference of two numbers rounded at 1e9, is anything.
-//    The backward's scores start at bias - m, so that no large number is left to round.
+//  * With a bias the scores of both directions start at the bias and m is taken off the result, so that the backward's P are the
+//    forward's to 32 bits: at -1e9 the bias takes up all of q . k, the keys of such a row weigh the same, and they have to weigh
+//    the same in the gradients (with scores that start at bias - m a row's P added up to 1.2 to 2.8).
 //  * The axis that streams comes by LDS-DMA in blocks of 64 rows, two buffers, one barrier a block; rows past the valid
 //    length are sent out of range and arrive as zeros, so whatever they hold (NaN, infinities) is never multiplied.
 //  * Few rows: the streamed axis is cut into `splits`, each with its own workgroup and an fp32 partial that a small kernel
@@ -114,13 +116,13 @@ __device__ __forceinline__ int one_entry(const ExtArgs& a, int qt, int kt, int l
 // Whether all pairs of 32 queries and 32 keys fall on the table's first entry (0) or on its last (1), or neither (-1).  On a long
 // sequence that is most of them, and the dQ pass, which has their dS, sums them for the table's gradient.
 __device__ __forceinline__ int far_end(int2 q, int2 k, int top) { return q.y - k.x <= 0 ? 0 : q.x - k.y >= top ? 1 : -1; }
-// The scores' start: bias (+ add) of 16 pairs of a lane whose own code is `mine` and the others' codes lie in LDS at `codes`
-__device__ __forceinline__ void gather_bias(f32x16& st, const char* codes, int half, int mine, int lo, int hi, float add) {
+// The scores' start: the bias of 16 pairs of a lane whose own code is `mine` and the others' codes lie in LDS at `codes`
+__device__ __forceinline__ void gather_bias(f32x16& st, const char* codes, int half, int mine, int lo, int hi) {
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
         const i32x4 c = *reinterpret_cast<const i32x4*>(codes + (8 * jj + 4 * half) * 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) st[4 * jj + e] = lds_float(bias_at(mine, c[e], lo, hi)) + add;
+        for (int e = 0; e < 4; ++e) st[4 * jj + e] = lds_float(bias_at(mine, c[e], lo, hi));
     }
 }
 // v[i] of the pairs at table addresses at[i] into a wave's own histogram.  LDS float adds take a cycle a lane, and many times
@@ -284,7 +286,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
                     break;
                 }
                 if (BIAS) {
-                    gather_bias(st[kt], codes + buf * 1024 + kt * 128, half, qc, tab, top, 0.f);
+                    gather_bias(st[kt], codes + buf * 1024 + kt * 128, half, qc, tab, top);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
@@ -778,7 +780,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
             for (int kt = 0; kt < 2; ++kt) {
                 if (!ONE && kt == 1 && !both) break;
                 f32x16 sc, dp;
-                if (BIAS) gather_bias(sc, codes + buf * 1024 + kt * 128, half, qc, tab, top, mq);
+                if (BIAS) gather_bias(sc, codes + buf * 1024 + kt * 128, half, qc, tab, top);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     if (!BIAS) sc[i] = mq;
@@ -797,7 +799,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_bwd_q(ExtArgs a, const bf16* __r
                 float off = 0.f, sum_p = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lq));
+                    const float p = __builtin_amdgcn_exp2f(fmaf(BIAS ? sc[i] + mq : sc[i], a.c, lq));
                     if (FAR) sum_p += p;
                     if (ONE) pr[kt][i] = p;
                     dp[i] *= p;
@@ -1130,7 +1132,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
                     f32x16 sc, dp;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        sc[i] = bias[kt][i] + mq;
+                        sc[i] = bias[kt][i];
                         dp[i] = d;
                     }
 #pragma unroll
@@ -1144,7 +1146,7 @@ __global__ __launch_bounds__(256, 2) void k_rel_dbias(ExtArgs a, const bf16* __r
                             if (kb * 128 + kt * 32 + acc_row(i, half) >= len) sc[i] = -kInf;
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[kt][i] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lq)), dp[i], acc[kt][i]);
+                    for (int i = 0; i < 16; ++i) acc[kt][i] = fmaf(__builtin_amdgcn_exp2f(fmaf(sc[i] + mq, a.c, lq)), dp[i], acc[kt][i]);
                 }
             }
         }
@@ -1255,11 +1257,11 @@ __global__ __launch_bounds__(256) void k_rel_entries(ExtArgs a, const float* __r
 }
 
 // Key owner: dK and dV of 128 keys a workgroup; the rows of all G heads stream through. Four products
-// a tile for the row owner's three, and a row's numbers (-m, -log2 l, -D, code) come from LDS for every register: 87 us, 153, 170 and 54 at the
+// a tile for the row owner's three, and a row's numbers (-m, -log2 l, -D, code) come from LDS for every register: 92 us, 160, 170 and 54 at the
 // sizes given at the forward, LDS and vector instructions half busy each. -D and the exponent by a matrix instruction with ones
 // instead: 99 and 67; the exponent as one number with a branch for large maxima: 101.
 template <int HD, bool BIAS>
-__global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, const bf16* __restrict__ dout, const float* __restrict__ stat,
+__global__ __launch_bounds__(256, HD > 64 ? 1 : BIAS ? 3 : 2) void k_ext_bwd_kv(ExtArgs a, const bf16* __restrict__ dout, const float* __restrict__ stat,
                                                     const float* __restrict__ dsum, bf16* __restrict__ dk, bf16* __restrict__ dv,
                                                     float* __restrict__ part_k, float* __restrict__ part_v, int tiles, int splits) {
     using G = AttnGeo<HD>;
@@ -1338,17 +1340,23 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
             for (int rt = 0; rt < 2; ++rt) {
                 if (HD <= 64 && rt == 1 && rb * 64 + 32 >= j.rows) break;
                 f32x16 sc, dp;
-                f32x4 lr[4];
+                // With a bias -m is needed after the products.  Held through them, -m and -log2 l cost a SIMD its third wave at head_dim
+                // 64 (103 us at 128 x 197 x 12 heads where read late 91); at 128, with one wave, late reads wait (196 us for 171).
+                constexpr bool LATE = BIAS && HD <= 64;
+                f32x4 lr[4], mr[4];
 #pragma unroll
                 for (int jj = 0; jj < 4; ++jj) {
                     const int w = (rt * 32 + 8 * jj + 4 * half) * 4;
-                    lr[jj] = *reinterpret_cast<const f32x4*>(st + w);
-                    const f32x4 dr = *reinterpret_cast<const f32x4*>(st + 1024 + w), mr = *reinterpret_cast<const f32x4*>(st + 3 * 1024 + w);
+                    if (!LATE) {
+                        lr[jj] = *reinterpret_cast<const f32x4*>(st + w);
+                        mr[jj] = *reinterpret_cast<const f32x4*>(st + 3 * 1024 + w);
+                    }
+                    const f32x4 dr = *reinterpret_cast<const f32x4*>(st + 1024 + w);
                     i32x4 qc = {0, 0, 0, 0};
                     if (BIAS) qc = *reinterpret_cast<const i32x4*>(st + 2048 + w);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        sc[4 * jj + e] = BIAS ? lds_float(bias_at(qc[e], kc, tab, top)) + mr[e] : mr[e];
+                        sc[4 * jj + e] = BIAS ? lds_float(bias_at(qc[e], kc, tab, top)) : mr[jj][e];
                         dp[4 * jj + e] = dr[e];
                     }
                 }
@@ -1359,10 +1367,20 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : 2) void k_ext_bwd_kv(ExtArgs a, 
                 }
                 // (no mask: a dead key is a lane of its own whose results are not stored; rows past the end have -log2 l = -inf)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, lr[i >> 2][i & 3]));
-                    sc[i] = p;
-                    dp[i] *= p;
+                for (int jj = 0; jj < 4; ++jj) {
+                    const int w = (rt * 32 + 8 * jj + 4 * half) * 4;
+                    if (LATE) {
+                        asm volatile("" ::: "memory");
+                        mr[jj] = *reinterpret_cast<const f32x4*>(st + 3 * 1024 + w);
+                        lr[jj] = *reinterpret_cast<const f32x4*>(st + w);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = 4 * jj + e;
+                        const float p = __builtin_amdgcn_exp2f(fmaf(BIAS ? sc[i] + mr[jj][e] : sc[i], a.c, lr[jj][e]));
+                        sc[i] = p;
+                        dp[i] *= p;
+                    }
                 }
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {

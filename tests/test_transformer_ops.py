@@ -893,3 +893,70 @@ def test_gated_residual_norm_past_the_caches(per_sample, post):
     """Activations of more than 64 MB."""
     assert 64 * 530 * 1024 * 2 >= 64 << 20
     _check_norm(_dev("cuda"), (64, 530, 1024), per_sample, post, 0.5)
+
+
+# ------------------------------------------------------------- rows whose every key has a very large negative bias
+LARGE = [dict(b=1, n=40, hd=64), dict(b=2, n=70, hd=32), dict(b=1, n=150, hd=128), dict(b=1, n=600, hd=64), dict(b=3, n=300, hd=128)]
+
+
+def _half_masked(n):
+    """Codes that put the first half of the queries on bucket 1 for every key, the others on bucket 0."""
+    q = torch.zeros(n, dtype=torch.int32)
+    q[:n // 2] = 1
+    return q, torch.zeros(n, dtype=torch.int32), torch.arange(2, dtype=torch.int32)
+
+
+@gpu
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -1e9, -1e6, -8e3])
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: f"b{c['b']}-n{c['n']}x{c['hd']}")
+def test_rel_bias_backward_has_the_forward_weights(case, low):
+    """V that names the first hd keys and dO that names the first hd queries show P in the output and in dV: one softmax."""
+    dev = _dev("cuda")
+    b, n, hd = case["b"], case["n"], case["hd"]
+    m = min(n, hd)
+    g = torch.Generator().manual_seed(31)
+    qkv = _rand(g, b, n, 2, 3 * hd).view(b, n, 3, 2, hd)
+    qkv[:, :, 2] = torch.eye(n, hd)[:, None]
+    do = torch.eye(n, hd)[:, None].expand(b, n, 2, hd).reshape(b, n, 2 * hd).to(torch.bfloat16).to(dev)
+    qkv = qkv.reshape(b, n, 6 * hd).to(dev).requires_grad_()
+    table = torch.tensor([[0.3, -0.2], [low, 0.5]], device=dev)
+    out = F.rel_bias_attention(qkv, table, *(t.to(dev) for t in _half_masked(n)), 2)
+    (dqkv,) = torch.autograd.grad(out, qkv, do)
+    forward = out.detach().view(b, n, 2, hd)[:, :m, :, :m].double()  # [b, query, head, key]
+    backward = dqkv[..., 4 * hd:].view(b, n, 2, hd)[:, :m, :, :m].double().transpose(1, 3)
+    # each of the two rounds P once and its result once; the scores of the two differ by roundings in 32 bits, which P takes up to
+    # 2^-9 of (|bias| sqrt(hd) at most 2^16 has steps of 2^-8, half of it at each of hd / 16 additions, times 1 / sqrt(hd))
+    _within(backward, forward, (4 * U + 2.0 ** -9 + hd / 16 * 2.0 ** -9 / math.sqrt(hd)) * forward + SLACK / n, "P")
+
+
+@gpu
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, -1e9])
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: f"b{c['b']}-n{c['n']}x{c['hd']}")
+def test_rel_bias_gradients_of_absorbed_scores(case, low):
+    """Where a bias takes up all of q . k a row's keys weigh the same, in every gradient too."""
+    dev = _dev("cuda")
+    heads, n, hd, b = 2, case["n"], case["hd"], case["b"]
+    codes = _half_masked(n)
+    table = torch.tensor([[0.3, -0.2], [low, 0.5]])
+    qkv, table, qc, kc, of, do, live, (qkv64, do64) = _rel_case(dev, b, codes, heads, hd, table=table)
+    leaf, tleaf = qkv.clone().requires_grad_(), table.clone().requires_grad_()
+    out = F.rel_bias_attention(leaf, tleaf, qc, kc, of, heads)
+    dqkv, dtable = torch.autograd.grad(out, [leaf, tleaf], do)
+    q, k, v = qkv64.view(b, n, 3, heads, hd).permute(2, 0, 3, 1, 4)
+    bias = table.double()[of.long()[(qc - kc[0]).long()]].t()[None, :, :, None].expand(b, heads, n, n).clone()
+    gone = slice(0, n // 2)
+    bias[:, 0, gone] = -(q[:, 0, gone] @ k[:, 0].transpose(-1, -2)) * hd ** -0.5  # the scores are nothing beside `low`
+    do4 = do64.view(b, n, heads, hd).transpose(1, 2)
+    (o, dq, dk, dv, ds, p), es = _attention64(q, k, v, bias, live, live.double(), do4)
+
+    def flat(t):
+        return t.transpose(1, 2).reshape(b, n, heads * hd)
+
+    _within(out, flat(o), flat(es[0]), "out")
+    for i, (name, w, e) in enumerate((("dq", dq, es[1]), ("dk", dk, es[2]), ("dv", dv, es[3]))):
+        _within(dqkv[..., i * heads * hd:(i + 1) * heads * hd], flat(w), flat(e), name)
+    # a bucket holds all pairs of its rows, whose dS add up to nothing; the bound is that of `_check_rel`
+    err = p * (2.0 ** -15 * (do4.abs() * (o.abs() + p @ v.abs())).sum(-1, keepdim=True) + SLACK / 8 * (do4.abs() @ v.abs().transpose(-1, -2)))
+    by_row = (err + 2.0 ** -20 * ds.abs()).sum((0, 3)), ds.sum((0, 3))
+    bound, want = (torch.stack([t[:, n // 2:].sum(1), t[:, :n // 2].sum(1)]) for t in by_row)
+    _within(dtable, want, bound, "dtable")
