@@ -49,6 +49,13 @@ void no_second_backward(const char* op) {
     TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the backward pass cannot be differentiated again");
 }
 
+// The kernels are called at once, outside the dispatcher: what autograd has beyond a backward pass would be lost without a word.  A
+// tensor with a tangent (forward-mode derivatives) does not require a gradient, so that a node alone would not see it.
+void check_plain(const char* op, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->defined()) TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), op, ": no forward-mode derivative, only a backward pass");
+}
+
 // A backward pass that is captured while an eager graph of the same leaves lives accumulates on the eager graph's stream: the
 // engine would wait for a stream outside the capture, in a thread whose exception ends the process.  Refused at the forward.
 void check_capture(std::initializer_list<const Tensor*> leaves) {
@@ -283,6 +290,7 @@ struct RelBiasFn : torch::autograd::Function<RelBiasFn> {
         no_second_backward("rel_bias_attention");
         torch::autograd::variable_list r(7);
         if (!g[0].defined()) return r;
+        check_plain("rel_bias_attention", {&g[0]});
         const auto s = ctx->get_saved_variables();
         auto [dqkv, dtable] = rel_bias_attention_bwd(dense16(g[0]), s[0], s[1], s[2], s[3], s[4], s[5], ctx->saved_data["buckets"].toInt(),
                                                      ctx->saved_data["heads"].toInt(), opt(s[6]), ctx->needs_input_grad(1));
@@ -302,6 +310,7 @@ OptTensor rel_bias_attention(const Tensor& qkv, const Tensor& table, const Tenso
     for (const Tensor* t : {&q_codes, &k_codes, &bucket_of})
         if (!is_index(*t) || t->device() != qkv.device()) return {};
     if (table.device() != qkv.device()) return {};
+    check_plain("rel_bias_attention", {&qkv, &table});
     if (!wants_grad({&qkv, &table}))
         return std::get<0>(rel_bias_attention_fwd(rows3(qkv), param32(table), int32(q_codes), int32(k_codes), int32(bucket_of), heads,
                                                   given(lens) ? opt(int32(*lens)) : lens, false));
@@ -353,6 +362,7 @@ struct CrossFn : torch::autograd::Function<CrossFn> {
         no_second_backward("cross_attention");
         torch::autograd::variable_list r(5);
         if (!g[0].defined()) return r;
+        check_plain("cross_attention", {&g[0]});
         const auto s = ctx->get_saved_variables();
         auto [dq, dkv] = cross_attention_bwd(dense16(g[0]), s[0], s[1], s[2], s[3], ctx->saved_data["heads"].toInt(),
                                              ctx->saved_data["kv_heads"].toInt(), opt(s[4]));
@@ -366,6 +376,7 @@ OptTensor cross_attention(const Tensor& q, const Tensor& kv, int64_t heads, int6
         kv_heads < 1 || heads % kv_heads || !attention_dim_ok(q.size(2), heads) || kv.size(2) != 2 * kv_heads * (q.size(2) / heads) ||
         q.size(0) != kv.size(0) || q.device() != kv.device() || !lengths_fit(lens, q))
         return {};
+    check_plain("cross_attention", {&q, &kv});
     if (!wants_grad({&q, &kv}))
         return std::get<0>(cross_attention_fwd(rows3(q), rows3(kv), heads, kv_heads, given(lens) ? opt(int32(*lens)) : lens, false));
     check_capture({&q, &kv});
@@ -477,6 +488,7 @@ struct GatedNormFn : torch::autograd::Function<GatedNormFn> {
         no_second_backward("gated_residual_norm");
         torch::autograd::variable_list r(9);
         if (!g[0].defined() && !g[1].defined()) return r;
+        check_plain("gated_residual_norm", {&g[0], &g[1]});
         const auto s = ctx->get_saved_variables();
         const auto types = ctx->saved_data["types"].toIntVector();
         const auto d = gated_norm_bwd(opt(dense16(g[0])), opt(dense16(g[1])), s[0], s[1], s[2], s[3], s[4], opt(s[5]), opt(s[6]), s[7],
@@ -501,6 +513,7 @@ c10::optional<std::tuple<Tensor, Tensor>> gated_residual_norm(const Tensor& x, c
         if (!t->defined()) continue;
         if (t->device() != x.device() || !at::isFloatingType(t->scalar_type()) || (t != &gate && t->sizes() != at::IntArrayRef({D}))) return {};
     }
+    check_plain("gated_residual_norm", {&x, &y, &gate, &w, &b, &pw, &pb});
     if (!wants_grad({&x, &y, &gate, &w, &b, &pw, &pb})) {
         auto [u, n, stats] = gated_norm_fwd(dense16(x), dense16(y), param32(gate), param32(w), param32(b), opt(param32(pw)),
                                             opt(param32(pb)), eps, scale, false);

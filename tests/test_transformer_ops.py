@@ -960,3 +960,42 @@ def test_rel_bias_gradients_of_absorbed_scores(case, low):
     by_row = (err + 2.0 ** -20 * ds.abs()).sum((0, 3)), ds.sum((0, 3))
     bound, want = (torch.stack([t[:, n // 2:].sum(1), t[:, :n // 2].sum(1)]) for t in by_row)
     _within(dtable, want, bound, "dtable")
+
+
+# ----------------------------------------------------------------------- what autograd has beyond a backward pass
+def _three_calls(dev, seed=41):
+    """-> (name, call, tensors that may get a tangent or a gradient): small calls that the kernels take"""
+    g = torch.Generator().manual_seed(seed)
+    qc, kc, of = (t.to(dev) for t in _log(9))
+    qkv, q, kv = (_rand(g, 2, 9, w, device=dev) for w in (192, 64, 128))
+    table, gate = (_rand(g, *s, dtype=torch.float32, device=dev) for s in ((8, 1), (64,)))
+    one = torch.ones(64, device=dev)
+    return [("rel_bias_attention", lambda a, b: F.rel_bias_attention(a, b, qc, kc, of, 1), [qkv, table]),
+            ("cross_attention", lambda a, b: F.cross_attention(a, b, 1), [q, kv]),
+            ("gated_residual_norm", lambda a, b: F.gated_residual_norm(a, a * 0.5, b, one, one)[1], [q, gate])]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_forward_mode_is_refused(device):
+    """A tangent that the kernels would drop reads as a derivative of zero."""
+    import torch.autograd.forward_ad as fwd
+
+    for name, call, inputs in _three_calls(_dev(device)):
+        for i in range(2):
+            for grad in (False, True):
+                with fwd.dual_level(), torch.set_grad_enabled(grad):
+                    args = [t.clone().requires_grad_(grad) for t in inputs]
+                    args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+                    with pytest.raises((RuntimeError, NotImplementedError)):
+                        call(*args)
+        # a tangent that reaches the backward pass alone, from a later layer's weight
+        args = [t.clone().requires_grad_() for t in inputs]
+        with fwd.dual_level():
+            out = call(*args)
+            w = fwd.make_dual(torch.ones_like(out), torch.ones_like(out))
+            if device == "cuda":
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    torch.autograd.grad((out * w).sum(), args)
+            else:  # elementary operations: the backward pass is linear in w
+                got = fwd.unpack_dual(torch.autograd.grad((out * w).sum(), args)[0])
+                assert got.tangent is not None and torch.equal(got.tangent, got.primal)
