@@ -4,7 +4,10 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -49,11 +52,27 @@ void no_second_backward(const char* op) {
     TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the backward pass cannot be differentiated again");
 }
 
-// The kernels are called at once, outside the dispatcher: what autograd has beyond a backward pass would be lost without a word.  A
-// tensor with a tangent (forward-mode derivatives) does not require a gradient, so that a node alone would not see it.
+// A tracer, and a mode whose tensors are proxies, fakes or wrappers, sees only the allocation of the outputs: what it records
+// would return memory that nobody has written.  Other modes (counters of operations and the like) may be on.
+bool is_recording() {
+    using Mode = c10::impl::TorchDispatchModeKey;
+    if (torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch)) return true;
+    if (!c10::impl::TorchDispatchModeTLS::any_modes_set()) return false;
+    for (Mode m : {Mode::FAKE, Mode::PROXY, Mode::FUNCTIONAL})
+        if (c10::impl::TorchDispatchModeTLS::get_mode(m).has_value()) return true;
+    return false;
+}
+// The kernels are called at once, outside the dispatcher: what autograd and the transforms have beyond a backward pass would be
+// lost without a word.  A tensor with a tangent (forward-mode derivatives) does not require a gradient, so that a node alone would
+// not see it; a tensor of a transform or a wrapper may say that it is on the GPU and have no memory there.
 void check_plain(const char* op, std::initializer_list<const Tensor*> ts) {
-    for (const Tensor* t : ts)
-        if (t->defined()) TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), op, ": no forward-mode derivative, only a backward pass");
+    TORCH_CHECK(!is_recording(), op, ": cannot be traced, exported or run on fake tensors (its kernels are called outside the dispatcher)");
+    for (const Tensor* t : ts) {
+        if (!t->defined()) continue;
+        TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), op, ": no forward-mode derivative, only a backward pass");
+        TORCH_CHECK(t->has_storage() && (t->numel() == 0 || t->const_data_ptr()), op,
+                    ": expected tensors with memory of their own (no vmap, no torch.func, no wrappers)");
+    }
 }
 
 // A backward pass that is captured while an eager graph of the same leaves lives accumulates on the eager graph's stream: the
@@ -310,7 +329,7 @@ OptTensor rel_bias_attention(const Tensor& qkv, const Tensor& table, const Tenso
     for (const Tensor* t : {&q_codes, &k_codes, &bucket_of})
         if (!is_index(*t) || t->device() != qkv.device()) return {};
     if (table.device() != qkv.device()) return {};
-    check_plain("rel_bias_attention", {&qkv, &table});
+    check_plain("rel_bias_attention", {&qkv, &table, &q_codes, &k_codes, &bucket_of, given(lens) ? &*lens : &qkv});
     if (!wants_grad({&qkv, &table}))
         return std::get<0>(rel_bias_attention_fwd(rows3(qkv), param32(table), int32(q_codes), int32(k_codes), int32(bucket_of), heads,
                                                   given(lens) ? opt(int32(*lens)) : lens, false));
@@ -376,7 +395,7 @@ OptTensor cross_attention(const Tensor& q, const Tensor& kv, int64_t heads, int6
         kv_heads < 1 || heads % kv_heads || !attention_dim_ok(q.size(2), heads) || kv.size(2) != 2 * kv_heads * (q.size(2) / heads) ||
         q.size(0) != kv.size(0) || q.device() != kv.device() || !lengths_fit(lens, q))
         return {};
-    check_plain("cross_attention", {&q, &kv});
+    check_plain("cross_attention", {&q, &kv, given(lens) ? &*lens : &q});
     if (!wants_grad({&q, &kv}))
         return std::get<0>(cross_attention_fwd(rows3(q), rows3(kv), heads, kv_heads, given(lens) ? opt(int32(*lens)) : lens, false));
     check_capture({&q, &kv});

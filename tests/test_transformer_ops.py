@@ -999,3 +999,71 @@ def test_forward_mode_is_refused(device):
             else:  # elementary operations: the backward pass is linear in w
                 got = fwd.unpack_dual(torch.autograd.grad((out * w).sum(), args)[0])
                 assert got.tangent is not None and torch.equal(got.tangent, got.primal)
+
+
+@pytest.mark.skipif(not pdt.native_available(), reason="extension not built")
+def test_fake_tensors_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    for inside in (True, False):
+        mode = FakeTensorMode()
+        with mode:
+            def e(*s, dtype=torch.bfloat16):
+                return torch.empty(*s, dtype=dtype, device="cuda")
+            qkv, q, kv, table, gate = e(2, 9, 192), e(2, 9, 64), e(2, 9, 128), e(8, 1, dtype=torch.float32), e(64, dtype=torch.float32)
+            codes = [torch.empty(n, dtype=torch.int32, device="cuda") for n in (9, 9, 33)]
+            calls = [lambda: F.rel_bias_attention(qkv, table, *codes, 1), lambda: F.cross_attention(q, kv, 1),
+                     lambda: F.gated_residual_norm(q, q, gate, gate, gate)]
+            if inside:
+                for call in calls:
+                    with pytest.raises(RuntimeError, match="fake"):
+                        call()
+        if not inside:
+            for call in calls:
+                with pytest.raises(RuntimeError):
+                    call()
+
+
+@gpu
+def test_tracers_and_transforms_are_refused():
+    """They see only the allocation of the outputs; what they recorded would return memory that nobody has written."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+
+    for name, call, (a, b) in _three_calls(_dev("cuda")):
+        want = call(a, b)
+        for grad in (False, True):
+            x, y = a.clone().requires_grad_(grad), b.clone().requires_grad_(grad)
+            for record in (lambda: torch.jit.trace(call, (x, y)), lambda: make_fx(call)(x, y), lambda: make_fx(call, pre_dispatch=True)(x, y),
+                           lambda: make_fx(call, tracing_mode="fake")(x, y)):
+                with pytest.raises(RuntimeError, match="cannot be traced"):
+                    record()
+            with pytest.raises(RuntimeError):
+                torch.func.vmap(lambda t: call(t, y))(torch.stack([x, x]))
+            with pytest.raises(RuntimeError):
+                torch.func.grad(lambda t: call(t, y).float().sum())(x)
+        # what only looks on, or leaves the calls out of what it records, works
+        with FlopCounterMode(display=False):
+            assert torch.equal(call(a, b), want)
+        assert torch.equal(torch.compile(call, backend="eager")(a, b), want)
+
+
+@pytest.mark.skipif(not pdt.native_available(), reason="extension not built")
+def test_wrappers_without_memory_are_refused():
+    """A subclass may say that it is on the GPU and hold its data elsewhere; its address is null."""
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, *shape, dtype=torch.bfloat16):
+            return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype, device="cuda")
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise AssertionError("the call was not refused before its first operation")
+
+    f32, i32 = torch.float32, torch.int32
+    qkv, q, kv, table, gate = Wrapper(2, 9, 192), Wrapper(2, 9, 64), Wrapper(2, 9, 128), Wrapper(8, 1, dtype=f32), Wrapper(64, dtype=f32)
+    codes = [Wrapper(n, dtype=i32) for n in (9, 9, 33)]
+    for call in (lambda: F.rel_bias_attention(qkv, table, *codes, 1), lambda: F.cross_attention(q, kv, 1),
+                 lambda: F.cross_attention(q, kv, 1, lengths=Wrapper(2, dtype=i32)), lambda: F.gated_residual_norm(q, q, gate, gate, gate)):
+        with pytest.raises(RuntimeError, match="memory of their own"):
+            call()
