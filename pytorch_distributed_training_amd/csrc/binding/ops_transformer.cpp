@@ -7,6 +7,8 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
@@ -48,8 +50,31 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
         if (t->defined() && t->requires_grad()) return true;
     return false;
 }
-void no_second_backward(const char* op) {
-    TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the backward pass cannot be differentiated again");
+// The gradients of a node's backward pass under create_graph: constants whose own derivative raises.  (Only then: a model may have
+// another term that does need second derivatives.)  The raising node hangs on all that the gradients depend on, the node's inputs
+// and the gradients that came in, so that no way to ask for the derivative finds nothing to differentiate.
+template <typename F>
+torch::autograd::variable_list first_order(const char* op, const torch::autograd::variable_list& g, F&& backward) {
+    if (!at::GradMode::is_enabled()) return backward();
+    torch::autograd::variable_list r;
+    {
+        at::NoGradGuard no_grad;
+        r = backward();
+    }
+    torch::autograd::edge_list edges;
+    if (const auto node = torch::autograd::get_current_node())
+        for (const auto& e : node->next_edges())
+            if (e.is_valid()) edges.push_back(e);
+    for (const Tensor& t : g)
+        if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+    const auto raise = std::make_shared<torch::autograd::Error>(std::string(op) + ": the backward pass cannot be differentiated again",
+                                                                std::move(edges));
+    for (Tensor& t : r) {
+        if (!t.defined()) continue;
+        if (t.is_view()) t = t.clone();  // (a history of its own)
+        torch::autograd::set_history(t, raise);
+    }
+    return r;
 }
 
 // A tracer, and a mode whose tensors are proxies, fakes or wrappers, sees only the allocation of the outputs: what it records
@@ -306,7 +331,9 @@ struct RelBiasFn : torch::autograd::Function<RelBiasFn> {
         return out;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
-        no_second_backward("rel_bias_attention");
+        return first_order("rel_bias_attention", g, [&] { return gradients(ctx, g); });
+    }
+    static torch::autograd::variable_list gradients(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& g) {
         torch::autograd::variable_list r(7);
         if (!g[0].defined()) return r;
         check_plain("rel_bias_attention", {&g[0]});
@@ -378,7 +405,9 @@ struct CrossFn : torch::autograd::Function<CrossFn> {
         return out;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
-        no_second_backward("cross_attention");
+        return first_order("cross_attention", g, [&] { return gradients(ctx, g); });
+    }
+    static torch::autograd::variable_list gradients(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& g) {
         torch::autograd::variable_list r(5);
         if (!g[0].defined()) return r;
         check_plain("cross_attention", {&g[0]});
@@ -504,7 +533,9 @@ struct GatedNormFn : torch::autograd::Function<GatedNormFn> {
         return {u, n};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
-        no_second_backward("gated_residual_norm");
+        return first_order("gated_residual_norm", g, [&] { return gradients(ctx, g); });
+    }
+    static torch::autograd::variable_list gradients(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& g) {
         torch::autograd::variable_list r(9);
         if (!g[0].defined() && !g[1].defined()) return r;
         check_plain("gated_residual_norm", {&g[0], &g[1]});

@@ -1067,3 +1067,27 @@ def test_wrappers_without_memory_are_refused():
                  lambda: F.cross_attention(q, kv, 1, lengths=Wrapper(2, dtype=i32)), lambda: F.gated_residual_norm(q, q, gate, gate, gate)):
         with pytest.raises(RuntimeError, match="memory of their own"):
             call()
+
+
+@pytest.mark.parametrize("device", [pytest.param("cuda", marks=gpu)])
+def test_create_graph_raises_only_for_a_second_derivative(device):
+    dev = _dev(device)
+    for name, call, (a, b) in _three_calls(dev):
+        x, y = a.clone().requires_grad_(), b.clone().requires_grad_()
+        z = torch.full((3,), 0.5, device=dev, requires_grad=True)
+
+        def loss():
+            out = call(x, y)
+            return (out * out).float().sum() + (z ** 3).sum()
+
+        want = torch.autograd.grad(loss(), [x, y, z])
+        got = torch.autograd.grad(loss(), [x, y, z], create_graph=True)
+        assert all(torch.equal(u, v) for u, v in zip(want, got))
+        (second,) = torch.autograd.grad(got[2].square().sum(), z)  # another term's
+        assert torch.equal(second, 36 * z.detach() ** 3)
+        for ask in (lambda d: torch.autograd.grad(d.float().sum(), x), lambda d: torch.autograd.grad(d.float().sum(), [x, y], allow_unused=True),
+                    lambda d: (d.float().sum() + z.sum()).backward()):
+            for i in (0, 1):
+                got = torch.autograd.grad(loss(), [x, y], create_graph=True)
+                with pytest.raises(RuntimeError):
+                    ask(got[i])
