@@ -564,7 +564,7 @@ class _RelBiasAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @reference.first_order("rel_bias_attention")
     def backward(ctx, dout):
         qkv, table, q_codes, k_codes, bucket_of, lengths = ctx.saved_tensors
         dqkv, dtable = reference.rel_bias_attention_bwd(dout, qkv, table, q_codes, k_codes, bucket_of, ctx.heads, lengths,
@@ -621,7 +621,7 @@ class _CrossAttentionFn(torch.autograd.Function):
         return reference.cross_attention_fwd(q, kv, heads, kv_heads, lengths)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @reference.first_order("cross_attention")
     def backward(ctx, dout):
         q, kv, lengths = ctx.saved_tensors
         dq, dkv = reference.cross_attention_bwd(dout, q, kv, *ctx.cfg, lengths)

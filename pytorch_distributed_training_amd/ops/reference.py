@@ -9,6 +9,8 @@ Conventions shared with the native ops: image tensors are logical ``[B,C,H,W]``
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn.functional as F
 
@@ -201,6 +203,42 @@ def layernorm_bwd(dy, x, mean, rstd, gamma, addend=None):
 
 
 # ----------------------- attention with relative positions, cross attention
+class _Constants(torch.autograd.Function):
+    """The first ``n`` tensors, unchanged; a derivative with respect to any of the tensors raises."""
+
+    @staticmethod
+    def forward(ctx, op, n, *tensors):
+        ctx.op = op
+        return tuple(t.clone() for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.op}: the backward pass cannot be differentiated again")
+
+
+def first_order(op: str):
+    """For the backward pass of a node: under create_graph its gradients are constants whose own derivative raises, as those of
+    the kernels' nodes are.  (``once_differentiable`` leaves them without a history where the incoming gradient has none, so
+    that a sum with other terms loses them without a word.)"""
+    def decorate(backward):
+        @functools.wraps(backward)
+        def run(ctx, *grads):
+            with torch.no_grad():
+                out = backward(ctx, *grads)
+            if not torch.is_grad_enabled():
+                return out
+            got = [t for t in out if t is not None]
+            if not got:
+                return out
+            needs = [t for t in (*ctx.saved_tensors, *grads) if t is not None and t.requires_grad]
+            got = iter(_Constants.apply(op, len(got), *got, *needs))
+            return tuple(None if t is None else next(got) for t in out)
+
+        return run
+
+    return decorate
+
+
 def _ext_probs(q, k, bias, lengths):
     """fp32 softmax probabilities ``[B, H, Sq, Sk]`` over the first ``lengths[b]`` keys; rows without a key are zero"""
     s = torch.matmul(q, k.transpose(2, 3)) * q.shape[-1] ** -0.5
@@ -370,7 +408,7 @@ class GatedResidualNorm(torch.autograd.Function):
         return gated_norm_fwd(x, branch, gate, weight, bias, post_weight, post_bias, eps, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order("gated_residual_norm")
     def backward(ctx, dnew, dnormed):
         if dnew is None and dnormed is None:
             return (None,) * 9

@@ -1069,7 +1069,7 @@ def test_wrappers_without_memory_are_refused():
             call()
 
 
-@pytest.mark.parametrize("device", [pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
 def test_create_graph_raises_only_for_a_second_derivative(device):
     dev = _dev(device)
     for name, call, (a, b) in _three_calls(dev):
