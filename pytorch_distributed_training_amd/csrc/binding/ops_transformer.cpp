@@ -150,6 +150,11 @@ void check_dense(const Tensor& t, at::IntArrayRef shape, at::ScalarType type, co
     TORCH_CHECK(t.numel() == 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, ": data pointer must be 16-B aligned");
     check_same_device(t, like, name);
 }
+void check_codes(const Tensor& t, long S, const Tensor& like, const char* name) {
+    TORCH_CHECK(is_index(t) && t.is_contiguous() && t.dim() == 1 && t.size(0) == S, name, ": expected ", S, " contiguous integers, got ",
+                t.scalar_type(), " ", t.sizes());
+    check_same_device(t, like, name);
+}
 ExtView view_of(const Tensor& t, int G) {
     return {t.size(0) < 2 ? 0 : (long)t.stride(0), t.size(1) < 2 ? (long)t.size(2) : (long)t.stride(1), make_fastdiv((uint32_t)G)};
 }
@@ -283,14 +288,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> rel_bias_attention_fwd(const Tensor& 
     TORCH_CHECK(NB < (1L << 24) && S < (1L << 29) && heads < 65536, "rel_bias_attention: ", NB, " buckets, ", S, " positions, ", heads,
                 " heads (below 2^24, 2^29 and 2^16)");
     check_dense(table, {NB, heads}, at::kFloat, qkv, "table");
-    check_dense(q_codes, {S}, at::kInt, qkv, "q_codes");
-    check_dense(k_codes, {S}, at::kInt, qkv, "k_codes");
+    check_codes(q_codes, S, qkv, "q_codes");
+    check_codes(k_codes, S, qkv, "k_codes");
     check_dense(bucket_of, {R}, at::kInt, qkv, "bucket_of");
     c10::hip::HIPGuardMasqueradingAsCUDA guard(qkv.device());
     const long Rp = (R + 3) / 4 * 4, Sp = (S + 127) / 128 * 128;
-    Tensor tab = at::empty({heads, Rp}, table.options()), codes = at::empty({2 * Sp + Sp / 8}, q_codes.options());
-    launch_bias_tables(table.data_ptr<float>(), bucket_of.data_ptr<int>(), q_codes.data_ptr<int>(), k_codes.data_ptr<int>(),
-                       tab.data_ptr<float>(), codes.data_ptr<int>(), (int)R, (int)Rp, (int)NB, (int)heads,
+    Tensor tab = at::empty({heads, Rp}, table.options()), codes = at::empty({2 * Sp + Sp / 8}, q_codes.options().dtype(at::kInt));
+    launch_bias_tables(table.data_ptr<float>(), bucket_of.data_ptr<int>(), q_codes.data_ptr(), q_codes.scalar_type() == at::kLong,
+                       k_codes.data_ptr(), k_codes.scalar_type() == at::kLong, tab.data_ptr<float>(), codes.data_ptr<int>(), (int)R, (int)Rp, (int)NB, (int)heads,
                        (int)S, (int)Sp, (float)std::sqrt((double)hd), stream_of(qkv));
     const Tensor q = qkv.narrow(2, 0, D), k = qkv.narrow(2, D, D), v = qkv.narrow(2, 2 * D, D);
     ExtArgs a = ext_args(q, k, v, heads, heads, lens, hd, true);
@@ -322,7 +327,7 @@ struct RelBiasFn : torch::autograd::Function<RelBiasFn> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& qkv_, const Tensor& table_, const Tensor& q_codes,
                           const Tensor& k_codes, const Tensor& bucket_of_, const OptTensor& lens_, int64_t heads) {
         const Tensor qkv = rows3(qkv_), bucket_of = int32(bucket_of_), lens = given(lens_) ? int32(*lens_) : Tensor();
-        auto [out, stat, tab, codes] = rel_bias_attention_fwd(qkv, param32(table_), int32(q_codes), int32(k_codes), bucket_of, heads, opt(lens), true);
+        auto [out, stat, tab, codes] = rel_bias_attention_fwd(qkv, param32(table_), q_codes.contiguous(), k_codes.contiguous(), bucket_of, heads, opt(lens), true);
         ctx->save_for_backward({qkv, out, stat, tab, codes, bucket_of, lens});
         ctx->set_materialize_grads(false);
         ctx->saved_data["heads"] = heads;
@@ -358,7 +363,7 @@ OptTensor rel_bias_attention(const Tensor& qkv, const Tensor& table, const Tenso
     if (table.device() != qkv.device()) return {};
     check_plain("rel_bias_attention", {&qkv, &table, &q_codes, &k_codes, &bucket_of, given(lens) ? &*lens : &qkv});
     if (!wants_grad({&qkv, &table}))
-        return std::get<0>(rel_bias_attention_fwd(rows3(qkv), param32(table), int32(q_codes), int32(k_codes), int32(bucket_of), heads,
+        return std::get<0>(rel_bias_attention_fwd(rows3(qkv), param32(table), q_codes.contiguous(), k_codes.contiguous(), int32(bucket_of), heads,
                                                   given(lens) ? opt(int32(*lens)) : lens, false));
     check_capture({&qkv, &table});
     return RelBiasFn::apply(qkv, table, q_codes, k_codes, bucket_of, lens, heads);

@@ -50,8 +50,9 @@ long ext_ends(const ExtArgs& a, const ExtPlan& q);
 void launch_ext_fwd(const ExtArgs& a, const ExtPlan& p, int hd, void* out, float* stat, float* part, float* part_ml,
                     hipStream_t s);
 void launch_ext_bwd(const ExtArgs& a, const ExtBwd& w, int hd, hipStream_t s);
-// codes [2 Sp + 4 Sp / 32]
-void launch_bias_tables(const float* table, const int* bucket_of, const int* q_codes, const int* k_codes, float* tab, int* codes, int R, int Rp, int NB, int H, int S, int Sp, float inv_scale, hipStream_t s);
+// codes [2 Sp + 4 Sp / 32]; position codes of 64 bits (wide) or 32
+void launch_bias_tables(const float* table, const int* bucket_of, const void* q_codes, bool q_wide, const void* k_codes, bool k_wide,
+                        float* tab, int* codes, int R, int Rp, int NB, int H, int S, int Sp, float inv_scale, hipStream_t s);
 // the bias table's gradient: after launch_ext_bwd (which leaves D in dsum)
 struct RelBlocks {
     int h0, heads, q0, qblocks, kblocks;  // of this launch: heads, blocks of 128 queries; blocks of 128 keys of all

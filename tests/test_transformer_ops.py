@@ -1091,3 +1091,40 @@ def test_create_graph_raises_only_for_a_second_derivative(device):
                 got = torch.autograd.grad(loss(), [x, y], create_graph=True)
                 with pytest.raises(RuntimeError):
                     ask(got[i])
+
+
+@gpu
+@pytest.mark.parametrize("base", [2 ** 27, 2 ** 31 - 400, -2 ** 31, 1_765_000_000_000, -2 ** 62])
+def test_rel_bias_codes_of_any_size(base):
+    """Only differences count: positions that count from far away (clocks) give the bits of those that count from zero."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(43)
+    qc, kc, of = (t.to(dev).long() for t in _log(150))
+    qkv, w = _rand(g, 2, 150, 384, device=dev), _rand(g, 2, 150, 128, device=dev)
+    table = _rand(g, 8, 2, dtype=torch.float32, device=dev)
+
+    def run(q, k):
+        a, t = qkv.clone().requires_grad_(), table.clone().requires_grad_()
+        out = F.rel_bias_attention(a, t, q, k, of, 2)
+        return (out, *torch.autograd.grad(out, [a, t], w))
+
+    want = run(qc, kc)
+    assert all(torch.equal(x, y) for x, y in zip(want, run(qc.int(), kc)))
+    q, k = qc + base, kc + base
+    forms = [(q, k)] if max(abs(base), abs(base + 400)) >= 2 ** 31 and base != -2 ** 31 else [(q, k), (q.int(), k.int()), (q, k.int())]
+    for f in forms:
+        assert all(torch.equal(x, y) for x, y in zip(want, run(*f)))
+    strided = torch.stack([q, q + 1], 1)[:, 0]
+    assert all(torch.equal(x, y) for x, y in zip(want, run(strided, k)))
+    # apart from the first key by almost 2^27: the far token is past the table's reach; by more: no number at all
+    q2, k2 = q.clone(), k.clone()
+    k2[-1] = k2[0] - 1 + 2 ** 27
+    got = run(q2, k2)
+    bucket = of[(qc[:, None] - (k2 - base)[None]).clamp(0, of.numel() - 1)]
+    bias = table.double()[bucket].permute(2, 0, 1)
+    x, y, v = qkv.double().view(2, 150, 3, 2, 64).permute(2, 0, 3, 1, 4)
+    (o, *_), (e, *_) = _attention64(x, y, v, bias, _live(None, 2, 150, dev), torch.ones(2, 150, device=dev).double(), torch.zeros_like(x))
+    _within(got[0], o.transpose(1, 2).reshape(2, 150, 128), e.transpose(1, 2).reshape(2, 150, 128), "out")
+    k2[-1] += 1
+    out, dqkv, dtable = run(q2, k2)
+    assert out.isnan().all() and dqkv.isnan().all() and dtable.isnan().any()  # (a bucket that no pair falls on keeps its zero)
