@@ -194,12 +194,15 @@ __device__ __forceinline__ Job job_of(const ExtArgs& a, int tiles, int splits) {
     return j;
 }
 
-// the row's statistics; where nothing was attended to, -log2 l = -inf makes every P of the backward zero.  Where l was summed
-// from 2^(c s + base) with base = -c m rounded, `rounding` = c m + base goes into log2 l
-__device__ __forceinline__ void put_stat(const ExtArgs& a, float* stat, long at, bool some, float m, float l, float rounding) {
+// the row's statistics; where nothing was attended to, -log2 l = -inf makes every P of the backward zero
+__device__ __forceinline__ void put_stat(const ExtArgs& a, float* stat, long at, bool some, float m, float l) {
     stat[at] = some ? -m : 0.f;
-    stat[a.stat_n + at] = some ? rounding - __builtin_amdgcn_logf(l) : -kInf;
+    stat[a.stat_n + at] = some ? -__builtin_amdgcn_logf(l) : -kInf;
 }
+// The exponents of a sweep are c s + base with base = -c m, rounded: l and O are 2^off times what they are for the m that is handed
+// on, off = c m + base (2^-15 at scores of 500).  Where m grows, the old sums go to the new off; at the end off is taken out, so that
+// parts can be joined and the backward's P add up to 1.
+__device__ __forceinline__ float sweep_end(float m, float off) { return m == -kInf ? 1.f : __builtin_amdgcn_exp2f(-off); }
 
 template <int HD>
 __device__ __forceinline__ void own_frags(bf16x8* f, const bf16* p, bool live, int half) {
@@ -243,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
     for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
-    float m = -kInf, l = 0.f, base = 0.f;
+    float m = -kInf, l = 0.f, off = 0.f;
 
     if (any) {
         const bf16* kbase = a.k + (long)j.b * a.kv.bs + (long)j.hkv * HD;
@@ -304,9 +307,12 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
             }
             mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
             const float mx = mb == -kInf ? 0.f : mb;  // (every key so far forbidden: m counts as 0, all P are 0)
-            base = -mx * a.c;
+            // one multiply-add a score, but for a bias of, say, -1e9 over a whole row: its product leaves nothing of the scores
+            const bool large = BIAS && !__all(fabsf(mx) < 65536.f);
+            const float base = large ? 0.f : -mx * a.c;
             if (__any(mb > m)) {
-                const float alpha = __builtin_amdgcn_exp2f((m - mx) * a.c);
+                const float now = large ? 0.f : fmaf(mx, a.c, base), alpha = __builtin_amdgcn_exp2f(fmaf(m - mx, a.c, now - off));
+                off = now;
                 l *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < G::DT; ++dt)
@@ -314,13 +320,11 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
                     for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
                 m = mb;
             }
-            // one multiply-add a score, but for a bias of, say, -1e9 over a whole row: its product leaves nothing of the scores
-            if (BIAS && !__all(fabsf(mx) < 65536.f)) {
+            if (large) {
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) st[kt][i] -= mx;
-                base = 0.f;
             }
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
@@ -342,7 +346,8 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
             }
         }
     }
-    l += __shfl_xor(l, 32, 64);
+    const float end = sweep_end(m, off);
+    l = (l + __shfl_xor(l, 32, 64)) * end;
     if (splits > 1) {
         if (r < a.M) {
             const long at = ((long)j.bh * splits + j.split) * a.M + r;
@@ -352,7 +357,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
                 for (int jj = 0; jj < 4; ++jj) {
                     f32x4 t;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) t[e] = o[dt][4 * jj + e];
+                    for (int e = 0; e < 4; ++e) t[e] = o[dt][4 * jj + e] * end;
                     *reinterpret_cast<f32x4*>(part + at * HD + dt * 32 + 8 * jj + 4 * half) = t;
                 }
             if (half == 0) {
@@ -362,8 +367,8 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
         }
         return;
     }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    if (stat && half == 0 && r < a.Mp) put_stat(a, stat, (long)j.bh * a.Mp + r, live && (l > 0.f || l != l), m, l, BIAS && base == 0.f ? 0.f : fmaf(m, a.c, base));
+    const float inv = l > 0.f || l != l ? end / l : 0.f;
+    if (stat && half == 0 && r < a.Mp) put_stat(a, stat, (long)j.bh * a.Mp + r, live && (l > 0.f || l != l), m, l);
     if (r < a.M) {
 #pragma unroll
         for (int dt = 0; dt < G::DT; ++dt)
@@ -411,7 +416,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
     for (int dt = 0; dt < G::DT; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
-    float m = -kInf, l = 0.f;
+    float m = -kInf, l = 0.f, off = 0.f;
     int buf = 0;
     if (t0 + wave < t1) issue(t0 + wave, 0);  // (before the rows: 8.5 us for 9.5 on 8 x 12 heads of up to 1500 keys)
     bf16x8 bq[G::STEPS];
@@ -446,7 +451,8 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
         mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
         const float base = -mb * a.c;
         if (__any(mb > m)) {
-            const float alpha = __builtin_amdgcn_exp2f(fmaf(m, a.c, base));
+            const float now = fmaf(mb, a.c, base), alpha = __builtin_amdgcn_exp2f(fmaf(m - mb, a.c, now - off));
+            off = now;
             l *= alpha;
 #pragma unroll
             for (int dt = 0; dt < G::DT; ++dt)
@@ -467,7 +473,8 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
                 o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(G::cols(Vs, blk * 16, dt * 32, lane), p, o[dt], 0, 0, 0);
         }
     }
-    l += __shfl_xor(l, 32, 64);
+    const float end = sweep_end(m, off);
+    l = (l + __shfl_xor(l, 32, 64)) * end;
     // the waves' (m, l, O) through LDS, over their rings
     float* ml = reinterpret_cast<float*>(smem + 8 * STAGE);
     if (half == 0) {
@@ -484,7 +491,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
             for (int jj = 0; jj < 4; ++jj) {
                 f32x4 t;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t[e] = o[dt][4 * jj + e];
+                for (int e = 0; e < 4; ++e) t[e] = o[dt][4 * jj + e] * end;
                 *reinterpret_cast<f32x4*>(acc + l31 * HD + dt * 32 + 8 * jj + 4 * half) = t;
             }
     }
@@ -516,11 +523,11 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
 #pragma unroll
             for (int e = 0; e < 4; ++e) w4[e] = (bf16)(t[e] * inv);
             *reinterpret_cast<bf16x4*>(out + (long)j.b * a.o.bs + row_offset(a.o, r, j.hkv, a.G, HD) + d) = w4;
-            if (stat && d == 0) put_stat(a, stat, (long)j.bh * a.Mp + r, j.len > 0, mx, sum, 0.f);
+            if (stat && d == 0) put_stat(a, stat, (long)j.bh * a.Mp + r, j.len > 0, mx, sum);
         }
     }
     if (stat && splits == 1)
-        for (int r = a.M + tid; r < a.Mp; r += 256) put_stat(a, stat, (long)j.bh * a.Mp + r, false, 0.f, 0.f, 0.f);
+        for (int r = a.M + tid; r < a.Mp; r += 256) put_stat(a, stat, (long)j.bh * a.Mp + r, false, 0.f, 0.f);
 }
 
 // (m, l, O) of the splits -> out (and stat).  HD / 4 lanes take a row's channels.  MANY: a workgroup has one row, and 1024 / HD
@@ -539,7 +546,7 @@ __global__ __launch_bounds__(256) void k_ext_join(ExtArgs a, const float* __rest
     const long at0 = (long)bh * splits * a.M + r;
     if (stat && r == a.M - 1)  // padding rows of the statistics
         for (int i = a.M + (MANY ? (int)threadIdx.x : d >> 2); i < a.Mp; i += MANY ? 256 : W)
-            put_stat(a, stat, (long)bh * a.Mp + i, false, 0.f, 0.f, 0.f);
+            put_stat(a, stat, (long)bh * a.Mp + i, false, 0.f, 0.f);
     float mx = -kInf, sum = 0.f;
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) mx = fmaxf(mx, part_ml[2 * (at0 + (long)s * a.M)]);
@@ -582,7 +589,7 @@ __global__ __launch_bounds__(256) void k_ext_join(ExtArgs a, const float* __rest
 #pragma unroll
     for (int e = 0; e < 4; ++e) w4[e] = (bf16)(some ? t[e] * inv : 0.f);
     *reinterpret_cast<bf16x4*>(out + o) = w4;
-    if (stat && d == 0) put_stat(a, stat, (long)bh * a.Mp + r, some, mx, sum, 0.f);
+    if (stat && d == 0) put_stat(a, stat, (long)bh * a.Mp + r, some, mx, sum);
 }
 
 // ------------------------------------------------------------------------------------------------------- backward

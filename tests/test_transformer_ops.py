@@ -1128,3 +1128,51 @@ def test_rel_bias_codes_of_any_size(base):
     k2[-1] += 1
     out, dqkv, dtable = run(q2, k2)
     assert out.isnan().all() and dqkv.isnan().all() and dtable.isnan().any()  # (a bucket that no pair falls on keeps its zero)
+
+
+@gpu
+@pytest.mark.parametrize("case", [dict(b=1, n=600, heads=2), dict(b=2, n=300, heads=2), dict(b=1, n=1100, heads=1)], ids=lambda c: f"b{c['b']}-n{c['n']}-h{c['heads']}")
+def test_rel_bias_table_gradient_at_large_scores(case):
+    """Scores of some 500, launches whole and split: the weights of the backward add up to 1, not to what the rounding of
+    log2(e) * maximum makes of them.  q . k is the same for all pairs and the bias grows towards the query's own position, so
+    that all rows have one maximum (and one rounding, which would not average out), and parts of the keys have smaller ones."""
+    dev = _dev("cuda")
+    b, n, heads, hd = case["b"], case["n"], case["heads"], 64
+    c = torch.tensor(math.log2(math.e) / 8, dtype=torch.float32)
+
+    def off(t):  # of the exponents' base where the maximum is (512 + t) * 8
+        m = torch.tensor((512 + t) * 8, dtype=torch.float32)
+        return float(c.double() * m.double() - (c * m).double())
+
+    steps = [max((k / 16 + 0.25 * j for j in range(4)), key=lambda t: abs(off(t))) for k in range(0, 128, 16)]  # one of each unit
+    assert max(abs(off(t)) for t in steps) > 2.0 ** -16
+    qc, kc, of = (t.to(dev) for t in _log(n))
+    near = torch.zeros(8)  # buckets of _log: 0 the same place, 1 to 3 behind it, 4 (never), 5 to 7 ahead
+    near[[0, 1, 2, 3, 5, 6, 7]] = torch.tensor([steps[7], steps[5], steps[3], steps[1], steps[6], steps[4], steps[2]])
+    table = near[:, None].repeat(1, heads).to(dev).requires_grad_()
+    qkv = torch.zeros(b, n, 3, heads, hd)
+    qkv[:, :, :2, :, 0] = 64  # 512 of every score
+    turn = torch.arange(n) * (math.pi / 24)  # dP = cos of the distance: near pairs and far ones get dS of one sign each
+    wave = torch.stack([turn.cos(), turn.sin()], -1)[None, :, None]
+    qkv[:, :, 2, :, :2] = wave
+    do = torch.zeros(b, n, heads, hd)
+    do[..., :2] = wave
+    flat, do = (t.reshape(b, n, -1).to(torch.bfloat16).to(dev) for t in (qkv, do))
+    out = F.rel_bias_attention(flat, table, qc, kc, of, heads)
+    (got,) = torch.autograd.grad(out, table, do)
+    q, k, v = flat.double().view(b, n, 3, heads, hd).permute(2, 0, 3, 1, 4)
+    bucket = of.long()[(qc.long()[:, None] - kc.long()[None]).clamp(0, of.numel() - 1)]
+    s = q @ k.transpose(-1, -2) * hd ** -0.5 + table.detach().double()[bucket].permute(2, 0, 1)
+    p = torch.softmax(s, -1)
+    do4 = do.double().view(b, n, heads, hd).transpose(1, 2)
+    dp = do4 @ v.transpose(-1, -2)
+    d = (p * dp).sum(-1, keepdim=True)
+
+    def by_bucket(t):
+        z = torch.zeros(8, heads, dtype=torch.float64, device=dev)
+        return z.index_add_(0, bucket.reshape(-1), t.sum(0).reshape(heads, -1).t().contiguous())
+
+    # the scores are exact (multiples of 2^-4 below 2^10).  P: an exponential (2^-23), a logarithm (of a sum below 2^11: 11 * 2^-24)
+    # and c (2^-25 of an exponent below 2^4); dP has two terms; a sum over up to 2^11 keys, 2^6 sequential additions: 2^-20 covers them
+    err = 2.0 ** -20 * p * (dp.abs() + d.abs() + 2)
+    _within(got, by_bucket(p * (dp - d)), by_bucket(err), "dtable")
