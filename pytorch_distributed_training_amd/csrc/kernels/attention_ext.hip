@@ -449,9 +449,9 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
 #pragma unroll
         for (int i = 0; i < 16; ++i) mb = fmaxf(mb, st[i]);
         mb = fmaxf(mb, __shfl_xor(mb, 32, 64));
-        const float base = -mb * a.c;
+        const float mx = mb == -kInf ? 0.f : mb, base = -mx * a.c;  // (every score so far -inf: m counts as 0, all P are 0)
         if (__any(mb > m)) {
-            const float now = fmaf(mb, a.c, base), alpha = __builtin_amdgcn_exp2f(fmaf(m - mb, a.c, now - off));
+            const float now = fmaf(mx, a.c, base), alpha = __builtin_amdgcn_exp2f(fmaf(m - mx, a.c, now - off));
             off = now;
             l *= alpha;
 #pragma unroll
@@ -518,12 +518,13 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restr
                 part_ml[2 * at + 1] = sum;
             }
         } else {
-            const float inv = j.len > 0 ? 1.f / sum : 0.f;
+            const bool some = sum > 0.f || sum != sum;
+            const float inv = some ? 1.f / sum : 0.f;
             bf16x4 w4;
 #pragma unroll
             for (int e = 0; e < 4; ++e) w4[e] = (bf16)(t[e] * inv);
             *reinterpret_cast<bf16x4*>(out + (long)j.b * a.o.bs + row_offset(a.o, r, j.hkv, a.G, HD) + d) = w4;
-            if (stat && d == 0) put_stat(a, stat, (long)j.bh * a.Mp + r, j.len > 0, mx, sum);
+            if (stat && d == 0) put_stat(a, stat, (long)j.bh * a.Mp + r, some, mx, sum);
         }
     }
     if (stat && splits == 1)

@@ -1176,3 +1176,26 @@ def test_rel_bias_table_gradient_at_large_scores(case):
     # and c (2^-25 of an exponent below 2^4); dP has two terms; a sum over up to 2^11 keys, 2^6 sequential additions: 2^-20 covers them
     err = 2.0 ** -20 * p * (dp.abs() + d.abs() + 2)
     _within(got, by_bucket(p * (dp - d)), by_bucket(err), "dtable")
+
+
+@gpu
+@pytest.mark.parametrize("case", [dict(nq=1, nk=200), dict(nq=1, nk=3000), dict(nq=40, nk=200), dict(nq=40, nk=1500)], ids=lambda c: f"{c['nq']}x{c['nk']}")
+def test_cross_attention_scores_of_minus_infinity(case):
+    """Keys with an infinite channel whose scores are -inf weigh nothing, whole tiles of them too; all keys so: zeros."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(53)
+    nq, nk, heads, hd = case["nq"], case["nk"], 2, 64
+    q, kv = _rand(g, 2, nq, heads * hd, device=dev), _rand(g, 2, nk, 2 * heads * hd, device=dev)
+    q.view(2, nq, heads, hd)[..., 0] = 1
+    key0 = kv.view(2, nk, 2, heads, hd)[:, :, 0, :, 0]
+    key0[0, :nk - 40] = -math.inf
+    key0[0, 100:110] = 0.5
+    key0[1] = -math.inf
+    out = F.cross_attention(q, kv, heads)
+    live = (key0[0, :, 0] > -math.inf).expand(2, nk)
+    q4 = q.double().view(2, nq, heads, hd).transpose(1, 2)
+    k4, v4 = kv.double().view(2, nk, 2, heads, hd).permute(2, 0, 3, 1, 4)
+    k4 = k4.nan_to_num(neginf=0.0)
+    (o, *_), (e, *_) = _attention64(q4, k4, v4, None, live, torch.ones(2, nq, device=dev).double(), torch.zeros_like(q4))
+    _within(out[:1], o[:1].transpose(1, 2).reshape(1, nq, -1), e[:1].transpose(1, 2).reshape(1, nq, -1), "out")
+    assert not out[1].any()
