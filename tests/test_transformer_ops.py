@@ -1199,3 +1199,24 @@ def test_cross_attention_scores_of_minus_infinity(case):
     (o, *_), (e, *_) = _attention64(q4, k4, v4, None, live, torch.ones(2, nq, device=dev).double(), torch.zeros_like(q4))
     _within(out[:1], o[:1].transpose(1, 2).reshape(1, nq, -1), e[:1].transpose(1, 2).reshape(1, nq, -1), "out")
     assert not out[1].any()
+
+
+@gpu
+def test_gated_residual_norm_with_a_gate_for_each_of_many_rows():
+    dev = _dev("cuda")
+    n, d = (1 << 23) + 1, 4
+    x = torch.randn(n, d, device=dev, generator=torch.Generator(dev).manual_seed(59)).to(torch.bfloat16).requires_grad_()
+    y = x.detach().flip(0).requires_grad_()
+    gate = torch.linspace(-1, 1, n, device=dev)[:, None].repeat(1, d).requires_grad_()
+    w, b = torch.full((d,), 1.5, device=dev, requires_grad=True), torch.zeros(d, device=dev, requires_grad=True)
+    u, normed = F.gated_residual_norm(x, y, gate, w, b)
+    got = torch.autograd.grad(u, [x, y, gate], torch.ones_like(u), retain_graph=True)
+    assert torch.equal(got[0], torch.ones_like(x)) and torch.equal(got[1], gate.to(torch.bfloat16)) and torch.equal(got[2], y.float())
+    (db,) = torch.autograd.grad(normed, b, torch.ones_like(normed))
+    assert ((db - n).abs() <= 2.0 ** -10 * n).all()  # 2^14 rows a workgroup in one 32-bit sum each, all terms 1
+    # the last rows of all against the form in 64 bits
+    last = slice(n - 5, n)
+    u64 = x[last].double() + gate[last].double() * y[last].double()
+    n64 = torch.nn.functional.layer_norm(u64, (d,), w.double(), b.double(), 1e-6).detach()
+    # (four channels: 2^-20 of what a division by a deviation of at least 2^-6 leaves)
+    assert (n64 - normed[last].double()).abs().max() <= U * n64.abs().max() + 2.0 ** -14
