@@ -394,8 +394,9 @@ def gated_norm_bwd(dnew, dnormed, x, branch, gate, weight, bias, post_weight, po
     rows = tuple(range(x.dim() - 1))
     dz = du * g
     dy = dz if post_weight is None else norm_grad(dz * post_weight.to(f), yh, yr)
-    grads = [(scale * du).to(x.dtype), dy.to(x.dtype), (du * z).sum(rows if gate.dim() == 1 else rows[1:]), (dn * nh).sum(rows),
-             dn.sum(rows)]
+    own = rows if gate.dim() == 1 else rows[1:]
+    dgate = (du * z).sum(own) if own else du * z  # (a gate for every row: a sum over no dimension would take them all)
+    grads = [(scale * du).to(x.dtype), dy.to(x.dtype), dgate, (dn * nh).sum(rows), dn.sum(rows)]
     return grads if post_weight is None else grads + [(dz * yh).sum(rows), dz.sum(rows)]
 
 

@@ -1220,3 +1220,16 @@ def test_gated_residual_norm_with_a_gate_for_each_of_many_rows():
     n64 = torch.nn.functional.layer_norm(u64, (d,), w.double(), b.double(), 1e-6).detach()
     # (four channels: 2^-20 of what a division by a deviation of at least 2^-6 leaves)
     assert (n64 - normed[last].double()).abs().max() <= U * n64.abs().max() + 2.0 ** -14
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_gated_residual_norm_with_a_gate_for_each_row(device):
+    """``x`` of two dimensions: the gate's first is the rows."""
+    _check_norm(_dev(device), (37, 64), True, True, 0.5)
+    _check_norm(_dev(device), (37, 64), True, False, 1.0)
+
+
+def test_gated_residual_norm_oracle_with_a_gate_for_each_row_against_differences():
+    g = torch.Generator().manual_seed(61)
+    x, y, gate, w, b, pw, pb = (torch.randn(*s, generator=g, dtype=torch.float64, requires_grad=True) for s in ((3, 8),) * 3 + ((8,),) * 4)
+    assert torch.autograd.gradcheck(lambda *t: F.gated_residual_norm(*t[:5], 1e-6, *t[5:], 0.5), (x, y, gate, w, b, pw, pb))
