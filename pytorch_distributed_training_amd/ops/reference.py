@@ -310,14 +310,14 @@ def rel_bias_attention_bwd(dout, qkv, table, q_codes, k_codes, bucket_of, heads:
     q, k, v = _rel_parts(qkv, heads, lengths)
     bucket, buckets = _rel_buckets(q_codes, k_codes, bucket_of), table.shape[0]
     p, real = _rel_probs(q, k, table, bucket, lengths)
-    do = _no_dead_rows(dout.to(q.dtype).view(b, s, heads, -1).transpose(1, 2), lengths)
+    do = _no_dead_rows(dout.to(q.dtype).view(b, s, heads, w // (3 * heads)).transpose(1, 2), lengths)
     dq, dk, dv, ds = _ext_grads(do, q, k, v, p)
     dqkv = torch.stack([dq, dk, dv]).permute(1, 3, 0, 2, 4).reshape(b, s, w).to(qkv.dtype)
     if not want_table:
         return dqkv, None
     dtable = torch.zeros((buckets, heads), dtype=q.dtype, device=q.device)
     if buckets:
-        by_pair = (ds.sum(0) * real).view(heads, -1).t()
+        by_pair = (ds.sum(0) * real).view(heads, s * s).t()
         dtable.index_add_(0, bucket.clamp(0, buckets - 1).reshape(-1), by_pair.contiguous())
     return dqkv, dtable
 
@@ -326,7 +326,7 @@ def _cross_parts(q, kv, heads, kv_heads, lengths):
     b, sq, w = q.shape
     hd = w // heads
     f = _work_type(q)
-    qf = q.to(f).view(b, sq, kv_heads, heads // kv_heads, hd).permute(0, 2, 3, 1, 4).reshape(b, kv_heads, -1, hd)
+    qf = q.to(f).view(b, sq, kv_heads, heads // kv_heads, hd).permute(0, 2, 3, 1, 4).reshape(b, kv_heads, heads // kv_heads * sq, hd)
     k, v = kv.to(f).view(b, kv.shape[1], 2, kv_heads, hd).permute(2, 0, 3, 1, 4).unbind(0)
     return qf, _no_dead_rows(k, lengths), _no_dead_rows(v, lengths)
 
@@ -345,11 +345,10 @@ def cross_attention_fwd(q, kv, heads: int, kv_heads: int, lengths=None):
 
 def cross_attention_bwd(dout, q, kv, heads: int, kv_heads: int, lengths=None):
     """-> (dq, dkv)"""
-    b, sk = kv.shape[:2]
     qf, k, v = _cross_parts(q, kv, heads, kv_heads, lengths)
     do = _cross_parts(dout, kv, heads, kv_heads, None)[0]
     dq, dk, dv, _ = _ext_grads(do, qf, k, v, _ext_probs(qf, k, None, lengths))
-    dkv = torch.stack([dk, dv]).permute(1, 3, 0, 2, 4).reshape(b, sk, -1).to(kv.dtype)
+    dkv = torch.stack([dk, dv]).permute(1, 3, 0, 2, 4).reshape(kv.shape).to(kv.dtype)
     return _cross_rows(dq, q, heads, kv_heads), dkv
 
 

@@ -1233,3 +1233,33 @@ def test_gated_residual_norm_oracle_with_a_gate_for_each_row_against_differences
     g = torch.Generator().manual_seed(61)
     x, y, gate, w, b, pw, pb = (torch.randn(*s, generator=g, dtype=torch.float64, requires_grad=True) for s in ((3, 8),) * 3 + ((8,),) * 4)
     assert torch.autograd.gradcheck(lambda *t: F.gated_residual_norm(*t[:5], 1e-6, *t[5:], 0.5), (x, y, gate, w, b, pw, pb))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_no_sequences_no_queries_no_keys(device):
+    dev = _dev(device)
+    g = torch.Generator().manual_seed(67)
+
+    def leaf(*s, dtype=torch.bfloat16):
+        return _rand(g, *s, dtype=dtype, device=dev).requires_grad_()
+
+    for b, nq, nk in ((0, 3, 4), (2, 0, 4), (2, 3, 0), (0, 0, 0), (2, 0, 0)):
+        for lens in (None, torch.full((b,), 1, device=dev)):
+            q, kv = leaf(b, nq, 128), leaf(b, nk, 128)
+            out = F.cross_attention(q, kv, 4, 2, lens)
+            got = torch.autograd.grad(out, [q, kv], torch.ones_like(out))
+            assert out.shape == q.shape and got[0].shape == q.shape and got[1].shape == kv.shape
+            assert not any(t.any() for t in (out, *got) if nk == 0 or nq == 0)
+    for b, n in ((0, 3), (2, 0), (0, 0)):
+        for lens in (None, torch.full((b,), 1, device=dev)):
+            qkv, table = leaf(b, n, 192), leaf(8, 2, dtype=torch.float32)
+            out = F.rel_bias_attention(qkv, table, *(t.to(dev) for t in _log(n)), 2, lens)
+            got = torch.autograd.grad(out, [qkv, table], torch.ones_like(out))
+            assert out.shape == (b, n, 64) and got[0].shape == qkv.shape and got[1].shape == table.shape and not got[1].any()
+    for shape in ((0, 8), (0, 3, 8), (3, 0, 8)):
+        for gate in (leaf(8, dtype=torch.float32), leaf(shape[0], 8, dtype=torch.float32)):
+            x, w = leaf(*shape), leaf(8, dtype=torch.float32)
+            new, normed = F.gated_residual_norm(x, x, gate, w, w, 1e-6, w, w)
+            got = torch.autograd.grad([new, normed], [x, gate, w], [torch.ones_like(x)] * 2)
+            assert new.shape == normed.shape == x.shape and got[0].shape == x.shape and got[1].shape == gate.shape
+            assert not any(t.any() for t in got)
