@@ -6,8 +6,8 @@
 
 namespace pdt {
 
-// entries of a relative-position table that a head keeps in LDS: 16 KiB beside 64 of keys at head_dim 128, so that a CU still holds
-// two workgroups; four histograms of the gradient are 64 KiB
+// entries of a relative-position table that a head keeps in LDS: 16 KiB beside 66 of keys and codes at head_dim 128, where a CU's 160
+// hold two workgroups up to 3584 entries and one above; four histograms of the gradient are 64 KiB
 constexpr int kExtMaxEntries = 4096;
 
 // rows of a [B, rows, heads, hd] tensor: element strides, and the division of a row by the heads that share a key head
