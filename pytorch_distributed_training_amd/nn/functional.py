@@ -585,7 +585,8 @@ def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, leng
     ``lengths`` (``[B]`` integers, on the device of ``qkv``): sequence ``b`` is its first ``lengths[b]`` tokens; the rows behind
     it are neither attended to nor read, their outputs and gradients are zero, and so is a row whose every key is forbidden.
     On bf16 GPU tensors with head_dim 32 / 64 / 128 and at most 4096 entries the HIP kernels of csrc/kernels/attention_ext.hip run;
-    the PyTorch oracle elsewhere."""
+    the PyTorch oracle elsewhere (and its ``[B, H, S, S]`` scores).  The table's gradient takes a workspace of up to 1 GiB (sums of dS over
+    the batch, 4 bytes a pair and head; more pairs go in groups) and 4 * heads * len(bucket_of) bytes for every 32 tokens."""
     heads = int(heads)
     be = backend_for(qkv)
     if be is not reference:

@@ -1263,3 +1263,36 @@ def test_no_sequences_no_queries_no_keys(device):
             got = torch.autograd.grad([new, normed], [x, gate, w], [torch.ones_like(x)] * 2)
             assert new.shape == normed.shape == x.shape and got[0].shape == x.shape and got[1].shape == gate.shape
             assert not any(t.any() for t in got)
+
+
+@gpu
+@pytest.mark.parametrize("case", [dict(n=4000, heads=17, far=2047), dict(n=4200, heads=16, far=16), dict(n=16500, heads=1, far=16),
+                                  dict(n=16500, heads=2, far=16)], ids=lambda c: f"n{c['n']}-h{c['heads']}-far{c['far']}")
+def test_rel_bias_table_gradient_in_groups(case):
+    """More than 1 GiB of sums over pairs: groups of heads (16 + 1, 15 + 1) and blocks of queries (127 + 2 of 128), each both with
+    the far pairs summed by the dQ pass (more positions than entries, dQ in one part) and without."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(71)
+    n, heads, hd = case["n"], case["heads"], 32
+    qc, kc, of = (t.to(dev) for t in _log(n, case["far"], 8))
+    qkv, do = _rand(g, 1, n, 3 * heads * hd, device=dev), _rand(g, 1, n, heads * hd, std=0.1, device=dev)
+    table = _rand(g, 8, heads, dtype=torch.float32, device=dev).requires_grad_()
+    out = F.rel_bias_attention(qkv, table, qc, kc, of, heads)
+    (got,) = torch.autograd.grad(out, table, do)
+    want, bound = (torch.zeros(8, heads, dtype=torch.float64, device=dev) for _ in range(2))
+    for h in range(heads):
+        q, k, v = qkv.view(n, 3, heads, hd)[:, :, h].double().unbind(1)
+        w = do.view(n, heads, hd)[:, h].double()
+        for rows in torch.arange(n, device=dev).split(2048):
+            bucket = of.long()[(qc[rows, None] - kc[None]).clamp(0, of.numel() - 1).long()]
+            p = torch.softmax(q[rows] @ k.t() * hd ** -0.5 + table.detach()[bucket, h].double(), -1)
+            o, dp, x = p @ v, w[rows] @ v.t(), w[rows]
+            ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+            # the bound of `_check_rel`
+            err = p * (2.0 ** -15 * (x.abs() * (o.abs() + p @ v.abs())).sum(-1, keepdim=True) + SLACK / 8 * (x.abs() @ v.abs().t()))
+            err += 2.0 ** -20 * ds.abs()
+            for i in range(8):
+                here = (bucket == i).double()
+                want[i, h] += (ds * here).sum()
+                bound[i, h] += (err * here).sum()
+    _within(got, want, bound, "dtable")
