@@ -168,7 +168,11 @@ def log_position_buckets(length: int, buckets: int = 32, far: int = 128, bidirec
     """``(q_codes, k_codes, bucket_of)`` for ``functional.rel_bias_attention`` on ``length`` positions in a row: with
     ``bidirectional`` half of the ``buckets`` for keys behind the query's position and half for those after it, else all for
     those behind (a key after it is in bucket 0).  Of those for one side, the first half are one distance each and the others
-    grow logarithmically up to ``far``, past which the last one holds."""
+    grow logarithmically up to ``far``, past which the last one holds.
+
+    The buckets alone forbid nothing: keys after the query are attended to as those of bucket 0 are.  For a decoder, which must not,
+    give their entries a bucket of their own, ``bucket_of[:far] = buckets``, and the table a last row of -inf for it
+    (``torch.cat([table, table.new_full((1, heads), -math.inf)])``)."""
     sides = buckets // 2 if bidirectional else buckets
     exact = sides // 2
     if length < 0 or exact < 1 or far <= exact:

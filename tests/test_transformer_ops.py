@@ -1296,3 +1296,31 @@ def test_rel_bias_table_gradient_in_groups(case):
                 want[i, h] += (ds * here).sum()
                 bound[i, h] += (err * here).sum()
     _within(got, want, bound, "dtable")
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("n", [1, 45, 300])
+def test_unidirectional_buckets_for_a_decoder(device, n):
+    """As its documentation has it: later keys in a bucket of their own whose row is -inf."""
+    dev = _dev(device)
+    g = torch.Generator().manual_seed(73)
+    heads, hd, buckets, far = 2, 32, 8, 20
+    qc, kc, of = pdt.nn.log_position_buckets(n, buckets, far, bidirectional=False)
+    of[:far] = buckets
+    qc, kc, of = (t.to(dev) for t in (qc, kc, of))
+    qkv, do = _rand(g, 2, n, 3 * heads * hd, device=dev).requires_grad_(), _rand(g, 2, n, heads * hd, std=0.1, device=dev)
+    learned = _rand(g, buckets, heads, dtype=torch.float32, device=dev).requires_grad_()
+    table = torch.cat([learned, learned.new_full((1, heads), -math.inf)])
+    out = F.rel_bias_attention(qkv, table, qc, kc, of, heads)
+    dqkv, dtable = torch.autograd.grad(out, [qkv, learned], do)
+    q, k, v = qkv.detach().double().view(2, n, 3, heads, hd).permute(2, 0, 3, 1, 4)
+    i = torch.arange(n, device=dev)
+    near = (i[:, None] - i[None]).clamp(min=0)
+    bucket = of.long()[(near + far).clamp(max=2 * far)]
+    bias = learned.detach().double()[bucket].permute(2, 0, 1).masked_fill(i[None] > i[:, None], -math.inf)
+    do4 = do.double().view(2, n, heads, hd).transpose(1, 2)
+    one = torch.ones(2, n, device=dev)
+    (o, dq, dk, dv, ds, _), es = _attention64(q, k, v, bias, one.bool(), one.double(), do4)
+    for i, (got, w, e) in enumerate(zip((out, *dqkv.split(heads * hd, -1)), (o, dq, dk, dv), es)):
+        _within(got, w.transpose(1, 2).reshape(2, n, -1), e.transpose(1, 2).reshape(2, n, -1), ("out", "dq", "dk", "dv")[i])
+    assert torch.isfinite(dtable).all()
