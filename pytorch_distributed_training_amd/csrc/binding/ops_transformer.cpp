@@ -15,6 +15,7 @@
 #include <cmath>
 #include <initializer_list>
 #include <limits>
+#include <unordered_set>
 
 #include "../kernels/attention_ext.h"
 #include "../kernels/gated_norm.h"
@@ -100,20 +101,34 @@ void check_plain(const char* op, std::initializer_list<const Tensor*> ts) {
     }
 }
 
-// A backward pass that is captured while an eager graph of the same leaves lives accumulates on the eager graph's stream: the
-// engine would wait for a stream outside the capture, in a thread whose exception ends the process.  Refused at the forward.
-void check_capture(std::initializer_list<const Tensor*> leaves) {
+// The engine hands a gradient to the stream on which the tensor's own node was made.  Where that is a node of an eager graph (an
+// input computed before the capture, or a leaf of a graph that lives), a captured backward pass would leave the capture, and the
+// process ends.  Refused at the forward, for the inputs and for all that they were computed from within the capture.
+bool outside_capture(const torch::autograd::Node& node) {
+    auto& n = const_cast<torch::autograd::Node&>(node);
+    if (!n.stream()) return false;
+    const hipStream_t s = c10::hip::HIPStreamMasqueradingAsCUDA(c10::hip::HIPStreamMasqueradingAsCUDA::UNCHECKED, *n.stream()).stream();
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (s) (void)hipStreamIsCapturing(s, &status);
+    return status != hipStreamCaptureStatusActive;
+}
+void check_capture(std::initializer_list<const Tensor*> inputs) {
+    using torch::autograd::Node;
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    for (const Tensor* t : leaves) {
-        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (!node || !node->stream()) continue;
-        const hipStream_t s = c10::hip::HIPStreamMasqueradingAsCUDA(c10::hip::HIPStreamMasqueradingAsCUDA::UNCHECKED, *node->stream()).stream();
-        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        if (s) (void)hipStreamIsCapturing(s, &status);
-        TORCH_CHECK(status == hipStreamCaptureStatusActive,
-                    "a forward pass with gradients is being captured while an eager graph of the same parameters lives on another stream: "
-                    "release that graph's outputs first");
+    std::vector<std::shared_ptr<Node>> todo;
+    std::unordered_set<const Node*> seen;
+    auto visit = [&](std::shared_ptr<Node> n) {
+        if (n && seen.insert(n.get()).second) todo.push_back(std::move(n));
+    };
+    for (const Tensor* t : inputs)
+        if (t->defined() && t->requires_grad()) visit(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    while (!todo.empty()) {
+        const std::shared_ptr<Node> n = std::move(todo.back());
+        todo.pop_back();
+        TORCH_CHECK(!outside_capture(*n),
+                    "a forward pass with gradients is being captured while an eager graph of the same parameters or inputs lives on "
+                    "another stream: release that graph's outputs first, or detach the inputs from it");
+        for (const auto& e : n->next_edges()) visit(e.function);
     }
 }
 

@@ -1324,3 +1324,45 @@ def test_unidirectional_buckets_for_a_decoder(device, n):
     for i, (got, w, e) in enumerate(zip((out, *dqkv.split(heads * hd, -1)), (o, dq, dk, dv), es)):
         _within(got, w.transpose(1, 2).reshape(2, n, -1), e.transpose(1, 2).reshape(2, n, -1), ("out", "dq", "dk", "dv")[i])
     assert torch.isfinite(dtable).all()
+
+
+@gpu
+def test_capture_beside_an_eager_graph_of_leaves_behind_the_inputs_is_refused():
+    """Parameters that are cast and expanded before the call (an attention pool's query) are leaves of its backward pass too."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(79)
+    qc, kc, of = (t.to(dev) for t in _log(9))
+    table, q, gate = (_rand(g, *s, dtype=torch.float32, device=dev).requires_grad_() for s in ((4, 1), (1, 1, 64), (64,)))
+    qkv, kv, x = (_rand(g, 2, 9, w, device=dev) for w in (192, 128, 64))
+    one = torch.ones(64, device=dev)
+    for call, leaf in ((lambda: F.rel_bias_attention(qkv, torch.cat([table, table * 0.5]), qc, kc, of, 1), table),
+                       (lambda: F.cross_attention(q.to(torch.bfloat16).expand(2, -1, -1), kv, 1), q),
+                       (lambda: F.gated_residual_norm(x, x, gate * 2, one, one)[0], gate)):
+        alive = call()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                one * 2
+                call()
+        want = torch.autograd.grad(alive, leaf, torch.ones_like(alive))[0]
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+            (got,) = torch.autograd.grad(out, leaf, torch.ones_like(out))
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+        # an input computed before the capture: its gradient would go to the stream of its own node, outside
+        y = leaf * 1.0
+        late = {table: lambda: F.rel_bias_attention(qkv, torch.cat([y, y * 0.5]), qc, kc, of, 1),
+                q: lambda: F.cross_attention(y.to(torch.bfloat16).expand(2, -1, -1), kv, 1),
+                gate: lambda: F.gated_residual_norm(x, x, y, one, one)[0]}[leaf]
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                one * 2
+                late()
+        y = y.detach().requires_grad_()
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            late()
