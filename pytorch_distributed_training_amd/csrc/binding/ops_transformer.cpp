@@ -33,15 +33,21 @@ bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 // The operators are differentiable calls with their nodes in C++: with Python functions a backward spent 20 to 50 us more on the
 // interpreter (lock, unpacking of saved tensors), more than its kernels take on small inputs.  A call whose operands the kernels
 // do not take (or that nobody should make) returns nothing: the Python side has the words for why.
+// with the numbers in memory that the tensor stands for (autograd hands out views that are negated when they are read, and zeros
+// without memory)
+Tensor written_out(const Tensor& t) {
+    if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
+    return t.is_neg() ? t.resolve_neg() : t;
+}
 Tensor dense16(const Tensor& t) {  // contiguous and 16-B aligned, by a copy where it is not
     if (!t.defined()) return t;
-    Tensor c = t.contiguous();
+    Tensor c = written_out(t).contiguous();
     return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 Tensor param32(const Tensor& t) { return t.defined() ? dense16(t.scalar_type() == at::kFloat ? t : t.to(at::kFloat)) : t; }
 Tensor int32(const Tensor& t) {
     if (!t.defined() || t.scalar_type() == at::kInt) return dense16(t);
-    return t.clamp(std::numeric_limits<int32_t>::min(), std::numeric_limits<int32_t>::max()).to(at::kInt);
+    return written_out(t).clamp(std::numeric_limits<int32_t>::min(), std::numeric_limits<int32_t>::max()).to(at::kInt);
 }
 bool is_index(const Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
@@ -96,7 +102,7 @@ void check_plain(const char* op, std::initializer_list<const Tensor*> ts) {
     for (const Tensor* t : ts) {
         if (!t->defined()) continue;
         TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), op, ": no forward-mode derivative, only a backward pass");
-        TORCH_CHECK(t->has_storage() && (t->numel() == 0 || t->const_data_ptr()), op,
+        TORCH_CHECK(t->has_storage() && (t->numel() == 0 || t->_is_zerotensor() || t->const_data_ptr()), op,
                     ": expected tensors with memory of their own (no vmap, no torch.func, no wrappers)");
     }
 }
@@ -145,7 +151,8 @@ void check_rows(const Tensor& t, const char* name) {
     TORCH_CHECK(t.size(0) < 2 || (t.stride(0) % 8 == 0 && t.stride(0) >= 0), name, ": batch stride ", t.stride(0));
 }
 // `t` where its rows are as check_rows wants them, else a copy
-Tensor rows3(const Tensor& t) {
+Tensor rows3(const Tensor& given) {
+    const Tensor t = written_out(given);
     const bool ok = t.stride(2) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
                     (t.size(1) < 2 || (t.stride(1) % 8 == 0 && t.stride(1) >= t.size(2) && t.stride(1) < (1L << 23))) &&
                     (t.size(0) < 2 || t.stride(0) % 8 == 0);
@@ -342,7 +349,7 @@ struct RelBiasFn : torch::autograd::Function<RelBiasFn> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& qkv_, const Tensor& table_, const Tensor& q_codes,
                           const Tensor& k_codes, const Tensor& bucket_of_, const OptTensor& lens_, int64_t heads) {
         const Tensor qkv = rows3(qkv_), bucket_of = int32(bucket_of_), lens = given(lens_) ? int32(*lens_) : Tensor();
-        auto [out, stat, tab, codes] = rel_bias_attention_fwd(qkv, param32(table_), q_codes.contiguous(), k_codes.contiguous(), bucket_of, heads, opt(lens), true);
+        auto [out, stat, tab, codes] = rel_bias_attention_fwd(qkv, param32(table_), written_out(q_codes).contiguous(), written_out(k_codes).contiguous(), bucket_of, heads, opt(lens), true);
         ctx->save_for_backward({qkv, out, stat, tab, codes, bucket_of, lens});
         ctx->set_materialize_grads(false);
         ctx->saved_data["heads"] = heads;
@@ -378,7 +385,7 @@ OptTensor rel_bias_attention(const Tensor& qkv, const Tensor& table, const Tenso
     if (table.device() != qkv.device()) return {};
     check_plain("rel_bias_attention", {&qkv, &table, &q_codes, &k_codes, &bucket_of, given(lens) ? &*lens : &qkv});
     if (!wants_grad({&qkv, &table}))
-        return std::get<0>(rel_bias_attention_fwd(rows3(qkv), param32(table), q_codes.contiguous(), k_codes.contiguous(), int32(bucket_of), heads,
+        return std::get<0>(rel_bias_attention_fwd(rows3(qkv), param32(table), written_out(q_codes).contiguous(), written_out(k_codes).contiguous(), int32(bucket_of), heads,
                                                   given(lens) ? opt(int32(*lens)) : lens, false));
     check_capture({&qkv, &table});
     return RelBiasFn::apply(qkv, table, q_codes, k_codes, bucket_of, lens, heads);

@@ -1366,3 +1366,32 @@ def test_capture_beside_an_eager_graph_of_leaves_behind_the_inputs_is_refused():
         y = y.detach().requires_grad_()
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             late()
+
+
+@gpu
+def test_negated_views():
+    """The imaginary part of a conjugate is a view of numbers that are yet to be negated."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(83)
+
+    def negated(t):
+        v = torch.imag(torch.complex(torch.zeros_like(t), t).conj()) if t.dtype == torch.float32 else torch._neg_view(t)
+        assert v.is_neg()
+        return v
+
+    x, w = _rand(g, 2, 9, 64, device=dev), _rand(g, 2, 9, 64, device=dev)
+    v = _rand(g, 64, dtype=torch.float32, device=dev)
+    for u, n in zip(F.gated_residual_norm(negated(x), x, negated(v), negated(v), v), F.gated_residual_norm(-x, x, -v, -v, v)):
+        assert torch.equal(u, n)
+    kv, lens = _rand(g, 2, 40, 128, device=dev), torch.tensor([-7, -40], device=dev, dtype=torch.int32)
+    assert torch.equal(F.cross_attention(negated(x), negated(kv), 1, None, negated(lens)), F.cross_attention(-x, -kv, 1, None, -lens))
+    qc, kc, of = (t.to(dev) for t in _log(40))
+    qkv, table = _rand(g, 2, 40, 192, device=dev), _rand(g, 8, 1, dtype=torch.float32, device=dev)
+    assert torch.equal(F.rel_bias_attention(negated(qkv), negated(table), negated(kc), negated(qc), of, 1),
+                       F.rel_bias_attention(-qkv, -table, -kc, -qc, of, 1))
+    q = x.clone().requires_grad_()
+    for grad in (negated(w), torch._efficientzerotensor(w.shape, dtype=w.dtype, device=dev)):
+        out = F.cross_attention(q, kv, 1)
+        (a,) = torch.autograd.grad(out, q, grad, retain_graph=True)
+        (b,) = torch.autograd.grad(out, q, grad + torch.zeros_like(w))
+        assert torch.equal(a, b)
