@@ -1395,3 +1395,36 @@ def test_negated_views():
         (a,) = torch.autograd.grad(out, q, grad, retain_graph=True)
         (b,) = torch.autograd.grad(out, q, grad + torch.zeros_like(w))
         assert torch.equal(a, b)
+
+
+@gpu
+def test_modes_around_the_calls():
+    """Inference mode, checkpointing of both kinds and saved tensors that wait on the host give the bits of a plain call."""
+    from torch.utils.checkpoint import checkpoint
+
+    for name, call, inputs in _three_calls(_dev("cuda")):
+        args = [t.clone().requires_grad_() for t in inputs]
+        out = call(*args)
+        w = torch.ones_like(out)
+        w[:, 1::2] = -0.5
+        want = torch.autograd.grad(out, args, w)
+        with torch.inference_mode():
+            assert torch.equal(call(*inputs), out)
+            assert torch.equal(call(*(t.clone() for t in inputs)), out)
+        with torch.no_grad():
+            assert torch.equal(call(*args), out)
+        for reentrant in (False, True):
+            again = [t.clone().requires_grad_() for t in inputs]
+            checkpoint(call, *again, use_reentrant=reentrant).backward(w)
+            assert all(torch.equal(t.grad, g) for t, g in zip(again, want))
+        with torch.autograd.graph.save_on_cpu(pin_memory=True):
+            out = call(*args)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, args, w), want))
+        # an input changed between the passes is an error, not a wrong gradient
+        x = inputs[0].clone().requires_grad_()
+        y = x * 1.0
+        out = call(y, inputs[1])
+        with torch.no_grad():
+            y.mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out, x, w)
