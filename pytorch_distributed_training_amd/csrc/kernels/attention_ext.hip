@@ -386,7 +386,7 @@ __global__ __launch_bounds__(256, 2) void k_ext_fwd(ExtArgs a, bf16* __restrict_
 // every fourth tile of 32 keys each, through an LDS ring of their own (no barrier until the join): the kernel is a stream over
 // K and V, 16 to 64 KiB of it in flight per workgroup, and bound by memory: 4 sequences of 65536 keys, 8 key heads of 128, four rows
 // each: 169 us, 6.4 TB/s (with the kernel above, whose waves would have one tile of rows for four: 193); 512 of 197 on 12 heads
-// of 64: 62 us, 5.0 TB/s (80 there, and the backward 275 for the 139 of its counterpart).
+// of 64: 64 us, 4.8 TB/s (80 there, and the backward 275 for the 139 of its counterpart).
 template <int HD, bool STREAM>
 __global__ __launch_bounds__(256, 2) void k_ext_fwd_few(ExtArgs a, bf16* __restrict__ out, float* __restrict__ stat,
                                                      float* __restrict__ part, float* __restrict__ part_ml, int splits) {
@@ -1062,7 +1062,7 @@ __global__ __launch_bounds__(256) void k_ext_dsum(float* __restrict__ dsum, long
 // dS summed over a part of the batch, for 128 queries x 128 keys of a head a workgroup (a wave: 32 queries, four tiles of 32
 // keys).  The bias of the block and the sums stay in registers while the batch streams through, so a pair costs two
 // multiply-adds and an exponential per sequence; written in register order, [tile][4][64 lanes] x 4 floats.  Its bound is what the
-// blocks move from L2, 64 KiB for 128 x 128 pairs of head_dim 64, at 6 to 7 TB/s: 58 us, 137 and 41 at the sizes given at the
+// blocks move from L2, 64 KiB for 128 x 128 pairs of head_dim 64, at 6 to 7 TB/s: 60 us, 139 and 39 at the sizes given at the
 // forward.  Blocks of 256 x 256 with the bias gathered for every sequence (no registers left for it) took 85 and 248, a second buffer
 // for K and V 64 and 149.
 template <int HD>
