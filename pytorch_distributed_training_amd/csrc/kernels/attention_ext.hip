@@ -1425,22 +1425,34 @@ __global__ __launch_bounds__(256, HD > 64 ? 1 : BIAS ? 3 : 2) void k_ext_bwd_kv(
 // tab[h][r] = table[bucket_of[r]][h] * sqrt(hd) (the scores are scaled after the bias is added), zero where the entry names no
 // bucket; byte offsets of the position codes, padded with the last one to a multiple of 128 (what is past the end then falls
 // on an entry that its neighbours use).  Offsets, their differences and an LDS address fit 32 bits where the codes are below
-// 2^27 in magnitude.  Only differences count, so where some are not, all are taken from the first key's; where that leaves some
-// too, the table is NaN, and so is every result: a limit without a sync, but not without a word.  (Every workgroup looks at
-// all codes by itself: 2.3 -> 3.1 us on 50 tokens, 4.7 -> 5.0 on 197 to 2047.)
-constexpr long kCodeReach = 1L << 27;
+// kCodeReach in magnitude.  What matters of a difference is its place in a table of at most 4096 entries, so larger codes move in:
+// those above the reach keep their distances from the lowest of them, kCodeSpan of them, and are kCodeGap from the others where they
+// are further; those below likewise.  Left are pairs past the span on one side: where a query and a key are, the table is NaN,
+// and so is every result: a limit without a sync, but not without a word.  (Every workgroup looks at all codes by itself: 2.3 ->
+// 3.1 us on 50 tokens, 4.7 -> 5.0 on 197 to 2047.)
+constexpr long kCodeReach = 1L << 27, kCodeSpan = (1L << 27) - (1L << 18), kCodeGap = 2 * kExtMaxEntries;
+static_assert(8 * (kCodeReach + kCodeSpan + 2 * kCodeGap) + 163840 < 1L << 31, "byte offsets' differences and an LDS address fit 32 bits");
+struct CodeEdges {
+    long low, high;  // the largest code below -kCodeReach, the smallest from kCodeReach on
+};
 __device__ __forceinline__ long code_at(const void* codes, bool wide, int i) {
     return wide ? static_cast<const long*>(codes)[i] : (long)static_cast<const int*>(codes)[i];
 }
-// bit 0: a code is past the reach; bit 1: one is so from `base` on (256 threads, four loads of each axis in flight)
+// how far past the span of its side a code is, or less than 0
+__device__ __forceinline__ long past_span(long c, const CodeEdges& e) {
+    return c >= kCodeReach ? c - e.high - kCodeSpan : c < -kCodeReach ? e.low - c - kCodeSpan : -1;
+}
+__device__ __forceinline__ int moved_in(long c, const CodeEdges& e) {
+    if (c >= -kCodeReach && c < kCodeReach) return (int)c;
+    const bool up = c >= kCodeReach;
+    const long gap = up ? e.high - kCodeReach : -kCodeReach - e.low;  // (from the reach to the first)
+    const long out = kCodeReach + min(gap, kCodeGap) + (past_span(c, e) >= 0 ? kCodeSpan + kCodeGap : up ? c - e.high : e.low - c);
+    return (int)(up ? out : -out);
+}
+// whether a code is past the reach (256 threads, four loads of each axis in flight)
 template <typename Q, typename K>
-__device__ __forceinline__ int codes_past_reach(const void* q_codes, const void* k_codes, int S, long base) {
-    bool from_zero = false, from_base = false;
-    auto look = [&](long c) {
-        long d;
-        from_zero |= c < -kCodeReach || c >= kCodeReach;
-        from_base |= __builtin_sub_overflow(c, base, &d) || d < -kCodeReach || d >= kCodeReach;
-    };
+__device__ __forceinline__ bool codes_past_reach(const void* q_codes, const void* k_codes, int S) {
+    bool past = false;
     for (int i0 = (int)threadIdx.x; i0 < S; i0 += 1024) {
         Q q[4];
         K k[4];
@@ -1451,18 +1463,47 @@ __device__ __forceinline__ int codes_past_reach(const void* q_codes, const void*
             k[n] = static_cast<const K*>(k_codes)[i];
         }
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            look(q[n]);
-            look(k[n]);
-        }
+        for (int n = 0; n < 4; ++n) past |= q[n] < -kCodeReach || q[n] >= kCodeReach || k[n] < -kCodeReach || k[n] >= kCodeReach;
     }
-    return (from_zero ? 1 : 0) | (from_base ? 2 : 0);
+    return past;
+}
+// the edges of both sides, and whether a query's and a key's code are both past the span of one
+__device__ __forceinline__ bool code_edges(const void* q_codes, bool q_wide, const void* k_codes, bool k_wide, int S, CodeEdges& e) {
+    __shared__ long edge[2][4];
+    __shared__ int past[4];
+    const int wave = threadIdx.x >> 6;
+    e = {-__LONG_MAX__ - 1, __LONG_MAX__};
+    for (int i = (int)threadIdx.x; i < 2 * S; i += 256) {
+        const long c = i < S ? code_at(q_codes, q_wide, i) : code_at(k_codes, k_wide, i - S);
+        if (c >= kCodeReach) e.high = min(e.high, c);
+        if (c < -kCodeReach) e.low = max(e.low, c);
+    }
+    for (int n = 1; n < 64; n *= 2) {
+        e.high = min(e.high, __shfl_xor(e.high, n, 64));
+        e.low = max(e.low, __shfl_xor(e.low, n, 64));
+    }
+    edge[0][wave] = e.low;  // (all lanes the same)
+    edge[1][wave] = e.high;
+    __syncthreads();
+    for (int n = 0; n < 4; ++n) {
+        e.low = max(e.low, edge[0][n]);
+        e.high = min(e.high, edge[1][n]);
+    }
+    int bits = 0;  // 1, 2: a query's above, below; 4, 8: a key's
+    for (int i = (int)threadIdx.x; i < 2 * S; i += 256) {
+        const long c = i < S ? code_at(q_codes, q_wide, i) : code_at(k_codes, k_wide, i - S);
+        if (past_span(c, e) >= 0) bits |= (c > 0 ? 1 : 2) << (i < S ? 0 : 2);
+    }
+    for (int n = 1; n < 64; n *= 2) bits |= __shfl_xor(bits, n, 64);
+    past[wave] = bits;
+    __syncthreads();
+    bits = past[0] | past[1] | past[2] | past[3];
+    return ((bits & 5) == 5) || ((bits & 10) == 10);
 }
 __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ table, const int* __restrict__ bucket_of,
                                                      const void* __restrict__ q_codes, bool q_wide, const void* __restrict__ k_codes, bool k_wide,
                                                      float* __restrict__ tab, int* __restrict__ codes /* q4 [Sp], k4 [Sp], ranges of 32 */, int R,
                                                      int Rp, int NB, int H, int S, int Sp, float inv_scale, int tab_blocks) {
-    __shared__ int past[4];
     const bool is_tab = (int)blockIdx.x < tab_blocks;
     // what this thread writes, loaded before the codes are looked at: an entry, or a code
     const uint32_t i = blockIdx.x * 256 + threadIdx.x, h = i / (uint32_t)Rp, r = i - h * (uint32_t)Rp;
@@ -1477,21 +1518,18 @@ __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ t
         if (v < -kBiasFloor && v > -kInf) v = -kBiasFloor;
         if (v > kBiasFloor && v < kInf) v = kBiasFloor;
     }
-    const long first = S > 0 ? code_at(k_codes, k_wide, 0) : 0;
-    int bits = !q_wide && !k_wide ? codes_past_reach<int, int>(q_codes, k_codes, S, first)
-               : !q_wide          ? codes_past_reach<int, long>(q_codes, k_codes, S, first)
-               : !k_wide          ? codes_past_reach<long, int>(q_codes, k_codes, S, first)
-                                  : codes_past_reach<long, long>(q_codes, k_codes, S, first);
-    bits = (__any(bits & 1) ? 1 : 0) | (__any(bits & 2) ? 2 : 0);
-    if ((threadIdx.x & 63) == 0) past[threadIdx.x >> 6] = bits;
-    __syncthreads();
-    bits = past[0] | past[1] | past[2] | past[3];
-    const bool too_far = bits == 3;
+    const bool past = !q_wide && !k_wide ? codes_past_reach<int, int>(q_codes, k_codes, S)
+                      : !q_wide          ? codes_past_reach<int, long>(q_codes, k_codes, S)
+                      : !k_wide          ? codes_past_reach<long, int>(q_codes, k_codes, S)
+                                         : codes_past_reach<long, long>(q_codes, k_codes, S);
+    CodeEdges edges{};
+    bool too_far = false;
+    if (__syncthreads_or(past)) too_far = code_edges(q_codes, q_wide, k_codes, k_wide, S, edges);
     if (is_tab) {
         if (h < (uint32_t)H) tab[i] = too_far ? __builtin_nanf("") : v * inv_scale;
         return;
     }
-    const int c = too_far ? 0 : (int)(code - (bits & 1 ? first : 0)) * 4;
+    const int c = moved_in(code, edges) * 4;
     codes[w] = c;
     int lo = c, hi = c;
 #pragma unroll

@@ -1093,8 +1093,20 @@ def test_create_graph_raises_only_for_a_second_derivative(device):
                     ask(got[i])
 
 
+def _check_codes(qkv, table, q, k, of):
+    """The output for 64-bit codes against the plain form (codes are clamped where their differences would not fit)."""
+    dev, (b, n, _), heads = qkv.device, qkv.shape, table.shape[1]
+    out = F.rel_bias_attention(qkv, table, q, k, of, heads)
+    limit = 2 ** 62 + 2 ** 28
+    bucket = of[(q.clamp(-limit, limit)[:, None] - k.clamp(-limit, limit)[None]).clamp(0, of.numel() - 1)]
+    x, y, v = qkv.double().view(b, n, 3, heads, -1).permute(2, 0, 3, 1, 4)
+    live = _live(None, b, n, dev)
+    (o, *_), (e, *_) = _attention64(x, y, v, table.double()[bucket].permute(2, 0, 1), live, live.double(), torch.zeros_like(x))
+    _within(out, o.transpose(1, 2).reshape(out.shape), e.transpose(1, 2).reshape(out.shape), "out")
+
+
 @gpu
-@pytest.mark.parametrize("base", [2 ** 27, 2 ** 31 - 400, -2 ** 31, 1_765_000_000_000, -2 ** 62])
+@pytest.mark.parametrize("base", [2 ** 27, 2 ** 27 - 80, -2 ** 27 - 80, 2 ** 31 - 400, -2 ** 31, 1_765_000_000_000, -2 ** 62])
 def test_rel_bias_codes_of_any_size(base):
     """Only differences count: positions that count from far away (clocks) give the bits of those that count from zero."""
     dev = _dev("cuda")
@@ -1111,23 +1123,42 @@ def test_rel_bias_codes_of_any_size(base):
     want = run(qc, kc)
     assert all(torch.equal(x, y) for x, y in zip(want, run(qc.int(), kc)))
     q, k = qc + base, kc + base
-    forms = [(q, k)] if max(abs(base), abs(base + 400)) >= 2 ** 31 and base != -2 ** 31 else [(q, k), (q.int(), k.int()), (q, k.int())]
+    forms = [(q, k)]
+    if abs(base) < 2 ** 31 or base == -2 ** 31:
+        forms += [(q.int(), k.int()), (q, k.int()), (q.int(), k)] if q.max() < 2 ** 31 else []
     for f in forms:
         assert all(torch.equal(x, y) for x, y in zip(want, run(*f)))
     strided = torch.stack([q, q + 1], 1)[:, 0]
     assert all(torch.equal(x, y) for x, y in zip(want, run(strided, k)))
-    # apart from the first key by almost 2^27: the far token is past the table's reach; by more: no number at all
+    # one token far from the others, among the keys, among the queries; in both: no number at all
+    step = 2 ** 27 if base > 0 else -2 ** 27
     q2, k2 = q.clone(), k.clone()
-    k2[-1] = k2[0] - 1 + 2 ** 27
-    got = run(q2, k2)
-    bucket = of[(qc[:, None] - (k2 - base)[None]).clamp(0, of.numel() - 1)]
-    bias = table.double()[bucket].permute(2, 0, 1)
-    x, y, v = qkv.double().view(2, 150, 3, 2, 64).permute(2, 0, 3, 1, 4)
-    (o, *_), (e, *_) = _attention64(x, y, v, bias, _live(None, 2, 150, dev), torch.ones(2, 150, device=dev).double(), torch.zeros_like(x))
-    _within(got[0], o.transpose(1, 2).reshape(2, 150, 128), e.transpose(1, 2).reshape(2, 150, 128), "out")
-    k2[-1] += 1
+    q2[-1] += step
+    k2[-1] += step
+    _check_codes(qkv, table, q, k2, of)
+    _check_codes(qkv, table, q2, k, of)
     out, dqkv, dtable = run(q2, k2)
     assert out.isnan().all() and dqkv.isnan().all() and dtable.isnan().any()  # (a bucket that no pair falls on keeps its zero)
+
+
+@gpu
+@pytest.mark.parametrize("base", [0, 2 ** 40])
+@pytest.mark.parametrize("marks", [(2 ** 31 - 1, None), (None, -2 ** 31), (-2 ** 40, -2 ** 40), (-2 ** 63, 5), (2 ** 27, -2 ** 27 - 1), (-2 ** 27, 2 ** 27)], ids=str)
+def test_rel_bias_marked_codes(marks, base):
+    """Tokens marked by codes far from all others, on one axis or both: past the table's reach, and next to one another."""
+    dev = _dev("cuda")
+    g = torch.Generator().manual_seed(89)
+    qc, kc, of = (t.to(dev).long() for t in _log(90))
+    qkv, table = _rand(g, 2, 90, 384, device=dev), _rand(g, 8, 2, dtype=torch.float32, device=dev)
+    q, k = qc + base, kc + base
+    for t, mark in ((q, marks[0]), (k, marks[1])):
+        if mark is not None:
+            t[:5] = mark
+    if base and any(m is not None and 2 ** 27 <= m for m in marks):
+        # (a mark of 2^27 or more is where that side's distances count from: 2^40 is too far from it for queries and keys)
+        assert F.rel_bias_attention(qkv, table, q, k, of, 2).isnan().all()
+    else:
+        _check_codes(qkv, table, q, k, of)
 
 
 @gpu
