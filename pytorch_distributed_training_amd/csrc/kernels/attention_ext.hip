@@ -37,7 +37,13 @@ namespace pdt {
 namespace {
 
 constexpr float kInf = __builtin_inff();
-constexpr float kBiasFloor = 1e30f;  // finite biases are clamped here: times sqrt(hd) they stay finite (-inf stays -inf: never attended)
+// Finite biases stay finite times sqrt(hd), and apart: from 2^120 on in magnitude what is over counts a sixteenth (lower stays lower
+// by at least 2^92, equal stays equal; the type's lowest value, 2^128, becomes 2^124).  -inf stays -inf: never attended.
+constexpr float kBiasFull = 0x1p120f;
+__device__ __forceinline__ float finite_bias(float v) {
+    const float over = fabsf(v) - kBiasFull;
+    return over > 0.f && over < kInf ? copysignf(fmaf(over, 0.0625f, kBiasFull), v) : v;
+}
 
 // one 4-byte-aligned 16-B piece per lane into LDS (lane-linear), descriptor from wave-uniform words
 __device__ __forceinline__ i32x4 uniform_rsrc(const void* base, uint32_t bytes) {
@@ -1514,9 +1520,7 @@ __global__ __launch_bounds__(256) void k_bias_tables(const float* __restrict__ t
         code = code_at(w < Sp ? q_codes : k_codes, w < Sp ? q_wide : k_wide, at < S ? at : S - 1);
     } else if (h < (uint32_t)H) {
         const int n = r < (uint32_t)R ? bucket_of[r] : -1;
-        v = n >= 0 && n < NB ? table[(long)n * H + h] : 0.f;
-        if (v < -kBiasFloor && v > -kInf) v = -kBiasFloor;
-        if (v > kBiasFloor && v < kInf) v = kBiasFloor;
+        v = n >= 0 && n < NB ? finite_bias(table[(long)n * H + h]) : 0.f;
     }
     const bool past = !q_wide && !k_wide ? codes_past_reach<int, int>(q_codes, k_codes, S)
                       : !q_wide          ? codes_past_reach<int, long>(q_codes, k_codes, S)

@@ -1459,3 +1459,19 @@ def test_modes_around_the_calls():
             y.mul_(2)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(out, x, w)
+
+
+@gpu
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_rel_bias_masks_of_different_depth(hd):
+    """Rows of several masking values only: the least low wins, as in the plain form, up to the ends of the type."""
+    dev = _dev("cuda")
+    lowest, low16 = torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min
+    g = torch.Generator().manual_seed(97)
+    n = 60
+    qc, kc = torch.arange(n, dtype=torch.int32) % 5 * 100, -torch.arange(n, dtype=torch.int32) % 7  # an entry a pair of residues
+    of = torch.randint(0, 4, (420,), generator=g)
+    for values in ((lowest, -1e30, -1e30, lowest), (low16, lowest, low16, lowest), (-2e38, -3e38, -1e37, -1e36), (-math.inf, lowest, -math.inf, lowest),
+                   (3e38, 1e38, -3e38, lowest)):
+        table = torch.tensor(values)[:, None].repeat(1, 2)
+        _check_rel(dev, 2, (qc, kc, of), 2, hd, table=table, seed=int(g.initial_seed()))
