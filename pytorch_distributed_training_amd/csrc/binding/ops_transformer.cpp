@@ -33,7 +33,8 @@ bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 // The operators are differentiable calls with their nodes in C++: with Python functions a backward spent 20 to 50 us more on the
 // interpreter (lock, unpacking of saved tensors), more than its kernels take on small inputs.  A call whose operands the kernels
 // do not take (or that nobody should make) returns nothing: the Python side has the words for why.
-// with the numbers in memory that the tensor stands for (autograd hands out views that are negated when they are read, and zeros
+
+// `t` with the numbers in memory that the tensor stands for (autograd hands out views that are negated when they are read, and zeros
 // without memory)
 Tensor written_out(const Tensor& t) {
     if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
@@ -110,10 +111,10 @@ void check_plain(const char* op, std::initializer_list<const Tensor*> ts) {
 // The engine hands a gradient to the stream on which the tensor's own node was made.  Where that is a node of an eager graph (an
 // input computed before the capture, or a leaf of a graph that lives), a captured backward pass would leave the capture, and the
 // process ends.  Refused at the forward, for the inputs and for all that they were computed from within the capture.
-bool outside_capture(const torch::autograd::Node& node) {
-    auto& n = const_cast<torch::autograd::Node&>(node);
-    if (!n.stream()) return false;
-    const hipStream_t s = c10::hip::HIPStreamMasqueradingAsCUDA(c10::hip::HIPStreamMasqueradingAsCUDA::UNCHECKED, *n.stream()).stream();
+bool outside_capture(torch::autograd::Node& node) {
+    const auto stream = node.stream();
+    if (!stream) return false;
+    const hipStream_t s = c10::hip::HIPStreamMasqueradingAsCUDA(c10::hip::HIPStreamMasqueradingAsCUDA::UNCHECKED, *stream).stream();
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (s) (void)hipStreamIsCapturing(s, &status);
     return status != hipStreamCaptureStatusActive;

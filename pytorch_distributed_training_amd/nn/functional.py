@@ -579,8 +579,9 @@ def rel_bias_attention(qkv, table, q_codes, k_codes, bucket_of, heads: int, leng
     The bias of query ``i`` and key ``j`` in head ``h`` is ``table[bucket, h]`` (``table`` ``[buckets, heads]``, learned) with
     ``bucket = bucket_of[clamp(q_codes[i] - k_codes[j], 0, len(bucket_of) - 1)]``; ``nn.grid_position_buckets`` and
     ``nn.log_position_buckets`` make the three integer tensors.  An entry of ``bucket_of`` outside the table means no bias; a table
-    entry of ``-inf`` forbids the pair.  Codes may be of any size; on the GPU the results are NaN where a query's and a key's
-    are both some 2^27 past the nearest code of 2^27 or more on their side (a clock that runs that long within one call).
+    entry of ``-inf`` forbids the pair (NaN or ``inf`` may reach every gradient, from rows behind a sequence's end too).  Codes may
+    be of any size; on the GPU the results are NaN where a query's and a key's are both some 2^27 past the nearest code of 2^27 or
+    more on their side (a clock that runs that long within one call).
 
     ``lengths`` (``[B]`` integers, on the device of ``qkv``): sequence ``b`` is its first ``lengths[b]`` tokens; the rows behind
     it are neither attended to nor read, their outputs and gradients are zero, and so is a row whose every key is forbidden.
